@@ -29,6 +29,7 @@ from .ops import (  # noqa: F401
     table_size,
     transfer_edge_id,
 )
+from .dropouts import Dropout, dropout  # noqa: F401
 from .sampler import Block, DataLoader, FusedMapSampler, PendingBatch, transpose_blocks  # noqa: F401
 from .conv import (  # noqa: F401
     GAT,

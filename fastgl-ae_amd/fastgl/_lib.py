@@ -76,6 +76,8 @@ SIGNATURES = {
     "fgl_row_product_sum": (_i32, [_vp, _i64, _vp, _i64, _i32, _vp, _i64, _vp, _i64, _i32, _i32, _i64, _i32, _i32, _vp, _vp, _i64, _vp]),
     "fgl_row_product_add": (_i32, [_vp, _i64, _vp, _i64, _i32, _i64, _i32, _i32, _i32, _vp, _i64, _vp]),
     "fgl_row_product": (_i32, [_vp, _i64, _vp, _i64, _i32, _i64, _i32, _i32, _i32, _vp, _vp, _i64, _vp]),
+    "fgl_dropout": (_i32, [_vp, _i64, _i64, _i64, _i32, C.c_double, _u64, _u32, _vp, _i32, _vp, _vp]),
+    "fgl_dropout_relu_backward": (_i32, [_vp, _vp, _i64, _i32, C.c_double, _vp, _vp]),
     "fgl_rmat_keys": (_i32, [_i64, _i64, _i32, _i64, _u64, _vp, _vp]),
 }
 

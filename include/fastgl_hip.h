@@ -453,6 +453,20 @@ int fgl_weight_grad(const void* d_a, int64_t lda, const void* d_b, int64_t ldb, 
 const char* fgl_product_last_kernel(void);
 
 /* ---------------------------------------------------------------------------------
+ * Dropout between layers (the reference's nn.Dropout, GraphConv.py:71,84-85) with a mask that is never stored.  For element
+ * i = row * n_cols + column of x (row stride ldx):
+ *   words = philox4x32_10(counter = (i / 4 low, i / 4 high, stream_id + *d_stream_offset, 0x44524F50), key = (seed low, seed high))
+ *   out[i] = words[i % 4] >= round(p 2^32) ? f(x[i]) / (1 - p) : 0,   f = max(x, 0) where relu is not zero, else x itself
+ * d_stream_offset (device int32, may be NULL) is read when the kernel runs: a captured call draws another mask at every replay whose
+ * caller changed it.  p = 0 keeps everything, p = 1 nothing.  out: [n_rows, n_cols] without gaps; x and out of `dtype`, at most 2^35 elements.
+ * Its gradient: the same call (relu = 0) on the output's gradient; with relu, fgl_dropout_relu_backward, which takes the
+ * output in the mask's place: dx[i] = out[i] <= 0 ? 0 : dout[i] / (1 - p), n elements without gaps.
+ * ------------------------------------------------------------------------------- */
+int fgl_dropout(const void* d_x, int64_t ldx, int64_t n_rows, int64_t n_cols, int dtype, double p, uint64_t seed, uint32_t stream_id,
+                const int32_t* d_stream_offset, int relu, void* d_out, void* stream);
+int fgl_dropout_relu_backward(const void* d_dout, const void* d_out, int64_t n, int dtype, double p, void* d_dx, void* stream);
+
+/* ---------------------------------------------------------------------------------
  * Seeded R-MAT key generator for the synthetic graphs (a=.57 b=.19 c=.19 d=.05).
  * For draw e in [first_edge, first_edge+n_edges): writes the two symmetrised keys
  * (row<<32 | col) of the in-neighbour CSR, or INT64_MAX twice for a self loop / an
