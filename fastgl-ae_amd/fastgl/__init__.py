@@ -46,4 +46,5 @@ from .conv import (  # noqa: F401
     SAGEConv,
     edge_softmax_torch,
 )
+from .losses import LinearCrossEntropy, linear_cross_entropy  # noqa: F401
 from . import graph  # noqa: F401

@@ -20,6 +20,8 @@ F32, BF16 = 0, 1
 AGG_SUM, AGG_MEAN, AGG_GCN, AGG_COLMEAN, AGG_EDGE, AGG_COLMEAN_PTR, AGG_GCN_OWN, AGG_GCN_OWN_PTR = 0, 1, 2, 3, 4, 5, 6, 7
 ZERO_COPY_SELF, ZERO_ZEROS = 0, 1
 ABI_VERSION = 11  # FGL_ABI_VERSION of include/fastgl_hip.h that the signatures below follow
+REDUCE = {"none": 0, "sum": 1, "mean": 2}
+XENT_ROWS, XENT_WEIGHTS, XENT_MAX_DIM = 1, 2, 512
 STATUS_TABLE_FULL, STATUS_UNIQ_OVERFLOW, STATUS_MISSING_KEY, STATUS_BAD_SEED, STATUS_BAD_ID = 1, 2, 4, 8, 16
 IDMAP_ORDERED, IDMAP_ARRIVAL, IDMAP_FINAL, IDMAP_LEAVE_TABLE_EMPTY = 0, 1, 2, 8
 BLOCKS_TABLE_EMPTY, BLOCKS_LEAVE_TABLE_EMPTY, BLOCKS_SORT_TRANSPOSED = 4, 8, 16
@@ -78,6 +80,10 @@ SIGNATURES = {
     "fgl_row_product": (_i32, [_vp, _i64, _vp, _i64, _i32, _i64, _i32, _i32, _i32, _vp, _vp, _i64, _vp]),
     "fgl_dropout": (_i32, [_vp, _i64, _i64, _i64, _i32, C.c_double, _u64, _u32, _vp, _i32, _vp, _vp]),
     "fgl_dropout_relu_backward": (_i32, [_vp, _vp, _i64, _i32, C.c_double, _vp, _vp]),
+    "fgl_linear_cross_entropy_state_bytes": (_sz, [_i64, _i64, _i32, _i32, _i32]),
+    "fgl_linear_cross_entropy_workspace_bytes": (_sz, [_i64, _i64, _i32, _i32, _i32, _i32]),
+    "fgl_linear_cross_entropy": (_i32, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i32, _i64, _i64, _i64, _i32, _i32, _i32, _i32, _vp, _vp, _sz, _vp, _sz, _vp]),
+    "fgl_linear_cross_entropy_backward": (_i32, [_vp, _i64, _i64, _i32, _i32, _i32, _i32, _vp, _sz, _vp, _vp, _vp, _vp, _sz, _vp]),
     "fgl_rmat_keys": (_i32, [_i64, _i64, _i32, _i64, _u64, _vp, _vp]),
 }
 

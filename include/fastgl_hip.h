@@ -44,6 +44,12 @@ enum fgl_error {
 
 enum fgl_dtype { FGL_F32 = 0, FGL_BF16 = 1 };
 
+/* what a loss over rows becomes */
+enum fgl_reduction { FGL_REDUCE_NONE = 0, FGL_REDUCE_SUM = 1, FGL_REDUCE_MEAN = 2 };
+
+/* gradients that fgl_linear_cross_entropy prepares for, or'ed */
+enum fgl_xent_want { FGL_XENT_ROWS = 1, FGL_XENT_WEIGHTS = 2 };
+
 /* per-edge weight of fgl_aggregate (row = output row, col = gathered row) */
 enum fgl_agg_mode {
     FGL_AGG_SUM = 0,     /* w = 1                                             (GIN)  */
@@ -465,6 +471,27 @@ const char* fgl_product_last_kernel(void);
 int fgl_dropout(const void* d_x, int64_t ldx, int64_t n_rows, int64_t n_cols, int dtype, double p, uint64_t seed, uint32_t stream_id,
                 const int32_t* d_stream_offset, int relu, void* d_out, void* stream);
 int fgl_dropout_relu_backward(const void* d_dout, const void* d_out, int64_t n, int dtype, double p, void* d_dx, void* stream);
+
+/* ---------------------------------------------------------------------------------
+ * A model's last product and its loss as one operator, without the logits ever lying in memory: softmax cross entropy of
+ * x W^T + b (replaces the last layer's product followed by nn.CrossEntropyLoss, train_fastgl.py:328,383).
+ *   s_iv = sum_d x[i, d] w[v, d] + b[v],   loss_i = log(sum_v exp(s_iv)) - s_i,label(i)
+ * x [n_rows, dim] and w [n_classes, dim] of `dtype`, any strides (in elements); d_bias [n_classes] of `dtype` or NULL, where -1e30 and less, -infinity among them, leave a class out;
+ * labels int32 or (label64) int64.  A row labelled ignore_index has loss 0 and no gradient; one with a label outside [0, n_classes) has a
+ * loss and gradients that are not numbers.  d_loss: float, n_rows of them (FGL_REDUCE_NONE), or the sum, or the sum over the number of rows with a
+ * label.  dim 1 .. 512, other sizes 1 .. 2^31 - 65.
+ * want: what the backward pass will be asked for, FGL_XENT_ROWS (dx; formed here up to its factor) and FGL_XENT_WEIGHTS (dw, db).  The state
+ * goes to the backward pass, which may run several times; the workspace is free afterwards.  Both on 256-byte boundaries.
+ * Backward: d_loss_grad, float, n_rows of them or one; d_dx [n_rows, dim], d_dw [n_classes, dim], d_db [n_classes] without gaps, of
+ * `dtype`, each may be NULL (d_db without d_dw may not).  The same bits on every run.
+ * ------------------------------------------------------------------------------- */
+size_t fgl_linear_cross_entropy_state_bytes(int64_t n_rows, int64_t n_classes, int dim, int dtype, int want);
+size_t fgl_linear_cross_entropy_workspace_bytes(int64_t n_rows, int64_t n_classes, int dim, int dtype, int want, int backward);
+int fgl_linear_cross_entropy(const void* d_x, int64_t x_row_stride, int64_t x_col_stride, const void* d_w, int64_t w_row_stride, int64_t w_col_stride,
+                             const void* d_bias, const void* d_labels, int label64, int64_t ignore_index, int64_t n_rows, int64_t n_classes, int dim,
+                             int dtype, int reduction, int want, float* d_loss, void* d_state, size_t state_bytes, void* d_ws, size_t ws_bytes, void* stream);
+int fgl_linear_cross_entropy_backward(const float* d_loss_grad, int64_t n_rows, int64_t n_classes, int dim, int dtype, int reduction, int want,
+                                      void* d_state, size_t state_bytes, void* d_dx, void* d_dw, void* d_db, void* d_ws, size_t ws_bytes, void* stream);
 
 /* ---------------------------------------------------------------------------------
  * Seeded R-MAT key generator for the synthetic graphs (a=.57 b=.19 c=.19 d=.05).

@@ -1,0 +1,338 @@
+"""fastgl.linear_cross_entropy against the definition in float64.
+
+Tolerances.  Let u = 2^-24 (fp32) and L the largest sum of magnitudes sum_d |x_id w_vd| + |b_v| of a row.  A logit is off by at most c u L
+with c = 3 + d / 32 (three-part products are exact to 2^-24 of each term; one addition for every 32 columns), in bf16, whose products
+are exact and are added up one instruction of 16 columns after another, with c = 2 + d / 16; the exponentials by 2 u and u times their
+argument in powers of two, at most 2 L log2(e), more.  So a share p is off by eps = 4 u (c + 4) (L + 4) of itself and a loss by eps, and a
+sum of n shares adds at most log-many roundings by tiles and one for each tile: (n / 32 + 8) u.  Gradients are sums of p (bf16: rounded, 2^-8 more)
+times finite values: their error is at most that share of the sum of the terms' magnitudes, plus half a step of the result."""
+import pytest
+import torch
+
+import fastgl
+
+pytestmark = pytest.mark.gpu
+
+HALF = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8}
+
+
+def definition(x, w, b, y, ignore, reduction, g):
+    """(loss, dx, dw, db) in 64 bits, and the sums of the magnitudes of the gradients' terms."""
+    x, w = x.detach().double(), w.detach().double()
+    s = x @ w.t()
+    if b is not None:
+        s = s + b.detach().double()
+    valid = y != ignore
+    label = torch.where(valid, y, torch.zeros_like(y)).long()
+    rows = torch.arange(x.size(0), device=x.device)
+    log_p = s - torch.logsumexp(s, 1, keepdim=True)
+    # (in 64 bits too, a loss of e^-30 has few bits left as a difference of logits)
+    others = (s - s[rows, label][:, None]).exp().scatter(1, label[:, None], 0.0).sum(1)
+    own = torch.where(others < 1e100, torch.log1p(others), -log_p[rows, label])
+    losses = torch.where(valid, own, 0.0)
+    count = valid.sum()
+    loss = losses if reduction == "none" else losses.sum() / (count if reduction == "mean" else 1)
+    d = log_p.exp()
+    d[rows, label] = torch.expm1(-own)
+    d *= torch.where(valid, g.double() / (count if reduction == "mean" else 1), 0.0)[:, None] if reduction != "none" else torch.where(valid, g.double(), 0.0)[:, None]
+    d[~valid] = 0.0
+    return (losses, loss, d @ w, d.t() @ x, d.sum(0)), (d.abs() @ w.abs(), d.abs().t() @ x.abs(), d.abs().sum(0))
+
+
+def share_error(x, w, b, n_terms):
+    u, d = 2.0 ** -24, x.size(1)
+    # (magnitudes of a few thousand classes at a time)
+    most = max(float((x.detach().abs().double() @ w.detach()[k:k + 4096].abs().double().t()).max()) for k in range(0, w.size(0), 4096))
+    if b is not None:
+        most += float(b.detach().double().abs().masked_fill(b.detach().isinf(), 0.0).max())
+    c = 3 + d / 32 if x.dtype == torch.float32 else 2 + d / 16
+    return 4 * u * (c + 4) * (most + 4) + (n_terms / 32 + 8) * u
+
+
+def check(x, w, b, y, reduction="mean", ignore=-100, g=None, limit_scale=1.0):
+    gen = torch.Generator(device=x.device).manual_seed(1)
+    n = x.size(0)
+    if g is None:
+        g = torch.rand(n if reduction == "none" else (), generator=gen, device=x.device) + 0.5
+    leaves = [t.detach().requires_grad_() for t in (x, w) + (() if b is None else (b,))]
+    loss = fastgl.linear_cross_entropy(leaves[0], leaves[1], y, leaves[2] if b is not None else None, ignore, reduction)
+    assert loss.dtype == torch.float32 and loss.shape == ((n,) if reduction == "none" else ())
+    grads = torch.autograd.grad(loss, leaves, g)
+    (losses, want, *want_grads), sums = definition(x, w, b, y, ignore, reduction, g)
+    eps = share_error(x, w, b, w.size(0))
+    loss_limit = eps * (1 + losses) if reduction == "none" else eps * (1 + losses.max()) * (n if reduction == "sum" else 1)
+    assert ((loss.detach().double() - want).abs() <= loss_limit).all(), float((loss.detach().double() - want).abs().max())
+    half = HALF[x.dtype]
+    for name, got, exact, total in zip(("dx", "dw", "db"), grads, want_grads, sums):
+        assert got.dtype == x.dtype and got.shape == exact.shape
+        terms = n if name != "dx" else w.size(0)
+        # (the maximum's factor, up to 2^8, is the same for all of a row's terms; bf16: dx holds one more term, rounded with w)
+        limit = (2 * eps + (terms / 32 + 16) * 2.0 ** -24 + (half if x.dtype == torch.bfloat16 else 0.0)) * total + half * exact.abs() + 2.0 ** -120
+        off = (got.double() - exact).abs()
+        assert (off <= limit).all(), (name, float((off / limit).max()))
+    with torch.no_grad():  # nobody records: the loss alone
+        alone = fastgl.linear_cross_entropy(x, w, y, b, ignore, reduction)
+    assert ((alone.double() - want).abs() <= loss_limit).all()
+    return loss.detach(), grads
+
+
+def make(cuda, n, v, d, dtype, bias=True, ignored=0.2, seed=0, label_dtype=torch.int64):
+    gen = torch.Generator(device=cuda).manual_seed(seed + n + 7 * v + 31 * d)
+    normal = lambda *size: torch.randn(size, generator=gen, device=cuda)  # noqa: E731
+    w = normal(v, d) / d ** 0.5
+    y = torch.randint(0, v, (n,), generator=gen, device=cuda)
+    x = normal(n, d) + w[y] * 8 * torch.rand((n, 1), generator=gen, device=cuda)
+    y = torch.where(torch.rand(n, generator=gen, device=cuda) < ignored, torch.full_like(y, -100), y)
+    if ignored < 1:
+        y[0] = v - 1
+    return x.to(dtype), w.to(dtype), normal(v).to(dtype) if bias else None, y.to(label_dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,v,d", [(1, 1, 1), (1, 2, 3), (2, 33, 31), (31, 32, 32), (33, 31, 33), (100, 47, 64), (128, 64, 65), (129, 129, 96), (257, 172, 100), (64, 1000, 128),
+                                   (300, 161, 160), (500, 300, 192), (96, 4097, 200), (1000, 47, 256), (40, 500, 257), (70, 333, 300), (130, 100, 384), (33, 700, 400),
+                                   (200, 65, 512), (5, 20011, 64), (4100, 5, 16), (2500, 2100, 48)])
+def test_losses_and_gradients(cuda, dtype, n, v, d):
+    print("linear_cross_entropy %d x %d, %d classes, %s" % (n, d, v, dtype), flush=True)
+    check(*make(cuda, n, v, d, dtype))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("label_dtype", [torch.int32, torch.int64])
+def test_reductions_biases_and_labels(cuda, dtype, reduction, bias, label_dtype):
+    check(*make(cuda, 150, 75, 70, dtype, bias=bias, label_dtype=label_dtype), reduction=reduction)
+    x, w, b, y = make(cuda, 60, 75, 70, dtype, bias=bias, label_dtype=label_dtype, ignored=0.0)
+    y[3:9] = 7
+    check(x, w, b, y, reduction=reduction, ignore=7)
+    g = torch.randn(60, device=cuda) if reduction == "none" else torch.tensor(-3.0, device=cuda)
+    check(x, w, b, y, reduction=reduction, ignore=-1, g=g)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_strides(cuda, dtype):
+    x, w, b, y = make(cuda, 77, 90, 45, dtype)
+    want_loss, want = check(x, w, b, y)
+    wide = torch.zeros((77, 61), dtype=dtype, device=cuda)
+    wide[:, 3:48] = x
+    for xs in (wide[:, 3:48], x.t().contiguous().t()):
+        for ws in (w.t().contiguous().t(), torch.stack([w, w], 2)[:, :, 0]):
+            loss, grads = check(xs, ws, b, y)
+            assert torch.equal(loss, want_loss) and all(torch.equal(p, q) for p, q in zip(grads, want))
+    row = x[5:6].expand(77, 45)  # (one row many times)
+    check(row, w, b, y)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_only_some_gradients(cuda, dtype):
+    x, w, b, y = make(cuda, 90, 200, 64, dtype)
+    _, (dx, dw, db) = check(x, w, b, y)
+    for needs in ((1, 0, 0), (0, 1, 0), (0, 0, 1), (1, 1, 0), (0, 1, 1), (1, 0, 1)):
+        leaves = [t.detach().requires_grad_(bool(k)) for t, k in zip((x, w, b), needs)]
+        loss = fastgl.linear_cross_entropy(leaves[0], leaves[1], y, leaves[2])
+        gen = torch.Generator(device=cuda).manual_seed(1)
+        loss.backward(torch.rand((), generator=gen, device=cuda) + 0.5)
+        for t, k, want in zip(leaves, needs, (dx, dw, db)):
+            assert t.grad is None if not k else torch.equal(t.grad, want)
+
+
+def test_two_backward_passes_and_no_third_order(cuda):
+    x, w, b, y = make(cuda, 90, 200, 64, torch.float32)
+    leaves = [t.detach().requires_grad_() for t in (x, w, b)]
+    loss = fastgl.linear_cross_entropy(leaves[0], leaves[1], y, leaves[2])
+    first = torch.autograd.grad(loss, leaves, retain_graph=True)
+    twice = torch.autograd.grad(loss, leaves, torch.tensor(2.0, device=cuda), retain_graph=True)
+    again = torch.autograd.grad(loss, leaves, create_graph=True)
+    assert all(torch.equal(2 * p, q) for p, q in zip(first, twice)) and all(torch.equal(p, q.detach()) for p, q in zip(first, again))
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(again[0].sum(), leaves)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rows_certain_of_their_label_keep_their_bits(cuda, dtype):
+    # every loss about e^-20: a difference of logits would have none of its bits
+    x, w, _, y = make(cuda, 64, 40, 32, dtype, bias=False, ignored=0.0)
+    x = (w[y].float() / w[y].float().square().sum(1, keepdim=True) * 24).to(dtype)
+    w = (w.float() * 0.2).to(dtype)
+    for r in range(64):
+        w[y[r]] = (x[r].float() / 24 ).to(dtype)
+    leaves = [t.detach().requires_grad_() for t in (x, w)]
+    losses = fastgl.linear_cross_entropy(leaves[0], leaves[1], y, reduction="none")
+    g = torch.ones(64, device=cuda)
+    dx, = torch.autograd.grad(losses, leaves[:1], g)
+    (exact, _, want, _, _), (total, _, _) = definition(x, w, None, y, -100, "none", g)
+    eps = share_error(x, w, None, 40)
+    small = exact < 1e-3
+    assert int(small.sum()) > 8
+    assert ((losses.detach().double() - exact).abs()[small] <= 3 * eps * exact[small]).all()
+    assert ((dx.double() - want).abs()[small] <= (3 * eps + 2 * HALF[dtype]) * total[small] + HALF[dtype] * want.abs()[small] + 2.0 ** -120).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("lowest", [True, False])
+def test_masked_classes(cuda, dtype, lowest):
+    x, w, b, y = make(cuda, 70, 300, 40, dtype, ignored=0.0)
+    off = torch.arange(300, device=cuda) % 3 == 1
+    off[:64] = True  # (whole tiles, the first among them)
+    y = torch.where(off[y], torch.full_like(y, 68), y)
+    assert not off[68]
+    b = torch.where(off, torch.full_like(b, torch.finfo(dtype).min if lowest else float("-inf")), b)
+    leaves = [t.detach().requires_grad_() for t in (x, w, b)]
+    loss = fastgl.linear_cross_entropy(leaves[0], leaves[1], y, leaves[2])
+    grads = torch.autograd.grad(loss, leaves)
+    kept = (~off).nonzero()[:, 0]
+    names = torch.full((300,), -1, device=cuda, dtype=torch.int64)
+    names[kept] = torch.arange(kept.numel(), device=cuda)
+    (_, want, dx, dw, db), (tx, tw, tb) = definition(x, w[kept], b[kept], names[y], -100, "mean", torch.ones((), device=cuda))
+    eps = share_error(x, w[kept], b[kept], 300)
+    assert abs(float(loss.detach()) - float(want)) <= eps * (1 + 2 * float(want) + 8)
+    for got, exact, total in ((grads[0], dx, tx), (grads[1][kept], dw, tw), (grads[2][kept], db, tb)):
+        assert ((got.double() - exact).abs() <= (2 * eps + 2 * HALF[dtype]) * total + HALF[dtype] * exact.abs() + 1e-30).all()
+    assert (grads[1][off] == 0).all() and (grads[2][off] == 0).all()
+    # a label that is left out
+    y2 = y.clone()
+    y2[0] = 0
+    loss = fastgl.linear_cross_entropy(x, w, y2, b, reduction="none")
+    assert float(loss[0]) == float("inf") and torch.isfinite(loss[1:]).all()
+    # no class that is not
+    assert fastgl.linear_cross_entropy(x, w, y, torch.full_like(b, float("-inf")), reduction="none").isnan().all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_no_labels_and_bad_ones(cuda, dtype):
+    x, w, b, y = make(cuda, 50, 30, 20, dtype, ignored=0.0)
+    none = torch.full_like(y, -100)
+    leaves = [t.detach().requires_grad_() for t in (x, w, b)]
+    loss = fastgl.linear_cross_entropy(leaves[0], leaves[1], none, leaves[2])
+    assert torch.isnan(loss)
+    assert all((g == 0).all() for g in torch.autograd.grad(loss, leaves))
+    assert float(fastgl.linear_cross_entropy(x, w, none, b, reduction="sum")) == 0
+    bad = y.clone()
+    bad[7], bad[9] = 30, -3
+    losses = fastgl.linear_cross_entropy(x, w, bad, b, reduction="none")
+    assert losses.isnan().nonzero()[:, 0].tolist() == [7, 9]
+    # a row that is not a number is the row's matter in the losses and in dx, an ignored one nobody's
+    x2 = x.clone()
+    x2[4] = float("nan")
+    leaves = [t.detach().requires_grad_() for t in (x2, w, b)]
+    losses = fastgl.linear_cross_entropy(leaves[0], leaves[1], y, leaves[2], reduction="none")
+    assert losses.isnan().nonzero()[:, 0].tolist() == [4]
+    dx, dw = torch.autograd.grad(losses.sum(), leaves[:2])
+    assert dx.isnan().any(1).nonzero()[:, 0].tolist() == [4] and dw.isnan().all()
+    # nothing at all
+    for reduction, want in (("none", []), ("sum", 0.0)):
+        leaves = [t.detach().requires_grad_() for t in (x[:0], w, b)]
+        loss = fastgl.linear_cross_entropy(leaves[0], leaves[1], y[:0], leaves[2], reduction=reduction)
+        assert loss.tolist() == want
+        dx, dw, db = torch.autograd.grad(loss.sum(), leaves)
+        assert dx.shape == (0, 20) and (dw == 0).all() and (db == 0).all()
+    assert torch.isnan(fastgl.linear_cross_entropy(x[:0], w, y[:0]))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_gradients_against_differences(cuda, dtype):
+    x, w, b, y = make(cuda, 9, 12, 7, torch.float32, ignored=0.1)
+    leaves = [t.to(dtype).detach().requires_grad_() for t in (x, w, b)]
+    loss = fastgl.linear_cross_entropy(leaves[0], leaves[1], y, leaves[2], reduction="sum")
+    grads = torch.autograd.grad(loss, leaves)
+    h = 2.0 ** -3  # (central differences of third order: off by h^4 / 30 times a fifth derivative of the order of the gradients' own scale)
+    for t, g in zip(leaves, grads):
+        flat = t.detach().reshape(-1)
+        for i in range(0, flat.numel(), 5):
+            def at(step):
+                moved = [u.detach().double() for u in leaves]
+                k = [u is t for u in leaves].index(True)
+                moved[k].reshape(-1)[i] += step
+                s = moved[0] @ moved[1].t() + moved[2]
+                keep = y != -100
+                return float(torch.nn.functional.cross_entropy(s[keep], y[keep], reduction="sum"))
+            slope = (8 * (at(h) - at(-h)) - (at(2 * h) - at(-2 * h))) / (12 * h)
+            assert abs(float(g.reshape(-1)[i]) - slope) <= 2e-2 * (1 + abs(slope))
+
+
+def test_refusals(cuda):
+    x, w, b, y = make(cuda, 10, 6, 8, torch.float32)
+    ce = fastgl.linear_cross_entropy
+    for bad in (lambda: ce(x, w[:, :7], y), lambda: ce(x[0], w, y), lambda: ce(x, w.bfloat16(), y), lambda: ce(x, w, y, b.bfloat16()), lambda: ce(x.half(), w.half(), y),
+                lambda: ce(x, w, y, b[:5]), lambda: ce(x, w, y, torch.stack([b, b], 1)[:, 0]), lambda: ce(x, w, y[:9]), lambda: ce(x, w, y.float()),
+                lambda: ce(x, w, y.short()), lambda: ce(x, w, y.cpu()), lambda: ce(x, w, torch.stack([y, y], 1)[:, 0]), lambda: ce(x, w, y, reduction="max"),
+                lambda: ce(x, w[:0], y), lambda: ce(x[:, :0], w[:, :0], y), lambda: ce(torch.zeros((3, 513), device=cuda), torch.zeros((4, 513), device=cuda), y[:3])):
+        with pytest.raises(RuntimeError):
+            bad()
+
+
+def test_autocast_takes_its_type(cuda):
+    x, w, b, y = make(cuda, 40, 20, 16, torch.float32)
+    leaves = [t.detach().requires_grad_() for t in (x, w, b)]
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        loss = fastgl.linear_cross_entropy(leaves[0], leaves[1], y, leaves[2])
+    assert torch.equal(loss, fastgl.linear_cross_entropy(x.bfloat16(), w.bfloat16(), y, b.bfloat16()))
+    assert all(g.dtype == torch.float32 for g in torch.autograd.grad(loss, leaves))
+
+
+def test_same_bits_on_every_run_and_on_another_stream(cuda):
+    x, w, b, y = make(cuda, 700, 900, 128, torch.float32)
+    run = lambda: check(x, w, b, y)  # noqa: E731
+    first = run()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        second = run()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    assert torch.equal(first[0], second[0]) and all(torch.equal(p, q) for p, q in zip(first[1], second[1]))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_captured_and_replayed(cuda, dtype):
+    x, w, b, y = make(cuda, 300, 180, 100, dtype)
+    d = torch.ones((), device=cuda)
+    held = [x.clone(), w.clone(), b.clone(), y.clone()]
+
+    def step():
+        leaves = [t.detach().requires_grad_() for t in held[:3]]
+        loss = fastgl.linear_cross_entropy(leaves[0], leaves[1], held[3], leaves[2])
+        return loss.detach(), torch.autograd.grad(loss, leaves, d)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss, grads = step()
+    for k in range(4):
+        nx, nw, nb, ny = make(cuda, 300, 180, 100, dtype, seed=50 + k)
+        for t, u in zip(held, (nx, nw, nb, ny)):
+            t.copy_(u)
+        graph.replay()
+        torch.cuda.synchronize()
+        want_loss, want = step()
+        torch.cuda.synchronize()
+        assert torch.equal(loss, want_loss) and all(torch.equal(p, q) for p, q in zip(grads, want))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_logits_far_apart(cuda, dtype):
+    # maxima that move many times, and far: classes in ascending order of their logits
+    n, v = 40, 2000
+    w = torch.zeros((v, 8), device=cuda)
+    w[:, 0] = torch.linspace(-100, 100, v, device=cuda)
+    x = torch.zeros((n, 8), device=cuda)
+    x[:, 0] = torch.linspace(-4, 4, n, device=cuda)
+    y = torch.randint(0, v, (n,), generator=torch.Generator(device=cuda).manual_seed(3), device=cuda)
+    check(x.to(dtype), w.to(dtype), None, y, reduction="none")
+
+
+def test_layer(cuda):
+    torch.manual_seed(0)
+    layer = fastgl.LinearCrossEntropy(48, 37).to(cuda)
+    x, _, _, y = make(cuda, 80, 37, 48, torch.float32)
+    want = torch.nn.functional.cross_entropy(layer.logits(x), y)
+    loss = layer(x, y)
+    assert torch.allclose(loss, want, rtol=1e-5)
+    loss.backward()
+    assert layer.weight.grad.shape == (37, 48) and layer.bias.grad.shape == (37,)
+    assert fastgl.LinearCrossEntropy(48, 37, bias=False).bias is None
