@@ -12,6 +12,7 @@
 #include <string>
 #include <vector>
 
+#include "fastgl_autograd.h"
 #include "fastgl_hip.h"
 
 namespace {
@@ -128,4 +129,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
         }));
     m.def("sample_blocks", &sample_blocks);
     m.def("trim", &trim);
+    bind_recorded_operators(m);
 }
