@@ -28,8 +28,10 @@
 // product with log2 e is not rounded where the maximum's is: logits up to some 1e9 are no matter, the difference of 2^-25 of the maximum is the
 // same for all of a row's shares and their sum.)
 //
-// Split: the passed rows are shared among `splits` workgroups so that the chip is full; each leaves its O, maximum and sum in
-// scratch, and xe_combine adds them up in order (the same bits on every run).
+// Work: four kept tiles (a group, one a wave) times the passed tiles, dealt out to as many workgroups as the chip holds (XePlan): a group is shared by
+// several, each with a part of the passed tiles, or a workgroup goes on from one group to the next in the middle of it.  Who has but a
+// part of a group's tiles leaves its O, maximum and sum in scratch, and a combining kernel adds the parts up in order (the same bits on every
+// run).
 #include "fgl_common.hpp"
 #include "fgl_kernels.hpp"
 #include "fgl_split.hpp"
@@ -42,7 +44,7 @@ typedef float XeF4 __attribute__((ext_vector_type(4)));
 
 constexpr int kXeWaves = kBlock / kWave;
 constexpr int kXeChunk = 1024;  // bytes of an operand of one matrix instruction
-constexpr int kXeMaxSplits = 64;
+constexpr int kXeMaxParts = 64;  // of a group whose rows are kept (a loss)
 constexpr int kXeMaxDim = 512;
 constexpr float kXeLog2e = 1.44269504088896340736f;
 constexpr float kXeLn2 = 0.69314718055994530942f;
@@ -54,7 +56,8 @@ enum { kXeLoss = 0, kXeLossAndRows = 1, kXeWeights = 2 };
 // A tile's first kilobyte, in floats.  Classes: their biases.  Rows: -maximum (powers of two), factor, label, the label's value.
 constexpr int kXeShift = 0, kXeFactor = 32, kXeLabel = 64, kXeOwn = 96;
 
-// Sizes of a problem as the kernels see it: blocks of 32 columns, padded, in one slice or two (O of one slice fits a wave's registers).
+// Sizes of a problem as the kernels see it: blocks of 32 columns, padded; beyond 256 columns in two slices, each with
+// half of O, which otherwise did not fit a wave's registers (S is formed for either).
 struct XeShape {
     int blocks;  // in a slice
     int slices;
@@ -69,8 +72,9 @@ inline XeShape xe_shape(int dim, int dtype)
     const int n = (int)ceil_div(dim, 32);
     XeShape s;
     s.parts = dtype == FGL_F32 ? 3 : 1;
-    s.slices = n > 8 ? 2 : 1;
-    s.blocks = n <= 4 ? n : n <= 6 || (n > 8 && n <= 12) ? 6 : 8;
+    const int blocks = n <= 4 ? n : n <= 6 ? 6 : n <= 8 ? 8 : n <= 12 ? 12 : 16;
+    s.slices = blocks > 8 ? 2 : 1;
+    s.blocks = blocks / s.slices;
     return s;
 }
 
@@ -201,16 +205,45 @@ __global__ __launch_bounds__(kBlock) void xe_images_kernel(const XeImagesArgs g)
 }
 
 // ---- the passes ----------------------------------------------------------------------------------------------------
+// How the groups' tiles are dealt out to workgroups.
+struct XePlan {
+    int groups;  // of four kept tiles (times slices)
+    int tiles;   // passed, of each
+    int per;     // tiles of a workgroup, of those that are shared
+    int shared;  // > 0: that many workgroups to a group
+    // shared = 0: each of `room` workgroups has whole groups, one in every round, of the first `whole` ones, all at the same tile at the same time (which
+    // the XCDs' L2s are for), and then `per` tiles of the others', counted through without regard for the groups' ends
+    int room, whole;
+
+    int64_t workgroups() const { return shared > 0 ? (int64_t)groups * shared : room; }
+    int64_t slots() const { return shared > 0 ? (int64_t)groups * shared : (int64_t)room + groups; }  // parts of groups at most
+    // A group's first and last workgroup among those that share it, and the place of one's part
+    __host__ __device__ int first(int group) const { return shared > 0 ? group * shared : group < whole ? 0 : (group - whole) * tiles / per; }
+    __host__ __device__ int last(int group) const { return shared > 0 ? group * shared + shared - 1 : group < whole ? 0 : ((group - whole + 1) * tiles - 1) / per; }
+    __host__ __device__ int slot(int workgroup, int group) const { return shared > 0 ? workgroup : group < whole ? group : group + workgroup; }
+};
+
+// Memory that all lanes have in common, its address in scalar registers: the compiler otherwise adds a lane's part to what the loops have in
+// common and keeps the sums in registers.
+template <typename T>
+using XeGlobal = __attribute__((address_space(1))) T;
+template <typename T>
+__device__ __forceinline__ XeGlobal<T>* xe_uniform(T* p)
+{
+    XeGlobal<T>* q = (XeGlobal<T>*)p;
+    asm("" : "+s"(q));
+    return q;
+}
+
 struct XeArgs {
+    XePlan plan;
     const char* kept;      // S images
     const char* passed;
     const char* passed_p;  // P image
-    int64_t kept_tiles, passed_tiles;
-    int64_t tiles_per_split;
-    int splits;
-    float* stats;  // [split][kept row]: maximum, others' sum, label's logit, -  (weights: sum, -, -, -)
-    float* part;   // [split][slice][kept tile][block][quarter][lane][4]
-    // weights without splits: straight to the result
+    int kept_tiles;
+    float* stats;  // [slot][wave][row of 32]: maximum, others' sum, label's logit, -  (weights: sum, -, -, -)
+    float* part;   // [slot][wave][block][quarter][lane][4]
+    // weights of groups that one workgroup has alone: straight to the result
     void* d_w;
     void* d_b;
     int64_t kept_rows;
@@ -218,17 +251,25 @@ struct XeArgs {
     int bf16;
 };
 
-// A wave's part of a copy to LDS of `chunks` kilobytes: neither a register nor an address calculation per lane beyond the first.
+// The value that the lane with the same kept row in the wave's other half has.
+__device__ __forceinline__ float xe_other_half(float v)
+{
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);  // (the lower lanes' values, the upper ones')
+    return __uint_as_float(lane_id() < 32 ? r[1] : r[0]);
+}
+
+// A wave's part of a copy of CHUNKS kilobytes to LDS, past the registers.  (Through a buffer's descriptor: after a copy from a plain address, which
+// might be LDS for all that the compiler knows, it waits for every read of LDS before it uses the first.)
 template <int CHUNKS>
 __device__ __forceinline__ void xe_stage(const char* src, char* dst)
 {
-    const int wave = (int)(threadIdx.x / kWave), lane = lane_id();
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x / kWave)), lane = lane_id();
+    const __amdgpu_buffer_rsrc_t from = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(src), 0, CHUNKS * kXeChunk, 0x00027000);
 #pragma unroll
     for (int c0 = 0; c0 < CHUNKS; c0 += kXeWaves) {
-        const int c = c0 + __builtin_amdgcn_readfirstlane(wave);
+        const int c = c0 + wave;
         if (CHUNKS % kXeWaves == 0 || c < CHUNKS)
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src + (int64_t)c * kXeChunk + lane * 16),
-                                             (__attribute__((address_space(3))) void*)(dst + c * kXeChunk), 16, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (__attribute__((address_space(3))) void*)(dst + c * kXeChunk), 16, lane * 16, c * kXeChunk, 0, 0);
     }
 }
 
@@ -240,26 +281,67 @@ __device__ __forceinline__ void xe_staged()
 
 __device__ __forceinline__ Bf16x8 xe_operand(const char* chunk) { return *reinterpret_cast<const Bf16x8*>(chunk + lane_id() * 16); }
 
+__device__ __forceinline__ Bf16x8 xe_operand(const XeGlobal<const char>* chunk) { return *reinterpret_cast<const XeGlobal<const Bf16x8>*>(chunk + lane_id() * 16); }
+
 __device__ __forceinline__ SpF32x16 xe_mfma(Bf16x8 a, Bf16x8 b, SpF32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+
+// N products of an operand from LDS each: at(i) is the i-th one's place, use(i, operand) multiplies.  Operands are read kAhead products before
+// they are used, and the compiler is kept from moving either: left to itself it reads two, waits for them and multiplies.
+template <int N, typename At, typename Use>
+__device__ __forceinline__ void xe_products(const At& at, const Use& use)
+{
+    constexpr int kAhead = N < 4 ? N : 4;
+    Bf16x8 a[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) a[i] = xe_operand(at(i));
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        use(i, a[i % kAhead]);
+        if (i + kAhead < N) a[i % kAhead] = xe_operand(at(i + kAhead));
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
+
+// The same for operands in three parts (at neighbouring places) and with six products each: the next one's parts are read while this one's are
+// multiplied.
+template <int N, typename At, typename Use>
+__device__ __forceinline__ void xe_products_in_parts(const At& at, const Use& use)
+{
+    Bf16x8 a[2][3];
+#pragma unroll
+    for (int p = 0; p < 3; ++p) a[0][p] = xe_operand(at(0) + p * kXeChunk);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+#pragma unroll
+        for (int p = 0; p < 3; ++p)
+            if (i + 1 < N) a[(i + 1) & 1][p] = xe_operand(at(i + 1) + p * kXeChunk);
+        use(i, a[i & 1]);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
 
 constexpr int kXePa[6] = {2, 0, 1, 1, 0, 0}, kXePb[6] = {0, 2, 1, 0, 1, 0};  // the small products first
 
 // Waves that a SIMD (and so workgroups that a CU) holds at once: the kept rows take 8 registers a block and part, O 16 a block, of 512.
+// WIDE: in two slices; in fp32 with the kept rows from memory.
 __host__ __device__ constexpr int xe_waves(int blocks, int parts, int use, bool wide)
 {
-    if (use == kXeLoss) return wide ? (parts == 1 ? 2 : 1) : parts == 1 ? 4 : blocks <= 2 ? 4 : blocks <= 4 ? 3 : blocks <= 6 ? 2 : 1;
-    if (wide) return parts == 1 ? 2 : 1;
-    return parts == 1 ? (blocks <= 2 ? 4 : blocks <= 3 ? 3 : 2) : blocks <= 1 ? 4 : blocks <= 4 ? 2 : 1;
+    if (wide) return parts == 1 && (use == kXeLoss || blocks <= 6) ? 2 : 1;
+    if (use == kXeLoss) return parts == 1 ? 4 : blocks <= 2 ? 4 : blocks <= 4 ? 3 : blocks <= 6 ? 2 : 1;
+    return parts == 1 ? (blocks <= 2 ? 4 : blocks <= 3 ? 3 : blocks <= 8 ? 2 : 1) : blocks <= 1 ? 4 : blocks <= 4 ? 2 : 1;
 }
 
 template <int DB, int PARTS, int USE, bool WIDE>
 struct XeWave {
     static constexpr int kSteps = WIDE ? 4 * DB : 2 * DB;
     static constexpr int kSChunks = 1 + kSteps * PARTS, kPChunks = 2 * DB * PARTS;
-    static constexpr int kKept = WIDE ? 1 : kSteps;
+    static constexpr bool kFromMemory = WIDE && PARTS == 3;
+    static constexpr int kKept = kFromMemory ? 1 : kSteps;
 
     Bf16x8 kept[kKept][PARTS];
-    const char* kept_at;  // WIDE: they are taken from memory for each tile
+    const XeGlobal<const char>* kept_at;  // kFromMemory
     SpF32x16 o[USE == kXeLoss ? 1 : DB];
     SpF32x16 start;       // weights: the class's bias sixteen times
     float top, sum, own;  // running maximum (a power of two), sum, the label's logit
@@ -268,7 +350,7 @@ struct XeWave {
 
     __device__ __forceinline__ Bf16x8 kept_part(int step, int p) const
     {
-        if constexpr (WIDE) return xe_operand(kept_at + (int64_t)(step * PARTS + p) * kXeChunk);
+        if constexpr (kFromMemory) return xe_operand(kept_at + (int64_t)(step * PARTS + p) * kXeChunk);
         else return kept[step][p];
     }
 
@@ -286,40 +368,31 @@ struct XeWave {
                 for (int c = 0; c < 4; ++c) acc[4 * q + c] = b[c];
             }
         }
-        const char* at = s + kXeChunk;
+        const auto at = [&](int k) { return s + (1 + k * PARTS) * kXeChunk; };
         if constexpr (PARTS == 1) {
-#pragma unroll
-            for (int k = 0; k < kSteps; ++k) acc = xe_mfma(xe_operand(at + k * kXeChunk), kept_part(k, 0), acc);
+            xe_products<kSteps>(at, [&](int k, Bf16x8 a) { acc = xe_mfma(a, kept_part(k, 0), acc); });
         } else {
+            SpF32x16 chunk = {};
+            xe_products_in_parts<kSteps>(at, [&](int k, const Bf16x8 (&a)[3]) {
 #pragma unroll
-            for (int k = 0; k < kSteps; k += 2) {
-                SpF32x16 chunk = {};
-                Bf16x8 a[2][3], b[2][3];
+                for (int q = 0; q < 6; ++q) chunk = xe_mfma(a[kXePa[q]], kept_part(k, kXePb[q]), chunk);
+                if (k % 2 == 1) {
 #pragma unroll
-                for (int u = 0; u < 2; ++u)
-#pragma unroll
-                    for (int p = 0; p < 3; ++p) {
-                        a[u][p] = xe_operand(at + ((k + u) * 3 + p) * kXeChunk);
-                        b[u][p] = kept_part(k + u, p);
-                    }
-#pragma unroll
-                for (int q = 0; q < 6; ++q)
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) chunk = xe_mfma(a[u][kXePa[q]], b[u][kXePb[q]], chunk);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) acc[i] += chunk[i];
-            }
+                    for (int i = 0; i < 16; ++i) acc[i] += chunk[i];
+                    chunk = SpF32x16{};
+                }
+            });
         }
         return acc;
     }
 
     // S^T -> P^T, with the running maximum, sum and the label's logit.  v0: the tile's first class.
-    __device__ __forceinline__ void shares(SpF32x16& s, int64_t v0)
+    __device__ __forceinline__ void shares(SpF32x16& s, int v0)
     {
         float most = s[0];
 #pragma unroll
         for (int i = 1; i < 16; ++i) most = fmaxf(most, s[i]);
-        most = fmaxf(most, __shfl_xor(most, 32, kWave)) * kXeLog2e;
+        most = fmaxf(most, xe_other_half(most)) * kXeLog2e;
         if (__any(most > top + kXeStep)) {
             const float now = fmaxf(top, most);
             const float scale = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top - now);
@@ -333,12 +406,13 @@ struct XeWave {
             }
         }
         const float shift = top == -INFINITY ? 0.0f : -top;
-        const int64_t in_tile = label - v0;
+        const int in_tile = label - v0;
         const bool here = label >= 0 && in_tile >= 0 && in_tile < 32;
         if (__any(here)) {
+            const int at = here ? in_tile - 4 * (lane_id() / 32) : -1;  // (of the lane's values, if it has it)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                if (here && (int)in_tile == 8 * (i / 4) + 4 * (lane_id() / 32) + i % 4) {
+                if (at == 8 * (i / 4) + i % 4) {
                     own = s[i];
                     s[i] = -INFINITY;
                 }
@@ -358,7 +432,7 @@ struct XeWave {
     }
 
     // S^T -> the gradient of the logits, from the maxima, factors and labels of the tile's rows
-    __device__ __forceinline__ void gradients(SpF32x16& s, const char* tile, int64_t v0)
+    __device__ __forceinline__ void gradients(SpF32x16& s, const char* tile, int v0)
     {
         const float* c = reinterpret_cast<const float*>(tile);
         const int* l = reinterpret_cast<const int*>(tile);
@@ -369,7 +443,7 @@ struct XeWave {
 #pragma unroll
             for (int j = 0; j < 4; ++j) s[4 * q + j] = __builtin_amdgcn_exp2f(fmaf(s[4 * q + j], kXeLog2e, shift[j])) * factor[j];
         }
-        const int64_t in_tile = l[kXeLabel + lane_id() % 32] - v0;
+        const int in_tile = l[kXeLabel + lane_id() % 32] - v0;
         if (__any(in_tile >= 0 && in_tile < 32)) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
@@ -387,10 +461,7 @@ struct XeWave {
             Bf16x8 w[2];
 #pragma unroll
             for (int i = 0; i < 16; ++i) w[i / 8][i % 8] = (__bf16)s[i];
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int d = 0; d < DB; ++d) o[d] = xe_mfma(xe_operand(p + (h * DB + d) * kXeChunk), w[h], o[d]);
+            xe_products<2 * DB>([&](int i) { return p + i * kXeChunk; }, [&](int i, Bf16x8 a) { o[i % DB] = xe_mfma(a, w[i / DB], o[i % DB]); });
         } else {
             SpU4 w[2][3];
             uint32_t rest = 0;
@@ -401,26 +472,21 @@ struct XeWave {
                 for (int j = 0; j < 8; ++j) v[j] = s[8 * h + j];
                 sp_split(v, w[h], rest);
             }
+            SpF32x16 chunk = {};
+            xe_products_in_parts<2 * DB>([&](int i) { return p + (i % 2 * DB + i / 2) * 3 * kXeChunk; }, [&](int i, const Bf16x8 (&a)[3]) {
 #pragma unroll
-            for (int d = 0; d < DB; ++d) {
-                SpF32x16 chunk = {};
-                Bf16x8 a[2][3];
+                for (int q = 0; q < 6; ++q) chunk = xe_mfma(a[kXePa[q]], __builtin_bit_cast(Bf16x8, w[i % 2][kXePb[q]]), chunk);
+                if (i % 2 == 1) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int q = 0; q < 3; ++q) a[h][q] = xe_operand(p + ((h * DB + d) * 3 + q) * kXeChunk);
-#pragma unroll
-                for (int q = 0; q < 6; ++q)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) chunk = xe_mfma(a[h][kXePa[q]], __builtin_bit_cast(Bf16x8, w[h][kXePb[q]]), chunk);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) o[d][i] += chunk[i];
-            }
+                    for (int c = 0; c < 16; ++c) o[i / 2][c] += chunk[c];
+                    chunk = SpF32x16{};
+                }
+            });
         }
     }
 
     // One tile: copies what comes next to `next` while it works on `s`
-    __device__ __forceinline__ void first_half(const char* __restrict__ s, char* __restrict__ next, const char* src, SpF32x16& p, int64_t n0, int64_t v0, bool active)
+    __device__ __forceinline__ void first_half(const char* __restrict__ s, char* __restrict__ next, const char* src, SpF32x16& p, int n0, int v0, bool active)
     {
         if constexpr (USE == kXeLoss) {
             if (src != nullptr) xe_stage<kSChunks>(src, next);
@@ -439,6 +505,50 @@ struct XeWave {
     }
 };
 
+// Four neighbouring columns of a result's row.
+__device__ __forceinline__ void xe_store4(void* out, bool bf16, int64_t row, int col, int dim, const XeF4& v)
+{
+    const int64_t to = row * dim + col;
+    if (bf16) {
+        typedef __bf16 Vec __attribute__((ext_vector_type(4), aligned(2)));
+        __bf16* p = static_cast<__bf16*>(out) + to;
+        if (col + 4 <= dim) {
+            *reinterpret_cast<Vec*>(p) = Vec{(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
+        } else {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                if (col + c < dim) p[c] = (__bf16)v[c];
+        }
+    } else {
+        typedef float Vec __attribute__((ext_vector_type(4), aligned(4)));
+        float* p = static_cast<float*>(out) + to;
+        if (col + 4 <= dim) {
+            *reinterpret_cast<Vec*>(p) = Vec{v[0], v[1], v[2], v[3]};
+        } else {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                if (col + c < dim) p[c] = v[c];
+        }
+    }
+}
+
+template <int DB, int N>
+__device__ __forceinline__ void xe_store_weights(const XeArgs& g, const SpF32x16 (&o)[N], int64_t row, int slice, float sum)
+{
+    if (row >= g.kept_rows) return;
+    int half = lane_id() / 32;
+    asm volatile("" : "+v"(half));  // (else what the columns make of it is kept in registers through all tiles)
+    if (g.d_b != nullptr && half == 0 && slice == 0) {
+        if (g.bf16) static_cast<__bf16*>(g.d_b)[row] = (__bf16)sum;
+        else static_cast<float*>(g.d_b)[row] = sum;
+    }
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            xe_store4(g.d_w, g.bf16 != 0, row, 32 * (slice * DB + d) + 8 * q + 4 * half, g.dim, XeF4{o[d][4 * q], o[d][4 * q + 1], o[d][4 * q + 2], o[d][4 * q + 3]});
+}
+
 template <int DB, int PARTS, int USE, bool WIDE>
 __global__ __launch_bounds__(kBlock, xe_waves(DB, PARTS, USE, WIDE)) void xe_kernel(const XeArgs g)
 {
@@ -449,17 +559,40 @@ __global__ __launch_bounds__(kBlock, xe_waves(DB, PARTS, USE, WIDE)) void xe_ker
     __shared__ __attribute__((aligned(16))) char p_buf[(USE != kXeLoss ? Wave::kPChunks : kTwo ? Wave::kSChunks : 1) * kXeChunk];
     constexpr int kSlices = WIDE && USE != kXeLoss ? 2 : 1;
     constexpr int64_t kSBytes = (int64_t)Wave::kSChunks * kXeChunk, kPBytes = (int64_t)Wave::kPChunks * (WIDE ? 2 : 1) * kXeChunk;
-    const int split = (int)(blockIdx.x % (unsigned)g.splits);
-    const int rest = (int)(blockIdx.x / (unsigned)g.splits), slice = rest % kSlices;
-    const int lane = lane_id();
-    const int64_t tile = (int64_t)(rest / kSlices) * kXeWaves + __builtin_amdgcn_readfirstlane((int)(threadIdx.x / kWave));
+    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x / kWave));
+    const XePlan plan = g.plan;
+    const int workgroup = (int)blockIdx.x;
+    // this workgroup's groups: whole ones first, then parts
+    int next = workgroup, whole = plan.shared > 0 ? 0 : plan.whole, t0 = 0, left = 0;
+    for (bool parts = false;;) {
+    int group;
+    if (next < whole) {
+        group = next;
+        next += plan.room;
+        left = plan.tiles;
+    } else if (!parts) {
+        parts = true;
+        const int later = plan.shared > 0 ? 0 : workgroup * plan.per / plan.tiles;
+        group = plan.shared > 0 ? workgroup / plan.shared : whole + later;
+        t0 = plan.shared > 0 ? workgroup % plan.shared * plan.per : workgroup * plan.per - later * plan.tiles;
+        left = plan.shared > 0 && plan.per > plan.tiles - t0 ? plan.tiles - t0 : plan.per;
+        next = group + 1;
+        whole = 0;
+        if (group >= plan.groups) break;
+    } else {
+        if (left <= 0 || next >= plan.groups) break;
+        group = next++;
+        t0 = 0;
+    }
+    const int t1 = left < plan.tiles - t0 ? t0 + left : plan.tiles;
+    left -= t1 - t0;
+    const int slice = group % kSlices, tile = group / kSlices * kXeWaves + wave;
     const bool active = tile < g.kept_tiles;
-    const int64_t mine = active ? tile : g.kept_tiles - 1;
-    const char* own = g.kept + mine * kSBytes;
+    const XeGlobal<const char>* own = xe_uniform(g.kept + (active ? tile : g.kept_tiles - 1) * kSBytes);
 
     Wave w;
     w.kept_at = own + kXeChunk;
-    if constexpr (!WIDE) {
+    if constexpr (!Wave::kFromMemory) {
 #pragma unroll
         for (int k = 0; k < Wave::kSteps; ++k)
 #pragma unroll
@@ -471,28 +604,27 @@ __global__ __launch_bounds__(kBlock, xe_waves(DB, PARTS, USE, WIDE)) void xe_ker
     w.sum = w.own = 0.0f;
     w.bias_sum = g.d_b != nullptr;
     if constexpr (USE == kXeWeights) {
-        w.label = (int)(32 * tile) + lane % 32;
-        const float b = reinterpret_cast<const float*>(own)[lane % 32];
+        w.label = 32 * tile + lane % 32;
+        const float b = reinterpret_cast<const XeGlobal<const float>*>(own)[lane % 32];
 #pragma unroll
         for (int i = 0; i < 16; ++i) w.start[i] = b;
     } else {
-        w.label = reinterpret_cast<const int*>(own)[kXeLabel + lane % 32];
+        w.label = reinterpret_cast<const XeGlobal<const int>*>(own)[kXeLabel + lane % 32];
     }
 
-    const int64_t t0 = split * g.tiles_per_split, t1 = t0 + g.tiles_per_split < g.passed_tiles ? t0 + g.tiles_per_split : g.passed_tiles;
-    const int64_t v0 = 32 * tile;
+    const int v0 = 32 * tile;
     SpF32x16 p = {};
     xe_stage<Wave::kSChunks>(g.passed + t0 * kSBytes, s_buf);
     xe_staged();
     if constexpr (USE == kXeLoss && !kTwo) {
-        for (int64_t t = t0; t < t1; ++t) {
+        for (int t = t0; t < t1; ++t) {
             w.first_half(s_buf, p_buf, nullptr, p, 32 * t, v0, active);
             __syncthreads();
             if (t + 1 < t1) xe_stage<Wave::kSChunks>(g.passed + (t + 1) * kSBytes, s_buf);
             xe_staged();
         }
     } else if constexpr (USE == kXeLoss) {
-        for (int64_t t = t0; t < t1; t += 2) {
+        for (int t = t0; t < t1; t += 2) {
             w.first_half(s_buf, p_buf, t + 1 < t1 ? g.passed + (t + 1) * kSBytes : nullptr, p, 32 * t, v0, active);
             xe_staged();
             if (t + 1 == t1) break;
@@ -501,82 +633,52 @@ __global__ __launch_bounds__(kBlock, xe_waves(DB, PARTS, USE, WIDE)) void xe_ker
         }
     } else {
         const char* passed_p = g.passed_p + slice * (int64_t)Wave::kPChunks * kXeChunk;
-        for (int64_t t = t0; t < t1; ++t) {
+        for (int t = t0; t < t1; ++t) {
             w.first_half(s_buf, p_buf, passed_p + t * kPBytes, p, 32 * t, v0, active);
             xe_staged();
             w.second_half(p_buf, s_buf, t + 1 < t1 ? g.passed + (t + 1) * kSBytes : nullptr, p, active);
             xe_staged();
         }
     }
-    if (!active) return;
+    if (!active) continue;
 
-    w.sum += __shfl_xor(w.sum, 32, kWave);
-    w.own += __shfl_xor(w.own, 32, kWave);
-    const int half = lane / 32;
-    if constexpr (USE == kXeWeights) {
-        if (g.splits == 1) {
-            const int64_t row = v0 + lane % 32;
-            if (row >= g.kept_rows) return;
-            if (g.d_b != nullptr && half == 0 && slice == 0) {
-                if (g.bf16) static_cast<__bf16*>(g.d_b)[row] = (__bf16)w.sum;
-                else static_cast<float*>(g.d_b)[row] = w.sum;
-            }
-#pragma unroll
-            for (int d = 0; d < DB; ++d)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int col = 32 * (slice * DB + d) + 8 * q + 4 * half;
-                    const int64_t to = row * g.dim + col;
-                    float v[4];
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) v[c] = w.o[d][4 * q + c];
-                    if (g.bf16) {
-                        typedef __bf16 Vec __attribute__((ext_vector_type(4), aligned(2)));
-                        __bf16* out = static_cast<__bf16*>(g.d_w) + to;
-                        if (col + 4 <= g.dim) *reinterpret_cast<Vec*>(out) = Vec{(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
-                        else
-#pragma unroll
-                            for (int c = 0; c < 4; ++c)
-                                if (col + c < g.dim) out[c] = (__bf16)v[c];
-                    } else {
-                        typedef float Vec __attribute__((ext_vector_type(4), aligned(4)));
-                        float* out = static_cast<float*>(g.d_w) + to;
-                        if (col + 4 <= g.dim) *reinterpret_cast<Vec*>(out) = Vec{v[0], v[1], v[2], v[3]};
-                        else
-#pragma unroll
-                            for (int c = 0; c < 4; ++c)
-                                if (col + c < g.dim) out[c] = v[c];
-                    }
-                }
-            return;
-        }
+    w.sum += xe_other_half(w.sum);
+    w.own += xe_other_half(w.own);
+    if (USE == kXeWeights && t1 - t0 == plan.tiles) {
+        xe_store_weights<USE == kXeWeights ? DB : 1>(g, w.o, v0 + lane % 32, slice, w.sum);
+        continue;
     }
-    if (half == 0 && slice == 0) {
+    const int64_t place = (int64_t)plan.slot(workgroup, group) * kXeWaves + wave;
+    if (lane < 32) {  // (of either slice: they are cut in other places)
         const XeF4 v = USE == kXeWeights ? XeF4{w.sum, 0.0f, 0.0f, 0.0f} : XeF4{w.top, w.sum, w.own, 0.0f};
-        *reinterpret_cast<XeF4*>(g.stats + 4 * (split * 32 * g.kept_tiles + v0 + lane)) = v;
+        *reinterpret_cast<XeGlobal<XeF4>*>(xe_uniform(g.stats + 4 * place * 32) + 4 * lane) = v;
     }
     if constexpr (USE != kXeLoss) {
-        float* to = g.part + (((int64_t)split * kSlices + slice) * g.kept_tiles + tile) * (DB * 4 * kWave * 4) + lane * 4;
+        int at_lane = lane * 4;
+        asm volatile("" : "+v"(at_lane));  // (as in xe_store_weights)
+        XeGlobal<float>* to = xe_uniform(g.part + place * (DB * 4 * kWave * 4)) + at_lane;
 #pragma unroll
         for (int d = 0; d < DB; ++d)
 #pragma unroll
             for (int q = 0; q < 4; ++q)
-                *reinterpret_cast<XeF4*>(to + (d * 4 + q) * kWave * 4) = XeF4{w.o[d][4 * q], w.o[d][4 * q + 1], w.o[d][4 * q + 2], w.o[d][4 * q + 3]};
+                *reinterpret_cast<XeGlobal<XeF4>*>(to + (d * 4 + q) * kWave * 4) = XeF4{w.o[d][4 * q], w.o[d][4 * q + 1], w.o[d][4 * q + 2], w.o[d][4 * q + 3]};
+    }
     }
 }
 
-// ---- what the splits left, added up --------------------------------------------------------------------------------
+// ---- what the parts of groups left, added up -----------------------------------------------------------------------
 struct XeRow {  // of a row, for the backward pass
     float top, inverse, others;  // maximum (a power of two), 1 / sum, the other classes' share
     int label;
 };
 
 struct XeCombineArgs {
+    XePlan plan;
     const float* stats;
     const float* part;
     const char* rows;  // S image of the rows (labels)
-    int64_t tiles, n_rows, s_bytes;
-    int splits, blocks, slices;
+    int64_t n_rows, s_bytes;
+    int blocks, slices;
     const void* w;  // classes
     int64_t w_row, w_col;
     int dim, bf16;
@@ -586,51 +688,63 @@ struct XeCombineArgs {
     float* d_x;        // [row][padded columns], up to its factor, or null
 };
 
-// (one workgroup a tile of 32 rows)
+// One workgroup a tile of 32 rows and block of 32 columns.  Each forms the rows' sums from their parts (a row eight threads), the first of
+// a tile's keeps them; then a wave takes eight columns.
 __global__ __launch_bounds__(kBlock) void xe_combine_kernel(const XeCombineArgs g)
 {
-    __shared__ float scale[kXeMaxSplits * 32];
+    constexpr int kEach = kBlock / 32;
+    __shared__ float scale[kXeMaxParts * 32];
+    __shared__ float top_of[kEach][32], own_of[kEach][32], rest_of[kEach][32];
     __shared__ float others[32];
     __shared__ int labels[32];
-    const int64_t tile = blockIdx.x, row0 = 32 * tile;
-    const int thread = (int)threadIdx.x;
-    if (thread < kWave) {
-        const int i = thread % 32;
-        const bool there = row0 + i < g.n_rows;
-        const int label = reinterpret_cast<const int*>(g.rows + tile * g.s_bytes)[kXeLabel + i];
-        const XeF4* s = reinterpret_cast<const XeF4*>(g.stats) + row0 + i;
-        const int64_t step = 32 * g.tiles;
-        float top = -INFINITY, own = 0.0f;
-        for (int k = 0; k < g.splits; ++k) {
-            const XeF4 v = s[k * step];
-            top = fmaxf(top, v[0]);
-            own += v[2];
-        }
-        const float own2 = own * kXeLog2e;
-        if (label >= 0) top = fmaxf(top, own2);
-        float rest = 0.0f;
-        for (int k = 0; k < g.splits; ++k) {
-            const XeF4 v = s[k * step];
-            const float f = v[0] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(v[0] - top);
-            rest += v[0] == -INFINITY ? v[1] : v[1] * f;  // (what is not a number stays it)
-            if (thread < 32) scale[k * 32 + i] = f;
-        }
-        const float mine = label >= 0 ? __builtin_amdgcn_exp2f(own2 - top) : 0.0f;
-        const float total = rest + mine, inverse = 1.0f / total;
+    const int tile = (int)blockIdx.x, block = (int)blockIdx.y, group = tile / kXeWaves * g.slices + block / g.blocks;
+    const int64_t row0 = 32LL * tile;
+    const int thread = (int)threadIdx.x, wave = tile % kXeWaves, i = thread % 32, each = thread / 32;
+    const int b0 = g.plan.first(group), parts = g.plan.last(group) - b0 + 1;
+    const XeF4* s = reinterpret_cast<const XeF4*>(g.stats) + ((int64_t)g.plan.slot(b0, group) * kXeWaves + wave) * 32 + i;
+    const bool there = row0 + i < g.n_rows;
+    const int label = reinterpret_cast<const int*>(g.rows + tile * g.s_bytes)[kXeLabel + i];
+    float top = -INFINITY, own = 0.0f;
+    for (int k = each; k < parts; k += kEach) {
+        const XeF4 v = s[k * kXeWaves * 32];
+        top = fmaxf(top, v[0]);
+        own += v[2];
+    }
+    top_of[each][i] = top;
+    own_of[each][i] = own;
+    __syncthreads();
+    own = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+        top = fmaxf(top, top_of[k][i]);
+        own += own_of[k][i];
+    }
+    const float own2 = own * kXeLog2e;
+    if (label >= 0) top = fmaxf(top, own2);
+    float rest = 0.0f;
+    for (int k = each; k < parts; k += kEach) {
+        const XeF4 v = s[k * kXeWaves * 32];
+        const float f = v[0] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(v[0] - top);
+        rest += v[0] == -INFINITY ? v[1] : v[1] * f;  // (what is not a number stays it)
+        scale[k * 32 + i] = f;
+    }
+    rest_of[each][i] = rest;
+    __syncthreads();
+    rest = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) rest += rest_of[k][i];
+    const float mine = label >= 0 ? __builtin_amdgcn_exp2f(own2 - top) : 0.0f;
+    const float total = rest + mine, inverse = 1.0f / total;
+    float share = rest * inverse;
+    if (blockIdx.y == 0 && thread < kWave) {
         float loss = top - own2 < 64.0f ? log1pf(rest / mine) : kXeLn2 * top + logf(total) - own;
-        float share = rest * inverse;
-        if (label == -2) loss = share = NAN;
-        if (label == -1) loss = share = 0.0f;
-        if (thread < 32) {
-            if (there) {
-                if (g.losses != nullptr) g.losses[row0 + i] = loss;
-                if (g.kept != nullptr) g.kept[row0 + i] = XeRow{top, inverse, share, label};
-            }
-            others[i] = share;
-            labels[i] = there ? label : -1;
-            for (int k = 0; k < g.splits; ++k) scale[k * 32 + i] *= inverse;
+        if (label == -2) loss = NAN;
+        if (label == -1) loss = 0.0f;
+        if (thread < 32 && there) {
+            if (g.losses != nullptr) g.losses[row0 + i] = loss;
+            if (g.kept != nullptr) g.kept[row0 + i] = XeRow{top, inverse, label == -2 ? NAN : share, label};
         }
-        float sum = there && thread < 32 ? loss : 0.0f, count = there && thread < 32 && label != -1 ? 1.0f : 0.0f;
+        float sum = there ? loss : 0.0f, count = there && label != -1 ? 1.0f : 0.0f;
 #pragma unroll
         for (int d = 16; d >= 1; d >>= 1) {
             sum += __shfl_xor(sum, d, kWave);
@@ -642,33 +756,36 @@ __global__ __launch_bounds__(kBlock) void xe_combine_kernel(const XeCombineArgs 
         }
     }
     if (g.d_x == nullptr) return;
-    __syncthreads();
-    const int cols = 32 * g.blocks * g.slices, per_slice = g.blocks * 4 * kWave;
-    const int64_t slice_step = g.tiles * per_slice;
-    for (int at = thread; at < per_slice * g.slices; at += kBlock) {
-        const int slice = at / per_slice, in_slice = at % per_slice, lane = in_slice % kWave, i = lane % 32;
-        const int col = 32 * (slice * g.blocks) + in_slice / kWave * 8 + lane / 32 * 4;
-        if (row0 + i >= g.n_rows) continue;
-        const XeF4* p = reinterpret_cast<const XeF4*>(g.part) + (slice * g.tiles + tile) * per_slice + in_slice;
-        XeF4 sum = {};
-        for (int k = 0; k < g.splits; ++k) {
-            const XeF4 v = p[k * g.slices * slice_step];
-            const float f = scale[k * 32 + i];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) sum[c] += v[c] * f;
-        }
-        const int label = labels[i];
-        if (label >= 0) {
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                if (col + c >= g.dim) continue;
-                const int64_t from = label * g.w_row + (col + c) * g.w_col;
-                const float v = g.bf16 ? (float)static_cast<const __bf16*>(g.w)[from] : static_cast<const float*>(g.w)[from];
-                sum[c] -= others[i] * v;
-            }
-        }
-        *reinterpret_cast<XeF4*>(g.d_x + (row0 + i) * cols + col) = sum;
+    for (int k = each; k < parts; k += kEach) scale[k * 32 + i] *= inverse;
+    if (thread < 32) {
+        others[i] = label == -2 ? NAN : share;
+        labels[i] = there ? label : -1;
     }
+    __syncthreads();
+    const int cols = 32 * g.blocks * g.slices, lane = thread % kWave;
+    const int col = 32 * block + thread / kWave * 8 + lane / 32 * 4;
+    if (!there) return;
+    const int64_t step = (int64_t)kXeWaves * g.blocks * 4 * kWave;  // of a slot, in fours
+    const XeF4* p = reinterpret_cast<const XeF4*>(g.part) + (int64_t)g.plan.slot(b0, group) * step +
+                    ((int64_t)wave * g.blocks + block % g.blocks) * 4 * kWave + thread;
+    XeF4 sum = {};
+#pragma unroll 4
+    for (int k = 0; k < parts; ++k) {
+        const XeF4 v = p[k * step];
+        const float f = scale[k * 32 + i];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) sum[c] += v[c] * f;
+    }
+    if (labels[i] >= 0) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            if (col + c >= g.dim) continue;
+            const int64_t from = labels[i] * g.w_row + (col + c) * g.w_col;
+            const float v = g.bf16 ? (float)static_cast<const __bf16*>(g.w)[from] : static_cast<const float*>(g.w)[from];
+            sum[c] -= others[i] * v;
+        }
+    }
+    *reinterpret_cast<XeF4*>(g.d_x + (row0 + i) * cols + col) = sum;
 }
 
 // the tiles' losses -> *loss; *count: rows with a label
@@ -703,12 +820,12 @@ struct XeRowsArgs {
     const float* count;
     int reduction;
     char* rows;  // S image of the rows, or null: the factors of the weights' gradient
-    int64_t tiles, n_rows, s_bytes;
+    int64_t n_rows, s_bytes;
     int cols, dim, bf16;
     void* out;
 };
 
-// The factors of a tile's 32 rows, and dx from them.
+// The factors of a tile's 32 rows, and dx from them, 32 columns a workgroup.
 __global__ __launch_bounds__(kBlock) void xe_rows_kernel(const XeRowsArgs g)
 {
     __shared__ float factor[32];
@@ -723,7 +840,7 @@ __global__ __launch_bounds__(kBlock) void xe_rows_kernel(const XeRowsArgs g)
         const bool with = r.label != -1;
         factor[thread] = r.label == -2 ? NAN : f;
         labels[thread] = r.label;
-        if (g.rows != nullptr) {
+        if (g.rows != nullptr && blockIdx.y == 0) {
             float* c = reinterpret_cast<float*>(g.rows + tile * g.s_bytes);
             c[kXeShift + thread] = with ? (r.label == -2 ? NAN : -r.top) : -INFINITY;
             c[kXeFactor + thread] = with ? f * r.inverse : 0.0f;
@@ -732,86 +849,102 @@ __global__ __launch_bounds__(kBlock) void xe_rows_kernel(const XeRowsArgs g)
     }
     if (g.out == nullptr) return;
     __syncthreads();
-    const int quads = (g.dim + 3) / 4;
-    for (int at = thread; at < 32 * quads; at += kBlock) {
-        const int i = at / quads, col = at % quads * 4;
-        if (row0 + i >= g.n_rows) break;
-        XeF4 v = *reinterpret_cast<const XeF4*>(g.d_x + (row0 + i) * g.cols + col);
-        const bool with = labels[i] != -1;
-        const int64_t to = (row0 + i) * g.dim + col;
+    const int i = thread / 8, col = 32 * (int)blockIdx.y + thread % 8 * 4;
+    if (row0 + i >= g.n_rows || col >= g.dim) return;
+    XeF4 v = *reinterpret_cast<const XeF4*>(g.d_x + (row0 + i) * g.cols + col);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            if (col + c >= g.dim) continue;
-            const float d = with ? v[c] * factor[i] : 0.0f;
-            if (g.bf16) static_cast<__bf16*>(g.out)[to + c] = (__bf16)d;
-            else static_cast<float*>(g.out)[to + c] = d;
-        }
-    }
+    for (int c = 0; c < 4; ++c) v[c] = labels[i] != -1 ? v[c] * factor[i] : 0.0f;
+    xe_store4(g.out, g.bf16 != 0, row0 + i, col, g.dim, v);
 }
 
 struct XeWeightsArgs {
+    XePlan plan;
     const float* stats;
     const float* part;
-    int64_t tiles, n_rows;
-    int splits, blocks, slices, dim, bf16;
+    int64_t n_rows;
+    int blocks, slices, dim, bf16;
     void* d_w;
     void* d_b;  // or null
 };
 
+// A wave 32 classes and eight columns.  Where there are many parts (TOGETHER) a workgroup's four share them.
+template <bool TOGETHER>
 __global__ __launch_bounds__(kBlock) void xe_weights_kernel(const XeWeightsArgs g)
 {
-    const int64_t tile = blockIdx.x, row0 = 32 * tile;
-    const int thread = (int)threadIdx.x;
-    if (g.d_b != nullptr && thread < 32 && row0 + thread < g.n_rows && blockIdx.y == 0) {
-        float sum = 0.0f;
-        for (int k = 0; k < g.splits; ++k) sum += g.stats[4 * (k * 32 * g.tiles + row0 + thread)];
-        if (g.bf16) static_cast<__bf16*>(g.d_b)[row0 + thread] = (__bf16)sum;
-        else static_cast<float*>(g.d_b)[row0 + thread] = sum;
+    __shared__ XeF4 sums[TOGETHER ? kXeWaves : 1][kWave];
+    __shared__ float biases[TOGETHER ? kXeWaves : 1][32];
+    const int tile = (int)blockIdx.x;
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x / kWave)), lane = lane_id();
+    const int chunk = TOGETHER ? (int)blockIdx.y : (int)blockIdx.y * kXeWaves + wave, slice = chunk / (4 * g.blocks);
+    const int group = tile / kXeWaves * g.slices + slice, b0 = g.plan.first(group), parts = g.plan.last(group) - b0 + 1;
+    if (parts == 1) return;  // (stored as it was formed)
+    const int64_t place = (int64_t)g.plan.slot(b0, group) * kXeWaves + tile % kXeWaves;
+    const int each = TOGETHER ? (parts + kXeWaves - 1) / kXeWaves : parts, k0 = TOGETHER ? wave * each : 0, k1 = k0 + each < parts ? k0 + each : parts;
+    const int64_t step = (int64_t)kXeWaves * g.blocks * 4 * kWave;
+    const XeF4* p = reinterpret_cast<const XeF4*>(g.part) + place * (g.blocks * 4 * kWave) + chunk % (4 * g.blocks) * kWave + lane;
+    const bool with_bias = g.d_b != nullptr && chunk == 0;
+    XeF4 sum = {};
+    float bias = 0.0f;
+#pragma unroll 4
+    for (int k = k0; k < k1; ++k) {
+        const XeF4 v = p[k * step];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) sum[c] += v[c];
     }
-    const int per_slice = g.blocks * 4 * kWave;
-    const int64_t slice_step = g.tiles * per_slice;
-    for (int at = (int)blockIdx.y * kBlock + thread; at < per_slice * g.slices; at += kBlock * (int)gridDim.y) {
-        const int slice = at / per_slice, in_slice = at % per_slice, lane = in_slice % kWave, i = lane % 32;
-        const int col = 32 * (slice * g.blocks) + in_slice / kWave * 8 + lane / 32 * 4;
-        if (row0 + i >= g.n_rows || col >= g.dim) continue;
-        const XeF4* p = reinterpret_cast<const XeF4*>(g.part) + (slice * g.tiles + tile) * per_slice + in_slice;
-        XeF4 sum = {};
-        for (int k = 0; k < g.splits; ++k) {
-            const XeF4 v = p[k * g.slices * slice_step];
+    if (with_bias)
+        for (int k = k0; k < k1; ++k) bias += g.stats[4 * ((place + (int64_t)k * kXeWaves) * 32 + lane % 32)];
+    if constexpr (TOGETHER) {
+        sums[wave][lane] = sum;
+        if (lane < 32) biases[wave][lane] = bias;
+        __syncthreads();
+        if (wave != 0) return;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) sum[c] += v[c];
-        }
-        const int64_t to = (row0 + i) * g.dim + col;
+        for (int k = 1; k < kXeWaves; ++k) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            if (col + c >= g.dim) continue;
-            if (g.bf16) static_cast<__bf16*>(g.d_w)[to + c] = (__bf16)sum[c];
-            else static_cast<float*>(g.d_w)[to + c] = sum[c];
+            for (int c = 0; c < 4; ++c) sum[c] += sums[k][lane][c];
+            bias += biases[k][lane % 32];
         }
+    }
+    const int64_t row = 32LL * tile + lane % 32;
+    if (row >= g.n_rows) return;
+    xe_store4(g.d_w, g.bf16 != 0, row, 8 * chunk + lane / 32 * 4, g.dim, sum);
+    if (with_bias && lane < 32) {
+        if (g.bf16) static_cast<__bf16*>(g.d_b)[row] = (__bf16)bias;
+        else static_cast<float*>(g.d_b)[row] = bias;
     }
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------------
-struct XeSplit {
-    int splits;
-    int64_t tiles;  // of each
-};
-
-inline XeSplit xe_split(const XeShape& s, int use, int64_t kept_tiles, int64_t passed_tiles)
+inline XePlan xe_plan(const XeShape& s, int use, int kept_tiles, int passed_tiles)
 {
-    const int64_t groups = ceil_div(kept_tiles, kXeWaves) * (use == kXeLoss ? 1 : s.slices);
-    int64_t n = 256LL * xe_waves(s.blocks, s.parts, use, s.slices == 2) / groups;
-    if (n > kXeMaxSplits) n = kXeMaxSplits;
-    if (n > passed_tiles) n = passed_tiles;
-    if (n < 1) n = 1;
-    XeSplit r;
-    r.tiles = ceil_div(passed_tiles, n);
-    r.splits = (int)ceil_div(passed_tiles, r.tiles);
-    return r;
+    XePlan p;
+    p.groups = (int)ceil_div(kept_tiles, kXeWaves) * (use == kXeLoss ? 1 : s.slices);
+    p.tiles = passed_tiles;
+    const int room = 256 * xe_waves(s.blocks, s.parts, use, s.slices == 2);
+    // at least: so that a part's kept rows and results are little beside its tiles, and its slots few enough to add up
+    int least = (int)ceil_div(passed_tiles, use == kXeWeights ? 128 : kXeMaxParts - 2);
+    if (least < 2) least = 2;
+    if (least > passed_tiles) least = passed_tiles;
+    p.shared = p.groups < room ? room / p.groups : 1;
+    p.per = (int)ceil_div(passed_tiles, p.shared);
+    if (p.per < least) p.per = least;
+    p.shared = (int)ceil_div(passed_tiles, p.per);
+    p.room = room;
+    p.whole = 0;
+    // Where that leaves an eighth of the chip idle, in the only round or the last of a few: no regard for the groups' ends
+    const int64_t full = (int64_t)p.groups * p.shared, rounds = ceil_div(full, room);
+    if (p.per > least && rounds <= 8 && full * 8 < rounds * room * 7 && (p.groups % room + 1LL) * passed_tiles < 1LL << 31) {
+        p.whole = p.groups / room * room;
+        p.per = (int)ceil_div((int64_t)(p.groups - p.whole) * passed_tiles, room);
+        if (p.per < least) p.per = least;
+        p.shared = 0;
+    }
+    return p;
 }
 
 struct XeProblem {
-    int64_t n, classes, row_tiles, class_tiles;
+    int64_t n, classes;
+    int row_tiles, class_tiles;
     int dim, dtype;
     XeShape shape;
 };
@@ -823,8 +956,8 @@ inline bool xe_problem(int64_t n, int64_t classes, int dim, int dtype, XeProblem
     p->classes = classes;
     p->dim = dim;
     p->dtype = dtype;
-    p->row_tiles = ceil_div(n, 32);
-    p->class_tiles = ceil_div(classes, 32);
+    p->row_tiles = (int)ceil_div(n, 32);
+    p->class_tiles = (int)ceil_div(classes, 32);
     p->shape = xe_shape(dim, dtype);
     return true;
 }
@@ -863,7 +996,7 @@ struct XeScratch {
 inline XeScratch xe_forward_scratch(const XeProblem& p, int want, void* base)
 {
     const int use = want & FGL_XENT_ROWS ? kXeLossAndRows : kXeLoss;
-    const XeSplit split = xe_split(p.shape, use, p.row_tiles, p.class_tiles);
+    const XePlan plan = xe_plan(p.shape, use, p.row_tiles, p.class_tiles);
     Carver c(base);
     XeScratch s = {};
     if (!(want & FGL_XENT_WEIGHTS)) {
@@ -872,9 +1005,9 @@ inline XeScratch xe_forward_scratch(const XeProblem& p, int want, void* base)
     }
     if (use == kXeLossAndRows) {
         s.classes_p = c.take<char>((size_t)(p.class_tiles * p.shape.p_bytes()));
-        s.part = c.take<float>((size_t)(split.splits * p.row_tiles) * 32 * p.shape.cols());
+        s.part = c.take<float>((size_t)plan.slots() * kXeWaves * 32 * 32 * p.shape.blocks);
     }
-    s.stats = c.take<float>((size_t)split.splits * p.row_tiles * 32 * 4);
+    s.stats = c.take<float>((size_t)plan.slots() * kXeWaves * 32 * 4);
     s.tile_loss = c.take<float>((size_t)p.row_tiles * 2);
     s.bytes = c.used();
     return s;
@@ -885,10 +1018,10 @@ inline XeScratch xe_backward_scratch(const XeProblem& p, int want, void* base)
     Carver c(base);
     XeScratch s = {};
     if (want & FGL_XENT_WEIGHTS) {
-        const XeSplit split = xe_split(p.shape, kXeWeights, p.class_tiles, p.row_tiles);
-        if (split.splits > 1) {
-            s.part = c.take<float>((size_t)(split.splits * p.class_tiles) * 32 * p.shape.cols());
-            s.stats = c.take<float>((size_t)split.splits * p.class_tiles * 32 * 4);
+        const XePlan plan = xe_plan(p.shape, kXeWeights, p.class_tiles, p.row_tiles);
+        if (plan.shared != 1) {
+            s.part = c.take<float>((size_t)plan.slots() * kXeWaves * 32 * 32 * p.shape.blocks);
+            s.stats = c.take<float>((size_t)plan.slots() * kXeWaves * 32 * 4);
         }
     }
     s.bytes = c.used();
@@ -896,9 +1029,9 @@ inline XeScratch xe_backward_scratch(const XeProblem& p, int want, void* base)
 }
 
 template <int PARTS, int USE>
-void launch_xe_parts(const XeShape& s, const XeArgs& g, unsigned groups, hipStream_t stream)
+void launch_xe_parts(const XeShape& s, const XeArgs& g, unsigned workgroups, hipStream_t stream)
 {
-    const dim3 grid(groups), block(kBlock);
+    const dim3 grid(workgroups), block(kBlock);
     if (s.slices == 2) {
         if (s.blocks == 6) hipLaunchKernelGGL((xe_kernel<6, PARTS, USE, true>), grid, block, 0, stream, g);
         else hipLaunchKernelGGL((xe_kernel<8, PARTS, USE, true>), grid, block, 0, stream, g);
@@ -915,18 +1048,16 @@ void launch_xe_parts(const XeShape& s, const XeArgs& g, unsigned groups, hipStre
 }
 
 template <int USE>
-int launch_xe(const XeShape& s, XeArgs& g, hipStream_t stream)
+int launch_xe(const XeShape& s, XeArgs& g, int passed_tiles, hipStream_t stream)
 {
-    const XeSplit split = xe_split(s, USE, g.kept_tiles, g.passed_tiles);
-    g.splits = split.splits;
-    g.tiles_per_split = split.tiles;
-    const int64_t groups = ceil_div(g.kept_tiles, kXeWaves) * (USE == kXeLoss ? 1 : s.slices) * split.splits;
-    if (groups >= 1 << 24) {
+    g.plan = xe_plan(s, USE, g.kept_tiles, passed_tiles);
+    const int64_t workgroups = g.plan.workgroups();
+    if (workgroups >= 1 << 24) {
         set_error("linear_cross_entropy: grid too large");
         return FGL_ERR_UNSUPPORTED;
     }
-    if (s.parts == 3) launch_xe_parts<3, USE>(s, g, (unsigned)groups, stream);
-    else launch_xe_parts<1, USE>(s, g, (unsigned)groups, stream);
+    if (s.parts == 3) launch_xe_parts<3, USE>(s, g, (unsigned)workgroups, stream);
+    else launch_xe_parts<1, USE>(s, g, (unsigned)workgroups, stream);
     return FGL_OK;
 }
 
@@ -976,7 +1107,7 @@ FGL_EXPORT int fgl_linear_cross_entropy(const void* d_x, int64_t x_row_stride, i
     im.label64 = label64;
     im.ignore = ignore_index;
     im.classes = n_classes;
-    const int64_t tiles = p.row_tiles + p.class_tiles;
+    const int64_t tiles = (int64_t)p.row_tiles + p.class_tiles;
     FGL_REQUIRE(tiles < 1 << 24, "linear_cross_entropy: grid too large");
     const dim3 grid((unsigned)tiles, (unsigned)ceil_div(s.cols(), kXeCols)), block(kBlock);
     if (dtype == FGL_F32) hipLaunchKernelGGL((xe_images_kernel<float, 3>), grid, block, 0, to, im);
@@ -988,23 +1119,21 @@ FGL_EXPORT int fgl_linear_cross_entropy(const void* d_x, int64_t x_row_stride, i
     g.passed = im.m[1].s_image;
     g.passed_p = ws.classes_p;
     g.kept_tiles = p.row_tiles;
-    g.passed_tiles = p.class_tiles;
     g.stats = ws.stats;
     g.part = ws.part;
-    const int rc = want & FGL_XENT_ROWS ? launch_xe<kXeLossAndRows>(s, g, to) : launch_xe<kXeLoss>(s, g, to);
+    const int rc = want & FGL_XENT_ROWS ? launch_xe<kXeLossAndRows>(s, g, p.class_tiles, to) : launch_xe<kXeLoss>(s, g, p.class_tiles, to);
     if (rc != FGL_OK) return rc;
     FGL_CHECK_LAUNCH("xe_kernel");
 
     XeCombineArgs c = {};
+    c.plan = g.plan;
     c.stats = ws.stats;
     c.part = ws.part;
     c.rows = g.kept;
-    c.tiles = p.row_tiles;
     c.n_rows = n_rows;
     c.s_bytes = s.s_bytes();
-    c.splits = g.splits;
     c.blocks = s.blocks;
-    c.slices = s.slices;
+    c.slices = want & FGL_XENT_ROWS ? s.slices : 1;
     c.w = d_w;
     c.w_row = w_row_stride;
     c.w_col = w_col_stride;
@@ -1014,7 +1143,7 @@ FGL_EXPORT int fgl_linear_cross_entropy(const void* d_x, int64_t x_row_stride, i
     c.tile_loss = reduction == FGL_REDUCE_NONE ? nullptr : ws.tile_loss;
     c.kept = st.kept;
     c.d_x = st.d_x;
-    hipLaunchKernelGGL(xe_combine_kernel, dim3((unsigned)p.row_tiles), block, 0, to, c);
+    hipLaunchKernelGGL(xe_combine_kernel, dim3((unsigned)p.row_tiles, want & FGL_XENT_ROWS ? (unsigned)(s.blocks * s.slices) : 1u), block, 0, to, c);
     FGL_CHECK_LAUNCH("xe_combine_kernel");
     if (reduction != FGL_REDUCE_NONE) {
         hipLaunchKernelGGL(xe_total_kernel, dim3(1), block, 0, to, ws.tile_loss, p.row_tiles, (int)(reduction == FGL_REDUCE_MEAN), d_loss, st.count);
@@ -1050,14 +1179,13 @@ FGL_EXPORT int fgl_linear_cross_entropy_backward(const float* d_loss_grad, int64
     r.count = st.count;
     r.reduction = reduction;
     r.rows = d_dw != nullptr ? st.rows_s : nullptr;
-    r.tiles = p.row_tiles;
     r.n_rows = n_rows;
     r.s_bytes = s.s_bytes();
     r.cols = s.cols();
     r.dim = dim;
     r.bf16 = dtype == FGL_BF16;
     r.out = d_dx;
-    hipLaunchKernelGGL(xe_rows_kernel, dim3((unsigned)p.row_tiles), block, 0, to, r);
+    hipLaunchKernelGGL(xe_rows_kernel, dim3((unsigned)p.row_tiles, d_dx != nullptr ? (unsigned)ceil_div(dim, 32) : 1u), block, 0, to, r);
     FGL_CHECK_LAUNCH("xe_rows_kernel");
     if (d_dw == nullptr) return FGL_OK;
 
@@ -1066,7 +1194,6 @@ FGL_EXPORT int fgl_linear_cross_entropy_backward(const float* d_loss_grad, int64
     g.passed = st.rows_s;
     g.passed_p = st.rows_p;
     g.kept_tiles = p.class_tiles;
-    g.passed_tiles = p.row_tiles;
     g.stats = ws.stats;
     g.part = ws.part;
     g.d_w = d_dw;
@@ -1074,23 +1201,25 @@ FGL_EXPORT int fgl_linear_cross_entropy_backward(const float* d_loss_grad, int64
     g.kept_rows = n_classes;
     g.dim = dim;
     g.bf16 = dtype == FGL_BF16;
-    const int rc = launch_xe<kXeWeights>(s, g, to);
+    const int rc = launch_xe<kXeWeights>(s, g, p.row_tiles, to);
     if (rc != FGL_OK) return rc;
     FGL_CHECK_LAUNCH("xe_kernel");
-    if (g.splits > 1) {
+    if (g.plan.shared != 1) {
         XeWeightsArgs c = {};
+        c.plan = g.plan;
         c.stats = ws.stats;
         c.part = ws.part;
-        c.tiles = p.class_tiles;
         c.n_rows = n_classes;
-        c.splits = g.splits;
         c.blocks = s.blocks;
         c.slices = s.slices;
         c.dim = dim;
         c.bf16 = g.bf16;
         c.d_w = d_dw;
         c.d_b = d_db;
-        hipLaunchKernelGGL(xe_weights_kernel, dim3((unsigned)p.class_tiles, (unsigned)s.blocks), block, 0, to, c);
+        const bool together = g.plan.shared > 8;
+        const dim3 combine((unsigned)p.class_tiles, (unsigned)((together ? kXeWaves : 1) * s.blocks * s.slices));
+        if (together) hipLaunchKernelGGL(xe_weights_kernel<true>, combine, block, 0, to, c);
+        else hipLaunchKernelGGL(xe_weights_kernel<false>, combine, block, 0, to, c);
         FGL_CHECK_LAUNCH("xe_weights_kernel");
     }
     return FGL_OK;

@@ -91,7 +91,8 @@ def make(cuda, n, v, d, dtype, bias=True, ignored=0.2, seed=0, label_dtype=torch
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("n,v,d", [(1, 1, 1), (1, 2, 3), (2, 33, 31), (31, 32, 32), (33, 31, 33), (100, 47, 64), (128, 64, 65), (129, 129, 96), (257, 172, 100), (64, 1000, 128),
                                    (300, 161, 160), (500, 300, 192), (96, 4097, 200), (1000, 47, 256), (40, 500, 257), (70, 333, 300), (130, 100, 384), (33, 700, 400),
-                                   (200, 65, 512), (5, 20011, 64), (4100, 5, 16), (2500, 2100, 48)])
+                                   (200, 65, 512), (5, 20011, 64), (4100, 5, 16), (2500, 2100, 48),
+                                   (12900, 230, 300), (230, 12900, 300), (40_000, 500, 250), (500, 90_000, 250), (33_000, 70, 30)])
 def test_losses_and_gradients(cuda, dtype, n, v, d):
     print("linear_cross_entropy %d x %d, %d classes, %s" % (n, d, v, dtype), flush=True)
     check(*make(cuda, n, v, d, dtype))
