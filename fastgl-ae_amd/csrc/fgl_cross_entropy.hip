@@ -13,18 +13,23 @@
 // S^T rather than S: a lane of a matrix result has one column, so a lane has one kept row -- its running maximum, sum and
 // rescaling are the lane's own -- and the sixteen values of S^T that it has are, rounded, an operand of the second product as they
 // are (its k, the passed rows, is taken in the order in which the lanes have it).  O^T for the same reason.
-// The running maximum is moved only where a row's largest value passes it by 2^8 (fp32 and bf16 hold p up to there with
-// the same relative error), so that O is rescaled a few times a pass and not once a tile.
+// The running maximum is moved only where a row's largest value passes it by 2^8, so that O is rescaled a few times a pass and not once a
+// tile.  The label's own share is no part of maximum, sum and O.
 //
 // Operands: "images" (xe_images_kernel), a copy of x and w in the order in which the lanes take them, 1 KB for each 32 x 16 values, rows
 // and columns padded with zeros: once as operand of S (lane: row, eight columns) and once of O (lane: column, eight rows).  So a tile is
 // copied to LDS straight, without a register or a bank conflict, and no access is out of bounds whatever the sizes.  A tile's
 // first kilobyte has what belongs to its 32 rows: biases, or labels and the backward pass's factors.
 //
-// fp32: each value in three bf16 parts (fgl_split.hpp), six matrix instructions a product, their sum over 32 k added to fp32 accumulators.
-// bf16: P and the results are rounded to bf16, as the operands are; sums, maxima and losses are fp32 in both.
-// Values must be finite, and below 3.38e38 in fp32, where a part would round to infinity: others make losses and gradients that are not
-// numbers.  A bias of -1e30 or less, -infinity among them, leaves its class out: no share, no gradient.  (Shares are exp2 of one fma, whose
+// bf16: P is rounded to bf16, as the operands are.
+// fp32: each value is the sum of two fp16 values, of 11 bits each, and a product three matrix instructions (high low, low high, high high; what is
+// left out is 2^-22 of it), whose sum over 64 k is added to fp32 accumulators.  fp16's range is short, so x and w are first multiplied by a power of two
+// that takes their largest value to 2^14 (xe_most_kernel); what lies 2^39 below it is lost, which is nothing beside the logits and sums that it would
+// go into.  P is scaled likewise, by the running maximum, and the gradient of the logits by a running bound of its own.  Against 64 bits, 2-norm,
+// 8192 x 128 and 20 K classes: @ERR@; the same in fp32 products by the library 1.7e-6, in three bf16 parts and six instructions 1.9e-7, in
+// @SIX@ of the time.
+// Sums, maxima and losses are fp32 in both.  x and w must be finite, in fp32 below 2^74: others make losses and gradients that are not numbers.
+// A bias of -1e30 or less, -infinity among them, leaves its class out: no share, no gradient.  (Shares are exp2 of one fma, whose
 // product with log2 e is not rounded where the maximum's is: logits up to some 1e9 are no matter, the difference of 2^-25 of the maximum is the
 // same for all of a row's shares and their sum.)
 //
@@ -34,13 +39,15 @@
 // run).
 #include "fgl_common.hpp"
 #include "fgl_kernels.hpp"
-#include "fgl_split.hpp"
 
 #include <math.h>
 
 namespace fgl {
 
 typedef float XeF4 __attribute__((ext_vector_type(4)));
+typedef float XeF32x16 __attribute__((ext_vector_type(16)));
+typedef uint32_t XeOp __attribute__((ext_vector_type(4)));  // eight values of a matrix instruction's operand
+typedef _Float16 XeF16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kXeWaves = kBlock / kWave;
 constexpr int kXeChunk = 1024;  // bytes of an operand of one matrix instruction
@@ -50,6 +57,8 @@ constexpr float kXeLog2e = 1.44269504088896340736f;
 constexpr float kXeLn2 = 0.69314718055994530942f;
 constexpr float kXeLeftOut = -1e30f;  // a bias of this or less leaves its class out, as -infinity does
 constexpr float kXeStep = 8.0f;       // powers of two that a row's values may pass its running maximum by
+constexpr float kXeRise = 6.0f;       // fp16: powers of two that P is multiplied by, so that it fills the range
+constexpr int kXeTop = 14;            // fp16: power of two that largest values are taken to
 
 enum { kXeLoss = 0, kXeLossAndRows = 1, kXeWeights = 2 };
 
@@ -71,7 +80,7 @@ inline XeShape xe_shape(int dim, int dtype)
 {
     const int n = (int)ceil_div(dim, 32);
     XeShape s;
-    s.parts = dtype == FGL_F32 ? 3 : 1;
+    s.parts = dtype == FGL_F32 ? 2 : 1;
     const int blocks = n <= 4 ? n : n <= 6 ? 6 : n <= 8 ? 8 : n <= 12 ? 12 : 16;
     s.slices = blocks > 8 ? 2 : 1;
     s.blocks = blocks / s.slices;
@@ -96,26 +105,100 @@ struct XeImagesArgs {
     int label64;
     int64_t ignore;
     int64_t classes;
+    const float* most;  // fp32: [2][kBlock], the largest magnitudes of parts of the matrices (xe_most_kernel)
+    float* scales;      // fp32: the powers of two that the matrices are multiplied by
 };
 
 constexpr int kXeCols = 128;  // columns that a workgroup lays out, of 32 rows
 constexpr int kXePitch = kXeCols + 4;
 
-template <int PARTS>
-__device__ __forceinline__ void xe_put(const float (&v)[8], char* to)
+// v = hi + lo, fp16 each, to 2^-22 of it
+__device__ __forceinline__ void xe_split(const float (&v)[8], XeOp& hi, XeOp& lo)
 {
-    if constexpr (PARTS == 3) {
-        SpU4 p[3];
-        uint32_t rest = 0;  // (bits below 2^-133: nothing beside a logit, and beside a gradient of x's own size)
-        sp_split(v, p, rest);
+    XeF16x8 h, l;
 #pragma unroll
-        for (int q = 0; q < 3; ++q) *reinterpret_cast<SpU4*>(to + q * kXeChunk) = p[q];
-    } else {
-        Bf16x8 o;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) o[j] = (__bf16)v[j];
-        *reinterpret_cast<Bf16x8*>(to) = o;
+    for (int j = 0; j < 8; ++j) {
+        h[j] = (_Float16)v[j];
+        l[j] = (_Float16)(v[j] - (float)h[j]);
     }
+    hi = __builtin_bit_cast(XeOp, h);
+    lo = __builtin_bit_cast(XeOp, l);
+}
+
+__device__ __forceinline__ XeOp xe_bf16(const float (&v)[8])
+{
+    Bf16x8 o;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o[j] = (__bf16)v[j];
+    return __builtin_bit_cast(XeOp, o);
+}
+
+template <int PARTS>
+__device__ __forceinline__ void xe_put(float (&v)[8], float scale, char* to)
+{
+    XeOp* p = reinterpret_cast<XeOp*>(to);
+    if constexpr (PARTS == 2) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] *= scale;
+        XeOp hi, lo;
+        xe_split(v, hi, lo);
+        p[0] = hi;
+        p[kXeChunk / sizeof(XeOp)] = lo;
+    } else {
+        p[0] = xe_bf16(v);
+    }
+}
+
+__device__ __forceinline__ float xe_block_max(float v, float* shared)
+{
+#pragma unroll
+    for (int d = kWave / 2; d >= 1; d >>= 1) v = fmaxf(v, __shfl_xor(v, d, kWave));
+    if (lane_id() == 0) shared[threadIdx.x / kWave] = v;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kXeWaves; ++k) v = fmaxf(v, shared[k]);
+    return v;
+}
+
+// Workgroup (i, m) of kBlock x 2: the largest magnitude of part i of matrix m (what is not a number is passed over).
+__global__ __launch_bounds__(kBlock) void xe_most_kernel(const XeMatrix m0, const XeMatrix m1, int dim, float* __restrict__ most)
+{
+    __shared__ float shared[kXeWaves];
+    const XeMatrix& m = blockIdx.y == 0 ? m0 : m1;
+    const float* src = static_cast<const float*>(m.src);
+    float v = 0.0f;
+    // a wave takes 1024 values of a line at a time: of a row, or of a column where those lie side by side, or of all rows if there is no gap between them
+    const bool rows = m.col_stride == 1, one = rows && m.row_stride == dim;
+    const int64_t lines = one ? 1 : rows ? m.rows : dim, length = one ? m.rows * dim : rows ? dim : m.rows;
+    const int64_t step = rows ? m.row_stride : m.col_stride, unit = rows ? 1 : m.row_stride, each = (length + 1023) / 1024;
+    const int lane = lane_id();
+    for (int64_t k = (int64_t)blockIdx.x * kXeWaves + threadIdx.x / kWave; k < lines * each; k += (int64_t)gridDim.x * kXeWaves) {
+        const int64_t line = k / each, first = (k - line * each) * 1024;
+        const float* p = src + line * step;
+        if (unit == 1 && first + 1024 <= length) {
+            typedef float Vec __attribute__((ext_vector_type(4), aligned(4)));
+            Vec q[4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) q[c] = *reinterpret_cast<const Vec*>(p + first + c * 256 + 4 * lane);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) v = fmaxf(v, fmaxf(fmaxf(fabsf(q[c][0]), fabsf(q[c][1])), fmaxf(fabsf(q[c][2]), fabsf(q[c][3]))));
+        } else {
+            const int64_t end = first + 1024 < length ? first + 1024 : length;
+#pragma unroll 4
+            for (int64_t c = first + lane; c < end; c += kWave) v = fmaxf(v, fabsf(p[c * unit]));
+        }
+    }
+    v = xe_block_max(v, shared);
+    if (threadIdx.x == 0) most[blockIdx.y * kBlock + blockIdx.x] = v;
+}
+
+// The power of two that takes a largest magnitude to 2^14 .. 2^15; bounded, so that two of them and a bias are no infinity.
+__device__ __forceinline__ float xe_scale(float most)
+{
+    int e = kXeTop + 127 - (int)(__float_as_uint(most) >> 23);
+    if (most == 0.0f) e = 0;
+    e = e < -60 ? -60 : e > 45 ? 45 : e;
+    return __uint_as_float((uint32_t)(127 + e) << 23);
 }
 
 template <typename T, int PARTS>
@@ -128,6 +211,17 @@ __global__ __launch_bounds__(kBlock) void xe_images_kernel(const XeImagesArgs g)
     const int64_t t = classes ? id - g.first_tiles : id, row0 = 32 * t;
     const int col0 = kXeCols * (int)blockIdx.y, thread = (int)threadIdx.x;
     const T* src = static_cast<const T*>(m.src);
+    float scale_x = 1.0f, scale_w = 1.0f;
+    if constexpr (PARTS == 2) {
+        __shared__ float shared[2][kXeWaves];
+        scale_x = xe_scale(xe_block_max(g.most[thread], shared[0]));
+        scale_w = xe_scale(xe_block_max(g.most[kBlock + thread], shared[1]));
+        if (id == 0 && blockIdx.y == 0 && thread == 0) {
+            g.scales[0] = scale_x;
+            g.scales[1] = scale_w;
+        }
+    }
+    const float scale = classes ? scale_w : scale_x;
     if (m.col_stride == 1) {
         typedef T Vec __attribute__((ext_vector_type(8), aligned(sizeof(T))));
 #pragma unroll
@@ -169,7 +263,7 @@ __global__ __launch_bounds__(kBlock) void xe_images_kernel(const XeImagesArgs g)
                 b = m.bias != nullptr ? (float)static_cast<const T*>(m.bias)[row] : 0.0f;
                 if (b <= kXeLeftOut) b = -INFINITY;
             }
-            reinterpret_cast<float*>(s_tile)[thread] = b;
+            reinterpret_cast<float*>(s_tile)[thread] = b * scale_x * scale_w;  // (it goes where their products go)
         } else {
             int label = -1;  // none
             if (row < m.rows) {
@@ -187,7 +281,7 @@ __global__ __launch_bounds__(kBlock) void xe_images_kernel(const XeImagesArgs g)
         float v[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = tile[lane % 32 * kXePitch + at / kWave * 16 + lane / 32 * 8 + j];
-        xe_put<PARTS>(v, s_tile + kXeChunk * (1 + (int64_t)step * PARTS) + lane * 16);
+        xe_put<PARTS>(v, scale, s_tile + kXeChunk * (1 + (int64_t)step * PARTS) + lane * 16);
     }
     if (m.p_image == nullptr) return;
     char* p_tile = m.p_image + t * kXeChunk * ((int64_t)steps * PARTS);
@@ -200,7 +294,7 @@ __global__ __launch_bounds__(kBlock) void xe_images_kernel(const XeImagesArgs g)
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = tile[(half * 16 + j / 4 * 8 + lane / 32 * 4 + j % 4) * kXePitch + own * 32 + lane % 32];
         const int slice = block / g.blocks, in_slice = block % g.blocks;
-        xe_put<PARTS>(v, p_tile + kXeChunk * ((((int64_t)slice * 2 + half) * g.blocks + in_slice) * PARTS) + lane * 16);
+        xe_put<PARTS>(v, scale, p_tile + kXeChunk * ((((int64_t)slice * 2 + half) * g.blocks + in_slice) * PARTS) + lane * 16);
     }
 }
 
@@ -243,6 +337,7 @@ struct XeArgs {
     int kept_tiles;
     float* stats;  // [slot][wave][row of 32]: maximum, others' sum, label's logit, -  (weights: sum, -, -, -)
     float* part;   // [slot][wave][block][quarter][lane][4]
+    const float* scales;  // fp32: of rows and classes
     // weights of groups that one workgroup has alone: straight to the result
     void* d_w;
     void* d_b;
@@ -279,85 +374,67 @@ __device__ __forceinline__ void xe_staged()
     __syncthreads();
 }
 
-__device__ __forceinline__ Bf16x8 xe_operand(const char* chunk) { return *reinterpret_cast<const Bf16x8*>(chunk + lane_id() * 16); }
+__device__ __forceinline__ XeOp xe_operand(const char* chunk) { return *reinterpret_cast<const XeOp*>(chunk + lane_id() * 16); }
 
-__device__ __forceinline__ Bf16x8 xe_operand(const XeGlobal<const char>* chunk) { return *reinterpret_cast<const XeGlobal<const Bf16x8>*>(chunk + lane_id() * 16); }
+__device__ __forceinline__ XeOp xe_operand(const XeGlobal<const char>* chunk) { return *reinterpret_cast<const XeGlobal<const XeOp>*>(chunk + lane_id() * 16); }
 
-__device__ __forceinline__ SpF32x16 xe_mfma(Bf16x8 a, Bf16x8 b, SpF32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+template <int PARTS>
+__device__ __forceinline__ XeF32x16 xe_mfma(const XeOp& a, const XeOp& b, const XeF32x16& c)
+{
+    if constexpr (PARTS == 1) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(Bf16x8, a), __builtin_bit_cast(Bf16x8, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(XeF16x8, a), __builtin_bit_cast(XeF16x8, b), c, 0, 0, 0);
+}
 
-// N products of an operand from LDS each: at(i) is the i-th one's place, use(i, operand) multiplies.  Operands are read kAhead products before
-// they are used, and the compiler is kept from moving either: left to itself it reads two, waits for them and multiplies.
-template <int N, typename At, typename Use>
+// N products of an operand from LDS each, in PARTS parts at neighbouring places: at(i) is the i-th one's place, use(i, parts) multiplies.  Operands are
+// read a few products before they are used, and the compiler is kept from moving either: left to itself it reads two, waits for them and
+// multiplies.
+template <int N, int PARTS, typename At, typename Use>
 __device__ __forceinline__ void xe_products(const At& at, const Use& use)
 {
-    constexpr int kAhead = N < 4 ? N : 4;
-    Bf16x8 a[kAhead];
+    constexpr int kMost = PARTS == 1 ? 4 : 2, kAhead = N < kMost ? N : kMost;
+    XeOp a[kAhead + 1][PARTS];
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) a[i] = xe_operand(at(i));
-    __builtin_amdgcn_sched_barrier(0);
+    for (int i = 0; i < kAhead; ++i)
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        use(i, a[i % kAhead]);
-        if (i + kAhead < N) a[i % kAhead] = xe_operand(at(i + kAhead));
-        __builtin_amdgcn_sched_barrier(0);
-    }
-}
-
-// The same for operands in three parts (at neighbouring places) and with six products each: the next one's parts are read while this one's are
-// multiplied.
-template <int N, typename At, typename Use>
-__device__ __forceinline__ void xe_products_in_parts(const At& at, const Use& use)
-{
-    Bf16x8 a[2][3];
-#pragma unroll
-    for (int p = 0; p < 3; ++p) a[0][p] = xe_operand(at(0) + p * kXeChunk);
+        for (int p = 0; p < PARTS; ++p) a[i][p] = xe_operand(at(i) + p * kXeChunk);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
 #pragma unroll
-        for (int p = 0; p < 3; ++p)
-            if (i + 1 < N) a[(i + 1) & 1][p] = xe_operand(at(i + 1) + p * kXeChunk);
-        use(i, a[i & 1]);
+        for (int p = 0; p < PARTS; ++p)
+            if (i + kAhead < N) a[(i + kAhead) % (kAhead + 1)][p] = xe_operand(at(i + kAhead) + p * kXeChunk);
+        use(i, a[i % (kAhead + 1)]);
         __builtin_amdgcn_sched_barrier(0);
     }
 }
-
-constexpr int kXePa[6] = {2, 0, 1, 1, 0, 0}, kXePb[6] = {0, 2, 1, 0, 1, 0};  // the small products first
 
 // Waves that a SIMD (and so workgroups that a CU) holds at once: the kept rows take 8 registers a block and part, O 16 a block, of 512.
-// WIDE: in two slices; in fp32 with the kept rows from memory.
+// WIDE: in two slices.
 __host__ __device__ constexpr int xe_waves(int blocks, int parts, int use, bool wide)
 {
     if (wide) return parts == 1 && (use == kXeLoss || blocks <= 6) ? 2 : 1;
-    if (use == kXeLoss) return parts == 1 ? 4 : blocks <= 2 ? 4 : blocks <= 4 ? 3 : blocks <= 6 ? 2 : 1;
-    return parts == 1 ? (blocks <= 2 ? 4 : blocks <= 3 ? 3 : blocks <= 8 ? 2 : 1) : blocks <= 1 ? 4 : blocks <= 4 ? 2 : 1;
+    if (use == kXeLoss) return parts == 1 ? 4 : blocks <= 2 ? 4 : blocks <= 4 ? 3 : 2;
+    return parts == 1 ? (blocks <= 2 ? 4 : blocks <= 3 ? 3 : 2) : blocks <= 1 ? 4 : blocks <= 2 ? 3 : blocks <= 4 ? 2 : 1;
 }
 
 template <int DB, int PARTS, int USE, bool WIDE>
 struct XeWave {
     static constexpr int kSteps = WIDE ? 4 * DB : 2 * DB;
     static constexpr int kSChunks = 1 + kSteps * PARTS, kPChunks = 2 * DB * PARTS;
-    static constexpr bool kFromMemory = WIDE && PARTS == 3;
-    static constexpr int kKept = kFromMemory ? 1 : kSteps;
+    static constexpr float kRise = PARTS == 2 ? kXeRise : 0.0f;
 
-    Bf16x8 kept[kKept][PARTS];
-    const XeGlobal<const char>* kept_at;  // kFromMemory
-    SpF32x16 o[USE == kXeLoss ? 1 : DB];
-    SpF32x16 start;       // weights: the class's bias sixteen times
-    float top, sum, own;  // running maximum (a power of two), sum, the label's logit
+    XeOp kept[kSteps][PARTS];
+    XeF32x16 o[USE == kXeLoss ? 1 : DB];
+    XeF32x16 start;       // weights: the class's bias sixteen times
+    float unit;           // what S is to be multiplied by (fp32: its operands are scaled)
+    float top, sum, own;  // running maximum (a power of two; weights, fp32: what P is below, a power of two itself), sum, the label's logit
     int label;            // weights: the class
     bool bias_sum;
 
-    __device__ __forceinline__ Bf16x8 kept_part(int step, int p) const
-    {
-        if constexpr (kFromMemory) return xe_operand(kept_at + (int64_t)(step * PARTS + p) * kXeChunk);
-        else return kept[step][p];
-    }
-
     // S^T of the staged tile
-    __device__ __forceinline__ SpF32x16 logits(const char* s) const
+    __device__ __forceinline__ XeF32x16 logits(const char* s) const
     {
-        SpF32x16 acc;
+        XeF32x16 acc;
         if constexpr (USE == kXeWeights) {
             acc = start;
         } else {
@@ -370,16 +447,17 @@ struct XeWave {
         }
         const auto at = [&](int k) { return s + (1 + k * PARTS) * kXeChunk; };
         if constexpr (PARTS == 1) {
-            xe_products<kSteps>(at, [&](int k, Bf16x8 a) { acc = xe_mfma(a, kept_part(k, 0), acc); });
+            xe_products<kSteps, 1>(at, [&](int k, const XeOp (&a)[1]) { acc = xe_mfma<1>(a[0], kept[k][0], acc); });
         } else {
-            SpF32x16 chunk = {};
-            xe_products_in_parts<kSteps>(at, [&](int k, const Bf16x8 (&a)[3]) {
-#pragma unroll
-                for (int q = 0; q < 6; ++q) chunk = xe_mfma(a[kXePa[q]], kept_part(k, kXePb[q]), chunk);
-                if (k % 2 == 1) {
+            XeF32x16 chunk = {};
+            xe_products<kSteps, 2>(at, [&](int k, const XeOp (&a)[2]) {
+                chunk = xe_mfma<2>(a[1], kept[k][0], chunk);
+                chunk = xe_mfma<2>(a[0], kept[k][1], chunk);
+                chunk = xe_mfma<2>(a[0], kept[k][0], chunk);
+                if (k % 4 == 3 || k == kSteps - 1) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) acc[i] += chunk[i];
-                    chunk = SpF32x16{};
+                    chunk = XeF32x16{};
                 }
             });
         }
@@ -387,25 +465,9 @@ struct XeWave {
     }
 
     // S^T -> P^T, with the running maximum, sum and the label's logit.  v0: the tile's first class.
-    __device__ __forceinline__ void shares(SpF32x16& s, int v0)
+    __device__ __forceinline__ void shares(XeF32x16& s, int v0)
     {
-        float most = s[0];
-#pragma unroll
-        for (int i = 1; i < 16; ++i) most = fmaxf(most, s[i]);
-        most = fmaxf(most, xe_other_half(most)) * kXeLog2e;
-        if (__any(most > top + kXeStep)) {
-            const float now = fmaxf(top, most);
-            const float scale = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top - now);
-            top = now;
-            sum *= scale;
-            if constexpr (USE == kXeLossAndRows) {
-#pragma unroll
-                for (int d = 0; d < DB; ++d)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) o[d][i] *= scale;
-            }
-        }
-        const float shift = top == -INFINITY ? 0.0f : -top;
+        const float to2 = kXeLog2e * unit;
         const int in_tile = label - v0;
         const bool here = label >= 0 && in_tile >= 0 && in_tile < 32;
         if (__any(here)) {
@@ -413,17 +475,37 @@ struct XeWave {
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 if (at == 8 * (i / 4) + i % 4) {
-                    own = s[i];
+                    own = s[i] * unit;
                     s[i] = -INFINITY;
                 }
             }
         }
+        float most = s[0];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], kXeLog2e, shift));
+        for (int i = 1; i < 16; ++i) most = fmaxf(most, s[i]);
+        most = fmaxf(most, xe_other_half(most)) * to2;
+        if (__any(most > top + kXeStep)) {
+            const float now = fmaxf(top, most);
+            const float scale = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top - now);
+            top = now;
+            sum *= scale;
+            if constexpr (USE == kXeLossAndRows) rescale(scale);
+        }
+        const float shift = top == -INFINITY ? 0.0f : kRise - top;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], to2, shift));
         add_up(s);
     }
 
-    __device__ __forceinline__ void add_up(const SpF32x16& p)
+    __device__ __forceinline__ void rescale(float scale)
+    {
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[d][i] *= scale;
+    }
+
+    __device__ __forceinline__ void add_up(const XeF32x16& p)
     {
         float t[8];
 #pragma unroll
@@ -432,7 +514,7 @@ struct XeWave {
     }
 
     // S^T -> the gradient of the logits, from the maxima, factors and labels of the tile's rows
-    __device__ __forceinline__ void gradients(SpF32x16& s, const char* tile, int v0)
+    __device__ __forceinline__ void gradients(XeF32x16& s, const char* tile, int v0)
     {
         const float* c = reinterpret_cast<const float*>(tile);
         const int* l = reinterpret_cast<const int*>(tile);
@@ -441,7 +523,7 @@ struct XeWave {
         for (int q = 0; q < 4; ++q) {
             const XeF4 shift = *reinterpret_cast<const XeF4*>(c + kXeShift + 8 * q + first), factor = *reinterpret_cast<const XeF4*>(c + kXeFactor + 8 * q + first);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) s[4 * q + j] = __builtin_amdgcn_exp2f(fmaf(s[4 * q + j], kXeLog2e, shift[j])) * factor[j];
+            for (int j = 0; j < 4; ++j) s[4 * q + j] = __builtin_amdgcn_exp2f(fmaf(s[4 * q + j], kXeLog2e * unit, shift[j])) * factor[j];
         }
         const int in_tile = l[kXeLabel + lane_id() % 32] - v0;
         if (__any(in_tile >= 0 && in_tile < 32)) {
@@ -452,41 +534,53 @@ struct XeWave {
             }
         }
         if (bias_sum) add_up(s);
+        if constexpr (PARTS == 2) {  // to fp16's range: 2^14 is what a class's values are below, sixteen times its largest one when that was met
+            float most = fabsf(s[0]);
+#pragma unroll
+            for (int i = 1; i < 16; ++i) most = fmaxf(most, fabsf(s[i]));
+            most = fmaxf(most, xe_other_half(most));
+            if (__any(most > top)) {
+                const float now = most > top ? __uint_as_float((__float_as_uint(fminf(most, 0x1p100f)) & 0x7F800000u) + (4u << 23)) : top;
+                rescale(top / now);
+                top = now;
+            }
+            const float scale = (float)(1 << kXeTop) / top;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] *= scale;
+        }
     }
 
     // O^T += passed^T P^T
-    __device__ __forceinline__ void product(const SpF32x16& s, const char* p)
+    __device__ __forceinline__ void product(const XeF32x16& s, const char* p)
     {
+        XeOp w[2][PARTS];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = s[8 * h + j];
+            if constexpr (PARTS == 1) w[h][0] = xe_bf16(v);
+            else xe_split(v, w[h][0], w[h][1]);
+        }
         if constexpr (PARTS == 1) {
-            Bf16x8 w[2];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) w[i / 8][i % 8] = (__bf16)s[i];
-            xe_products<2 * DB>([&](int i) { return p + i * kXeChunk; }, [&](int i, Bf16x8 a) { o[i % DB] = xe_mfma(a, w[i / DB], o[i % DB]); });
+            xe_products<2 * DB, 1>([&](int i) { return p + i * kXeChunk; }, [&](int i, const XeOp (&a)[1]) { o[i % DB] = xe_mfma<1>(a[0], w[i / DB][0], o[i % DB]); });
         } else {
-            SpU4 w[2][3];
-            uint32_t rest = 0;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                float v[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = s[8 * h + j];
-                sp_split(v, w[h], rest);
-            }
-            SpF32x16 chunk = {};
-            xe_products_in_parts<2 * DB>([&](int i) { return p + (i % 2 * DB + i / 2) * 3 * kXeChunk; }, [&](int i, const Bf16x8 (&a)[3]) {
-#pragma unroll
-                for (int q = 0; q < 6; ++q) chunk = xe_mfma(a[kXePa[q]], __builtin_bit_cast(Bf16x8, w[i % 2][kXePb[q]]), chunk);
+            XeF32x16 chunk = {};
+            xe_products<2 * DB, 2>([&](int i) { return p + (i % 2 * DB + i / 2) * 2 * kXeChunk; }, [&](int i, const XeOp (&a)[2]) {
+                chunk = xe_mfma<2>(a[1], w[i % 2][0], chunk);
+                chunk = xe_mfma<2>(a[0], w[i % 2][1], chunk);
+                chunk = xe_mfma<2>(a[0], w[i % 2][0], chunk);
                 if (i % 2 == 1) {
 #pragma unroll
                     for (int c = 0; c < 16; ++c) o[i / 2][c] += chunk[c];
-                    chunk = SpF32x16{};
+                    chunk = XeF32x16{};
                 }
             });
         }
     }
 
     // One tile: copies what comes next to `next` while it works on `s`
-    __device__ __forceinline__ void first_half(const char* __restrict__ s, char* __restrict__ next, const char* src, SpF32x16& p, int n0, int v0, bool active)
+    __device__ __forceinline__ void first_half(const char* __restrict__ s, char* __restrict__ next, const char* src, XeF32x16& p, int n0, int v0, bool active)
     {
         if constexpr (USE == kXeLoss) {
             if (src != nullptr) xe_stage<kSChunks>(src, next);
@@ -498,7 +592,7 @@ struct XeWave {
         if constexpr (USE == kXeWeights) gradients(p, s, v0);
         else shares(p, n0);
     }
-    __device__ __forceinline__ void second_half(const char* __restrict__ s, char* __restrict__ next, const char* src, const SpF32x16& p, bool active)
+    __device__ __forceinline__ void second_half(const char* __restrict__ s, char* __restrict__ next, const char* src, const XeF32x16& p, bool active)
     {
         if (src != nullptr) xe_stage<kSChunks>(src, next);
         if (active) product(p, s);
@@ -533,7 +627,7 @@ __device__ __forceinline__ void xe_store4(void* out, bool bf16, int64_t row, int
 }
 
 template <int DB, int N>
-__device__ __forceinline__ void xe_store_weights(const XeArgs& g, const SpF32x16 (&o)[N], int64_t row, int slice, float sum)
+__device__ __forceinline__ void xe_store_weights(const XeArgs& g, const XeF32x16 (&o)[N], int64_t row, int slice, float sum)
 {
     if (row >= g.kept_rows) return;
     int half = lane_id() / 32;
@@ -553,10 +647,8 @@ template <int DB, int PARTS, int USE, bool WIDE>
 __global__ __launch_bounds__(kBlock, xe_waves(DB, PARTS, USE, WIDE)) void xe_kernel(const XeArgs g)
 {
     using Wave = XeWave<DB, PARTS, USE, WIDE>;
-    // the loss alone: two tiles in turn, or one where LDS has no room for two
-    constexpr bool kTwo = USE == kXeLoss && 2 * Wave::kSChunks <= 160;
     __shared__ __attribute__((aligned(16))) char s_buf[Wave::kSChunks * kXeChunk];
-    __shared__ __attribute__((aligned(16))) char p_buf[(USE != kXeLoss ? Wave::kPChunks : kTwo ? Wave::kSChunks : 1) * kXeChunk];
+    __shared__ __attribute__((aligned(16))) char p_buf[(USE == kXeLoss ? Wave::kSChunks : Wave::kPChunks) * kXeChunk];  // (the loss alone: two tiles in turn)
     constexpr int kSlices = WIDE && USE != kXeLoss ? 2 : 1;
     constexpr int64_t kSBytes = (int64_t)Wave::kSChunks * kXeChunk, kPBytes = (int64_t)Wave::kPChunks * (WIDE ? 2 : 1) * kXeChunk;
     const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x / kWave));
@@ -591,16 +683,15 @@ __global__ __launch_bounds__(kBlock, xe_waves(DB, PARTS, USE, WIDE)) void xe_ker
     const XeGlobal<const char>* own = xe_uniform(g.kept + (active ? tile : g.kept_tiles - 1) * kSBytes);
 
     Wave w;
-    w.kept_at = own + kXeChunk;
-    if constexpr (!Wave::kFromMemory) {
 #pragma unroll
-        for (int k = 0; k < Wave::kSteps; ++k)
+    for (int k = 0; k < Wave::kSteps; ++k)
 #pragma unroll
-            for (int p = 0; p < PARTS; ++p) w.kept[k][p] = xe_operand(w.kept_at + (k * PARTS + p) * kXeChunk);
-    }
+        for (int p = 0; p < PARTS; ++p) w.kept[k][p] = xe_operand(own + kXeChunk + (k * PARTS + p) * kXeChunk);
+    w.unit = 1.0f;
+    if constexpr (PARTS == 2) w.unit = 1.0f / g.scales[0] * (1.0f / g.scales[1]);
 #pragma unroll
-    for (int d = 0; d < (USE == kXeLoss ? 1 : DB); ++d) w.o[d] = SpF32x16{};
-    w.top = -INFINITY;
+    for (int d = 0; d < (USE == kXeLoss ? 1 : DB); ++d) w.o[d] = XeF32x16{};
+    w.top = USE == kXeWeights ? 0x1p-100f : -INFINITY;
     w.sum = w.own = 0.0f;
     w.bias_sum = g.d_b != nullptr;
     if constexpr (USE == kXeWeights) {
@@ -613,17 +704,10 @@ __global__ __launch_bounds__(kBlock, xe_waves(DB, PARTS, USE, WIDE)) void xe_ker
     }
 
     const int v0 = 32 * tile;
-    SpF32x16 p = {};
+    XeF32x16 p = {};
     xe_stage<Wave::kSChunks>(g.passed + t0 * kSBytes, s_buf);
     xe_staged();
-    if constexpr (USE == kXeLoss && !kTwo) {
-        for (int t = t0; t < t1; ++t) {
-            w.first_half(s_buf, p_buf, nullptr, p, 32 * t, v0, active);
-            __syncthreads();
-            if (t + 1 < t1) xe_stage<Wave::kSChunks>(g.passed + (t + 1) * kSBytes, s_buf);
-            xe_staged();
-        }
-    } else if constexpr (USE == kXeLoss) {
+    if constexpr (USE == kXeLoss) {
         for (int t = t0; t < t1; t += 2) {
             w.first_half(s_buf, p_buf, t + 1 < t1 ? g.passed + (t + 1) * kSBytes : nullptr, p, 32 * t, v0, active);
             xe_staged();
@@ -644,6 +728,11 @@ __global__ __launch_bounds__(kBlock, xe_waves(DB, PARTS, USE, WIDE)) void xe_ker
 
     w.sum += xe_other_half(w.sum);
     w.own += xe_other_half(w.own);
+    if constexpr (PARTS == 2) {
+        if constexpr (USE != kXeWeights) w.sum *= 1.0f / (1 << (int)kXeRise);
+        if constexpr (USE == kXeLossAndRows) w.rescale(1.0f / (1 << (int)kXeRise) / g.scales[1]);
+        if constexpr (USE == kXeWeights) w.rescale(w.top / (1 << kXeTop) / g.scales[0]);
+    }
     if (USE == kXeWeights && t1 - t0 == plan.tiles) {
         xe_store_weights<USE == kXeWeights ? DB : 1>(g, w.o, v0 + lane % 32, slice, w.sum);
         continue;
@@ -967,7 +1056,7 @@ struct XeState {
     char *rows_s, *rows_p, *classes_s;  // (weights' gradient)
     XeRow* kept;
     float* d_x;
-    float* count;
+    float *count, *scales;
     size_t bytes;
 };
 
@@ -975,7 +1064,8 @@ inline XeState xe_state(const XeProblem& p, int want, void* base)
 {
     Carver c(base);
     XeState s = {};
-    s.count = c.take<float>(1);
+    s.scales = c.take<float>(4);
+    s.count = s.scales + 2;
     if (want != 0) s.kept = c.take<XeRow>((size_t)p.n);
     if (want & FGL_XENT_ROWS) s.d_x = c.take<float>((size_t)p.n * p.shape.cols());
     if (want & FGL_XENT_WEIGHTS) {
@@ -989,7 +1079,7 @@ inline XeState xe_state(const XeProblem& p, int want, void* base)
 
 struct XeScratch {
     char *rows_s, *classes_s, *classes_p;
-    float *stats, *part, *tile_loss;
+    float *stats, *part, *tile_loss, *most;
     size_t bytes;
 };
 
@@ -1009,6 +1099,7 @@ inline XeScratch xe_forward_scratch(const XeProblem& p, int want, void* base)
     }
     s.stats = c.take<float>((size_t)plan.slots() * kXeWaves * 32 * 4);
     s.tile_loss = c.take<float>((size_t)p.row_tiles * 2);
+    s.most = c.take<float>(2 * kBlock);
     s.bytes = c.used();
     return s;
 }
@@ -1056,7 +1147,7 @@ int launch_xe(const XeShape& s, XeArgs& g, int passed_tiles, hipStream_t stream)
         set_error("linear_cross_entropy: grid too large");
         return FGL_ERR_UNSUPPORTED;
     }
-    if (s.parts == 3) launch_xe_parts<3, USE>(s, g, (unsigned)workgroups, stream);
+    if (s.parts == 2) launch_xe_parts<2, USE>(s, g, (unsigned)workgroups, stream);
     else launch_xe_parts<1, USE>(s, g, (unsigned)workgroups, stream);
     return FGL_OK;
 }
@@ -1110,8 +1201,15 @@ FGL_EXPORT int fgl_linear_cross_entropy(const void* d_x, int64_t x_row_stride, i
     const int64_t tiles = (int64_t)p.row_tiles + p.class_tiles;
     FGL_REQUIRE(tiles < 1 << 24, "linear_cross_entropy: grid too large");
     const dim3 grid((unsigned)tiles, (unsigned)ceil_div(s.cols(), kXeCols)), block(kBlock);
-    if (dtype == FGL_F32) hipLaunchKernelGGL((xe_images_kernel<float, 3>), grid, block, 0, to, im);
-    else hipLaunchKernelGGL((xe_images_kernel<__bf16, 1>), grid, block, 0, to, im);
+    im.most = ws.most;
+    im.scales = st.scales;
+    if (dtype == FGL_F32) {
+        hipLaunchKernelGGL(xe_most_kernel, dim3(kBlock, 2), block, 0, to, im.m[0], im.m[1], dim, ws.most);
+        FGL_CHECK_LAUNCH("xe_most_kernel");
+        hipLaunchKernelGGL((xe_images_kernel<float, 2>), grid, block, 0, to, im);
+    } else {
+        hipLaunchKernelGGL((xe_images_kernel<__bf16, 1>), grid, block, 0, to, im);
+    }
     FGL_CHECK_LAUNCH("xe_images_kernel");
 
     XeArgs g = {};
@@ -1121,6 +1219,7 @@ FGL_EXPORT int fgl_linear_cross_entropy(const void* d_x, int64_t x_row_stride, i
     g.kept_tiles = p.row_tiles;
     g.stats = ws.stats;
     g.part = ws.part;
+    g.scales = st.scales;
     const int rc = want & FGL_XENT_ROWS ? launch_xe<kXeLossAndRows>(s, g, p.class_tiles, to) : launch_xe<kXeLoss>(s, g, p.class_tiles, to);
     if (rc != FGL_OK) return rc;
     FGL_CHECK_LAUNCH("xe_kernel");
@@ -1196,6 +1295,7 @@ FGL_EXPORT int fgl_linear_cross_entropy_backward(const float* d_loss_grad, int64
     g.kept_tiles = p.class_tiles;
     g.stats = ws.stats;
     g.part = ws.part;
+    g.scales = st.scales;
     g.d_w = d_dw;
     g.d_b = d_db;
     g.kept_rows = n_classes;

@@ -1,11 +1,14 @@
 """fastgl.linear_cross_entropy against the definition in float64.
 
-Tolerances.  Let u = 2^-24 (fp32) and L the largest sum of magnitudes sum_d |x_id w_vd| + |b_v| of a row.  A logit is off by at most c u L
-with c = 3 + d / 32 (three-part products are exact to 2^-24 of each term; one addition for every 32 columns), in bf16, whose products
-are exact and are added up one instruction of 16 columns after another, with c = 2 + d / 16; the exponentials by 2 u and u times their
-argument in powers of two, at most 2 L log2(e), more.  So a share p is off by eps = 4 u (c + 4) (L + 4) of itself and a loss by eps, and a
-sum of n shares adds at most log-many roundings by tiles and one for each tile: (n / 32 + 8) u.  Gradients are sums of p (bf16: rounded, 2^-8 more)
-times finite values: their error is at most that share of the sum of the terms' magnitudes, plus half a step of the result."""
+Tolerances.  Let u = 2^-24 and M the largest sum of magnitudes sum_d |x_id w_vd| + |b_v| of a row.  bf16: products are exact, and added up one
+instruction of 16 columns after another: a logit is off by at most c u M, c = 2 + d / 16.  fp32: a value is taken as the sum of two fp16 values, off by
+2^-22 of it (half a step of the second, 2^-11, times 2^-11 for the first), and the product of the two second parts, 2^-22, is left out: 3 * 2^-22 = 12 u of
+each product; sums of 64 columns are added up: c = 14 + d / 64 + 64 / 16.  A value whose scaled second part is below fp16's normal numbers is off by
+2^-25 of 2^-14 times the matrix's largest: 2^-39 of it, once for either factor: 2^-38 d max|x| max|w| more.  The exponentials are off by 2 u and by u
+times their argument in powers of two, at most 2 M log2(e), more.  So a share p is off by eps = 4 u (c + 4) (M + 4) of itself and a loss by eps, and a sum
+of n shares adds one rounding for each tile of 32 and log-many: (n / 32 + 8) u.  Gradients are sums of p times finite values: bf16: p is
+rounded, 2^-8 more of each term; fp32: 3 * 2^-22 more, and as p is scaled by its row's largest, or by sixteen times that, 2^-25 of 2^-14 of those:
+2^-35 of the largest term's p, times the largest value, for each term.  At last half a step of the result."""
 import pytest
 import torch
 
@@ -36,7 +39,10 @@ def definition(x, w, b, y, ignore, reduction, g):
     d[rows, label] = torch.expm1(-own)
     d *= torch.where(valid, g.double() / (count if reduction == "mean" else 1), 0.0)[:, None] if reduction != "none" else torch.where(valid, g.double(), 0.0)[:, None]
     d[~valid] = 0.0
-    return (losses, loss, d @ w, d.t() @ x, d.sum(0)), (d.abs() @ w.abs(), d.abs().t() @ x.abs(), d.abs().sum(0))
+    # of the gradients' terms: the sums of their magnitudes, and the largest of a row times the largest value that p meets
+    sums = d.abs() @ w.abs(), d.abs().t() @ x.abs(), d.abs().sum(0)
+    largest = (d.abs().amax(1)[:, None] * w.abs().max(), d.abs().amax(0)[:, None] * x.abs().max(), 0.0) if min(d.shape) else (0.0, 0.0, 0.0)
+    return (losses, loss, d @ w, d.t() @ x, d.sum(0)), sums, largest
 
 
 def share_error(x, w, b, n_terms):
@@ -45,8 +51,9 @@ def share_error(x, w, b, n_terms):
     most = max(float((x.detach().abs().double() @ w.detach()[k:k + 4096].abs().double().t()).max()) for k in range(0, w.size(0), 4096))
     if b is not None:
         most += float(b.detach().double().abs().masked_fill(b.detach().isinf(), 0.0).max())
-    c = 3 + d / 32 if x.dtype == torch.float32 else 2 + d / 16
-    return 4 * u * (c + 4) * (most + 4) + (n_terms / 32 + 8) * u
+    c = 18 + d / 64 if x.dtype == torch.float32 else 2 + d / 16
+    scaled = 2.0 ** -38 * d * float(x.detach().abs().max()) * float(w.detach().abs().max()) if x.dtype == torch.float32 else 0.0
+    return 4 * u * (c + 4) * (most + 4) + (n_terms / 32 + 8) * u + 4 * scaled
 
 
 def check(x, w, b, y, reduction="mean", ignore=-100, g=None, limit_scale=1.0):
@@ -58,16 +65,17 @@ def check(x, w, b, y, reduction="mean", ignore=-100, g=None, limit_scale=1.0):
     loss = fastgl.linear_cross_entropy(leaves[0], leaves[1], y, leaves[2] if b is not None else None, ignore, reduction)
     assert loss.dtype == torch.float32 and loss.shape == ((n,) if reduction == "none" else ())
     grads = torch.autograd.grad(loss, leaves, g)
-    (losses, want, *want_grads), sums = definition(x, w, b, y, ignore, reduction, g)
+    (losses, want, *want_grads), sums, largest = definition(x, w, b, y, ignore, reduction, g)
     eps = share_error(x, w, b, w.size(0))
     loss_limit = eps * (1 + losses) if reduction == "none" else eps * (1 + losses.max()) * (n if reduction == "sum" else 1)
     assert ((loss.detach().double() - want).abs() <= loss_limit).all(), float((loss.detach().double() - want).abs().max())
     half = HALF[x.dtype]
-    for name, got, exact, total in zip(("dx", "dw", "db"), grads, want_grads, sums):
+    for name, got, exact, total, most in zip(("dx", "dw", "db"), grads, want_grads, sums, largest):
         assert got.dtype == x.dtype and got.shape == exact.shape
         terms = n if name != "dx" else w.size(0)
-        # (the maximum's factor, up to 2^8, is the same for all of a row's terms; bf16: dx holds one more term, rounded with w)
-        limit = (2 * eps + (terms / 32 + 16) * 2.0 ** -24 + (half if x.dtype == torch.bfloat16 else 0.0)) * total + half * exact.abs() + 2.0 ** -120
+        limit = (2 * eps + (terms / 32 + 16) * 2.0 ** -24 + (half if x.dtype == torch.bfloat16 else 12 * half)) * total + half * exact.abs() + 2.0 ** -120
+        if x.dtype == torch.float32:
+            limit = limit + terms * 2.0 ** -35 * most
         off = (got.double() - exact).abs()
         assert (off <= limit).all(), (name, float((off / limit).max()))
     with torch.no_grad():  # nobody records: the loss alone
@@ -162,12 +170,12 @@ def test_rows_certain_of_their_label_keep_their_bits(cuda, dtype):
     losses = fastgl.linear_cross_entropy(leaves[0], leaves[1], y, reduction="none")
     g = torch.ones(64, device=cuda)
     dx, = torch.autograd.grad(losses, leaves[:1], g)
-    (exact, _, want, _, _), (total, _, _) = definition(x, w, None, y, -100, "none", g)
+    (exact, _, want, _, _), (total, _, _), (largest, _, _) = definition(x, w, None, y, -100, "none", g)
     eps = share_error(x, w, None, 40)
     small = exact < 1e-3
     assert int(small.sum()) > 8
     assert ((losses.detach().double() - exact).abs()[small] <= 3 * eps * exact[small]).all()
-    assert ((dx.double() - want).abs()[small] <= (3 * eps + 2 * HALF[dtype]) * total[small] + HALF[dtype] * want.abs()[small] + 2.0 ** -120).all()
+    assert ((dx.double() - want).abs()[small] <= (3 * eps + (2 if dtype == torch.bfloat16 else 14) * HALF[dtype]) * total[small] + HALF[dtype] * want.abs()[small] + 40 * 2.0 ** -35 * largest[small] + 2.0 ** -120).all()
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
@@ -185,11 +193,11 @@ def test_masked_classes(cuda, dtype, lowest):
     kept = (~off).nonzero()[:, 0]
     names = torch.full((300,), -1, device=cuda, dtype=torch.int64)
     names[kept] = torch.arange(kept.numel(), device=cuda)
-    (_, want, dx, dw, db), (tx, tw, tb) = definition(x, w[kept], b[kept], names[y], -100, "mean", torch.ones((), device=cuda))
+    (_, want, dx, dw, db), (tx, tw, tb), largest = definition(x, w[kept], b[kept], names[y], -100, "mean", torch.ones((), device=cuda))
     eps = share_error(x, w[kept], b[kept], 300)
     assert abs(float(loss.detach()) - float(want)) <= eps * (1 + 2 * float(want) + 8)
-    for got, exact, total in ((grads[0], dx, tx), (grads[1][kept], dw, tw), (grads[2][kept], db, tb)):
-        assert ((got.double() - exact).abs() <= (2 * eps + 2 * HALF[dtype]) * total + HALF[dtype] * exact.abs() + 1e-30).all()
+    for got, exact, total, most in zip((grads[0], grads[1][kept], grads[2][kept]), (dx, dw, db), (tx, tw, tb), largest):
+        assert ((got.double() - exact).abs() <= (2 * eps + (2 if dtype == torch.bfloat16 else 14) * HALF[dtype]) * total + HALF[dtype] * exact.abs() + 300 * 2.0 ** -35 * most + 1e-30).all()
     assert (grads[1][off] == 0).all() and (grads[2][off] == 0).all()
     # a label that is left out
     y2 = y.clone()
