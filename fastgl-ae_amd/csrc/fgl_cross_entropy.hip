@@ -26,8 +26,8 @@
 // left out is 2^-22 of it), whose sum over 64 k is added to fp32 accumulators.  fp16's range is short, so x and w are first multiplied by a power of two
 // that takes their largest value to 2^14 (xe_most_kernel); what lies 2^39 below it is lost, which is nothing beside the logits and sums that it would
 // go into.  P is scaled likewise, by the running maximum, and the gradient of the logits by a running bound of its own.  Against 64 bits, 2-norm,
-// 8192 x 128 and 20 K classes: @ERR@; the same in fp32 products by the library 1.7e-6, in three bf16 parts and six instructions 1.9e-7, in
-// @SIX@ of the time.
+// 8192 x 128 and 20 K classes: 2.2e-7; the same in fp32 products by the library 1.7e-6, in three bf16 parts and six instructions 1.9e-7, in
+// 1.6 times the time.
 // Sums, maxima and losses are fp32 in both.  x and w must be finite, in fp32 below 2^74: others make losses and gradients that are not numbers.
 // A bias of -1e30 or less, -infinity among them, leaves its class out: no share, no gradient.  (Shares are exp2 of one fma, whose
 // product with log2 e is not rounded where the maximum's is: logits up to some 1e9 are no matter, the difference of 2^-25 of the maximum is the
@@ -41,6 +41,8 @@
 #include "fgl_kernels.hpp"
 
 #include <math.h>
+
+#include <type_traits>
 
 namespace fgl {
 
@@ -343,7 +345,6 @@ struct XeArgs {
     void* d_b;
     int64_t kept_rows;
     int dim;
-    int bf16;
 };
 
 // The value that the lane with the same kept row in the wave's other half has.
@@ -391,8 +392,8 @@ __device__ __forceinline__ XeF32x16 xe_mfma(const XeOp& a, const XeOp& b, const 
 template <int N, int PARTS, typename At, typename Use>
 __device__ __forceinline__ void xe_products(const At& at, const Use& use)
 {
-    constexpr int kMost = PARTS == 1 ? 4 : 2, kAhead = N < kMost ? N : kMost;
-    XeOp a[kAhead + 1][PARTS];
+    constexpr int kMost = PARTS == 1 ? 4 : 3, kAhead = N < kMost ? N : kMost;
+    XeOp a[kAhead][PARTS];
 #pragma unroll
     for (int i = 0; i < kAhead; ++i)
 #pragma unroll
@@ -400,10 +401,10 @@ __device__ __forceinline__ void xe_products(const At& at, const Use& use)
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
+        use(i, a[i % kAhead]);
 #pragma unroll
         for (int p = 0; p < PARTS; ++p)
-            if (i + kAhead < N) a[(i + kAhead) % (kAhead + 1)][p] = xe_operand(at(i + kAhead) + p * kXeChunk);
-        use(i, a[i % (kAhead + 1)]);
+            if (i + kAhead < N) a[i % kAhead][p] = xe_operand(at(i + kAhead) + p * kXeChunk);
         __builtin_amdgcn_sched_barrier(0);
     }
 }
@@ -425,7 +426,7 @@ struct XeWave {
 
     XeOp kept[kSteps][PARTS];
     XeF32x16 o[USE == kXeLoss ? 1 : DB];
-    XeF32x16 start;       // weights: the class's bias sixteen times
+    float start;          // weights: the class's bias
     float unit;           // what S is to be multiplied by (fp32: its operands are scaled)
     float top, sum, own;  // running maximum (a power of two; weights, fp32: what P is below, a power of two itself), sum, the label's logit
     int label;            // weights: the class
@@ -436,7 +437,8 @@ struct XeWave {
     {
         XeF32x16 acc;
         if constexpr (USE == kXeWeights) {
-            acc = start;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[i] = start;
         } else {
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
@@ -527,10 +529,13 @@ struct XeWave {
         }
         const int in_tile = l[kXeLabel + lane_id() % 32] - v0;
         if (__any(in_tile >= 0 && in_tile < 32)) {
+            typedef int I4 __attribute__((ext_vector_type(4)));
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int n = 8 * (i / 4) + first + i % 4;
-                if (l[kXeLabel + n] == label) s[i] = c[kXeOwn + n];
+            for (int q = 0; q < 4; ++q) {
+                const I4 labels = *reinterpret_cast<const I4*>(l + kXeLabel + 8 * q + first);
+                const XeF4 values = *reinterpret_cast<const XeF4*>(c + kXeOwn + 8 * q + first);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) s[4 * q + j] = labels[j] == label ? values[j] : s[4 * q + j];
             }
         }
         if (bias_sum) add_up(s);
@@ -599,48 +604,39 @@ struct XeWave {
     }
 };
 
-// Four neighbouring columns of a result's row.
-__device__ __forceinline__ void xe_store4(void* out, bool bf16, int64_t row, int col, int dim, const XeF4& v)
+// Four neighbouring columns of a result's row, as far as it has them; as one where all rows have whole fours.
+template <typename T>
+__device__ __forceinline__ void xe_store4(T* row, int col, int dim, const XeF4& v)
 {
-    const int64_t to = row * dim + col;
-    if (bf16) {
-        typedef __bf16 Vec __attribute__((ext_vector_type(4), aligned(2)));
-        __bf16* p = static_cast<__bf16*>(out) + to;
-        if (col + 4 <= dim) {
-            *reinterpret_cast<Vec*>(p) = Vec{(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
-        } else {
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-                if (col + c < dim) p[c] = (__bf16)v[c];
-        }
+    typedef T Vec __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+    if (dim % 4 == 0) {
+        if (col < dim) *reinterpret_cast<Vec*>(row + col) = Vec{(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
     } else {
-        typedef float Vec __attribute__((ext_vector_type(4), aligned(4)));
-        float* p = static_cast<float*>(out) + to;
-        if (col + 4 <= dim) {
-            *reinterpret_cast<Vec*>(p) = Vec{v[0], v[1], v[2], v[3]};
-        } else {
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
-                if (col + c < dim) p[c] = v[c];
-        }
+        for (int c = 0; c < 4; ++c)
+            if (col + c < dim) row[col + c] = (T)v[c];
     }
 }
+__device__ __forceinline__ void xe_store4(void* out, bool bf16, int64_t row, int col, int dim, const XeF4& v)
+{
+    if (bf16) xe_store4(static_cast<__bf16*>(out) + row * dim, col, dim, v);
+    else xe_store4(static_cast<float*>(out) + row * dim, col, dim, v);
+}
 
-template <int DB, int N>
-__device__ __forceinline__ void xe_store_weights(const XeArgs& g, const XeF32x16 (&o)[N], int64_t row, int slice, float sum)
+// What a lane has of a class's gradients, the class a group's alone.
+template <typename T, int DB>
+__device__ __forceinline__ void xe_store_weights(const XeArgs& g, const XeF32x16 (&o)[DB], int64_t row, int slice, float sum)
 {
     if (row >= g.kept_rows) return;
     int half = lane_id() / 32;
     asm volatile("" : "+v"(half));  // (else what the columns make of it is kept in registers through all tiles)
-    if (g.d_b != nullptr && half == 0 && slice == 0) {
-        if (g.bf16) static_cast<__bf16*>(g.d_b)[row] = (__bf16)sum;
-        else static_cast<float*>(g.d_b)[row] = sum;
-    }
+    if (g.d_b != nullptr && half == 0 && slice == 0) static_cast<T*>(g.d_b)[row] = (T)sum;
+    T* to = static_cast<T*>(g.d_w) + row * g.dim;
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
         for (int q = 0; q < 4; ++q)
-            xe_store4(g.d_w, g.bf16 != 0, row, 32 * (slice * DB + d) + 8 * q + 4 * half, g.dim, XeF4{o[d][4 * q], o[d][4 * q + 1], o[d][4 * q + 2], o[d][4 * q + 3]});
+            xe_store4(to, 32 * (slice * DB + d) + 8 * q + 4 * half, g.dim, XeF4{o[d][4 * q], o[d][4 * q + 1], o[d][4 * q + 2], o[d][4 * q + 3]});
 }
 
 template <int DB, int PARTS, int USE, bool WIDE>
@@ -696,9 +692,7 @@ __global__ __launch_bounds__(kBlock, xe_waves(DB, PARTS, USE, WIDE)) void xe_ker
     w.bias_sum = g.d_b != nullptr;
     if constexpr (USE == kXeWeights) {
         w.label = 32 * tile + lane % 32;
-        const float b = reinterpret_cast<const XeGlobal<const float>*>(own)[lane % 32];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) w.start[i] = b;
+        w.start = reinterpret_cast<const XeGlobal<const float>*>(own)[lane % 32];
     } else {
         w.label = reinterpret_cast<const XeGlobal<const int>*>(own)[kXeLabel + lane % 32];
     }
@@ -733,9 +727,11 @@ __global__ __launch_bounds__(kBlock, xe_waves(DB, PARTS, USE, WIDE)) void xe_ker
         if constexpr (USE == kXeLossAndRows) w.rescale(1.0f / (1 << (int)kXeRise) / g.scales[1]);
         if constexpr (USE == kXeWeights) w.rescale(w.top / (1 << kXeTop) / g.scales[0]);
     }
-    if (USE == kXeWeights && t1 - t0 == plan.tiles) {
-        xe_store_weights<USE == kXeWeights ? DB : 1>(g, w.o, v0 + lane % 32, slice, w.sum);
-        continue;
+    if constexpr (USE == kXeWeights) {
+        if (t1 - t0 == plan.tiles) {
+            xe_store_weights<typename std::conditional<PARTS == 1, __bf16, float>::type>(g, w.o, v0 + lane % 32, slice, w.sum);
+            continue;
+        }
     }
     const int64_t place = (int64_t)plan.slot(workgroup, group) * kXeWaves + wave;
     if (lane < 32) {  // (of either slice: they are cut in other places)
@@ -1300,7 +1296,6 @@ FGL_EXPORT int fgl_linear_cross_entropy_backward(const float* d_loss_grad, int64
     g.d_b = d_db;
     g.kept_rows = n_classes;
     g.dim = dim;
-    g.bf16 = dtype == FGL_BF16;
     const int rc = launch_xe<kXeWeights>(s, g, p.row_tiles, to);
     if (rc != FGL_OK) return rc;
     FGL_CHECK_LAUNCH("xe_kernel");
@@ -1313,7 +1308,7 @@ FGL_EXPORT int fgl_linear_cross_entropy_backward(const float* d_loss_grad, int64
         c.blocks = s.blocks;
         c.slices = s.slices;
         c.dim = dim;
-        c.bf16 = g.bf16;
+        c.bf16 = dtype == FGL_BF16;
         c.d_w = d_dw;
         c.d_b = d_db;
         const bool together = g.plan.shared > 8;
