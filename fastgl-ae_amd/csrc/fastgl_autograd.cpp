@@ -172,9 +172,11 @@ struct LossNode : torch::autograd::Function<LossNode> {
             if (need_b) d_b = make({classes});
             if (n > 0 && (need_x || need_w || need_b)) {
                 const Tensor d_loss = grads[0].contiguous();
-                Tensor ws = bytes_like(state, fgl_linear_cross_entropy_workspace_bytes(n, classes, (int)dim, dtype, want, 1));
+                const size_t ws_bytes = fgl_linear_cross_entropy_workspace_bytes(n, classes, (int)dim, dtype, want, 1);
+                Tensor ws;
+                if (ws_bytes > 0) ws = bytes_like(state, ws_bytes);
                 ok(fgl_linear_cross_entropy_backward(d_loss.data_ptr<float>(), n, classes, (int)dim, dtype, reduction, want, state.data_ptr(), (size_t)state.numel(),
-                                                     address(d_x), address(d_w), address(d_b), ws.data_ptr(), (size_t)ws.numel(), stream_of(state)));
+                                                     address(d_x), address(d_w), address(d_b), address(ws), ws_bytes, stream_of(state)));
             }
         }
         if (!need_w) d_w = Tensor();

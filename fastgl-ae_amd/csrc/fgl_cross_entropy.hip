@@ -107,8 +107,9 @@ struct XeImagesArgs {
     int label64;
     int64_t ignore;
     int64_t classes;
-    const float* most;  // fp32: [2][kBlock], the largest magnitudes of parts of the matrices (xe_most_kernel)
+    const float* most;  // fp32: [2][kBlock], the largest magnitudes of parts of the matrices (xe_most_kernel), or null: they are looked for here
     float* scales;      // fp32: the powers of two that the matrices are multiplied by
+    int* done;          // cleared: workgroups of xe_combine_kernel that have left their tile's loss
 };
 
 constexpr int kXeCols = 128;  // columns that a workgroup lays out, of 32 rows
@@ -162,19 +163,17 @@ __device__ __forceinline__ float xe_block_max(float v, float* shared)
     return v;
 }
 
-// Workgroup (i, m) of kBlock x 2: the largest magnitude of part i of matrix m (what is not a number is passed over).
-__global__ __launch_bounds__(kBlock) void xe_most_kernel(const XeMatrix m0, const XeMatrix m1, int dim, float* __restrict__ most)
+// The largest magnitude of what worker `worker` of `workers` (waves) has of a matrix (what is not a number is passed over).
+__device__ __forceinline__ float xe_most(const XeMatrix& m, int dim, int worker, int workers)
 {
-    __shared__ float shared[kXeWaves];
-    const XeMatrix& m = blockIdx.y == 0 ? m0 : m1;
     const float* src = static_cast<const float*>(m.src);
     float v = 0.0f;
-    // a wave takes 1024 values of a line at a time: of a row, or of a column where those lie side by side, or of all rows if there is no gap between them
+    // 1024 values of a line at a time: of a row, or of a column where those lie side by side, or of all rows if there is no gap between them
     const bool rows = m.col_stride == 1, one = rows && m.row_stride == dim;
     const int64_t lines = one ? 1 : rows ? m.rows : dim, length = one ? m.rows * dim : rows ? dim : m.rows;
     const int64_t step = rows ? m.row_stride : m.col_stride, unit = rows ? 1 : m.row_stride, each = (length + 1023) / 1024;
     const int lane = lane_id();
-    for (int64_t k = (int64_t)blockIdx.x * kXeWaves + threadIdx.x / kWave; k < lines * each; k += (int64_t)gridDim.x * kXeWaves) {
+    for (int64_t k = worker; k < lines * each; k += workers) {
         const int64_t line = k / each, first = (k - line * each) * 1024;
         const float* p = src + line * step;
         if (unit == 1 && first + 1024 <= length) {
@@ -190,7 +189,15 @@ __global__ __launch_bounds__(kBlock) void xe_most_kernel(const XeMatrix m0, cons
             for (int64_t c = first + lane; c < end; c += kWave) v = fmaxf(v, fabsf(p[c * unit]));
         }
     }
-    v = xe_block_max(v, shared);
+    return v;
+}
+
+// Workgroup (i, m) of kBlock x 2: part i of matrix m.
+__global__ __launch_bounds__(kBlock) void xe_most_kernel(const XeMatrix m0, const XeMatrix m1, int dim, float* __restrict__ most)
+{
+    __shared__ float shared[kXeWaves];
+    const int wave = (int)(threadIdx.x / kWave);
+    const float v = xe_block_max(xe_most(blockIdx.y == 0 ? m0 : m1, dim, (int)blockIdx.x * kXeWaves + wave, kBlock * kXeWaves), shared);
     if (threadIdx.x == 0) most[blockIdx.y * kBlock + blockIdx.x] = v;
 }
 
@@ -216,14 +223,23 @@ __global__ __launch_bounds__(kBlock) void xe_images_kernel(const XeImagesArgs g)
     float scale_x = 1.0f, scale_w = 1.0f;
     if constexpr (PARTS == 2) {
         __shared__ float shared[2][kXeWaves];
-        scale_x = xe_scale(xe_block_max(g.most[thread], shared[0]));
-        scale_w = xe_scale(xe_block_max(g.most[kBlock + thread], shared[1]));
+        float most_x, most_w;
+        if (g.most != nullptr) {
+            most_x = g.most[thread];
+            most_w = g.most[kBlock + thread];
+        } else {
+            most_x = xe_most(g.m[0], g.dim, thread / kWave, kXeWaves);
+            most_w = xe_most(g.m[1], g.dim, thread / kWave, kXeWaves);
+        }
+        scale_x = xe_scale(xe_block_max(most_x, shared[0]));
+        scale_w = xe_scale(xe_block_max(most_w, shared[1]));
         if (id == 0 && blockIdx.y == 0 && thread == 0) {
             g.scales[0] = scale_x;
             g.scales[1] = scale_w;
         }
     }
     const float scale = classes ? scale_w : scale_x;
+    if (id == 0 && blockIdx.y == 0 && thread == 0) *g.done = 0;
     if (m.col_stride == 1) {
         typedef T Vec __attribute__((ext_vector_type(8), aligned(sizeof(T))));
 #pragma unroll
@@ -331,6 +347,17 @@ __device__ __forceinline__ XeGlobal<T>* xe_uniform(T* p)
     return q;
 }
 
+// The loss's gradient for all rows, where it is the same for all: of a sum, or of a mean over the rows that have a label.
+struct XeFactor {
+    const float* d_loss;  // null: rows have one each, which is in their factors
+    const float* count;   // or null
+    __device__ __forceinline__ float value() const
+    {
+        if (d_loss == nullptr) return 1.0f;
+        return count == nullptr ? *d_loss : *count > 0.0f ? *d_loss / *count : 0.0f;  // (no labels at all: no gradients)
+    }
+};
+
 struct XeArgs {
     XePlan plan;
     const char* kept;      // S images
@@ -340,6 +367,7 @@ struct XeArgs {
     float* stats;  // [slot][wave][row of 32]: maximum, others' sum, label's logit, -  (weights: sum, -, -, -)
     float* part;   // [slot][wave][block][quarter][lane][4]
     const float* scales;  // fp32: of rows and classes
+    XeFactor factor;      // weights: of all results
     // weights of groups that one workgroup has alone: straight to the result
     void* d_w;
     void* d_b;
@@ -628,15 +656,17 @@ template <typename T, int DB>
 __device__ __forceinline__ void xe_store_weights(const XeArgs& g, const XeF32x16 (&o)[DB], int64_t row, int slice, float sum)
 {
     if (row >= g.kept_rows) return;
+    const float f = g.factor.value();
     int half = lane_id() / 32;
     asm volatile("" : "+v"(half));  // (else what the columns make of it is kept in registers through all tiles)
-    if (g.d_b != nullptr && half == 0 && slice == 0) static_cast<T*>(g.d_b)[row] = (T)sum;
+    if (g.d_b != nullptr && half == 0 && slice == 0) static_cast<T*>(g.d_b)[row] = (T)(sum * f);
     T* to = static_cast<T*>(g.d_w) + row * g.dim;
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
         for (int q = 0; q < 4; ++q)
-            xe_store4(to, 32 * (slice * DB + d) + 8 * q + 4 * half, g.dim, XeF4{o[d][4 * q], o[d][4 * q + 1], o[d][4 * q + 2], o[d][4 * q + 3]});
+            xe_store4(to, 32 * (slice * DB + d) + 8 * q + 4 * half, g.dim,
+                      XeF4{o[d][4 * q] * f, o[d][4 * q + 1] * f, o[d][4 * q + 2] * f, o[d][4 * q + 3] * f});
 }
 
 template <int DB, int PARTS, int USE, bool WIDE>
@@ -761,36 +791,88 @@ struct XeCombineArgs {
     XePlan plan;
     const float* stats;
     const float* part;
-    const char* rows;  // S image of the rows (labels)
+    char* rows;  // S image of the rows: their labels; what the weights' gradient needs of them goes there
     int64_t n_rows, s_bytes;
     int blocks, slices;
     const void* w;  // classes
     int64_t w_row, w_col;
     int dim, bf16;
     float* losses;     // a row each, or null
-    float* tile_loss;  // [tile][2]: sum, count
-    XeRow* kept;       // or null
-    float* d_x;        // [row][padded columns], up to its factor, or null
+    float* tile_loss;  // [tile][2]: sum, count; or null
+    int tiles, mean;
+    int* done;
+    float *loss, *count;
+    XeRow* kept;  // or null
+    int weights;  // whether their gradient is wanted
+    float* d_x;   // [row][padded columns], up to its factor, or null
 };
 
+// The tiles' losses -> the loss, and the rows that have a label.  By the last workgroup that left one, in their order.
+__device__ __forceinline__ void xe_total(const XeCombineArgs& g, double (&sums)[2][kXeWaves])
+{
+    double sum = 0.0, n = 0.0;
+    for (int t = (int)threadIdx.x; t < g.tiles; t += kBlock) {
+        sum += (double)__hip_atomic_load(g.tile_loss + 2 * t, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        n += (double)__hip_atomic_load(g.tile_loss + 2 * t + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+#pragma unroll
+    for (int d = kWave / 2; d >= 1; d >>= 1) {
+        sum += __shfl_xor(sum, d, kWave);
+        n += __shfl_xor(n, d, kWave);
+    }
+    if (lane_id() == 0) {
+        sums[0][threadIdx.x / kWave] = sum;
+        sums[1][threadIdx.x / kWave] = n;
+    }
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+#pragma unroll
+    for (int k = 1; k < kXeWaves; ++k) {
+        sum += sums[0][k];
+        n += sums[1][k];
+    }
+    *g.loss = (float)(g.mean ? sum / n : sum);  // (no labels at all: not a number, as the mean of nothing is)
+    *g.count = (float)n;
+}
+
 // One workgroup a tile of 32 rows and block of 32 columns.  Each forms the rows' sums from their parts (a row eight threads), the first of
-// a tile's keeps them; then a wave takes eight columns.
+// a tile's keeps them; then a wave takes eight columns.  What it needs from memory is asked for at once, at the start: the time of such a
+// launch is that of a few reads one after another.
 __global__ __launch_bounds__(kBlock) void xe_combine_kernel(const XeCombineArgs g)
 {
-    constexpr int kEach = kBlock / 32;
+    constexpr int kEach = kBlock / 32, kFirst = 4;
     __shared__ float scale[kXeMaxParts * 32];
     __shared__ float top_of[kEach][32], own_of[kEach][32], rest_of[kEach][32];
-    __shared__ float others[32];
-    __shared__ int labels[32];
+    __shared__ double totals[2][kXeWaves];
+    __shared__ int last;
     const int tile = (int)blockIdx.x, block = (int)blockIdx.y, group = tile / kXeWaves * g.slices + block / g.blocks;
     const int64_t row0 = 32LL * tile;
-    const int thread = (int)threadIdx.x, wave = tile % kXeWaves, i = thread % 32, each = thread / 32;
+    const int thread = (int)threadIdx.x, wave = tile % kXeWaves, i = thread % 32, each = thread / 32, lane = thread % kWave;
     const int b0 = g.plan.first(group), parts = g.plan.last(group) - b0 + 1;
-    const XeF4* s = reinterpret_cast<const XeF4*>(g.stats) + ((int64_t)g.plan.slot(b0, group) * kXeWaves + wave) * 32 + i;
-    const bool there = row0 + i < g.n_rows;
-    const int label = reinterpret_cast<const int*>(g.rows + tile * g.s_bytes)[kXeLabel + i];
-    float top = -INFINITY, own = 0.0f;
-    for (int k = each; k < parts; k += kEach) {
+    const int64_t place = (int64_t)g.plan.slot(b0, group) * kXeWaves + wave, step = (int64_t)kXeWaves * g.blocks * 4 * kWave;
+    const XeF4* s = reinterpret_cast<const XeF4*>(g.stats) + place * 32 + i;
+    const XeF4* p = reinterpret_cast<const XeF4*>(g.part) + (place * g.blocks + block % g.blocks) * 4 * kWave + thread;
+    char* own_tile = g.rows + tile * g.s_bytes;
+    const bool there = row0 + i < g.n_rows, with_x = g.d_x != nullptr;
+    const int col = 32 * block + thread / kWave * 8 + lane / 32 * 4;
+    XeF4 mine = {-INFINITY, 0.0f, 0.0f, 0.0f}, first[kFirst];
+    if (each < parts) mine = s[each * kXeWaves * 32];
+    const int label = reinterpret_cast<const int*>(own_tile)[kXeLabel + i];
+    if (with_x) {
+#pragma unroll
+        for (int k = 0; k < kFirst; ++k) first[k] = p[(k < parts ? k : 0) * step];
+    }
+    XeF4 w = {};
+    if (with_x && label >= 0) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            if (col + c >= g.dim) continue;
+            const int64_t from = label * g.w_row + (col + c) * g.w_col;
+            w[c] = g.bf16 ? (float)static_cast<const __bf16*>(g.w)[from] : static_cast<const float*>(g.w)[from];
+        }
+    }
+    float top = mine[0], own = mine[2];
+    for (int k = each + kEach; k < parts; k += kEach) {
         const XeF4 v = s[k * kXeWaves * 32];
         top = fmaxf(top, v[0]);
         own += v[2];
@@ -808,7 +890,7 @@ __global__ __launch_bounds__(kBlock) void xe_combine_kernel(const XeCombineArgs 
     if (label >= 0) top = fmaxf(top, own2);
     float rest = 0.0f;
     for (int k = each; k < parts; k += kEach) {
-        const XeF4 v = s[k * kXeWaves * 32];
+        const XeF4 v = k == each ? mine : s[k * kXeWaves * 32];
         const float f = v[0] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(v[0] - top);
         rest += v[0] == -INFINITY ? v[1] : v[1] * f;  // (what is not a number stays it)
         scale[k * 32 + i] = f;
@@ -818,16 +900,41 @@ __global__ __launch_bounds__(kBlock) void xe_combine_kernel(const XeCombineArgs 
     rest = 0.0f;
 #pragma unroll
     for (int k = 0; k < kEach; ++k) rest += rest_of[k][i];
-    const float mine = label >= 0 ? __builtin_amdgcn_exp2f(own2 - top) : 0.0f;
-    const float total = rest + mine, inverse = 1.0f / total;
-    float share = rest * inverse;
-    if (blockIdx.y == 0 && thread < kWave) {
-        float loss = top - own2 < 64.0f ? log1pf(rest / mine) : kXeLn2 * top + logf(total) - own;
+    const float own_part = label >= 0 ? __builtin_amdgcn_exp2f(own2 - top) : 0.0f;
+    const float total = rest + own_part, inverse = 1.0f / total, others = label == -2 ? NAN : rest * inverse;
+    if (with_x && there) {
+        XeF4 sum = {};
+#pragma unroll
+        for (int k = 0; k < kFirst; ++k) {
+            const float f = k < parts ? scale[k * 32 + i] : 0.0f;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) sum[c] += k < parts ? first[k][c] * f : 0.0f;
+        }
+#pragma unroll 4
+        for (int k = kFirst; k < parts; ++k) {
+            const XeF4 v = p[k * step];
+            const float f = scale[k * 32 + i];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) sum[c] += v[c] * f;
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) sum[c] = label >= 0 || label == -2 ? sum[c] * inverse - others * w[c] : 0.0f;
+        *reinterpret_cast<XeF4*>(g.d_x + (row0 + i) * (32 * g.blocks * g.slices) + col) = sum;
+    }
+    if (block != 0) return;  // (the tile's first workgroup alone keeps what is the rows')
+    if (thread < kWave) {
+        float loss = top - own2 < 64.0f ? log1pf(rest / own_part) : kXeLn2 * top + logf(total) - own;
         if (label == -2) loss = NAN;
         if (label == -1) loss = 0.0f;
-        if (thread < 32 && there) {
-            if (g.losses != nullptr) g.losses[row0 + i] = loss;
-            if (g.kept != nullptr) g.kept[row0 + i] = XeRow{top, inverse, label == -2 ? NAN : share, label};
+        if (thread < 32) {
+            if (there && g.losses != nullptr) g.losses[row0 + i] = loss;
+            if (there && g.kept != nullptr) g.kept[row0 + i] = XeRow{top, inverse, others, label};
+            if (g.weights) {  // (rows without a label and past the end: no share)
+                float* c = reinterpret_cast<float*>(own_tile);
+                c[kXeShift + i] = label == -1 ? -INFINITY : label == -2 ? NAN : -top;
+                c[kXeFactor + i] = label == -1 ? 0.0f : inverse;
+                c[kXeOwn + i] = -others;
+            }
         }
         float sum = there ? loss : 0.0f, count = there && label != -1 ? 1.0f : 0.0f;
 #pragma unroll
@@ -836,131 +943,78 @@ __global__ __launch_bounds__(kBlock) void xe_combine_kernel(const XeCombineArgs 
             count += __shfl_xor(count, d, kWave);
         }
         if (thread == 0 && g.tile_loss != nullptr) {
-            g.tile_loss[2 * tile] = sum;
-            g.tile_loss[2 * tile + 1] = count;
+            __hip_atomic_store(g.tile_loss + 2 * tile, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            __hip_atomic_store(g.tile_loss + 2 * tile + 1, count, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            // The two are where all of the chip sees them once their stores are counted as done; a release would write the L2's other contents back
+            // too, for each tile (8192 rows: 8 us of 19).
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            last = __hip_atomic_fetch_add(g.done, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == g.tiles - 1;
         }
     }
-    if (g.d_x == nullptr) return;
-    for (int k = each; k < parts; k += kEach) scale[k * 32 + i] *= inverse;
-    if (thread < 32) {
-        others[i] = label == -2 ? NAN : share;
-        labels[i] = there ? label : -1;
-    }
+    if (g.tile_loss == nullptr) return;
     __syncthreads();
-    const int cols = 32 * g.blocks * g.slices, lane = thread % kWave;
-    const int col = 32 * block + thread / kWave * 8 + lane / 32 * 4;
-    if (!there) return;
-    const int64_t step = (int64_t)kXeWaves * g.blocks * 4 * kWave;  // of a slot, in fours
-    const XeF4* p = reinterpret_cast<const XeF4*>(g.part) + (int64_t)g.plan.slot(b0, group) * step +
-                    ((int64_t)wave * g.blocks + block % g.blocks) * 4 * kWave + thread;
-    XeF4 sum = {};
-#pragma unroll 4
-    for (int k = 0; k < parts; ++k) {
-        const XeF4 v = p[k * step];
-        const float f = scale[k * 32 + i];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) sum[c] += v[c] * f;
-    }
-    if (labels[i] >= 0) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            if (col + c >= g.dim) continue;
-            const int64_t from = labels[i] * g.w_row + (col + c) * g.w_col;
-            const float v = g.bf16 ? (float)static_cast<const __bf16*>(g.w)[from] : static_cast<const float*>(g.w)[from];
-            sum[c] -= others[i] * v;
-        }
-    }
-    *reinterpret_cast<XeF4*>(g.d_x + (row0 + i) * cols + col) = sum;
+    if (last) xe_total(g, totals);
 }
 
-// the tiles' losses -> *loss; *count: rows with a label
-__global__ __launch_bounds__(kBlock) void xe_total_kernel(const float* __restrict__ tile_loss, int64_t tiles, int mean, float* __restrict__ loss, float* __restrict__ count)
+// Reductions that leave a loss for each row: the rows' factors, of the losses' gradients.
+__global__ __launch_bounds__(kBlock) void xe_factors_kernel(const XeRow* __restrict__ kept, const float* __restrict__ d_loss, int64_t n_rows, char* __restrict__ rows,
+                                                            int64_t s_bytes)
 {
-    __shared__ double s[kBlock], c[kBlock];
-    double sum = 0.0, n = 0.0;
-    for (int64_t t = threadIdx.x; t < tiles; t += kBlock) {
-        sum += (double)tile_loss[2 * t];
-        n += (double)tile_loss[2 * t + 1];
-    }
-    s[threadIdx.x] = sum;
-    c[threadIdx.x] = n;
-    __syncthreads();
-    for (int d = kBlock / 2; d >= 1; d >>= 1) {
-        if ((int)threadIdx.x < d) {
-            s[threadIdx.x] += s[threadIdx.x + d];
-            c[threadIdx.x] += c[threadIdx.x + d];
-        }
-        __syncthreads();
-    }
-    if (threadIdx.x == 0) {
-        *loss = (float)(mean ? s[0] / c[0] : s[0]);  // (no labels at all: not a number, as the mean of nothing is)
-        *count = (float)c[0];
-    }
+    const int64_t row = (int64_t)blockIdx.x * kBlock + threadIdx.x;
+    if (row >= n_rows) return;
+    const XeRow r = kept[row];
+    float* c = reinterpret_cast<float*>(rows + row / 32 * s_bytes) + row % 32;
+    const float f = d_loss[row];
+    c[kXeFactor] = r.label == -1 ? 0.0f : f * r.inverse;
+    c[kXeOwn] = -f * r.others;
 }
 
-struct XeRowsArgs {
+struct XeFinishArgs {
+    // dx (null: not wanted), 32 rows and 32 columns a workgroup, the first dx_groups of them
     const XeRow* kept;
-    const float* d_x;  // or null
-    const float* d_loss;
-    const float* count;
-    int reduction;
-    char* rows;  // S image of the rows, or null: the factors of the weights' gradient
-    int64_t n_rows, s_bytes;
+    const float* d_x;
+    const float* d_loss;  // of a row each, or null
+    XeFactor factor;
+    int64_t n_rows;
     int cols, dim, bf16;
     void* out;
-};
-
-// The factors of a tile's 32 rows, and dx from them, 32 columns a workgroup.
-__global__ __launch_bounds__(kBlock) void xe_rows_kernel(const XeRowsArgs g)
-{
-    __shared__ float factor[32];
-    __shared__ int labels[32];
-    const int64_t tile = blockIdx.x, row0 = 32 * tile;
-    const int thread = (int)threadIdx.x;
-    if (thread < 32) {
-        const bool there = row0 + thread < g.n_rows;
-        const XeRow r = there ? g.kept[row0 + thread] : XeRow{0.0f, 0.0f, 0.0f, -1};
-        float f = 0.0f;
-        if (there) f = g.reduction == FGL_REDUCE_NONE ? g.d_loss[row0 + thread] : g.reduction == FGL_REDUCE_SUM ? *g.d_loss : *g.d_loss / *g.count;
-        const bool with = r.label != -1;
-        factor[thread] = r.label == -2 ? NAN : f;
-        labels[thread] = r.label;
-        if (g.rows != nullptr && blockIdx.y == 0) {
-            float* c = reinterpret_cast<float*>(g.rows + tile * g.s_bytes);
-            c[kXeShift + thread] = with ? (r.label == -2 ? NAN : -r.top) : -INFINITY;
-            c[kXeFactor + thread] = with ? f * r.inverse : 0.0f;
-            c[kXeOwn + thread] = -f * r.others;
-        }
-    }
-    if (g.out == nullptr) return;
-    __syncthreads();
-    const int i = thread / 8, col = 32 * (int)blockIdx.y + thread % 8 * 4;
-    if (row0 + i >= g.n_rows || col >= g.dim) return;
-    XeF4 v = *reinterpret_cast<const XeF4*>(g.d_x + (row0 + i) * g.cols + col);
-#pragma unroll
-    for (int c = 0; c < 4; ++c) v[c] = labels[i] != -1 ? v[c] * factor[i] : 0.0f;
-    xe_store4(g.out, g.bf16 != 0, row0 + i, col, g.dim, v);
-}
-
-struct XeWeightsArgs {
+    int dx_groups;
+    // the weights' gradient from its parts
     XePlan plan;
     const float* stats;
     const float* part;
-    int64_t n_rows;
-    int blocks, slices, dim, bf16;
+    int64_t n_classes;
+    int blocks, slices, groups_per_tile;
     void* d_w;
     void* d_b;  // or null
 };
 
-// A wave 32 classes and eight columns.  Where there are many parts (TOGETHER) a workgroup's four share them.
+__device__ __forceinline__ void xe_finish_rows(const XeFinishArgs& g)
+{
+    const int col_groups = (g.dim + 31) / 32, thread = (int)threadIdx.x;
+    const int64_t row = 32LL * ((int)blockIdx.x / col_groups) + thread / 8;
+    const int col = (int)blockIdx.x % col_groups * 32 + thread % 8 * 4;
+    if (row >= g.n_rows || col >= g.dim) return;
+    XeF4 v = *reinterpret_cast<const XeF4*>(g.d_x + row * g.cols + col);
+    const int label = g.kept[row].label;
+    const float f = g.d_loss != nullptr ? g.d_loss[row] : g.factor.value();
+#pragma unroll
+    for (int c = 0; c < 4; ++c) v[c] = label != -1 ? v[c] * f : 0.0f;
+    xe_store4(g.out, g.bf16 != 0, row, col, g.dim, v);
+}
+
+// What is left to do for the gradients: dx from what the forward pass made of it, and the weights' gradient from the parts of shared groups.  A
+// wave takes 32 classes and eight columns; where there are many parts (TOGETHER), a workgroup's four share them.
 template <bool TOGETHER>
-__global__ __launch_bounds__(kBlock) void xe_weights_kernel(const XeWeightsArgs g)
+__global__ __launch_bounds__(kBlock) void xe_finish_kernel(const XeFinishArgs g)
 {
     __shared__ XeF4 sums[TOGETHER ? kXeWaves : 1][kWave];
     __shared__ float biases[TOGETHER ? kXeWaves : 1][32];
-    const int tile = (int)blockIdx.x;
+    const int id = (int)blockIdx.x - g.dx_groups;
+    if (id < 0) return xe_finish_rows(g);
+    const int tile = id / g.groups_per_tile, in_tile = id % g.groups_per_tile;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x / kWave)), lane = lane_id();
-    const int chunk = TOGETHER ? (int)blockIdx.y : (int)blockIdx.y * kXeWaves + wave, slice = chunk / (4 * g.blocks);
+    const int chunk = TOGETHER ? in_tile : in_tile * kXeWaves + wave, slice = chunk / (4 * g.blocks);
     const int group = tile / kXeWaves * g.slices + slice, b0 = g.plan.first(group), parts = g.plan.last(group) - b0 + 1;
     if (parts == 1) return;  // (stored as it was formed)
     const int64_t place = (int64_t)g.plan.slot(b0, group) * kXeWaves + tile % kXeWaves;
@@ -970,14 +1024,20 @@ __global__ __launch_bounds__(kBlock) void xe_weights_kernel(const XeWeightsArgs 
     const bool with_bias = g.d_b != nullptr && chunk == 0;
     XeF4 sum = {};
     float bias = 0.0f;
-#pragma unroll 4
-    for (int k = k0; k < k1; ++k) {
-        const XeF4 v = p[k * step];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) sum[c] += v[c];
-    }
-    if (with_bias)
+    if (with_bias) {
+#pragma unroll 8
         for (int k = k0; k < k1; ++k) bias += g.stats[4 * ((place + (int64_t)k * kXeWaves) * 32 + lane % 32)];
+    }
+    constexpr int kBatch = TOGETHER ? 8 : 4;  // parts that are asked for at once
+    for (int k = k0; k < k1; k += kBatch) {
+        XeF4 v[kBatch];
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) v[j] = p[(k + j < k1 ? k + j : k) * step];
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) sum[c] += k + j < k1 ? v[j][c] : 0.0f;
+    }
     if constexpr (TOGETHER) {
         sums[wave][lane] = sum;
         if (lane < 32) biases[wave][lane] = bias;
@@ -991,11 +1051,14 @@ __global__ __launch_bounds__(kBlock) void xe_weights_kernel(const XeWeightsArgs 
         }
     }
     const int64_t row = 32LL * tile + lane % 32;
-    if (row >= g.n_rows) return;
+    if (row >= g.n_classes) return;
+    const float f = g.factor.value();
+#pragma unroll
+    for (int c = 0; c < 4; ++c) sum[c] *= f;
     xe_store4(g.d_w, g.bf16 != 0, row, 8 * chunk + lane / 32 * 4, g.dim, sum);
     if (with_bias && lane < 32) {
-        if (g.bf16) static_cast<__bf16*>(g.d_b)[row] = (__bf16)bias;
-        else static_cast<float*>(g.d_b)[row] = bias;
+        if (g.bf16) static_cast<__bf16*>(g.d_b)[row] = (__bf16)(bias * f);
+        else static_cast<float*>(g.d_b)[row] = bias * f;
     }
 }
 
@@ -1013,12 +1076,14 @@ inline XePlan xe_plan(const XeShape& s, int use, int kept_tiles, int passed_tile
     p.shared = p.groups < room ? room / p.groups : 1;
     p.per = (int)ceil_div(passed_tiles, p.shared);
     if (p.per < least) p.per = least;
+    // (the weights' gradient of a few tiles: without parts there is a launch less)
+    if (use == kXeWeights && passed_tiles <= 6) p.per = passed_tiles;
     p.shared = (int)ceil_div(passed_tiles, p.per);
     p.room = room;
     p.whole = 0;
     // Where that leaves an eighth of the chip idle, in the only round or the last of a few: no regard for the groups' ends
     const int64_t full = (int64_t)p.groups * p.shared, rounds = ceil_div(full, room);
-    if (p.per > least && rounds <= 8 && full * 8 < rounds * room * 7 && (p.groups % room + 1LL) * passed_tiles < 1LL << 31) {
+    if (p.per > least && p.per > 6 && rounds <= 8 && full * 8 < rounds * room * 7 && (p.groups % room + 1LL) * passed_tiles < 1LL << 31) {
         p.whole = p.groups / room * room;
         p.per = (int)ceil_div((int64_t)(p.groups - p.whole) * passed_tiles, room);
         if (p.per < least) p.per = least;
@@ -1053,6 +1118,7 @@ struct XeState {
     XeRow* kept;
     float* d_x;
     float *count, *scales;
+    int* done;
     size_t bytes;
 };
 
@@ -1062,6 +1128,7 @@ inline XeState xe_state(const XeProblem& p, int want, void* base)
     XeState s = {};
     s.scales = c.take<float>(4);
     s.count = s.scales + 2;
+    s.done = reinterpret_cast<int*>(s.scales + 3);
     if (want != 0) s.kept = c.take<XeRow>((size_t)p.n);
     if (want & FGL_XENT_ROWS) s.d_x = c.take<float>((size_t)p.n * p.shape.cols());
     if (want & FGL_XENT_WEIGHTS) {
@@ -1197,11 +1264,16 @@ FGL_EXPORT int fgl_linear_cross_entropy(const void* d_x, int64_t x_row_stride, i
     const int64_t tiles = (int64_t)p.row_tiles + p.class_tiles;
     FGL_REQUIRE(tiles < 1 << 24, "linear_cross_entropy: grid too large");
     const dim3 grid((unsigned)tiles, (unsigned)ceil_div(s.cols(), kXeCols)), block(kBlock);
-    im.most = ws.most;
+    // Few values: each workgroup looks for the largest itself, which a launch of its own takes longer for.
+    const bool few = (n_rows + n_classes) * dim <= 16384;
+    im.most = few ? nullptr : ws.most;
     im.scales = st.scales;
+    im.done = st.done;
     if (dtype == FGL_F32) {
-        hipLaunchKernelGGL(xe_most_kernel, dim3(kBlock, 2), block, 0, to, im.m[0], im.m[1], dim, ws.most);
-        FGL_CHECK_LAUNCH("xe_most_kernel");
+        if (!few) {
+            hipLaunchKernelGGL(xe_most_kernel, dim3(kBlock, 2), block, 0, to, im.m[0], im.m[1], dim, ws.most);
+            FGL_CHECK_LAUNCH("xe_most_kernel");
+        }
         hipLaunchKernelGGL((xe_images_kernel<float, 2>), grid, block, 0, to, im);
     } else {
         hipLaunchKernelGGL((xe_images_kernel<__bf16, 1>), grid, block, 0, to, im);
@@ -1224,7 +1296,7 @@ FGL_EXPORT int fgl_linear_cross_entropy(const void* d_x, int64_t x_row_stride, i
     c.plan = g.plan;
     c.stats = ws.stats;
     c.part = ws.part;
-    c.rows = g.kept;
+    c.rows = im.m[0].s_image;
     c.n_rows = n_rows;
     c.s_bytes = s.s_bytes();
     c.blocks = s.blocks;
@@ -1236,14 +1308,16 @@ FGL_EXPORT int fgl_linear_cross_entropy(const void* d_x, int64_t x_row_stride, i
     c.bf16 = dtype == FGL_BF16;
     c.losses = reduction == FGL_REDUCE_NONE ? d_loss : nullptr;
     c.tile_loss = reduction == FGL_REDUCE_NONE ? nullptr : ws.tile_loss;
+    c.tiles = p.row_tiles;
+    c.mean = reduction == FGL_REDUCE_MEAN;
+    c.done = st.done;
+    c.loss = d_loss;
+    c.count = st.count;
     c.kept = st.kept;
+    c.weights = (want & FGL_XENT_WEIGHTS) != 0;
     c.d_x = st.d_x;
     hipLaunchKernelGGL(xe_combine_kernel, dim3((unsigned)p.row_tiles, want & FGL_XENT_ROWS ? (unsigned)(s.blocks * s.slices) : 1u), block, 0, to, c);
     FGL_CHECK_LAUNCH("xe_combine_kernel");
-    if (reduction != FGL_REDUCE_NONE) {
-        hipLaunchKernelGGL(xe_total_kernel, dim3(1), block, 0, to, ws.tile_loss, p.row_tiles, (int)(reduction == FGL_REDUCE_MEAN), d_loss, st.count);
-        FGL_CHECK_LAUNCH("xe_total_kernel");
-    }
     return FGL_OK;
 }
 
@@ -1255,67 +1329,69 @@ FGL_EXPORT int fgl_linear_cross_entropy_backward(const float* d_loss_grad, int64
                 (long long)n_rows, (long long)n_classes, dim, kXeMaxDim, dtype);
     FGL_REQUIRE(reduction == FGL_REDUCE_NONE || reduction == FGL_REDUCE_SUM || reduction == FGL_REDUCE_MEAN, "linear_cross_entropy_backward: reduction %d", reduction);
     FGL_REQUIRE((want & ~(FGL_XENT_ROWS | FGL_XENT_WEIGHTS)) == 0 && want != 0, "linear_cross_entropy_backward: want %d", want);
-    FGL_REQUIRE(d_loss_grad && d_state && d_ws && (d_dx == nullptr || (want & FGL_XENT_ROWS)) && ((d_dw == nullptr && d_db == nullptr) || (want & FGL_XENT_WEIGHTS)) &&
+    FGL_REQUIRE(d_loss_grad && d_state && (d_dx == nullptr || (want & FGL_XENT_ROWS)) && ((d_dw == nullptr && d_db == nullptr) || (want & FGL_XENT_WEIGHTS)) &&
                     (d_db == nullptr || d_dw != nullptr),
                 "linear_cross_entropy_backward: null pointer, or a gradient that the forward pass was not told of");
     const XeState st = xe_state(p, want, d_state);
     const XeScratch ws = xe_backward_scratch(p, want, d_ws);
-    if (state_bytes < st.bytes || ws_bytes < ws.bytes || ((uintptr_t)d_state | (uintptr_t)d_ws) % 256 != 0) {
+    if (state_bytes < st.bytes || ws_bytes < ws.bytes || (d_ws == nullptr && ws.bytes > 0) || ((uintptr_t)d_state | (uintptr_t)d_ws) % 256 != 0) {
         set_error("linear_cross_entropy_backward: needs %zu bytes of state and %zu of workspace on 256-byte boundaries, got %zu and %zu", st.bytes, ws.bytes, state_bytes, ws_bytes);
         return FGL_ERR_WORKSPACE;
     }
     const XeShape& s = p.shape;
     const hipStream_t to = as_stream(stream);
     const dim3 block(kBlock);
-    XeRowsArgs r = {};
-    r.kept = st.kept;
-    r.d_x = st.d_x;
-    r.d_loss = d_loss_grad;
-    r.count = st.count;
-    r.reduction = reduction;
-    r.rows = d_dw != nullptr ? st.rows_s : nullptr;
-    r.n_rows = n_rows;
-    r.s_bytes = s.s_bytes();
-    r.cols = s.cols();
-    r.dim = dim;
-    r.bf16 = dtype == FGL_BF16;
-    r.out = d_dx;
-    hipLaunchKernelGGL(xe_rows_kernel, dim3((unsigned)p.row_tiles, d_dx != nullptr ? (unsigned)ceil_div(dim, 32) : 1u), block, 0, to, r);
-    FGL_CHECK_LAUNCH("xe_rows_kernel");
-    if (d_dw == nullptr) return FGL_OK;
-
+    const XeFactor factor = {reduction == FGL_REDUCE_NONE ? nullptr : d_loss_grad, reduction == FGL_REDUCE_MEAN ? st.count : nullptr};
     XeArgs g = {};
-    g.kept = st.classes_s;
-    g.passed = st.rows_s;
-    g.passed_p = st.rows_p;
-    g.kept_tiles = p.class_tiles;
-    g.stats = ws.stats;
-    g.part = ws.part;
-    g.scales = st.scales;
-    g.d_w = d_dw;
-    g.d_b = d_db;
-    g.kept_rows = n_classes;
-    g.dim = dim;
-    const int rc = launch_xe<kXeWeights>(s, g, p.row_tiles, to);
-    if (rc != FGL_OK) return rc;
-    FGL_CHECK_LAUNCH("xe_kernel");
-    if (g.plan.shared != 1) {
-        XeWeightsArgs c = {};
-        c.plan = g.plan;
-        c.stats = ws.stats;
-        c.part = ws.part;
-        c.n_rows = n_classes;
-        c.blocks = s.blocks;
-        c.slices = s.slices;
-        c.dim = dim;
-        c.bf16 = dtype == FGL_BF16;
-        c.d_w = d_dw;
-        c.d_b = d_db;
-        const bool together = g.plan.shared > 8;
-        const dim3 combine((unsigned)p.class_tiles, (unsigned)((together ? kXeWaves : 1) * s.blocks * s.slices));
-        if (together) hipLaunchKernelGGL(xe_weights_kernel<true>, combine, block, 0, to, c);
-        else hipLaunchKernelGGL(xe_weights_kernel<false>, combine, block, 0, to, c);
-        FGL_CHECK_LAUNCH("xe_weights_kernel");
+    if (d_dw != nullptr) {
+        if (reduction == FGL_REDUCE_NONE) {
+            hipLaunchKernelGGL(xe_factors_kernel, dim3((unsigned)ceil_div(n_rows, kBlock)), block, 0, to, st.kept, d_loss_grad, n_rows, st.rows_s, s.s_bytes());
+            FGL_CHECK_LAUNCH("xe_factors_kernel");
+        }
+        g.kept = st.classes_s;
+        g.passed = st.rows_s;
+        g.passed_p = st.rows_p;
+        g.kept_tiles = p.class_tiles;
+        g.stats = ws.stats;
+        g.part = ws.part;
+        g.scales = st.scales;
+        g.factor = factor;
+        g.d_w = d_dw;
+        g.d_b = d_db;
+        g.kept_rows = n_classes;
+        g.dim = dim;
+        const int rc = launch_xe<kXeWeights>(s, g, p.row_tiles, to);
+        if (rc != FGL_OK) return rc;
+        FGL_CHECK_LAUNCH("xe_kernel");
     }
+    const bool parts = d_dw != nullptr && g.plan.shared != 1;
+    if (d_dx == nullptr && !parts) return FGL_OK;
+    const bool together = parts && g.plan.shared > 8;
+    XeFinishArgs f = {};
+    f.kept = st.kept;
+    f.d_x = st.d_x;
+    f.d_loss = reduction == FGL_REDUCE_NONE ? d_loss_grad : nullptr;
+    f.factor = factor;
+    f.n_rows = n_rows;
+    f.cols = s.cols();
+    f.dim = dim;
+    f.bf16 = dtype == FGL_BF16;
+    f.out = d_dx;
+    const int64_t dx_groups = d_dx != nullptr ? (int64_t)p.row_tiles * ceil_div(dim, 32) : 0;
+    f.plan = g.plan;
+    f.stats = ws.stats;
+    f.part = ws.part;
+    f.n_classes = n_classes;
+    f.blocks = s.blocks;
+    f.slices = s.slices;
+    f.groups_per_tile = (together ? 4 : 1) * s.blocks * s.slices;
+    f.d_w = d_dw;
+    f.d_b = d_db;
+    const int64_t groups = dx_groups + (parts ? (int64_t)p.class_tiles * f.groups_per_tile : 0);
+    FGL_REQUIRE(groups < 1 << 24, "linear_cross_entropy_backward: grid too large");
+    f.dx_groups = (int)dx_groups;
+    if (together) hipLaunchKernelGGL(xe_finish_kernel<true>, dim3((unsigned)groups), block, 0, to, f);
+    else hipLaunchKernelGGL(xe_finish_kernel<false>, dim3((unsigned)groups), block, 0, to, f);
+    FGL_CHECK_LAUNCH("xe_finish_kernel");
     return FGL_OK;
 }
