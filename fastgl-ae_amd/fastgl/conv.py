@@ -19,6 +19,7 @@ import torch
 from torch import nn
 
 from . import ops
+from .dropouts import Dropout
 from .sampler import Block
 
 
@@ -169,11 +170,16 @@ def _stack(conv, in_feats, n_hidden, n_classes, n_layers, weight):
     return layers
 
 
+def _between_layers(p, seed, relu=False):
+    """The dropout between a model's layers: torch's, or -- with a seed -- the one whose masks are a function of it (and of the call)."""
+    return nn.Dropout(p=p) if seed is None else Dropout(p, seed, relu)
+
+
 class GCN(nn.Module):
-    def __init__(self, in_feats, n_hidden, n_classes, n_layers, activation, weight, dropout):
+    def __init__(self, in_feats, n_hidden, n_classes, n_layers, activation, weight, dropout, dropout_seed=None):
         super().__init__()
         self.layers = _stack(GCNConv, in_feats, n_hidden, n_classes, n_layers, weight)
-        self.dropout = nn.Dropout(p=dropout)
+        self.dropout = _between_layers(dropout, dropout_seed)
 
     def forward(self, blocks, features, neighbor_list=[5, 10, 15]):
         h = features
@@ -226,10 +232,10 @@ class GINConv(_Conv):
 
 
 class GIN(nn.Module):
-    def __init__(self, in_feats, n_hidden, n_classes, n_layers, activation, weight, dropout):
+    def __init__(self, in_feats, n_hidden, n_classes, n_layers, activation, weight, dropout, dropout_seed=None):
         super().__init__()
         self.layers = _stack(GINConv, in_feats, n_hidden, n_classes, n_layers, weight)
-        self.dropout = nn.Dropout(p=dropout)
+        self.dropout = _between_layers(dropout, dropout_seed)
 
     def forward(self, blocks, features, neighbor_list=[5, 10, 15]):
         h = features
@@ -546,12 +552,12 @@ class SAGEConv(nn.Module):
 
 
 class SAGE(nn.Module):
-    def __init__(self, in_feats, n_hidden, n_classes, n_layers, activation=torch.relu, dropout=0.0):
+    def __init__(self, in_feats, n_hidden, n_classes, n_layers, activation=torch.relu, dropout=0.0, dropout_seed=None):
         super().__init__()
         dims = [in_feats] + [n_hidden] * (n_layers - 1) + [n_classes]
         self.layers = nn.ModuleList(SAGEConv(dims[i], dims[i + 1]) for i in range(n_layers))
         self.activation = activation
-        self.dropout = nn.Dropout(p=dropout)
+        self.dropout = _between_layers(dropout, dropout_seed, relu=activation in (torch.relu, nn.functional.relu))
 
     def forward(self, blocks, features, input_nodes=None):
         """``features``: the rows of the input nodes, or -- with ``input_nodes`` given -- the
@@ -568,7 +574,7 @@ class SAGE(nn.Module):
             else:
                 h = layer(block, h)
             if i != len(self.layers) - 1:
-                if self.activation is not None:
+                if self.activation is not None and not getattr(self.dropout, "relu", False):  # (else it goes with the dropout)
                     h = self.activation(h)
                 h = self.dropout(h)
         return h

@@ -38,15 +38,17 @@ def make_dataset(n_nodes, n_draws, feat_dim, n_classes, train_frac, seed, device
     return edge_ptr, edge_src, feat, label, train_nids
 
 
-def build_model(name, in_feats, n_hidden, n_classes, n_layers, dropout):
+def build_model(name, in_feats, n_hidden, n_classes, n_layers, dropout, dropout_seed=None):
     if name == "gcn":
-        return fastgl.GCN(in_feats, n_hidden, n_classes, n_layers, None, True, dropout)
+        return fastgl.GCN(in_feats, n_hidden, n_classes, n_layers, None, True, dropout, dropout_seed)
     if name == "gin":
-        return fastgl.GIN(in_feats, n_hidden, n_classes, n_layers, None, True, dropout)
+        return fastgl.GIN(in_feats, n_hidden, n_classes, n_layers, None, True, dropout, dropout_seed)
     if name == "gat":
+        if dropout_seed is not None:
+            raise ValueError("GAT has no dropout between its layers")
         return fastgl.GAT(in_feats, n_hidden, n_classes, n_layers, None, dropout, heads=4)
     if name == "sage":
-        return fastgl.SAGE(in_feats, n_hidden, n_classes, n_layers, dropout=dropout)
+        return fastgl.SAGE(in_feats, n_hidden, n_classes, n_layers, dropout=dropout, dropout_seed=dropout_seed)
     raise ValueError("unknown model %r" % name)
 
 
@@ -61,9 +63,11 @@ def run(args):
         print("config:{:}={:}".format(k, v))
     sampler = fastgl.FusedMapSampler(args.fanout, rng_seed=args.seed, id_order=args.id_order,
                                      deterministic=bool(args.deterministic)).set_graph(edge_ptr, edge_src)
-    model = build_model(args.model, args.feat_dim, args.num_hidden, args.classes, len(args.fanout), args.dropout).to(device)
-    loss_fcn = torch.nn.CrossEntropyLoss()
-    optimizer = torch.optim.Adam(model.parameters(), lr=args.lr, weight_decay=args.weight_decay)
+    # the last layer gives the classes' logits, or hidden rows that a layer of its own turns into the loss at once
+    outputs = args.classes if args.head == "layer" else args.num_hidden
+    model = build_model(args.model, args.feat_dim, args.num_hidden, outputs, len(args.fanout), args.dropout, args.dropout_seed).to(device)
+    loss_fcn = torch.nn.CrossEntropyLoss() if args.head == "layer" else fastgl.LinearCrossEntropy(args.num_hidden, args.classes).to(device)
+    optimizer = torch.optim.Adam([*model.parameters(), *loss_fcn.parameters()], lr=args.lr, weight_decay=args.weight_decay)
     sync = torch.cuda.synchronize
 
     # the reference wraps its sampler in DGL's DataLoader (train_fastgl.py:248-258); here the library's own, with the same
@@ -158,6 +162,12 @@ def parse_args(argv=None):
     ap.add_argument("--train_frac", type=float, default=0.1)
     ap.add_argument("--lr", type=float, default=0.01)
     ap.add_argument("--dropout", type=float, default=0.5)
+    ap.add_argument("--dropout_seed", type=int, default=None,
+                    help="gcn, gin, sage: dropout masks are a function of this seed and the call instead of torch's generator (a run with "
+                         "--deterministic 1 is then reproducible with dropout too)")
+    ap.add_argument("--head", default="layer", choices=["layer", "linear"],
+                    help="linear: the model gives num_hidden columns, and fastgl.LinearCrossEntropy the loss over the classes, without the "
+                         "logits in memory (for very many classes)")
     ap.add_argument("--weight_decay", type=float, default=0.0005)
     ap.add_argument("--seed", type=int, default=0)
     ap.add_argument("--id_order", default="first", choices=["first", "arrival"])
