@@ -83,7 +83,7 @@ inline XeShape xe_shape(int dim, int dtype)
     const int n = (int)ceil_div(dim, 32);
     XeShape s;
     s.parts = dtype == FGL_F32 ? 2 : 1;
-    const int blocks = n <= 4 ? n : n <= 6 ? 6 : n <= 8 ? 8 : n <= 12 ? 12 : 16;
+    const int blocks = n <= 8 ? n : n <= 12 ? 12 : 16;
     s.slices = blocks > 8 ? 2 : 1;
     s.blocks = blocks / s.slices;
     return s;
@@ -1212,7 +1212,9 @@ void launch_xe_parts(const XeShape& s, const XeArgs& g, unsigned workgroups, hip
     case 2: hipLaunchKernelGGL((xe_kernel<2, PARTS, USE, false>), grid, block, 0, stream, g); break;
     case 3: hipLaunchKernelGGL((xe_kernel<3, PARTS, USE, false>), grid, block, 0, stream, g); break;
     case 4: hipLaunchKernelGGL((xe_kernel<4, PARTS, USE, false>), grid, block, 0, stream, g); break;
+    case 5: hipLaunchKernelGGL((xe_kernel<5, PARTS, USE, false>), grid, block, 0, stream, g); break;
     case 6: hipLaunchKernelGGL((xe_kernel<6, PARTS, USE, false>), grid, block, 0, stream, g); break;
+    case 7: hipLaunchKernelGGL((xe_kernel<7, PARTS, USE, false>), grid, block, 0, stream, g); break;
     default: hipLaunchKernelGGL((xe_kernel<8, PARTS, USE, false>), grid, block, 0, stream, g); break;
     }
 }
