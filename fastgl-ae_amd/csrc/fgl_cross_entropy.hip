@@ -67,8 +67,10 @@ enum { kXeLoss = 0, kXeLossAndRows = 1, kXeWeights = 2 };
 // A tile's first kilobyte, in floats.  Classes: their biases.  Rows: -maximum (powers of two), factor, label, the label's value.
 constexpr int kXeShift = 0, kXeFactor = 32, kXeLabel = 64, kXeOwn = 96;
 
-// Sizes of a problem as the kernels see it: blocks of 32 columns, padded; beyond 256 columns in two slices, each with
-// half of O, which otherwise did not fit a wave's registers (S is formed for either).
+// Sizes of a problem as the kernels see it: blocks of 32 columns, padded.  Beyond 384 columns, in bf16 beyond 256, in two slices, each with half of O,
+// which otherwise did not fit a wave's registers, and S formed for either.  (bf16 could have 384 columns whole, with one wave a SIMD instead of
+// two: 8192 rows, 20 K classes, forward, 300 columns 340 us against 352 in slices, 370 columns 556 against 352.  fp32 has one wave a SIMD
+// from 129 columns on anyway: 300 columns 686 whole, 1115 in slices.)
 struct XeShape {
     int blocks;  // in a slice
     int slices;
@@ -83,8 +85,8 @@ inline XeShape xe_shape(int dim, int dtype)
     const int n = (int)ceil_div(dim, 32);
     XeShape s;
     s.parts = dtype == FGL_F32 ? 2 : 1;
-    const int blocks = n <= 8 ? n : n <= 12 ? 12 : 16;
-    s.slices = blocks > 8 ? 2 : 1;
+    s.slices = n > (s.parts == 2 ? 12 : 8) ? 2 : 1;
+    const int blocks = n <= 8 ? n : n <= 10 && s.parts == 2 ? 10 : n <= 12 ? 12 : 16;
     s.blocks = blocks / s.slices;
     return s;
 }
@@ -442,7 +444,7 @@ __device__ __forceinline__ void xe_products(const At& at, const Use& use)
 __host__ __device__ constexpr int xe_waves(int blocks, int parts, int use, bool wide)
 {
     if (wide) return parts == 1 && (use == kXeLoss || blocks <= 6) ? 2 : 1;
-    if (use == kXeLoss) return parts == 1 ? 4 : blocks <= 2 ? 4 : blocks <= 4 ? 3 : 2;
+    if (use == kXeLoss) return parts == 1 ? 4 : blocks <= 2 ? 4 : blocks <= 4 ? 3 : blocks <= 8 ? 2 : 1;
     return parts == 1 ? (blocks <= 2 ? 4 : blocks <= 3 ? 3 : 2) : blocks <= 1 ? 4 : blocks <= 2 ? 3 : blocks <= 4 ? 2 : 1;
 }
 
@@ -1203,9 +1205,21 @@ void launch_xe_parts(const XeShape& s, const XeArgs& g, unsigned workgroups, hip
 {
     const dim3 grid(workgroups), block(kBlock);
     if (s.slices == 2) {
-        if (s.blocks == 6) hipLaunchKernelGGL((xe_kernel<6, PARTS, USE, true>), grid, block, 0, stream, g);
-        else hipLaunchKernelGGL((xe_kernel<8, PARTS, USE, true>), grid, block, 0, stream, g);
+        if constexpr (PARTS == 1) {
+            if (s.blocks == 6) {
+                hipLaunchKernelGGL((xe_kernel<6, PARTS, USE, true>), grid, block, 0, stream, g);
+                return;
+            }
+        }
+        hipLaunchKernelGGL((xe_kernel<8, PARTS, USE, true>), grid, block, 0, stream, g);
         return;
+    }
+    if constexpr (PARTS == 2) {
+        if (s.blocks > 8) {
+            if (s.blocks == 10) hipLaunchKernelGGL((xe_kernel<10, PARTS, USE, false>), grid, block, 0, stream, g);
+            else hipLaunchKernelGGL((xe_kernel<12, PARTS, USE, false>), grid, block, 0, stream, g);
+            return;
+        }
     }
     switch (s.blocks) {
     case 1: hipLaunchKernelGGL((xe_kernel<1, PARTS, USE, false>), grid, block, 0, stream, g); break;

@@ -99,7 +99,7 @@ def make(cuda, n, v, d, dtype, bias=True, ignored=0.2, seed=0, label_dtype=torch
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("n,v,d", [(1, 1, 1), (1, 2, 3), (2, 33, 31), (31, 32, 32), (33, 31, 33), (100, 47, 64), (128, 64, 65), (129, 129, 96), (257, 172, 100), (64, 1000, 128),
                                    (300, 161, 160), (500, 300, 192), (96, 4097, 200), (1000, 47, 256), (40, 500, 257), (70, 333, 300), (130, 100, 384), (33, 700, 400),
-                                   (200, 65, 512), (5, 20011, 64), (4100, 5, 16), (2500, 2100, 48),
+                                   (200, 65, 512), (150, 140, 350), (90, 1000, 288), (5, 20011, 64), (4100, 5, 16), (2500, 2100, 48),
                                    (12900, 230, 300), (230, 12900, 300), (40_000, 500, 250), (500, 90_000, 250), (33_000, 70, 30)])
 def test_losses_and_gradients(cuda, dtype, n, v, d):
     print("linear_cross_entropy %d x %d, %d classes, %s" % (n, d, v, dtype), flush=True)
@@ -258,6 +258,40 @@ def test_gradients_against_differences(cuda, dtype):
                 return float(torch.nn.functional.cross_entropy(s[keep], y[keep], reduction="sum"))
             slope = (8 * (at(h) - at(-h)) - (at(2 * h) - at(-2 * h))) / (12 * h)
             assert abs(float(g.reshape(-1)[i]) - slope) <= 2e-2 * (1 + abs(slope))
+
+
+def test_values_beyond_2_to_the_31(cuda):
+    """A weight of 2^31 values and more: classes at its far end, against sums over pieces of the classes."""
+    n, v, d = 40, (1 << 31) // 256 + 3000, 256
+    gen = torch.Generator(device=cuda).manual_seed(2)
+    w = torch.empty((v, d), dtype=torch.bfloat16, device=cuda)
+    for k in range(0, v, 1 << 20):
+        w[k:k + (1 << 20)] = torch.randn((min(1 << 20, v - k), d), generator=gen, device=cuda) / 16
+    y = torch.randint(0, v, (n,), generator=gen, device=cuda)
+    y[:20] = v - 1 - torch.arange(20, device=cuda) * 97
+    x = torch.randn((n, d), generator=gen, device=cuda).bfloat16()
+    x[:20] += w[y[:20]] * 6
+    x, w = x.requires_grad_(), w.requires_grad_()
+    losses = fastgl.linear_cross_entropy(x, w, y, reduction="none")
+    dx, dw = torch.autograd.grad(losses, (x, w), torch.ones(n, device=cuda))
+    with torch.no_grad():
+        total = torch.zeros(n, dtype=torch.float64, device=cuda)
+        want_dx = torch.zeros((n, d), dtype=torch.float64, device=cuda)
+        for k in range(0, v, 1 << 19):
+            s = (x.float() @ w[k:k + (1 << 19)].float().t()).double()
+            total += s.exp().sum(1)
+            want_dx += (s.exp().float() @ w[k:k + (1 << 19)].float()).double()
+        own = (x.double() * w[y].double()).sum(1)
+        # (fp32 sums of 256 products on either side, shares rounded to bf16 on this: 2^-8 of sums of magnitudes, which are ten times the sums here)
+        assert ((losses.double() - (total.log() - own)).abs() <= 1e-5 * losses.abs()).all()
+        want_dx = want_dx / total[:, None] - w[y].double()
+        assert (dx.double() - want_dx).norm() <= 2.0 ** -7 * want_dx.norm()
+        last = slice(v - 2000, v)
+        p = (x.double() @ w[last].double().t()).exp() / total[:, None]
+        p[torch.arange(20, device=cuda), y[:20] - (v - 2000)] -= 1
+        want_dw = p.t() @ x.double()
+        assert (dw[last].double() - want_dw).norm() <= 2.0 ** -7 * want_dw.norm()
+        assert (dw[last].double() - want_dw).abs().amax() <= 2.0 ** -7 * want_dw.abs().amax()
 
 
 def test_refusals(cuda):
