@@ -696,7 +696,13 @@ __global__ __launch_bounds__(kBlock, xe_waves(DB, PARTS, USE, WIDE)) void xe_ker
     constexpr int64_t kSBytes = (int64_t)Wave::kSChunks * kXeChunk, kPBytes = (int64_t)Wave::kPChunks * (WIDE ? 2 : 1) * kXeChunk;
     const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x / kWave));
     const XePlan plan = g.plan;
-    const int workgroup = (int)blockIdx.x;
+    int workgroup = (int)blockIdx.x;
+    if (plan.shared > 0) {
+        // The workgroups of an XCD, every eighth one, take neighbouring places in an order by the part of the passed tiles, so that its L2 has to hold
+        // few of those parts
+        const int all = plan.groups * plan.shared, xcd = workgroup % 8, place = all / 8 * xcd + (xcd < all % 8 ? xcd : all % 8) + workgroup / 8;
+        workgroup = place % plan.groups * plan.shared + place / plan.groups;
+    }
     // this workgroup's groups: whole ones first, then parts
     int next = workgroup, whole = plan.shared > 0 ? 0 : plan.whole, t0 = 0, left = 0;
     for (bool parts = false;;) {
