@@ -642,6 +642,17 @@ struct XeWave {
         if constexpr (USE == kXeWeights) both = gradients(p, s, v0);
         else shares(p, n0);
     }
+    // The same where LDS has room for two S tiles: the next one is on its way from the start of this one
+    __device__ __forceinline__ void first_half_of_two(const char* __restrict__ s, char* __restrict__ next_p, char* __restrict__ next_s, const char* src_p, const char* src_s,
+                                                      XeF32x16& p, bool& both, int n0, int v0, bool active)
+    {
+        xe_stage<kPChunks>(src_p, next_p);
+        if (src_s != nullptr) xe_stage<kSChunks>(src_s, next_s);
+        if (!active) return;
+        p = logits(s);
+        if constexpr (USE == kXeWeights) both = gradients(p, s, v0);
+        else shares(p, n0);
+    }
     __device__ __forceinline__ void second_half(const char* __restrict__ s, char* __restrict__ next, const char* src, const XeF32x16& p, bool both, bool active)
     {
         if (src != nullptr) xe_stage<kSChunks>(src, next);
@@ -692,6 +703,10 @@ __global__ __launch_bounds__(kBlock, xe_waves(DB, PARTS, USE, WIDE)) void xe_ker
     using Wave = XeWave<DB, PARTS, USE, WIDE>;
     __shared__ __attribute__((aligned(16))) char s_buf[Wave::kSChunks * kXeChunk];
     __shared__ __attribute__((aligned(16))) char p_buf[(USE == kXeLoss ? Wave::kSChunks : Wave::kPChunks) * kXeChunk];  // (the loss alone: two tiles in turn)
+    // In slices S is most of the work and O too little to hide the next S tile's copy behind.  (8192 x 512, 10 K classes, backward 399 us with
+    // one S tile, 348 with two.  Slices of 192 columns, two waves a SIMD, have no registers left for it.)
+    constexpr bool kTwo = WIDE && DB == 8 && PARTS == 1 && USE != kXeLoss;
+    __shared__ __attribute__((aligned(16))) char s_other[(kTwo ? Wave::kSChunks : 1) * kXeChunk];
     constexpr int kSlices = WIDE && USE != kXeLoss ? 2 : 1;
     constexpr int64_t kSBytes = (int64_t)Wave::kSChunks * kXeChunk, kPBytes = (int64_t)Wave::kPChunks * (WIDE ? 2 : 1) * kXeChunk;
     const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x / kWave));
@@ -762,6 +777,19 @@ __global__ __launch_bounds__(kBlock, xe_waves(DB, PARTS, USE, WIDE)) void xe_ker
             if (t + 1 == t1) break;
             w.first_half(p_buf, s_buf, t + 2 < t1 ? g.passed + (t + 2) * kSBytes : nullptr, p, both, 32 * (t + 1), v0, active);
             xe_staged();
+        }
+    } else if constexpr (kTwo) {
+        const char* passed_p = g.passed_p + slice * (int64_t)Wave::kPChunks * kXeChunk;
+        for (int t = t0; t < t1; t += 2) {
+            w.first_half_of_two(s_buf, p_buf, s_other, passed_p + t * kPBytes, t + 1 < t1 ? g.passed + (t + 1) * kSBytes : nullptr, p, both, 32 * t, v0, active);
+            xe_staged();
+            if (active) w.product(p, p_buf, both);
+            __syncthreads();
+            if (t + 1 == t1) break;
+            w.first_half_of_two(s_other, p_buf, s_buf, passed_p + (t + 1) * kPBytes, t + 2 < t1 ? g.passed + (t + 2) * kSBytes : nullptr, p, both, 32 * (t + 1), v0, active);
+            xe_staged();
+            if (active) w.product(p, p_buf, both);
+            __syncthreads();
         }
     } else {
         const char* passed_p = g.passed_p + slice * (int64_t)Wave::kPChunks * kXeChunk;
