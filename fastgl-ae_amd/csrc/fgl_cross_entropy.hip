@@ -23,13 +23,14 @@
 //
 // bf16: P is rounded to bf16, as the operands are.
 // fp32: each value is the sum of two fp16 values, of 11 bits each, and a product three matrix instructions (high low, low high, high high; what is
-// left out is 2^-22 of it), whose sum over 64 k is added to fp32 accumulators.  fp16's range is short, so x and w are first multiplied by a power of two
-// that takes their largest value to 2^14 (xe_most_kernel); what lies 2^39 below it is lost, which is nothing beside the logits and sums that it would
-// go into.  P is scaled likewise, by the running maximum, and the gradient of the logits by a running bound of its own.  Against 64 bits, 2-norm,
-// 8192 x 128 and 20 K classes: 2.2e-7; the same in fp32 products by the library 1.7e-6, in three bf16 parts and six instructions 1.9e-7, in
-// 1.6 times the time.
-// Sums, maxima and losses are fp32 in both.  x and w must be finite, in fp32 below 2^74: others make losses and gradients that are not numbers.
-// A bias of -1e30 or less, -infinity among them, leaves its class out: no share, no gradient.  (Shares are exp2 of one fma, whose
+// left out is 2^-22 of it), whose sum over 64 k is added to fp32 accumulators.  fp16's range is short, so a tile is first multiplied by a power of two
+// that takes its largest value to 2^14; what lies 2^39 below that is lost.  In S a row that is 2^12 below its tile's largest value gets a
+// power of its own, which costs its tile a multiplication a logit.  P is scaled likewise, by the running maximum, and the gradient of the logits by a
+// running bound of its own.  Against 64 bits, 2-norm, 8192 x 128 and 20 K classes: 2.2e-7; the same in fp32 products by the library 1.7e-6, in three
+// bf16 parts and six instructions 1.9e-7, in 1.6 times the time.
+// Sums, maxima and losses are fp32 in both.  x and w must be finite: others make losses and gradients that are not numbers, but in rows
+// without a label, which are taken as zeros.
+// A bias of -1e30 or less, -infinity among them, leaves its class out: no share, no gradient.  (bf16: shares are exp2 of one fma, whose
 // product with log2 e is not rounded where the maximum's is: logits up to some 1e9 are no matter, the difference of 2^-25 of the maximum is the
 // same for all of a row's shares and their sum.)
 //
@@ -59,13 +60,17 @@ constexpr float kXeLog2e = 1.44269504088896340736f;
 constexpr float kXeLn2 = 0.69314718055994530942f;
 constexpr float kXeLeftOut = -1e30f;  // a bias of this or less leaves its class out, as -infinity does
 constexpr float kXeStep = 8.0f;       // powers of two that a row's values may pass its running maximum by
-constexpr float kXeRise = 6.0f;       // fp16: powers of two that P is multiplied by, so that it fills the range
+constexpr int kXeRise = 6;            // fp16: powers of two that P is multiplied by, so that it fills the range
 constexpr int kXeTop = 14;            // fp16: power of two that largest values are taken to
 
 enum { kXeLoss = 0, kXeLossAndRows = 1, kXeWeights = 2 };
 
-// A tile's first kilobyte, in floats.  Classes: their biases.  Rows: -maximum (powers of two), factor, label, the label's value.
+// A tile's first kilobyte, in floats.  Classes: their biases (fp32: times log2 e).  Rows: -maximum (powers of two), factor, label, the label's value.
 constexpr int kXeShift = 0, kXeFactor = 32, kXeLabel = 64, kXeOwn = 96;
+// fp32, with e the power of two that the tile is multiplied by, and f a row's in S: 2^-f, 2^(e - f) of each row; 2^-e, e, whether any f is not e
+constexpr int kXeRow = 128, kXeRowInTile = 160, kXeTile = 192, kXeExponent = 193, kXeMixed = 194;
+constexpr int kXeNear = 12;  // powers of two below the tile's largest value from where on a row has its own f
+constexpr int kXeFar = 120;  // how far f is from e at most: 2^(e - f) is a number
 
 // Sizes of a problem as the kernels see it: blocks of 32 columns, padded.  Beyond 384 columns, in bf16 beyond 256, in two slices, each with half of O,
 // which otherwise did not fit a wave's registers, and S formed for either.  (bf16 could have 384 columns whole, with one wave a SIMD instead of
@@ -109,9 +114,7 @@ struct XeImagesArgs {
     int label64;
     int64_t ignore;
     int64_t classes;
-    const float* most;  // fp32: [2][kBlock], the largest magnitudes of parts of the matrices (xe_most_kernel), or null: they are looked for here
-    float* scales;      // fp32: the powers of two that the matrices are multiplied by
-    int* done;          // cleared: workgroups of xe_combine_kernel that have left their tile's loss
+    int* done;  // cleared: workgroups of xe_combine_kernel that have left their tile's loss
 };
 
 constexpr int kXeCols = 128;  // columns that a workgroup lays out, of 32 rows
@@ -154,94 +157,93 @@ __device__ __forceinline__ void xe_put(float (&v)[8], float scale, char* to)
     }
 }
 
-__device__ __forceinline__ float xe_block_max(float v, float* shared)
+__device__ __forceinline__ float xe_power(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }  // 2^e, -127 < e < 128
+
+// The power of two that takes a largest magnitude to 2^14 .. 2^15, as far as it and its inverse are numbers; that of no values at all is as large
+// as any.
+__device__ __forceinline__ int xe_exponent(float most)
 {
-#pragma unroll
-    for (int d = kWave / 2; d >= 1; d >>= 1) v = fmaxf(v, __shfl_xor(v, d, kWave));
-    if (lane_id() == 0) shared[threadIdx.x / kWave] = v;
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < kXeWaves; ++k) v = fmaxf(v, shared[k]);
-    return v;
+    const int e = kXeTop + 127 - (int)(__float_as_uint(most) >> 23);
+    return e > 100 ? 100 : e;  // (at least -113)
 }
 
-// The largest magnitude of what worker `worker` of `workers` (waves) has of a matrix (what is not a number is passed over).
-__device__ __forceinline__ float xe_most(const XeMatrix& m, int dim, int worker, int workers)
-{
-    const float* src = static_cast<const float*>(m.src);
-    float v = 0.0f;
-    // 1024 values of a line at a time: of a row, or of a column where those lie side by side, or of all rows if there is no gap between them
-    const bool rows = m.col_stride == 1, one = rows && m.row_stride == dim;
-    const int64_t lines = one ? 1 : rows ? m.rows : dim, length = one ? m.rows * dim : rows ? dim : m.rows;
-    const int64_t step = rows ? m.row_stride : m.col_stride, unit = rows ? 1 : m.row_stride, each = (length + 1023) / 1024;
-    const int lane = lane_id();
-    for (int64_t k = worker; k < lines * each; k += workers) {
-        const int64_t line = k / each, first = (k - line * each) * 1024;
-        const float* p = src + line * step;
-        if (unit == 1 && first + 1024 <= length) {
-            typedef float Vec __attribute__((ext_vector_type(4), aligned(4)));
-            Vec q[4];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) q[c] = *reinterpret_cast<const Vec*>(p + first + c * 256 + 4 * lane);
-#pragma unroll
-            for (int c = 0; c < 4; ++c) v = fmaxf(v, fmaxf(fmaxf(fabsf(q[c][0]), fabsf(q[c][1])), fmaxf(fabsf(q[c][2]), fabsf(q[c][3]))));
-        } else {
-            const int64_t end = first + 1024 < length ? first + 1024 : length;
-#pragma unroll 4
-            for (int64_t c = first + lane; c < end; c += kWave) v = fmaxf(v, fabsf(p[c * unit]));
-        }
-    }
-    return v;
-}
-
-// Workgroup (i, m) of kBlock x 2: part i of matrix m.
-__global__ __launch_bounds__(kBlock) void xe_most_kernel(const XeMatrix m0, const XeMatrix m1, int dim, float* __restrict__ most)
-{
-    __shared__ float shared[kXeWaves];
-    const int wave = (int)(threadIdx.x / kWave);
-    const float v = xe_block_max(xe_most(blockIdx.y == 0 ? m0 : m1, dim, (int)blockIdx.x * kXeWaves + wave, kBlock * kXeWaves), shared);
-    if (threadIdx.x == 0) most[blockIdx.y * kBlock + blockIdx.x] = v;
-}
-
-// The power of two that takes a largest magnitude to 2^14 .. 2^15; bounded, so that two of them and a bias are no infinity.
-__device__ __forceinline__ float xe_scale(float most)
-{
-    int e = kXeTop + 127 - (int)(__float_as_uint(most) >> 23);
-    if (most == 0.0f) e = 0;
-    e = e < -60 ? -60 : e > 45 ? 45 : e;
-    return __uint_as_float((uint32_t)(127 + e) << 23);
-}
+__device__ __forceinline__ float xe_finite(float v) { return fabsf(v) < INFINITY ? fabsf(v) : 0.0f; }
 
 template <typename T, int PARTS>
 __global__ __launch_bounds__(kBlock) void xe_images_kernel(const XeImagesArgs g)
 {
     __shared__ float tile[32 * kXePitch];
+    __shared__ int live[32];  // rows that there are, and that have a label
     const int64_t id = blockIdx.x;
     const bool classes = id >= g.first_tiles;
     const XeMatrix& m = g.m[classes ? 1 : 0];
     const int64_t t = classes ? id - g.first_tiles : id, row0 = 32 * t;
     const int col0 = kXeCols * (int)blockIdx.y, thread = (int)threadIdx.x;
     const T* src = static_cast<const T*>(m.src);
-    float scale_x = 1.0f, scale_w = 1.0f;
-    if constexpr (PARTS == 2) {
-        __shared__ float shared[2][kXeWaves];
-        float most_x, most_w;
-        if (g.most != nullptr) {
-            most_x = g.most[thread];
-            most_w = g.most[kBlock + thread];
-        } else {
-            most_x = xe_most(g.m[0], g.dim, thread / kWave, kXeWaves);
-            most_w = xe_most(g.m[1], g.dim, thread / kWave, kXeWaves);
+    if (id == 0 && blockIdx.y == 0 && thread == 0) *g.done = 0;
+    float bias = -INFINITY;
+    int label = -1;  // none
+    if (thread < 32) {
+        const int64_t row = row0 + thread;
+        if (row < m.rows) {
+            if (classes) {
+                bias = m.bias != nullptr ? (float)static_cast<const T*>(m.bias)[row] : 0.0f;
+                bias = bias <= kXeLeftOut ? -INFINITY : PARTS == 2 ? bias * kXeLog2e : bias;
+            } else {
+                const int64_t y = g.label64 ? static_cast<const int64_t*>(m.labels)[row] : (int64_t) static_cast<const int32_t*>(m.labels)[row];
+                if (y != g.ignore) label = y >= 0 && y < g.classes ? (int)y : -2;  // (-2: no such class)
+            }
         }
-        scale_x = xe_scale(xe_block_max(most_x, shared[0]));
-        scale_w = xe_scale(xe_block_max(most_w, shared[1]));
-        if (id == 0 && blockIdx.y == 0 && thread == 0) {
-            g.scales[0] = scale_x;
-            g.scales[1] = scale_w;
+        live[thread] = row < m.rows && (classes || label != -1);
+    }
+    __syncthreads();
+    int exponent = 0;      // the tile's
+    float row_scale = 1.0f;  // of the row that this thread's lane has in S
+    bool mixed = false;
+    if constexpr (PARTS == 2) {
+        // the largest magnitude of each row, eight threads a row, what is not finite passed over
+        __shared__ float most[8][32];
+        const bool by_rows = m.col_stride == 1;
+        const int r = by_rows ? thread / 8 : thread % 32, part = by_rows ? thread % 8 : thread / 32;
+        float v = 0.0f;
+        if (live[r]) {
+            const T* p = src + (row0 + r) * m.row_stride;
+            typedef T Vec __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+            if (by_rows) {
+                int c = 4 * part;
+                for (; c + 4 <= g.dim; c += 32) {
+                    const Vec q = *reinterpret_cast<const Vec*>(p + c);
+                    v = fmaxf(v, fmaxf(fmaxf(xe_finite((float)q[0]), xe_finite((float)q[1])), fmaxf(xe_finite((float)q[2]), xe_finite((float)q[3]))));
+                }
+                for (; c < g.dim; ++c) v = fmaxf(v, xe_finite((float)p[c]));
+            } else {
+                for (int c = part; c < g.dim; c += 8) v = fmaxf(v, xe_finite((float)p[c * m.col_stride]));
+            }
+        }
+        most[part][r] = v;
+        __syncthreads();
+        float of_row = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) of_row = fmaxf(of_row, most[k][thread % 32]);
+        float of_tile = of_row;
+#pragma unroll
+        for (int d = 16; d >= 1; d >>= 1) of_tile = fmaxf(of_tile, __shfl_xor(of_tile, d, kWave));
+        exponent = xe_exponent(of_tile);
+        const int own = xe_exponent(of_row), above = own - exponent < kXeFar ? own - exponent : kXeFar;
+        const int f = of_row > 0.0f && above > kXeNear ? exponent + above : exponent;
+        mixed = __any(f != exponent);
+        row_scale = xe_power(f);
+        if (blockIdx.y == 0 && thread < 32) {
+            float* c = reinterpret_cast<float*>(m.s_image + t * kXeChunk * (1 + 2LL * g.blocks * g.slices * PARTS));
+            c[kXeRow + thread] = xe_power(-f);
+            c[kXeRowInTile + thread] = xe_power(exponent - f);
+            if (thread == 0) {
+                c[kXeTile] = xe_power(-exponent);
+                reinterpret_cast<int*>(c)[kXeExponent] = exponent;
+                reinterpret_cast<int*>(c)[kXeMixed] = mixed;
+            }
         }
     }
-    const float scale = classes ? scale_w : scale_x;
-    if (id == 0 && blockIdx.y == 0 && thread == 0) *g.done = 0;
     if (m.col_stride == 1) {
         typedef T Vec __attribute__((ext_vector_type(8), aligned(sizeof(T))));
 #pragma unroll
@@ -250,7 +252,7 @@ __global__ __launch_bounds__(kBlock) void xe_images_kernel(const XeImagesArgs g)
             float v[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[j] = 0.0f;
-            if (row0 + r < m.rows) {
+            if (live[r]) {
                 const T* p = src + (row0 + r) * m.row_stride + col0 + c;
                 if (left >= 8) {
                     const Vec q = *reinterpret_cast<const Vec*>(p);
@@ -269,29 +271,14 @@ __global__ __launch_bounds__(kBlock) void xe_images_kernel(const XeImagesArgs g)
 #pragma unroll
         for (int k = 0; k < 32 * kXeCols / kBlock; ++k) {
             const int at = thread + k * kBlock, r = at % 32, c = at / 32;
-            const bool there = row0 + r < m.rows && col0 + c < g.dim;
-            tile[r * kXePitch + c] = there ? (float)src[(row0 + r) * m.row_stride + (col0 + c) * m.col_stride] : 0.0f;
+            tile[r * kXePitch + c] = live[r] && col0 + c < g.dim ? (float)src[(row0 + r) * m.row_stride + (col0 + c) * m.col_stride] : 0.0f;
         }
     }
     const int all_blocks = g.blocks * g.slices, steps = 2 * all_blocks;
     char* s_tile = m.s_image + t * kXeChunk * (1 + (int64_t)steps * PARTS);
     if (blockIdx.y == 0 && thread < 32) {
-        const int64_t row = row0 + thread;
-        if (classes) {
-            float b = -INFINITY;
-            if (row < m.rows) {
-                b = m.bias != nullptr ? (float)static_cast<const T*>(m.bias)[row] : 0.0f;
-                if (b <= kXeLeftOut) b = -INFINITY;
-            }
-            reinterpret_cast<float*>(s_tile)[thread] = b * scale_x * scale_w;  // (it goes where their products go)
-        } else {
-            int label = -1;  // none
-            if (row < m.rows) {
-                const int64_t y = g.label64 ? static_cast<const int64_t*>(m.labels)[row] : (int64_t) static_cast<const int32_t*>(m.labels)[row];
-                if (y != g.ignore) label = y >= 0 && y < g.classes ? (int)y : -2;  // (-2: no such class)
-            }
-            reinterpret_cast<int*>(s_tile)[kXeLabel + thread] = label;
-        }
+        if (classes) reinterpret_cast<float*>(s_tile)[thread] = bias;
+        else reinterpret_cast<int*>(s_tile)[kXeLabel + thread] = label;
     }
     __syncthreads();
 #pragma unroll
@@ -301,7 +288,7 @@ __global__ __launch_bounds__(kBlock) void xe_images_kernel(const XeImagesArgs g)
         float v[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = tile[lane % 32 * kXePitch + at / kWave * 16 + lane / 32 * 8 + j];
-        xe_put<PARTS>(v, scale, s_tile + kXeChunk * (1 + (int64_t)step * PARTS) + lane * 16);
+        xe_put<PARTS>(v, row_scale, s_tile + kXeChunk * (1 + (int64_t)step * PARTS) + lane * 16);
     }
     if (m.p_image == nullptr) return;
     char* p_tile = m.p_image + t * kXeChunk * ((int64_t)steps * PARTS);
@@ -314,7 +301,7 @@ __global__ __launch_bounds__(kBlock) void xe_images_kernel(const XeImagesArgs g)
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = tile[(half * 16 + j / 4 * 8 + lane / 32 * 4 + j % 4) * kXePitch + own * 32 + lane % 32];
         const int slice = block / g.blocks, in_slice = block % g.blocks;
-        xe_put<PARTS>(v, scale, p_tile + kXeChunk * ((((int64_t)slice * 2 + half) * g.blocks + in_slice) * PARTS) + lane * 16);
+        xe_put<PARTS>(v, xe_power(exponent), p_tile + kXeChunk * ((((int64_t)slice * 2 + half) * g.blocks + in_slice) * PARTS) + lane * 16);
     }
 }
 
@@ -366,9 +353,8 @@ struct XeArgs {
     const char* passed;
     const char* passed_p;  // P image
     int kept_tiles;
-    float* stats;  // [slot][wave][row of 32]: maximum, others' sum, label's logit, -  (weights: sum, -, -, -)
+    float* stats;  // [slot][wave][row of 32]: maximum, others' sum, label's logit (powers of two), -  (weights: sum, -, -, -)
     float* part;   // [slot][wave][block][quarter][lane][4]
-    const float* scales;  // fp32: of rows and classes
     XeFactor factor;      // weights: of all results
     // weights of groups that one workgroup has alone: straight to the result
     void* d_w;
@@ -452,21 +438,22 @@ template <int DB, int PARTS, int USE, bool WIDE>
 struct XeWave {
     static constexpr int kSteps = WIDE ? 4 * DB : 2 * DB;
     static constexpr int kSChunks = 1 + kSteps * PARTS, kPChunks = 2 * DB * PARTS;
-    static constexpr float kRise = PARTS == 2 ? kXeRise : 0.0f;
 
     XeOp kept[kSteps][PARTS];
     XeF32x16 o[USE == kXeLoss ? 1 : DB];
     float start;          // weights: the class's bias
-    float unit;           // what S is to be multiplied by (fp32: its operands are scaled)
-    float top, sum, own;  // running maximum (a power of two; weights, fp32: what P is below, a power of two itself), sum, the label's logit
+    float unit;           // fp32: what the row's power of two makes of S
+    float top, sum, own;  // running maximum (a power of two; weights, fp32: what P is below, a power of two itself), sum, the label's logit (a power of two)
     int label;            // weights: the class
+    int rise;             // fp32, rows: power of two that O is multiplied by
     bool bias_sum;
 
     // S^T of the staged tile
     __device__ __forceinline__ XeF32x16 logits(const char* s) const
     {
-        XeF32x16 acc;
-        if constexpr (USE == kXeWeights) {
+        XeF32x16 acc = {};
+        if constexpr (PARTS == 2) {
+        } else if constexpr (USE == kXeWeights) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) acc[i] = start;
         } else {
@@ -496,10 +483,40 @@ struct XeWave {
         return acc;
     }
 
-    // S^T -> P^T, with the running maximum, sum and the label's logit.  v0: the tile's first class.
-    __device__ __forceinline__ void shares(XeF32x16& s, int v0)
+    // Four values of the staged tile's rows that a lane's values 4 q .. 4 q + 3 of S^T belong to.
+    static __device__ __forceinline__ XeF4 of_rows(const char* tile, int what, int q)
     {
-        const float to2 = kXeLog2e * unit;
+        return *reinterpret_cast<const XeF4*>(reinterpret_cast<const float*>(tile) + what + 8 * q + 4 * (lane_id() / 32));
+    }
+    static __device__ __forceinline__ int of_tile(const char* tile, int what) { return __builtin_amdgcn_readfirstlane(reinterpret_cast<const int*>(tile)[what]); }
+
+    // fp32: S^T in the tile's powers of two, and what takes it to powers of two of the shares
+    __device__ __forceinline__ float even(XeF32x16& s, const char* tile) const
+    {
+        if (of_tile(tile, kXeMixed)) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const XeF4 f = of_rows(tile, kXeRowInTile, q);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) s[4 * q + j] *= f[j];
+            }
+        }
+        return unit * (__int_as_float(of_tile(tile, kXeTile)) * kXeLog2e);
+    }
+
+    // S^T -> P^T, with the running maximum, sum and the label's logit.  v0: the tile's first class.
+    __device__ __forceinline__ void shares(XeF32x16& s, const char* tile, int v0)
+    {
+        if constexpr (PARTS == 2) {
+            const float to2 = even(s, tile);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const XeF4 bias = of_rows(tile, 0, q);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) s[4 * q + j] = fmaf(s[4 * q + j], to2, bias[j]);
+            }
+        }
+        constexpr float kTo2 = PARTS == 2 ? 1.0f : kXeLog2e;
         const int in_tile = label - v0;
         const bool here = label >= 0 && in_tile >= 0 && in_tile < 32;
         if (__any(here)) {
@@ -507,7 +524,7 @@ struct XeWave {
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 if (at == 8 * (i / 4) + i % 4) {
-                    own = s[i] * unit;
+                    own = s[i] * kTo2;
                     s[i] = -INFINITY;
                 }
             }
@@ -515,7 +532,7 @@ struct XeWave {
         float most = s[0];
 #pragma unroll
         for (int i = 1; i < 16; ++i) most = fmaxf(most, s[i]);
-        most = fmaxf(most, xe_other_half(most)) * to2;
+        most = fmaxf(most, xe_other_half(most)) * kTo2;
         if (__any(most > top + kXeStep)) {
             const float now = fmaxf(top, most);
             const float scale = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top - now);
@@ -523,10 +540,28 @@ struct XeWave {
             sum *= scale;
             if constexpr (USE == kXeLossAndRows) rescale(scale);
         }
-        const float shift = top == -INFINITY ? 0.0f : kRise - top;
+        const float shift = top == -INFINITY ? 0.0f : -top;
+        if constexpr (PARTS == 1) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], to2, shift));
-        add_up(s);
+            for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], kXeLog2e, shift));
+            add_up(s, 1.0f);
+        } else {
+            // P times 2^(rise - e), at most 2^14, so that with classes times 2^e all tiles' sums are times 2^rise (the loss alone: for the same bits)
+            const int most_rise = of_tile(tile, kXeExponent) + kXeRise;
+            if (most_rise < rise) {
+                if constexpr (USE == kXeLossAndRows) rescale(most_rise - rise < -126 ? 0.0f : xe_power(most_rise - rise));
+                rise = most_rise;
+            }
+            const int below = most_rise - rise, little = below < 60 ? below : 60;
+            const float up = shift + (float)(kXeRise - little);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(s[i] + up);
+            add_up(s, xe_power(little - kXeRise));
+            if (USE == kXeLossAndRows && below > little) {  // (classes so small beside others that fp16 has nothing of their sums; the shares count all the same)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[i] = 0.0f;
+            }
+        }
     }
 
     __device__ __forceinline__ void rescale(float scale)
@@ -537,25 +572,26 @@ struct XeWave {
             for (int i = 0; i < 16; ++i) o[d][i] *= scale;
     }
 
-    __device__ __forceinline__ void add_up(const XeF32x16& p)
+    __device__ __forceinline__ void add_up(const XeF32x16& p, float scale)
     {
         float t[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) t[i] = p[i] + p[i + 8];
-        sum += ((t[0] + t[4]) + (t[1] + t[5])) + ((t[2] + t[6]) + (t[3] + t[7]));
+        sum += (((t[0] + t[4]) + (t[1] + t[5])) + ((t[2] + t[6]) + (t[3] + t[7]))) * scale;
     }
 
     // S^T -> the gradient of the logits, from the maxima, factors and labels of the tile's rows.  Returns whether a label is among them.
     __device__ __forceinline__ bool gradients(XeF32x16& s, const char* tile, int v0)
     {
-        const float* c = reinterpret_cast<const float*>(tile);
         const int* l = reinterpret_cast<const int*>(tile);
-        const int first = 4 * (lane_id() / 32);
+        float to2 = kXeLog2e;
+        if constexpr (PARTS == 2) to2 = even(s, tile);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-            const XeF4 shift = *reinterpret_cast<const XeF4*>(c + kXeShift + 8 * q + first), factor = *reinterpret_cast<const XeF4*>(c + kXeFactor + 8 * q + first);
+            const XeF4 shift = of_rows(tile, kXeShift, q), factor = of_rows(tile, kXeFactor, q);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) s[4 * q + j] = __builtin_amdgcn_exp2f(fmaf(s[4 * q + j], kXeLog2e * unit, shift[j])) * factor[j];
+            for (int j = 0; j < 4; ++j)
+                s[4 * q + j] = __builtin_amdgcn_exp2f(fmaf(s[4 * q + j], to2, PARTS == 2 ? shift[j] + start : shift[j])) * factor[j];
         }
         const int in_tile = l[kXeLabel + lane_id() % 32] - v0;
         const bool labels_here = __any(in_tile >= 0 && in_tile < 32);
@@ -563,24 +599,26 @@ struct XeWave {
             typedef int I4 __attribute__((ext_vector_type(4)));
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                const I4 labels = *reinterpret_cast<const I4*>(l + kXeLabel + 8 * q + first);
-                const XeF4 values = *reinterpret_cast<const XeF4*>(c + kXeOwn + 8 * q + first);
+                const I4 labels = __builtin_bit_cast(I4, of_rows(tile, kXeLabel, q));
+                const XeF4 values = of_rows(tile, kXeOwn, q);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) s[4 * q + j] = labels[j] == label ? values[j] : s[4 * q + j];
             }
         }
-        if (bias_sum) add_up(s);
-        if constexpr (PARTS == 2) {  // to fp16's range: 2^14 is what a class's values are below, sixteen times its largest one when that was met
+        if (bias_sum) add_up(s, 1.0f);
+        if constexpr (PARTS == 2) {
+            // Times 2^-e, for rows times 2^e, and to fp16's range: 2^14 is what a class's values are below, sixteen times the largest one when that was met
+            const float of_e = __int_as_float(of_tile(tile, kXeTile));
             float most = fabsf(s[0]);
 #pragma unroll
             for (int i = 1; i < 16; ++i) most = fmaxf(most, fabsf(s[i]));
-            most = fmaxf(most, xe_other_half(most));
+            most = fmaxf(most, xe_other_half(most)) * of_e;
             if (__any(most > top)) {
-                const float now = most > top ? __uint_as_float((__float_as_uint(fminf(most, 0x1p100f)) & 0x7F800000u) + (4u << 23)) : top;
+                const float now = most > top ? __uint_as_float((__float_as_uint(fminf(most, 0x1p122f)) & 0x7F800000u) + (4u << 23)) : top;
                 rescale(top / now);
                 top = now;
             }
-            const float scale = (float)(1 << kXeTop) / top;
+            const float scale = fminf((float)(1 << kXeTop) / top * of_e, 0x1p120f);  // (more only where all values are zero)
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[i] *= scale;
         }
@@ -640,7 +678,7 @@ struct XeWave {
         if (!active) return;
         p = logits(s);
         if constexpr (USE == kXeWeights) both = gradients(p, s, v0);
-        else shares(p, n0);
+        else shares(p, s, n0);
     }
     // The same where LDS has room for two S tiles: the next one is on its way from the start of this one
     __device__ __forceinline__ void first_half_of_two(const char* __restrict__ s, char* __restrict__ next_p, char* __restrict__ next_s, const char* src_p, const char* src_s,
@@ -651,7 +689,7 @@ struct XeWave {
         if (!active) return;
         p = logits(s);
         if constexpr (USE == kXeWeights) both = gradients(p, s, v0);
-        else shares(p, n0);
+        else shares(p, s, n0);
     }
     __device__ __forceinline__ void second_half(const char* __restrict__ s, char* __restrict__ next, const char* src, const XeF32x16& p, bool both, bool active)
     {
@@ -752,7 +790,8 @@ __global__ __launch_bounds__(kBlock, xe_waves(DB, PARTS, USE, WIDE)) void xe_ker
 #pragma unroll
         for (int p = 0; p < PARTS; ++p) w.kept[k][p] = xe_operand(own + kXeChunk + (k * PARTS + p) * kXeChunk);
     w.unit = 1.0f;
-    if constexpr (PARTS == 2) w.unit = 1.0f / g.scales[0] * (1.0f / g.scales[1]);
+    if constexpr (PARTS == 2) w.unit = reinterpret_cast<const XeGlobal<const float>*>(own)[kXeRow + lane % 32];
+    w.rise = 1 << 20;
 #pragma unroll
     for (int d = 0; d < (USE == kXeLoss ? 1 : DB); ++d) w.o[d] = XeF32x16{};
     w.top = USE == kXeWeights ? 0x1p-100f : -INFINITY;
@@ -804,11 +843,8 @@ __global__ __launch_bounds__(kBlock, xe_waves(DB, PARTS, USE, WIDE)) void xe_ker
 
     w.sum += xe_other_half(w.sum);
     w.own += xe_other_half(w.own);
-    if constexpr (PARTS == 2) {
-        if constexpr (USE != kXeWeights) w.sum *= 1.0f / (1 << (int)kXeRise);
-        if constexpr (USE == kXeLossAndRows) w.rescale(1.0f / (1 << (int)kXeRise) / g.scales[1]);
-        if constexpr (USE == kXeWeights) w.rescale(w.top / (1 << kXeTop) / g.scales[0]);
-    }
+    if constexpr (PARTS == 2 && USE == kXeLossAndRows) w.rescale(xe_power(-w.rise));
+    if constexpr (PARTS == 2 && USE == kXeWeights) w.rescale(w.top / (1 << kXeTop));
     if constexpr (USE == kXeWeights) {
         if (t1 - t0 == plan.tiles) {
             xe_store_weights<typename std::conditional<PARTS == 1, __bf16, float>::type>(g, w.o, v0 + lane % 32, slice, w.sum);
@@ -938,8 +974,7 @@ __global__ __launch_bounds__(kBlock) void xe_combine_kernel(const XeCombineArgs 
         top = fmaxf(top, top_of[k][i]);
         own += own_of[k][i];
     }
-    const float own2 = own * kXeLog2e;
-    if (label >= 0) top = fmaxf(top, own2);
+    if (label >= 0) top = fmaxf(top, own);
     float rest = 0.0f;
     for (int k = each; k < parts; k += kEach) {
         const XeF4 v = k == each ? mine : s[k * kXeWaves * 32];
@@ -952,7 +987,7 @@ __global__ __launch_bounds__(kBlock) void xe_combine_kernel(const XeCombineArgs 
     rest = 0.0f;
 #pragma unroll
     for (int k = 0; k < kEach; ++k) rest += rest_of[k][i];
-    const float own_part = label >= 0 ? __builtin_amdgcn_exp2f(own2 - top) : 0.0f;
+    const float own_part = label >= 0 ? __builtin_amdgcn_exp2f(own - top) : 0.0f;
     const float total = rest + own_part, inverse = 1.0f / total, others = label == -2 ? NAN : rest * inverse;
     if (with_x && there) {
         XeF4 sum = {};
@@ -975,7 +1010,7 @@ __global__ __launch_bounds__(kBlock) void xe_combine_kernel(const XeCombineArgs 
     }
     if (block != 0) return;  // (the tile's first workgroup alone keeps what is the rows')
     if (thread < kWave) {
-        float loss = top - own2 < 64.0f ? log1pf(rest / own_part) : kXeLn2 * top + logf(total) - own;
+        float loss = top - own < 64.0f ? log1pf(rest / own_part) : kXeLn2 * (top - own) + logf(total);
         if (label == -2) loss = NAN;
         if (label == -1) loss = 0.0f;
         if (thread < 32) {
@@ -1169,7 +1204,7 @@ struct XeState {
     char *rows_s, *rows_p, *classes_s;  // (weights' gradient)
     XeRow* kept;
     float* d_x;
-    float *count, *scales;
+    float* count;
     int* done;
     size_t bytes;
 };
@@ -1178,9 +1213,8 @@ inline XeState xe_state(const XeProblem& p, int want, void* base)
 {
     Carver c(base);
     XeState s = {};
-    s.scales = c.take<float>(4);
-    s.count = s.scales + 2;
-    s.done = reinterpret_cast<int*>(s.scales + 3);
+    s.count = c.take<float>(2);
+    s.done = reinterpret_cast<int*>(s.count + 1);
     if (want != 0) s.kept = c.take<XeRow>((size_t)p.n);
     if (want & FGL_XENT_ROWS) s.d_x = c.take<float>((size_t)p.n * p.shape.cols());
     if (want & FGL_XENT_WEIGHTS) {
@@ -1194,7 +1228,7 @@ inline XeState xe_state(const XeProblem& p, int want, void* base)
 
 struct XeScratch {
     char *rows_s, *classes_s, *classes_p;
-    float *stats, *part, *tile_loss, *most;
+    float *stats, *part, *tile_loss;
     size_t bytes;
 };
 
@@ -1214,7 +1248,6 @@ inline XeScratch xe_forward_scratch(const XeProblem& p, int want, void* base)
     }
     s.stats = c.take<float>((size_t)plan.slots() * kXeWaves * 32 * 4);
     s.tile_loss = c.take<float>((size_t)p.row_tiles * 2);
-    s.most = c.take<float>(2 * kBlock);
     s.bytes = c.used();
     return s;
 }
@@ -1330,20 +1363,9 @@ FGL_EXPORT int fgl_linear_cross_entropy(const void* d_x, int64_t x_row_stride, i
     const int64_t tiles = (int64_t)p.row_tiles + p.class_tiles;
     FGL_REQUIRE(tiles < 1 << 24, "linear_cross_entropy: grid too large");
     const dim3 grid((unsigned)tiles, (unsigned)ceil_div(s.cols(), kXeCols)), block(kBlock);
-    // Few values: each workgroup looks for the largest itself, which a launch of its own takes longer for.
-    const bool few = (n_rows + n_classes) * dim <= 16384;
-    im.most = few ? nullptr : ws.most;
-    im.scales = st.scales;
     im.done = st.done;
-    if (dtype == FGL_F32) {
-        if (!few) {
-            hipLaunchKernelGGL(xe_most_kernel, dim3(kBlock, 2), block, 0, to, im.m[0], im.m[1], dim, ws.most);
-            FGL_CHECK_LAUNCH("xe_most_kernel");
-        }
-        hipLaunchKernelGGL((xe_images_kernel<float, 2>), grid, block, 0, to, im);
-    } else {
-        hipLaunchKernelGGL((xe_images_kernel<__bf16, 1>), grid, block, 0, to, im);
-    }
+    if (dtype == FGL_F32) hipLaunchKernelGGL((xe_images_kernel<float, 2>), grid, block, 0, to, im);
+    else hipLaunchKernelGGL((xe_images_kernel<__bf16, 1>), grid, block, 0, to, im);
     FGL_CHECK_LAUNCH("xe_images_kernel");
 
     XeArgs g = {};
@@ -1353,7 +1375,6 @@ FGL_EXPORT int fgl_linear_cross_entropy(const void* d_x, int64_t x_row_stride, i
     g.kept_tiles = p.row_tiles;
     g.stats = ws.stats;
     g.part = ws.part;
-    g.scales = st.scales;
     const int rc = want & FGL_XENT_ROWS ? launch_xe<kXeLossAndRows>(s, g, p.class_tiles, to) : launch_xe<kXeLoss>(s, g, p.class_tiles, to);
     if (rc != FGL_OK) return rc;
     FGL_CHECK_LAUNCH("xe_kernel");
@@ -1420,8 +1441,7 @@ FGL_EXPORT int fgl_linear_cross_entropy_backward(const float* d_loss_grad, int64
         g.kept_tiles = p.class_tiles;
         g.stats = ws.stats;
         g.part = ws.part;
-        g.scales = st.scales;
-        g.factor = factor;
+            g.factor = factor;
         g.d_w = d_dw;
         g.d_b = d_db;
         g.kept_rows = n_classes;

@@ -369,6 +369,55 @@ def test_logits_far_apart(cuda, dtype):
     check(x.to(dtype), w.to(dtype), None, y, reduction="none")
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("what", [float("nan"), float("inf"), 1e30])
+def test_what_padded_rows_hold_is_nobodys_matter(cuda, dtype, what):
+    x, w, b, y = make(cuda, 200, 130, 72, dtype, ignored=0.4)
+    x[y == -100] = 0.0
+    want_loss, want = check(x, w, b, y)
+    padded = x.clone()
+    padded[y == -100] = what
+    leaves = [t.detach().requires_grad_() for t in (padded, w, b)]
+    loss = fastgl.linear_cross_entropy(leaves[0], leaves[1], y, leaves[2])
+    gen = torch.Generator(device=cuda).manual_seed(1)
+    grads = torch.autograd.grad(loss, leaves, torch.rand((), generator=gen, device=cuda) + 0.5)
+    assert torch.equal(loss.detach(), want_loss) and all(torch.equal(p, q) for p, q in zip(grads, want))
+
+
+@pytest.mark.parametrize("far", [(0, 0), (-30, 10), (60, -50), (-90, 20)])
+def test_rows_and_classes_of_many_magnitudes(cuda, far):
+    """fp32: two kinds of rows and of classes in any order, powers of two apart, each with columns of its own; a kind's products are near 1.  A row's or
+    class's values that are within 2^12 of their tile's largest are taken with 2^-25 / 2^2 of their own largest, others with less: 2^-27 of it for either
+    factor, 2^-26 d max|x_i| max|w_v| for a logit."""
+    n, v, d = 150, 170, 64
+    gen = torch.Generator(device=cuda).manual_seed(5)
+    x, w, b = (torch.randn(s, generator=gen, device=cuda) for s in ((n, d), (v, d), (v,)))
+    w /= 4
+    scaled = torch.zeros(n, dtype=torch.float64, device=cuda)
+    rows, classes = (torch.randint(0, 2, (k,), generator=gen, device=cuda) for k in (n, v))
+    columns = torch.arange(d, device=cuda) // (d // 2)
+    power = 2.0 ** torch.tensor(far, device=cuda, dtype=torch.float64)
+    for k in (0, 1):
+        most = x[rows == k][:, columns == k].abs().amax(1).double() * float(w[classes == k][:, columns == k].abs().max())
+        scaled[rows == k] = 2.0 ** -26 * d * most
+    x = torch.where(rows[:, None] == columns, x * power[rows][:, None], 0.0).float()
+    w = torch.where(classes[:, None] == columns, w / power[classes][:, None], 0.0).float()
+    y = torch.randint(0, v, (n,), generator=gen, device=cuda)
+    leaves = [t.detach().requires_grad_() for t in (x, w, b)]
+    losses = fastgl.linear_cross_entropy(leaves[0], leaves[1], y, leaves[2], reduction="none")
+    g = torch.ones(n, device=cuda)
+    grads = torch.autograd.grad(losses, leaves, g)
+    (want, _, *want_grads), sums, largest = definition(x, w, b, y, -100, "none", g)
+    u = 2.0 ** -24
+    most = (x.abs().double() @ w.abs().double().t()).amax(1) + float(b.abs().max())
+    eps = 4 * u * (18 + d / 64 + 4) * (most + 4) + (v / 32 + 8) * u + 4 * scaled
+    assert ((losses.detach().double() - want).abs() <= eps * (1 + want)).all(), float(((losses.detach().double() - want).abs() / eps).max())
+    for name, got, exact, total, top in zip(("dx", "dw", "db"), grads, want_grads, sums, largest):
+        terms = n if name != "dx" else v
+        limit = (2 * eps.max() + (terms / 32 + 16) * u + 12 * u) * total + u * exact.abs() + terms * 2.0 ** -35 * top + 2.0 ** -120
+        assert ((got.double() - exact).abs() <= limit).all(), (name, float(((got.double() - exact).abs() / limit).max()))
+
+
 def test_layer(cuda):
     torch.manual_seed(0)
     layer = fastgl.LinearCrossEntropy(48, 37).to(cuda)
