@@ -1188,13 +1188,14 @@ struct XeProblem {
 
 inline bool xe_problem(int64_t n, int64_t classes, int dim, int dtype, XeProblem* p)
 {
-    if (n < 1 || n >= (1LL << 31) - 64 || classes < 1 || classes >= (1LL << 31) - 64 || dim < 1 || dim > kXeMaxDim || (dtype != FGL_F32 && dtype != FGL_BF16)) return false;
+    if (n < 1 || n >= 1LL << 29 || classes < 1 || classes >= 1LL << 29 || dim < 1 || dim > kXeMaxDim || (dtype != FGL_F32 && dtype != FGL_BF16)) return false;
     p->n = n;
     p->classes = classes;
     p->dim = dim;
     p->dtype = dtype;
     p->row_tiles = (int)ceil_div(n, 32);
     p->class_tiles = (int)ceil_div(classes, 32);
+    if (p->row_tiles + (int64_t)p->class_tiles >= 1 << 24 || p->row_tiles * ceil_div(dim, 32) >= 1 << 23) return false;  // (launches have fewer than 2^32 threads)
     p->shape = xe_shape(dim, dtype);
     return true;
 }
@@ -1301,17 +1302,11 @@ void launch_xe_parts(const XeShape& s, const XeArgs& g, unsigned workgroups, hip
 }
 
 template <int USE>
-int launch_xe(const XeShape& s, XeArgs& g, int passed_tiles, hipStream_t stream)
+void launch_xe(const XeShape& s, XeArgs& g, int passed_tiles, hipStream_t stream)
 {
     g.plan = xe_plan(s, USE, g.kept_tiles, passed_tiles);
-    const int64_t workgroups = g.plan.workgroups();
-    if (workgroups >= 1 << 24) {
-        set_error("linear_cross_entropy: grid too large");
-        return FGL_ERR_UNSUPPORTED;
-    }
-    if (s.parts == 2) launch_xe_parts<2, USE>(s, g, (unsigned)workgroups, stream);
-    else launch_xe_parts<1, USE>(s, g, (unsigned)workgroups, stream);
-    return FGL_OK;
+    if (s.parts == 2) launch_xe_parts<2, USE>(s, g, (unsigned)g.plan.workgroups(), stream);
+    else launch_xe_parts<1, USE>(s, g, (unsigned)g.plan.workgroups(), stream);
 }
 
 }  // namespace fgl
@@ -1360,9 +1355,7 @@ FGL_EXPORT int fgl_linear_cross_entropy(const void* d_x, int64_t x_row_stride, i
     im.label64 = label64;
     im.ignore = ignore_index;
     im.classes = n_classes;
-    const int64_t tiles = (int64_t)p.row_tiles + p.class_tiles;
-    FGL_REQUIRE(tiles < 1 << 24, "linear_cross_entropy: grid too large");
-    const dim3 grid((unsigned)tiles, (unsigned)ceil_div(s.cols(), kXeCols)), block(kBlock);
+    const dim3 grid((unsigned)(p.row_tiles + p.class_tiles), (unsigned)ceil_div(s.cols(), kXeCols)), block(kBlock);
     im.done = st.done;
     if (dtype == FGL_F32) hipLaunchKernelGGL((xe_images_kernel<float, 2>), grid, block, 0, to, im);
     else hipLaunchKernelGGL((xe_images_kernel<__bf16, 1>), grid, block, 0, to, im);
@@ -1375,8 +1368,8 @@ FGL_EXPORT int fgl_linear_cross_entropy(const void* d_x, int64_t x_row_stride, i
     g.kept_tiles = p.row_tiles;
     g.stats = ws.stats;
     g.part = ws.part;
-    const int rc = want & FGL_XENT_ROWS ? launch_xe<kXeLossAndRows>(s, g, p.class_tiles, to) : launch_xe<kXeLoss>(s, g, p.class_tiles, to);
-    if (rc != FGL_OK) return rc;
+    if (want & FGL_XENT_ROWS) launch_xe<kXeLossAndRows>(s, g, p.class_tiles, to);
+    else launch_xe<kXeLoss>(s, g, p.class_tiles, to);
     FGL_CHECK_LAUNCH("xe_kernel");
 
     XeCombineArgs c = {};
@@ -1441,13 +1434,12 @@ FGL_EXPORT int fgl_linear_cross_entropy_backward(const float* d_loss_grad, int64
         g.kept_tiles = p.class_tiles;
         g.stats = ws.stats;
         g.part = ws.part;
-            g.factor = factor;
+        g.factor = factor;
         g.d_w = d_dw;
         g.d_b = d_db;
         g.kept_rows = n_classes;
         g.dim = dim;
-        const int rc = launch_xe<kXeWeights>(s, g, p.row_tiles, to);
-        if (rc != FGL_OK) return rc;
+        launch_xe<kXeWeights>(s, g, p.row_tiles, to);
         FGL_CHECK_LAUNCH("xe_kernel");
     }
     const bool parts = d_dw != nullptr && g.plan.shared != 1;
@@ -1474,7 +1466,6 @@ FGL_EXPORT int fgl_linear_cross_entropy_backward(const float* d_loss_grad, int64
     f.d_w = d_dw;
     f.d_b = d_db;
     const int64_t groups = dx_groups + (parts ? (int64_t)p.class_tiles * f.groups_per_tile : 0);
-    FGL_REQUIRE(groups < 1 << 24, "linear_cross_entropy_backward: grid too large");
     f.dx_groups = (int)dx_groups;
     if (together) hipLaunchKernelGGL(xe_finish_kernel<true>, dim3((unsigned)groups), block, 0, to, f);
     else hipLaunchKernelGGL(xe_finish_kernel<false>, dim3((unsigned)groups), block, 0, to, f);

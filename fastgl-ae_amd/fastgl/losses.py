@@ -14,8 +14,11 @@ def linear_cross_entropy(x, weight, labels, bias=None, ignore_index=-100, reduct
     """``cross_entropy(x weight^T + bias, labels)`` in float32, with gradients for ``x`` [n, d], ``weight`` [classes, d] (a transposed view of a
     [d, classes] weight will do) and ``bias`` [classes]: float32 or bfloat16, all of one type, ``d`` up to 512.  The logits are formed in pieces
     and never stored; sums, maxima and losses are float32.  ``labels`` [n]: int32 or int64; rows labelled ``ignore_index`` have no loss and no
-    gradient; a label outside ``[0, classes)`` makes a loss that is not a number.  A bias of -1e30 or less, ``-inf`` and the type's lowest value among them, leaves its class out; ``x`` and
-    ``weight`` are finite, logits below 1e9 in magnitude.  ``reduction``: ``"mean"`` over the rows that have a label (not a number if none has), ``"sum"`` or ``"none"``.
+    gradient, whatever they hold; a label outside ``[0, classes)`` makes a loss that is not a number.  A bias of -1e30 or less, ``-inf`` and the type's
+    lowest value among them, leaves its class out; ``weight`` and the other rows of ``x`` are finite, logits below 1e9 in magnitude.  float32 values
+    2^39 times smaller than the largest one of their row, or in the gradients of the 32 rows or classes around it, count as zero.  Fewer than 2^29
+    rows and classes together, and 2^28 pieces of 32 columns of ``x``.  ``reduction``: ``"mean"`` over the rows that have a label (not a number if
+    none has), ``"sum"`` or ``"none"``.
     Under autocast, its type is taken.  No gradients of gradients."""
     if not all(isinstance(t, torch.Tensor) and t.is_cuda for t in (x, weight, labels)) or not (bias is None or (isinstance(bias, torch.Tensor) and bias.is_cuda)):
         raise RuntimeError("x, weight, labels and bias must be CUDA tensors")

@@ -46,3 +46,11 @@ def test_sizes_of_state_and_workspace():
                 for dtype in (0, 1):
                     for want in (0, 1, 2, 3):
                         assert state(n, v, d, dtype, want) > 0 and ws(n, v, d, dtype, want, 0) > 0
+
+
+def test_sizes_beyond_a_launch_are_refused_before_the_forward_pass():
+    lib = fastgl.lib()
+    for n, v, d in ((1 << 29, 3, 8), (3, 1 << 29, 8), (1 << 28, 1 << 28, 8), (1 << 24, 3, 512), (1 << 28, 3, 32)):
+        assert lib.fgl_linear_cross_entropy_state_bytes(n, v, d, 1, 3) == 0 and lib.fgl_linear_cross_entropy_workspace_bytes(n, v, d, 1, 3, 1) == 0
+        assert lib.fgl_linear_cross_entropy(256, d, 1, 256, d, 1, None, 256, 1, -100, n, v, d, 1, 2, 3, 256, 256, 1 << 40, 256, 1 << 40, None) == 1
+    assert lib.fgl_linear_cross_entropy_state_bytes((1 << 24) - 32, 3, 512, 1, 3) > 0 and lib.fgl_linear_cross_entropy_state_bytes((1 << 28) - 32, 1 << 20, 32, 1, 3) > 0
