@@ -1156,19 +1156,23 @@ inline XePlan xe_plan(const XeShape& s, int use, int kept_tiles, int passed_tile
     p.groups = (int)ceil_div(kept_tiles, kXeWaves) * (use == kXeLoss ? 1 : s.slices);
     p.tiles = passed_tiles;
     const int room = 256 * xe_waves(s.blocks, s.parts, use, s.slices == 2);
-    // at least: so that a part's kept rows and results are little beside its tiles, and its slots few enough to add up
-    int least = (int)ceil_div(passed_tiles, use == kXeWeights ? 128 : kXeMaxParts - 2);
+    // at least: so that a part's kept rows and results are little beside its tiles, and for a loss so many parts that the combining kernel holds their
+    // sums in LDS.  (100 rows, 500 K classes, bf16: 410 us with 62 parts, 1230 with 16.  Weights, 100 K rows, 47 classes, bf16: backward 42 us with 512
+    // parts, 53 with 128, 135 with 32, and 69 with 1024, which the kernel's first tile and last stores are much of.)
+    int least = (int)ceil_div(passed_tiles, use == kXeWeights ? 512 : kXeMaxParts - 2);
     if (least < 2) least = 2;
     if (least > passed_tiles) least = passed_tiles;
     p.shared = p.groups < room ? room / p.groups : 1;
     p.per = (int)ceil_div(passed_tiles, p.shared);
     if (p.per < least) p.per = least;
-    // (the weights' gradient of a few tiles: without parts there is a launch less)
-    if (use == kXeWeights && passed_tiles <= 6) p.per = passed_tiles;
+    // The weights' gradient of a few tiles and many classes: parts would cost more to write and add up than they save.  (190 rows, 256 columns,
+    // backward, whole and in parts: bf16, 4 K classes 19 us and 20, 16 K 19 and 25, 32 K 23 and 37; fp32, 8 K classes 32 and 20, 16 K 34 and 34.)
+    if (use == kXeWeights && passed_tiles <= 6 && p.groups > 48 * s.parts) p.per = passed_tiles;
     p.shared = (int)ceil_div(passed_tiles, p.per);
     p.room = room;
     p.whole = 0;
-    // Where that leaves an eighth of the chip idle, in the only round or the last of a few: no regard for the groups' ends
+    // Where that leaves an eighth of the chip idle, in the only round or the last of a few: no regard for the groups' ends.  (40 K rows x 256, 20 K
+    // classes, bf16: forward 877 us so, 977 in whole groups; 100 K x 128, 10 K classes: 618 and 732.)
     const int64_t full = (int64_t)p.groups * p.shared, rounds = ceil_div(full, room);
     if (p.per > least && p.per > 6 && rounds <= 8 && full * 8 < rounds * room * 7 && (p.groups % room + 1LL) * passed_tiles < 1LL << 31) {
         p.whole = p.groups / room * room;
@@ -1444,6 +1448,7 @@ FGL_EXPORT int fgl_linear_cross_entropy_backward(const float* d_loss_grad, int64
     }
     const bool parts = d_dw != nullptr && g.plan.shared != 1;
     if (d_dx == nullptr && !parts) return FGL_OK;
+    // (8192 x 256, 47 classes, fp32, 128 parts: backward 20 us with four waves on them, 28 with one; with eight parts there is no difference)
     const bool together = parts && g.plan.shared > 8;
     XeFinishArgs f = {};
     f.kept = st.kept;
