@@ -23,11 +23,11 @@
 //
 // bf16: P is rounded to bf16, as the operands are.
 // fp32: each value is the sum of two fp16 values, of 11 bits each, and a product three matrix instructions (high low, low high, high high; what is
-// left out is 2^-22 of it), whose sum over 64 k is added to fp32 accumulators.  fp16's range is short, so a tile is first multiplied by a power of two
+// left out is 2^-22 of it) that add to fp32 accumulators.  fp16's range is short, so a tile is first multiplied by a power of two
 // that takes its largest value to 2^14; what lies 2^39 below that is lost.  In S a row that is 2^12 below its tile's largest value gets a
 // power of its own, which costs its tile a multiplication a logit.  P is scaled likewise, by the running maximum, and the gradient of the logits by a
-// running bound of its own.  Against 64 bits, 2-norm, 8192 x 128 and 20 K classes: 2.2e-7; the same in fp32 products by the library 1.7e-6, in three
-// bf16 parts and six instructions 1.9e-7, in 1.6 times the time.
+// running bound of its own.  Against 64 bits, 2-norm, the weights' gradient, 2048 x 128 and 20 K classes: 2.6e-7; the same in
+// fp32 products by the library 8.1e-7.
 // Sums, maxima and losses are fp32 in both.  x and w must be finite: others make losses and gradients that are not numbers, but in rows
 // without a label, which are taken as zeros.
 // A bias of -1e30 or less, -infinity among them, leaves its class out: no share, no gradient.  (bf16: shares are exp2 of one fma, whose
@@ -50,6 +50,8 @@ namespace fgl {
 typedef float XeF4 __attribute__((ext_vector_type(4)));
 typedef float XeF32x16 __attribute__((ext_vector_type(16)));
 typedef uint32_t XeOp __attribute__((ext_vector_type(4)));  // eight values of a matrix instruction's operand
+typedef float XeF2 __attribute__((ext_vector_type(2)));
+typedef _Float16 XeF16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 XeF16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kXeWaves = kBlock / kWave;
@@ -124,10 +126,17 @@ constexpr int kXePitch = kXeCols + 4;
 __device__ __forceinline__ void xe_split(const float (&v)[8], XeOp& hi, XeOp& lo)
 {
     XeF16x8 h, l;
+    float minus = -1.0f;
+    asm("" : "+s"(minus));  // (so that the difference is the one instruction that takes an fp16 operand)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        h[j] = (_Float16)v[j];
-        l[j] = (_Float16)(v[j] - (float)h[j]);
+    for (int j = 0; j < 8; j += 2) {
+        const XeF16x2 both = __builtin_convertvector((XeF2){v[j], v[j + 1]}, XeF16x2);
+        const XeF2 rest = {fmaf((float)both[0], minus, v[j]), fmaf((float)both[1], minus, v[j + 1])};
+        const XeF16x2 second = __builtin_convertvector(rest, XeF16x2);
+        h[j] = both[0];
+        h[j + 1] = both[1];
+        l[j] = second[0];
+        l[j + 1] = second[1];
     }
     hi = __builtin_bit_cast(XeOp, h);
     lo = __builtin_bit_cast(XeOp, l);
@@ -468,16 +477,10 @@ struct XeWave {
         if constexpr (PARTS == 1) {
             xe_products<kSteps, 1>(at, [&](int k, const XeOp (&a)[1]) { acc = xe_mfma<1>(a[0], kept[k][0], acc); });
         } else {
-            XeF32x16 chunk = {};
             xe_products<kSteps, 2>(at, [&](int k, const XeOp (&a)[2]) {
-                chunk = xe_mfma<2>(a[1], kept[k][0], chunk);
-                chunk = xe_mfma<2>(a[0], kept[k][1], chunk);
-                chunk = xe_mfma<2>(a[0], kept[k][0], chunk);
-                if (k % 4 == 3 || k == kSteps - 1) {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) acc[i] += chunk[i];
-                    chunk = XeF32x16{};
-                }
+                acc = xe_mfma<2>(a[1], kept[k][0], acc);
+                acc = xe_mfma<2>(a[0], kept[k][1], acc);
+                acc = xe_mfma<2>(a[0], kept[k][0], acc);
             });
         }
         return acc;
@@ -552,15 +555,11 @@ struct XeWave {
                 if constexpr (USE == kXeLossAndRows) rescale(most_rise - rise < -126 ? 0.0f : xe_power(most_rise - rise));
                 rise = most_rise;
             }
-            const int below = most_rise - rise, little = below < 60 ? below : 60;
+            const int below = most_rise - rise, little = below < 60 ? below : 60;  // (fp16 has nothing of 2^-60 times P; the sum has)
             const float up = shift + (float)(kXeRise - little);
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(s[i] + up);
             add_up(s, xe_power(little - kXeRise));
-            if (USE == kXeLossAndRows && below > little) {  // (classes so small beside others that fp16 has nothing of their sums; the shares count all the same)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) s[i] = 0.0f;
-            }
         }
     }
 
@@ -653,15 +652,20 @@ struct XeWave {
                 xe_products<2 * DB, 1>([&](int i) { return p + i * kXeChunk; }, [&](int i, const XeOp (&a)[1]) { o[i % DB] = xe_mfma<1>(a[0], w[i / DB][0], o[i % DB]); });
             }
         } else {
-            XeF32x16 chunk = {};
+            // O beyond eight blocks lies in the accumulator registers, and the compiler moves all of it back and forth for instructions that add to it
+            // (8192 rows, 10 K classes, forward, 300 columns 444 us so and 382 with additions of their own, 384 columns 1192 and 452; 256 columns 299
+            // and 318).
+            constexpr bool kOwn = DB > 8 || WIDE;
+            XeF32x16 sum = {};
             xe_products<2 * DB, 2>([&](int i) { return p + (i % 2 * DB + i / 2) * 2 * kXeChunk; }, [&](int i, const XeOp (&a)[2]) {
-                chunk = xe_mfma<2>(a[1], w[i % 2][0], chunk);
-                chunk = xe_mfma<2>(a[0], w[i % 2][1], chunk);
-                chunk = xe_mfma<2>(a[0], w[i % 2][0], chunk);
-                if (i % 2 == 1) {
+                XeF32x16& to = kOwn ? sum : o[i / 2];
+                to = xe_mfma<2>(a[1], w[i % 2][0], to);
+                to = xe_mfma<2>(a[0], w[i % 2][1], to);
+                to = xe_mfma<2>(a[0], w[i % 2][0], to);
+                if (kOwn && i % 2 == 1) {
 #pragma unroll
-                    for (int c = 0; c < 16; ++c) o[i / 2][c] += chunk[c];
-                    chunk = XeF32x16{};
+                    for (int c = 0; c < 16; ++c) o[i / 2][c] += sum[c];
+                    sum = XeF32x16{};
                 }
             });
         }

@@ -3,11 +3,11 @@
 Tolerances.  Let u = 2^-24 and M the largest sum of magnitudes sum_d |x_id w_vd| + |b_v| of a row.  bf16: products are exact, and added up one
 instruction of 16 columns after another: a logit is off by at most c u M, c = 2 + d / 16.  fp32: a value is taken as the sum of two fp16 values, off by
 2^-22 of it (half a step of the second, 2^-11, times 2^-11 for the first), and the product of the two second parts, 2^-22, is left out: 3 * 2^-22 = 12 u of
-each product; sums of 64 columns are added up: c = 14 + d / 64 + 64 / 16.  A value whose scaled second part is below fp16's normal numbers is off by
+each product; three instructions for 16 columns: c = 14 + 3 d / 16.  A value whose scaled second part is below fp16's normal numbers is off by
 2^-25 of 2^-14 times the matrix's largest: 2^-39 of it, once for either factor: 2^-38 d max|x| max|w| more.  The exponentials are off by 2 u and by u
 times their argument in powers of two, at most 2 M log2(e), more.  So a share p is off by eps = 4 u (c + 4) (M + 4) of itself and a loss by eps, and a sum
 of n shares adds one rounding for each tile of 32 and log-many: (n / 32 + 8) u.  Gradients are sums of p times finite values: bf16: p is
-rounded, 2^-8 more of each term; fp32: 3 * 2^-22 more, and as p is scaled by its row's largest, or by sixteen times that, 2^-25 of 2^-14 of those:
+rounded, 2^-8 more of each term; fp32: 3 * 2^-22 more and six instructions for a tile's 32 terms, (6 n / 32 + 8) u, and as p is scaled by its row's largest, or by sixteen times that, 2^-25 of 2^-14 of those:
 2^-35 of the largest term's p, times the largest value, for each term.  At last half a step of the result."""
 import pytest
 import torch
@@ -51,7 +51,7 @@ def share_error(x, w, b, n_terms):
     most = max(float((x.detach().abs().double() @ w.detach()[k:k + 4096].abs().double().t()).max()) for k in range(0, w.size(0), 4096))
     if b is not None:
         most += float(b.detach().double().abs().masked_fill(b.detach().isinf(), 0.0).max())
-    c = 18 + d / 64 if x.dtype == torch.float32 else 2 + d / 16
+    c = 14 + 3 * d / 16 if x.dtype == torch.float32 else 2 + d / 16
     scaled = 2.0 ** -38 * d * float(x.detach().abs().max()) * float(w.detach().abs().max()) if x.dtype == torch.float32 else 0.0
     return 4 * u * (c + 4) * (most + 4) + (n_terms / 32 + 8) * u + 4 * scaled
 
@@ -73,7 +73,7 @@ def check(x, w, b, y, reduction="mean", ignore=-100, g=None, limit_scale=1.0):
     for name, got, exact, total, most in zip(("dx", "dw", "db"), grads, want_grads, sums, largest):
         assert got.dtype == x.dtype and got.shape == exact.shape
         terms = n if name != "dx" else w.size(0)
-        limit = (2 * eps + (terms / 32 + 16) * 2.0 ** -24 + (half if x.dtype == torch.bfloat16 else 12 * half)) * total + half * exact.abs() + 2.0 ** -120
+        limit = (2 * eps + ((6 if x.dtype == torch.float32 else 2) * terms / 32 + 16) * 2.0 ** -24 + (half if x.dtype == torch.bfloat16 else 12 * half)) * total + half * exact.abs() + 2.0 ** -120
         if x.dtype == torch.float32:
             limit = limit + terms * 2.0 ** -35 * most
         off = (got.double() - exact).abs()
@@ -410,11 +410,11 @@ def test_rows_and_classes_of_many_magnitudes(cuda, far):
     (want, _, *want_grads), sums, largest = definition(x, w, b, y, -100, "none", g)
     u = 2.0 ** -24
     most = (x.abs().double() @ w.abs().double().t()).amax(1) + float(b.abs().max())
-    eps = 4 * u * (18 + d / 64 + 4) * (most + 4) + (v / 32 + 8) * u + 4 * scaled
+    eps = 4 * u * (14 + 3 * d / 16 + 4) * (most + 4) + (v / 32 + 8) * u + 4 * scaled
     assert ((losses.detach().double() - want).abs() <= eps * (1 + want)).all(), float(((losses.detach().double() - want).abs() / eps).max())
     for name, got, exact, total, top in zip(("dx", "dw", "db"), grads, want_grads, sums, largest):
         terms = n if name != "dx" else v
-        limit = (2 * eps.max() + (terms / 32 + 16) * u + 12 * u) * total + u * exact.abs() + terms * 2.0 ** -35 * top + 2.0 ** -120
+        limit = (2 * eps.max() + (6 * terms / 32 + 16) * u + 12 * u) * total + u * exact.abs() + terms * 2.0 ** -35 * top + 2.0 ** -120
         assert ((got.double() - exact).abs() <= limit).all(), (name, float(((got.double() - exact).abs() / limit).max()))
 
 
