@@ -2,7 +2,8 @@
 // and autograd nodes.
 //
 // A training step calls them once a layer, on rows that take the GPU tens of microseconds; recorded by a Python function, forward and
-// backward cost 90 us (dropout) and 130 us (the loss) of the host's time, here 35 and 45.
+// backward cost 90 us (dropout) and 130 us (the loss) of the host's time, here 46 and 73, on a host where torch's relu takes 42 (27, 45 and 24 on
+// a faster one).
 #include "fastgl_autograd.h"
 
 #include <ATen/autocast_mode.h>

@@ -26,8 +26,8 @@
 // left out is 2^-22 of it) that add to fp32 accumulators.  fp16's range is short, so a tile is first multiplied by a power of two
 // that takes its largest value to 2^14; what lies 2^39 below that is lost.  In S a row that is 2^12 below its tile's largest value gets a
 // power of its own, which costs its tile a multiplication a logit.  P is scaled likewise, by the running maximum, and the gradient of the logits by a
-// running bound of its own.  Against 64 bits, 2-norm, the weights' gradient, 2048 x 128 and 20 K classes: 2.6e-7; the same in
-// fp32 products by the library 8.1e-7.
+// running bound of its own.  Against 64 bits, 2-norm, all results of 8192 x 128 and 20 K classes: 4.5e-7; the same in
+// fp32 products by the library 1.7e-6.
 // Sums, maxima and losses are fp32 in both.  x and w must be finite: others make losses and gradients that are not numbers, but in rows
 // without a label, which are taken as zeros.
 // A bias of -1e30 or less, -infinity among them, leaves its class out: no share, no gradient.  (bf16: shares are exp2 of one fma, whose
@@ -38,6 +38,12 @@
 // several, each with a part of the passed tiles, or a workgroup goes on from one group to the next in the middle of it.  Who has but a
 // part of a group's tiles leaves its O, maximum and sum in scratch, and a combining kernel adds the parts up in order (the same bits on every
 // run).
+//
+// What bounds it: for many classes the matrix cores and, beside them, LDS, whose operands at 1 KB for an instruction of 32 cycles would take all of its
+// rate if the cores were never idle.  8192 x 256, 100 K classes, bf16: 735 .. 785 us forward, 765 .. 815 backward, 1.07 .. 1.14 PFLOP/s (a large matrix product
+// of the library 1.24), matrix cores busy 58 % of the cycles at the 1.83 GHz that the power limit leaves.  8192 x 128, 20 K classes, fp32: 235 .. 250 us and
+// 246 .. 262, 0.96 .. 1.07 PFLOP/s of fp16, busy 56 % (vector instructions: four for a logit's exponential, four for its parts).  The loss alone, bf16, is bound by
+// them: 2000 x 100, 100 K classes 66 us, busy 34 %.  For a few classes: launches of 5 to 20 us, mostly latency.
 #include "fgl_common.hpp"
 #include "fgl_kernels.hpp"
 
@@ -77,7 +83,7 @@ constexpr int kXeFar = 120;  // how far f is from e at most: 2^(e - f) is a numb
 // Sizes of a problem as the kernels see it: blocks of 32 columns, padded.  Beyond 384 columns, in bf16 beyond 256, in two slices, each with half of O,
 // which otherwise did not fit a wave's registers, and S formed for either.  (bf16 could have 384 columns whole, with one wave a SIMD instead of
 // two: 8192 rows, 20 K classes, forward, 300 columns 340 us against 352 in slices, 370 columns 556 against 352.  fp32 has one wave a SIMD
-// from 129 columns on anyway: 300 columns 686 whole, 1115 in slices.)
+// from 129 columns on anyway: 300 columns 678 whole, 1061 in slices.)
 struct XeShape {
     int blocks;  // in a slice
     int slices;

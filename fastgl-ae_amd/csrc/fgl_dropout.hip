@@ -8,7 +8,9 @@
 // With f = max(x, 0) the backward pass needs no generator: an element is kept and positive if and only if the output is not zero or
 // below (it is no smaller than x, as 1 / (1 - p) >= 1), and the output is there for the next layer's own gradient anyway.
 //
-// What bounds it: the pass over memory in fp32; in bf16 the generator's forty 32-bit products for four elements come close to it.
+// What bounds it: the pass over memory.  60 K x 256 fp32, forward or backward: 21 us, 5.9 TB/s as the kernel sees it (what was written just before is
+// read from the last-level cache); 2.4 M x 64 of rows of 100 columns: 277 us, back without gaps 202 us (6.1 TB/s).  In bf16 the generator's forty
+// 32-bit products for four elements are as long: 87 K x 256 with relu 24.5 us forward, 20.7 us backward with 1.5 times the bytes and no generator.
 #include "fgl_common.hpp"
 #include "fgl_kernels.hpp"
 
@@ -17,7 +19,7 @@
 namespace fgl {
 
 constexpr uint32_t kDropTag = 0x44524F50u;
-constexpr int kDropQuads = 4;  // fours of elements a thread
+constexpr int kDropQuads = 4;  // fours of elements a thread: four loads on their way at once
 constexpr int kDropTile = kBlock * kDropQuads * 4;
 constexpr int64_t kDropMost = 1LL << 35;  // elements of a call: a launch has fewer than 2^32 threads
 
