@@ -469,8 +469,10 @@ struct XeWave {
         XeF32x16 acc = {};
         if constexpr (PARTS == 2) {
         } else if constexpr (USE == kXeWeights) {
+            float bias = start;
+            asm volatile("" : "+v"(bias));  // (else sixteen copies of it are kept in registers through all tiles)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) acc[i] = start;
+            for (int i = 0; i < 16; ++i) acc[i] = bias;
         } else {
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
@@ -701,6 +703,21 @@ struct XeWave {
         if constexpr (USE == kXeWeights) both = gradients(p, s, v0);
         else shares(p, s, n0);
     }
+    // The same where LDS has room for two tiles of both: the next one is on its way all the while
+    __device__ __forceinline__ void tile(const char* __restrict__ s, const char* __restrict__ p_tile, char* __restrict__ next_s, char* __restrict__ next_p, const char* src_s,
+                                         const char* src_p, int n0, int v0, bool active)
+    {
+        if (src_s != nullptr) {
+            xe_stage<kSChunks>(src_s, next_s);
+            xe_stage<kPChunks>(src_p, next_p);
+        }
+        if (!active) return;
+        XeF32x16 p = logits(s);
+        bool both = false;
+        if constexpr (USE == kXeWeights) both = gradients(p, s, v0);
+        else shares(p, s, n0);
+        product(p, p_tile, both);
+    }
     __device__ __forceinline__ void second_half(const char* __restrict__ s, char* __restrict__ next, const char* src, const XeF32x16& p, bool both, bool active)
     {
         if (src != nullptr) xe_stage<kSChunks>(src, next);
@@ -749,10 +766,14 @@ template <int DB, int PARTS, int USE, bool WIDE>
 __global__ __launch_bounds__(kBlock, xe_waves(DB, PARTS, USE, WIDE)) void xe_kernel(const XeArgs g)
 {
     using Wave = XeWave<DB, PARTS, USE, WIDE>;
-    __shared__ __attribute__((aligned(16))) char s_buf[Wave::kSChunks * kXeChunk];
-    __shared__ __attribute__((aligned(16))) char p_buf[(USE == kXeLoss ? Wave::kSChunks : Wave::kPChunks) * kXeChunk];  // (the loss alone: two tiles in turn)
+    // bf16 and 161 columns or more, the loss and its rows: two tiles of both in LDS, and one wait and barrier a tile.  (8192 rows, 40 K classes, forward, 256
+    // columns 345 us so and 357 with one tile, 300 columns 688 and 703, 192 columns 282 and 286; 128 columns and fp32 no difference.  The weights'
+    // gradient, which has a second product for some tiles, has no registers left for the one loop body: 955 us for 353.)
+    constexpr bool kAll = USE == kXeLossAndRows && PARTS == 1 && DB >= 6 && !(WIDE && DB == 8);
+    __shared__ __attribute__((aligned(16))) char s_buf[(kAll ? 2 : 1) * Wave::kSChunks * kXeChunk];
+    __shared__ __attribute__((aligned(16))) char p_buf[(kAll ? 2 : 1) * (USE == kXeLoss ? Wave::kSChunks : Wave::kPChunks) * kXeChunk];  // (the loss alone: two tiles in turn)
     // In slices S is most of the work and O too little to hide the next S tile's copy behind.  (8192 x 512, 10 K classes, backward 399 us with
-    // one S tile, 348 with two.  Slices of 192 columns, two waves a SIMD, have no registers left for it.)
+    // one S tile, 348 with two; two of P as well, 1250 us for 1147 of 40 K classes, forward.  Slices of 192 columns, two waves a SIMD, have no registers left for it.)
     constexpr bool kTwo = WIDE && DB == 8 && PARTS == 1 && USE != kXeLoss;
     __shared__ __attribute__((aligned(16))) char s_other[(kTwo ? Wave::kSChunks : 1) * kXeChunk];
     constexpr int kSlices = WIDE && USE != kXeLoss ? 2 : 1;
@@ -818,8 +839,21 @@ __global__ __launch_bounds__(kBlock, xe_waves(DB, PARTS, USE, WIDE)) void xe_ker
     XeF32x16 p = {};
     bool both = false;
     xe_stage<Wave::kSChunks>(g.passed + t0 * kSBytes, s_buf);
+    if constexpr (kAll) xe_stage<Wave::kPChunks>(g.passed_p + slice * (int64_t)Wave::kPChunks * kXeChunk + t0 * kPBytes, p_buf);
     xe_staged();
-    if constexpr (USE == kXeLoss) {
+    if constexpr (kAll) {
+        const char* passed_p = g.passed_p + slice * (int64_t)Wave::kPChunks * kXeChunk;
+        int at_s = 0, at_p = 0;
+        for (int t = t0; t < t1; ++t) {
+            const int to_s = Wave::kSChunks * kXeChunk - at_s, to_p = Wave::kPChunks * kXeChunk - at_p;
+            const bool more = t + 1 < t1;
+            w.tile(s_buf + at_s, p_buf + at_p, s_buf + to_s, p_buf + to_p, more ? g.passed + (t + 1) * kSBytes : nullptr, more ? passed_p + (t + 1) * kPBytes : nullptr,
+                   32 * t, v0, active);
+            xe_staged();
+            at_s = to_s;
+            at_p = to_p;
+        }
+    } else if constexpr (USE == kXeLoss) {
         for (int t = t0; t < t1; t += 2) {
             w.first_half(s_buf, p_buf, t + 1 < t1 ? g.passed + (t + 1) * kSBytes : nullptr, p, both, 32 * t, v0, active);
             xe_staged();
