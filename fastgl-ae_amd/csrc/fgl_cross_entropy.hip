@@ -40,10 +40,11 @@
 // run).
 //
 // What bounds it: for many classes the matrix cores and, beside them, LDS, whose operands at 1 KB for an instruction of 32 cycles would take all of its
-// rate if the cores were never idle.  8192 x 256, 100 K classes, bf16: 735 .. 785 us forward, 765 .. 815 backward, 1.07 .. 1.14 PFLOP/s (a large matrix product
-// of the library 1.24), matrix cores busy 58 % of the cycles at the 1.83 GHz that the power limit leaves.  8192 x 128, 20 K classes, fp32: 235 .. 250 us and
-// 246 .. 262, 0.96 .. 1.07 PFLOP/s of fp16, busy 56 % (vector instructions: four for a logit's exponential, four for its parts).  The loss alone, bf16, is bound by
-// them: 2000 x 100, 100 K classes 66 us, busy 34 %.  For a few classes: launches of 5 to 20 us, mostly latency.
+// rate if the cores were never idle.  8192 x 256, 100 K classes, bf16: 725 .. 770 us forward, 770 .. 835 backward (the clock falls as the chip warms up),
+// 1.00 .. 1.16 PFLOP/s (a large matrix product of the library 1.24), matrix cores busy 63 and 57 % of the cycles at the 1.8 GHz that the power limit
+// leaves.  8192 x 128, 20 K classes, fp32: 242 .. 260 us and 250 .. 274, 0.92 .. 1.04 PFLOP/s of fp16, busy 54 and 50 % beside the exponentials and splits.
+// The loss alone, bf16, is bound by the exponentials, maxima and sums: 2000 x 100, 100 K classes 66 us, busy 34 %.  For a few classes: launches of 5 to
+// 20 us, mostly latency.
 #include "fgl_common.hpp"
 #include "fgl_kernels.hpp"
 
