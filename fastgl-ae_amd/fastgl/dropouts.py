@@ -35,7 +35,8 @@ class Dropout(nn.Module):
     """``dropout`` as a layer: ``seed`` makes the masks of a run, every call in training takes the next stream (``calls`` counts them;
     set it to repeat or resume a run).  Layers of one model take a seed each, or share one instance.  ``relu=True``: the activation before it goes with it, in
     evaluation too.  ``stream_offset``: as for ``dropout``, for calls that are captured in a graph (whose stream numbers are those of the
-    capture: advance it by more than the calls that one replay makes)."""
+    capture: advance it by more than the calls that one replay makes).  A layer that is computed anew for its backward pass (activation
+    checkpoints) would take another stream there: call ``dropout`` with a ``stream`` of its own in such a layer."""
 
     def __init__(self, p=0.5, seed=0, relu=False):
         super().__init__()

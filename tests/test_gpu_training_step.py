@@ -2,6 +2,7 @@
 in the trainer."""
 import importlib.util
 import os
+import threading
 
 import pytest
 import torch
@@ -164,3 +165,74 @@ def test_compiled_modules_fall_back_to_the_operators(cuda):
     want = loss(x, y)
     drop.calls = 0
     assert torch.equal(torch.compile(loss, backend="eager")(x, y), want)
+
+
+def _ends(x, w, b, y, stream):
+    """Dropout and loss, forward and backward: (loss, gradients)."""
+    leaves = [t.detach().requires_grad_() for t in (x, w, b)]
+    h = fastgl.dropout(leaves[0], 0.4, 5, stream, relu=True)
+    loss = fastgl.linear_cross_entropy(h, leaves[1], y, leaves[2])
+    return [loss.detach(), *torch.autograd.grad(loss, leaves, torch.ones((), device=x.device))]
+
+
+def _some(cuda, k, dtype):
+    gen = torch.Generator(device=cuda).manual_seed(k)
+    n, v, d = 200 + 31 * k, 90 + 500 * k, 64 + 20 * k
+    normal = lambda *s: torch.randn(s, generator=gen, device=cuda).to(dtype)  # noqa: E731
+    return normal(n, d), normal(v, d) / 8, normal(v), torch.randint(0, v, (n,), generator=gen, device=cuda)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_calls_of_several_threads_at_once(cuda, dtype):
+    inputs = [_some(cuda, k, dtype) for k in range(4)]
+    want = [_ends(*t, stream=k) for k, t in enumerate(inputs)]
+    torch.cuda.synchronize()
+    got, errors = [[] for _ in inputs], []
+
+    def work(k):
+        try:
+            with torch.cuda.device(cuda), torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(8):
+                    got[k].append(_ends(*inputs[k], stream=k))
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    torch.cuda.synchronize()
+    for k, runs in enumerate(got):
+        assert len(runs) == 8 and all(torch.equal(p, q) for run in runs for p, q in zip(run, want[k]))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_two_graphs_replayed_at_once(cuda, dtype):
+    inputs = [_some(cuda, k, dtype) for k in (1, 3)]
+    want = [_ends(*t, stream=k) for k, t in enumerate(inputs)]
+    graphs, results = [], []
+    for k, t in enumerate(inputs):
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            _ends(*t, stream=k)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            results.append(_ends(*t, stream=k))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(5):
+        for r in results:
+            for t in r:
+                t.zero_()
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for r, e in zip(results, want) for p, q in zip(r, e))
+        assert all(torch.equal(p, q) for k, t in enumerate(inputs) for p, q in zip(_ends(*t, stream=k), want[k]))
