@@ -1205,7 +1205,10 @@ inline XePlan xe_plan(const XeShape& s, int use, int kept_tiles, int passed_tile
     // sums in LDS.  (100 rows, 500 K classes, bf16: 410 us with 62 parts, 1230 with 16.  Weights, 100 K rows, 47 classes, bf16: backward 42 us with 512
     // parts, 53 with 128, 135 with 32, and 69 with 1024, which the kernel's first tile and last stores are much of.)
     int least = (int)ceil_div(passed_tiles, use == kXeWeights ? 512 : kXeMaxParts - 2);
-    if (least < 2) least = 2;
+    // Two tiles, unless all of them are few beside the chip.  (1000 rows x 256, 64 classes, forward and backward with one and two: bf16 31 us and 34, fp32 39 and
+    // 43; 172 classes 37 and 36, 45 and 47.  8192 rows, bf16, 64 classes 51 and 50, 172 classes 69 and 57.)
+    const bool few = (int64_t)p.groups * passed_tiles < room / 4;
+    if (least < 2 && !few) least = 2;
     if (least > passed_tiles) least = passed_tiles;
     p.shared = p.groups < room ? room / p.groups : 1;
     p.per = (int)ceil_div(passed_tiles, p.shared);
