@@ -22,15 +22,14 @@
 // first kilobyte has what belongs to its 32 rows: biases, or labels and the backward pass's factors.
 //
 // bf16: P is rounded to bf16, as the operands are.
-// fp32: each value is the sum of two fp16 values, of 11 bits each, and a product three matrix instructions (high low, low high, high high; what is
-// left out is 2^-22 of it) that add to fp32 accumulators.  fp16's range is short, so a tile is first multiplied by a power of two
-// that takes its largest value to 2^14; what lies 2^39 below that is lost.  In S a row that is 2^12 below its tile's largest value gets a
-// power of its own, which costs its tile a multiplication a logit.  P is scaled likewise, by the running maximum, and the gradient of the logits by a
-// running bound of its own.  Against 64 bits, 2-norm, all results of 8192 x 128 and 20 K classes: 4.5e-7; the same in
-// fp32 products by the library 1.7e-6.
-// Sums, maxima and losses are fp32 in both.  x and w must be finite: others make losses and gradients that are not numbers, but in rows
-// without a label, which are taken as zeros.
-// A bias of -1e30 or less, -infinity among them, leaves its class out: no share, no gradient.  (bf16: shares are exp2 of one fma, whose
+// fp32: each value, P's and the logits' gradients' among them, is the sum of three bf16 values, exactly (fgl_split.hpp), and a product six matrix
+// instructions, the small ones first, that add to fp32 accumulators; what is left out is 2^-23 of the product at most.  So each term of a sum has
+// fp32's precision for itself, however far rows, columns and classes lie apart.  (Two fp16 parts and three instructions a product take
+// two thirds of the time, 8192 x 128, 20 K classes, forward and backward 498 us for 782, but share a power of two with the values around them and
+// hold nothing below 2^-39 of the largest of those: one column of x 2^30 times the others took half of the other columns' bits.)
+// Sums, maxima and losses are fp32 in both.  x and w must be finite, and below 3.38e38 in fp32, where a part would round to infinity: others make
+// losses and gradients that are not numbers, but in rows without a label, which are taken as zeros.
+// A bias of -1e30 or less, -infinity among them, leaves its class out: no share, no gradient.  (Shares are exp2 of one fma, whose
 // product with log2 e is not rounded where the maximum's is: logits up to some 1e9 are no matter, the difference of 2^-25 of the maximum is the
 // same for all of a row's shares and their sum.)
 //
@@ -47,6 +46,7 @@
 // 20 us, mostly latency.
 #include "fgl_common.hpp"
 #include "fgl_kernels.hpp"
+#include "fgl_split.hpp"
 
 #include <math.h>
 
@@ -57,9 +57,6 @@ namespace fgl {
 typedef float XeF4 __attribute__((ext_vector_type(4)));
 typedef float XeF32x16 __attribute__((ext_vector_type(16)));
 typedef uint32_t XeOp __attribute__((ext_vector_type(4)));  // eight values of a matrix instruction's operand
-typedef float XeF2 __attribute__((ext_vector_type(2)));
-typedef _Float16 XeF16x2 __attribute__((ext_vector_type(2)));
-typedef _Float16 XeF16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kXeWaves = kBlock / kWave;
 constexpr int kXeChunk = 1024;  // bytes of an operand of one matrix instruction
@@ -69,22 +66,18 @@ constexpr float kXeLog2e = 1.44269504088896340736f;
 constexpr float kXeLn2 = 0.69314718055994530942f;
 constexpr float kXeLeftOut = -1e30f;  // a bias of this or less leaves its class out, as -infinity does
 constexpr float kXeStep = 8.0f;       // powers of two that a row's values may pass its running maximum by
-constexpr int kXeRise = 6;            // fp16: powers of two that P is multiplied by, so that it fills the range
-constexpr int kXeTop = 14;            // fp16: power of two that largest values are taken to
 
 enum { kXeLoss = 0, kXeLossAndRows = 1, kXeWeights = 2 };
 
-// A tile's first kilobyte, in floats.  Classes: their biases (fp32: times log2 e).  Rows: -maximum (powers of two), factor, label, the label's value.
+// A tile's first kilobyte, in floats.  Classes: their biases.  Rows: -maximum (powers of two), factor, label, the label's value.
 constexpr int kXeShift = 0, kXeFactor = 32, kXeLabel = 64, kXeOwn = 96;
-// fp32, with e the power of two that the tile is multiplied by, and f a row's in S: 2^-f, 2^(e - f) of each row; 2^-e, e, whether any f is not e
-constexpr int kXeRow = 128, kXeRowInTile = 160, kXeTile = 192, kXeExponent = 193, kXeMixed = 194;
-constexpr int kXeNear = 12;  // powers of two below the tile's largest value from where on a row has its own f
-constexpr int kXeFar = 120;  // how far f is from e at most: 2^(e - f) is a number
 
-// Sizes of a problem as the kernels see it: blocks of 32 columns, padded.  Beyond 384 columns, in bf16 beyond 256, in two slices, each with half of O,
-// which otherwise did not fit a wave's registers, and S formed for either.  (bf16 could have 384 columns whole, with one wave a SIMD instead of
-// two: 8192 rows, 20 K classes, forward, 300 columns 340 us against 352 in slices, 370 columns 556 against 352.  fp32 has one wave a SIMD
-// from 129 columns on anyway: 300 columns 678 whole, 1061 in slices.)
+// Sizes of a problem as the kernels see it: blocks of 32 columns, padded.  Beyond 256 columns in bf16, 320 in fp32, in two slices, each with half of O,
+// which otherwise did not fit a wave's registers.  bf16 forms S for either.  In fp32 half of the columns of the kept rows is all that fits beside half of
+// O too: two waves share them, each forms its half of S, and they add the halves up.  (8192 rows, 10 K classes, 512 columns, forward and backward: 2261
+// us, 3140 with S formed for either and the kept rows' other half read from the L2 for each tile, 2293 by the library; 384 columns 1856, 1835 with S
+// formed for either, 1800 by the library.)  (bf16 could have 384 columns whole, with one wave a SIMD instead of
+// two: 8192 rows, 20 K classes, forward, 300 columns 340 us against 352 in slices, 370 columns 556 against 352.)
 struct XeShape {
     int blocks;  // in a slice
     int slices;
@@ -98,9 +91,9 @@ inline XeShape xe_shape(int dim, int dtype)
 {
     const int n = (int)ceil_div(dim, 32);
     XeShape s;
-    s.parts = dtype == FGL_F32 ? 2 : 1;
-    s.slices = n > (s.parts == 2 ? 12 : 8) ? 2 : 1;
-    const int blocks = n <= 8 ? n : n <= 10 && s.parts == 2 ? 10 : n <= 12 ? 12 : 16;
+    s.parts = dtype == FGL_F32 ? 3 : 1;
+    s.slices = n > (s.parts == 3 ? 10 : 8) ? 2 : 1;
+    const int blocks = n <= 8 ? n : n <= 10 && s.parts == 3 ? 10 : n <= 12 ? 12 : 16;
     s.blocks = blocks / s.slices;
     return s;
 }
@@ -129,26 +122,6 @@ struct XeImagesArgs {
 constexpr int kXeCols = 128;  // columns that a workgroup lays out, of 32 rows
 constexpr int kXePitch = kXeCols + 4;
 
-// v = hi + lo, fp16 each, to 2^-22 of it
-__device__ __forceinline__ void xe_split(const float (&v)[8], XeOp& hi, XeOp& lo)
-{
-    XeF16x8 h, l;
-    float minus = -1.0f;
-    asm("" : "+s"(minus));  // (so that the difference is the one instruction that takes an fp16 operand)
-#pragma unroll
-    for (int j = 0; j < 8; j += 2) {
-        const XeF16x2 both = __builtin_convertvector((XeF2){v[j], v[j + 1]}, XeF16x2);
-        const XeF2 rest = {fmaf((float)both[0], minus, v[j]), fmaf((float)both[1], minus, v[j + 1])};
-        const XeF16x2 second = __builtin_convertvector(rest, XeF16x2);
-        h[j] = both[0];
-        h[j + 1] = both[1];
-        l[j] = second[0];
-        l[j + 1] = second[1];
-    }
-    hi = __builtin_bit_cast(XeOp, h);
-    lo = __builtin_bit_cast(XeOp, l);
-}
-
 __device__ __forceinline__ XeOp xe_bf16(const float (&v)[8])
 {
     Bf16x8 o;
@@ -157,33 +130,26 @@ __device__ __forceinline__ XeOp xe_bf16(const float (&v)[8])
     return __builtin_bit_cast(XeOp, o);
 }
 
+// Eight values as an operand of one matrix instruction, or as three
 template <int PARTS>
-__device__ __forceinline__ void xe_put(float (&v)[8], float scale, char* to)
+__device__ __forceinline__ void xe_operands(const float (&v)[8], XeOp (&p)[PARTS])
 {
-    XeOp* p = reinterpret_cast<XeOp*>(to);
-    if constexpr (PARTS == 2) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] *= scale;
-        XeOp hi, lo;
-        xe_split(v, hi, lo);
-        p[0] = hi;
-        p[kXeChunk / sizeof(XeOp)] = lo;
+    if constexpr (PARTS == 3) {
+        uint32_t rest = 0;  // (bits below 2^-133: nothing beside a logit, and beside a gradient of x's own size)
+        sp_split(v, p, rest);
     } else {
         p[0] = xe_bf16(v);
     }
 }
 
-__device__ __forceinline__ float xe_power(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }  // 2^e, -127 < e < 128
-
-// The power of two that takes a largest magnitude to 2^14 .. 2^15, as far as it and its inverse are numbers; that of no values at all is as large
-// as any.
-__device__ __forceinline__ int xe_exponent(float most)
+template <int PARTS>
+__device__ __forceinline__ void xe_put(const float (&v)[8], char* to)
 {
-    const int e = kXeTop + 127 - (int)(__float_as_uint(most) >> 23);
-    return e > 100 ? 100 : e;  // (at least -113)
+    XeOp p[PARTS];
+    xe_operands<PARTS>(v, p);
+#pragma unroll
+    for (int q = 0; q < PARTS; ++q) *reinterpret_cast<XeOp*>(to + q * kXeChunk) = p[q];
 }
-
-__device__ __forceinline__ float xe_finite(float v) { return fabsf(v) < INFINITY ? fabsf(v) : 0.0f; }
 
 template <typename T, int PARTS>
 __global__ __launch_bounds__(kBlock) void xe_images_kernel(const XeImagesArgs g)
@@ -204,7 +170,7 @@ __global__ __launch_bounds__(kBlock) void xe_images_kernel(const XeImagesArgs g)
         if (row < m.rows) {
             if (classes) {
                 bias = m.bias != nullptr ? (float)static_cast<const T*>(m.bias)[row] : 0.0f;
-                bias = bias <= kXeLeftOut ? -INFINITY : PARTS == 2 ? bias * kXeLog2e : bias;
+                if (bias <= kXeLeftOut) bias = -INFINITY;
             } else {
                 const int64_t y = g.label64 ? static_cast<const int64_t*>(m.labels)[row] : (int64_t) static_cast<const int32_t*>(m.labels)[row];
                 if (y != g.ignore) label = y >= 0 && y < g.classes ? (int)y : -2;  // (-2: no such class)
@@ -213,53 +179,6 @@ __global__ __launch_bounds__(kBlock) void xe_images_kernel(const XeImagesArgs g)
         live[thread] = row < m.rows && (classes || label != -1);
     }
     __syncthreads();
-    int exponent = 0;      // the tile's
-    float row_scale = 1.0f;  // of the row that this thread's lane has in S
-    bool mixed = false;
-    if constexpr (PARTS == 2) {
-        // the largest magnitude of each row, eight threads a row, what is not finite passed over
-        __shared__ float most[8][32];
-        const bool by_rows = m.col_stride == 1;
-        const int r = by_rows ? thread / 8 : thread % 32, part = by_rows ? thread % 8 : thread / 32;
-        float v = 0.0f;
-        if (live[r]) {
-            const T* p = src + (row0 + r) * m.row_stride;
-            typedef T Vec __attribute__((ext_vector_type(4), aligned(sizeof(T))));
-            if (by_rows) {
-                int c = 4 * part;
-                for (; c + 4 <= g.dim; c += 32) {
-                    const Vec q = *reinterpret_cast<const Vec*>(p + c);
-                    v = fmaxf(v, fmaxf(fmaxf(xe_finite((float)q[0]), xe_finite((float)q[1])), fmaxf(xe_finite((float)q[2]), xe_finite((float)q[3]))));
-                }
-                for (; c < g.dim; ++c) v = fmaxf(v, xe_finite((float)p[c]));
-            } else {
-                for (int c = part; c < g.dim; c += 8) v = fmaxf(v, xe_finite((float)p[c * m.col_stride]));
-            }
-        }
-        most[part][r] = v;
-        __syncthreads();
-        float of_row = 0.0f;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) of_row = fmaxf(of_row, most[k][thread % 32]);
-        float of_tile = of_row;
-#pragma unroll
-        for (int d = 16; d >= 1; d >>= 1) of_tile = fmaxf(of_tile, __shfl_xor(of_tile, d, kWave));
-        exponent = xe_exponent(of_tile);
-        const int own = xe_exponent(of_row), above = own - exponent < kXeFar ? own - exponent : kXeFar;
-        const int f = of_row > 0.0f && above > kXeNear ? exponent + above : exponent;
-        mixed = __any(f != exponent);
-        row_scale = xe_power(f);
-        if (blockIdx.y == 0 && thread < 32) {
-            float* c = reinterpret_cast<float*>(m.s_image + t * kXeChunk * (1 + 2LL * g.blocks * g.slices * PARTS));
-            c[kXeRow + thread] = xe_power(-f);
-            c[kXeRowInTile + thread] = xe_power(exponent - f);
-            if (thread == 0) {
-                c[kXeTile] = xe_power(-exponent);
-                reinterpret_cast<int*>(c)[kXeExponent] = exponent;
-                reinterpret_cast<int*>(c)[kXeMixed] = mixed;
-            }
-        }
-    }
     if (m.col_stride == 1) {
         typedef T Vec __attribute__((ext_vector_type(8), aligned(sizeof(T))));
 #pragma unroll
@@ -304,7 +223,7 @@ __global__ __launch_bounds__(kBlock) void xe_images_kernel(const XeImagesArgs g)
         float v[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = tile[lane % 32 * kXePitch + at / kWave * 16 + lane / 32 * 8 + j];
-        xe_put<PARTS>(v, row_scale, s_tile + kXeChunk * (1 + (int64_t)step * PARTS) + lane * 16);
+        xe_put<PARTS>(v, s_tile + kXeChunk * (1 + (int64_t)step * PARTS) + lane * 16);
     }
     if (m.p_image == nullptr) return;
     char* p_tile = m.p_image + t * kXeChunk * ((int64_t)steps * PARTS);
@@ -317,14 +236,16 @@ __global__ __launch_bounds__(kBlock) void xe_images_kernel(const XeImagesArgs g)
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = tile[(half * 16 + j / 4 * 8 + lane / 32 * 4 + j % 4) * kXePitch + own * 32 + lane % 32];
         const int slice = block / g.blocks, in_slice = block % g.blocks;
-        xe_put<PARTS>(v, xe_power(exponent), p_tile + kXeChunk * ((((int64_t)slice * 2 + half) * g.blocks + in_slice) * PARTS) + lane * 16);
+        xe_put<PARTS>(v, p_tile + kXeChunk * ((((int64_t)slice * 2 + half) * g.blocks + in_slice) * PARTS) + lane * 16);
     }
 }
 
 // ---- the passes ----------------------------------------------------------------------------------------------------
 // How the groups' tiles are dealt out to workgroups.
 struct XePlan {
-    int groups;  // of four kept tiles (times slices)
+    int groups;  // of four kept tiles (times slices), or of two, for the pairs of waves
+    int slices;
+    bool pairs;
     int tiles;   // passed, of each
     int per;     // tiles of a workgroup, of those that are shared
     int shared;  // > 0: that many workgroups to a group
@@ -337,6 +258,9 @@ struct XePlan {
     // A group's first and last workgroup among those that share it, and the place of one's part
     __host__ __device__ int first(int group) const { return shared > 0 ? group * shared : group < whole ? 0 : (group - whole) * tiles / per; }
     __host__ __device__ int last(int group) const { return shared > 0 ? group * shared + shared - 1 : group < whole ? 0 : ((group - whole + 1) * tiles - 1) / per; }
+    // Who has a tile's slice
+    __host__ __device__ int group_of(int tile, int slice) const { return pairs ? tile / (kXeWaves / 2) : tile / kXeWaves * slices + slice; }
+    __host__ __device__ int wave_of(int tile, int slice) const { return pairs ? tile % (kXeWaves / 2) * 2 + slice : tile % kXeWaves; }
     __host__ __device__ int slot(int workgroup, int group) const { return shared > 0 ? workgroup : group < whole ? group : group + workgroup; }
 };
 
@@ -411,11 +335,9 @@ __device__ __forceinline__ XeOp xe_operand(const char* chunk) { return *reinterp
 
 __device__ __forceinline__ XeOp xe_operand(const XeGlobal<const char>* chunk) { return *reinterpret_cast<const XeGlobal<const XeOp>*>(chunk + lane_id() * 16); }
 
-template <int PARTS>
 __device__ __forceinline__ XeF32x16 xe_mfma(const XeOp& a, const XeOp& b, const XeF32x16& c)
 {
-    if constexpr (PARTS == 1) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(Bf16x8, a), __builtin_bit_cast(Bf16x8, b), c, 0, 0, 0);
-    else return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(XeF16x8, a), __builtin_bit_cast(XeF16x8, b), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(Bf16x8, a), __builtin_bit_cast(Bf16x8, b), c, 0, 0, 0);
 }
 
 // N products of an operand from LDS each, in PARTS parts at neighbouring places: at(i) is the i-th one's place, use(i, parts) multiplies.  Operands are
@@ -424,7 +346,7 @@ __device__ __forceinline__ XeF32x16 xe_mfma(const XeOp& a, const XeOp& b, const 
 template <int N, int PARTS, typename At, typename Use>
 __device__ __forceinline__ void xe_products(const At& at, const Use& use)
 {
-    constexpr int kMost = PARTS == 1 ? 4 : 3, kAhead = N < kMost ? N : kMost;
+    constexpr int kMost = PARTS == 1 ? 4 : 2, kAhead = N < kMost ? N : kMost;
     XeOp a[kAhead][PARTS];
 #pragma unroll
     for (int i = 0; i < kAhead; ++i)
@@ -441,35 +363,48 @@ __device__ __forceinline__ void xe_products(const At& at, const Use& use)
     }
 }
 
-// Waves that a SIMD (and so workgroups that a CU) holds at once: the kept rows take 8 registers a block and part, O 16 a block, of 512.
-// WIDE: in two slices.
+// a b + c, in three parts: the small products first
+__device__ __forceinline__ XeF32x16 xe_mfma(const XeOp (&a)[3], const XeOp (&b)[3], XeF32x16 c)
+{
+    constexpr int kA[6] = {2, 0, 1, 1, 0, 0}, kB[6] = {0, 2, 1, 0, 1, 0};
+#pragma unroll
+    for (int q = 0; q < 6; ++q) c = xe_mfma(a[kA[q]], b[kB[q]], c);
+    return c;
+}
+__device__ __forceinline__ XeF32x16 xe_mfma(const XeOp (&a)[1], const XeOp (&b)[1], const XeF32x16& c) { return xe_mfma(a[0], b[0], c); }
+
+// Waves that a SIMD (and so workgroups that a CU) holds at once: the kept rows take 8 registers a block and part, O 16 a block, of 512.  (The loss
+// alone in fp32, 7 blocks and more: LDS has room for one workgroup.)  WIDE: in two slices.
 __host__ __device__ constexpr int xe_waves(int blocks, int parts, int use, bool wide)
 {
     if (wide) return parts == 1 && (use == kXeLoss || blocks <= 6) ? 2 : 1;
-    if (use == kXeLoss) return parts == 1 ? 4 : blocks <= 2 ? 4 : blocks <= 4 ? 3 : blocks <= 8 ? 2 : 1;
+    if (use == kXeLoss) return parts == 1 ? 4 : blocks <= 2 ? 4 : blocks <= 4 ? 3 : blocks <= 6 ? 2 : 1;
     return parts == 1 ? (blocks <= 2 ? 4 : blocks <= 3 ? 3 : 2) : blocks <= 1 ? 4 : blocks <= 2 ? 3 : blocks <= 4 ? 2 : 1;
 }
+
+// fp32 in two slices: neighbouring waves share their kept rows, each with the columns of its slice.
+__host__ __device__ constexpr bool xe_pair(int parts, int use, bool wide) { return wide && parts == 3 && use != kXeLoss; }
 
 template <int DB, int PARTS, int USE, bool WIDE>
 struct XeWave {
     static constexpr int kSteps = WIDE ? 4 * DB : 2 * DB;
     static constexpr int kSChunks = 1 + kSteps * PARTS, kPChunks = 2 * DB * PARTS;
 
-    XeOp kept[kSteps][PARTS];
+    static constexpr bool kPair = xe_pair(PARTS, USE, WIDE);
+    static constexpr int kKept = kPair ? kSteps / 2 : kSteps;  // (a wave of a pair: its half of the columns)
+
+    XeOp kept[kKept][PARTS];
     XeF32x16 o[USE == kXeLoss ? 1 : DB];
     float start;          // weights: the class's bias
-    float unit;           // fp32: what the row's power of two makes of S
-    float top, sum, own;  // running maximum (a power of two; weights, fp32: what P is below, a power of two itself), sum, the label's logit (a power of two)
+    float top, sum, own;  // running maximum (a power of two), sum, the label's logit (a power of two)
     int label;            // weights: the class
-    int rise;             // fp32, rows: power of two that O is multiplied by
     bool bias_sum;
 
-    // S^T of the staged tile
-    __device__ __forceinline__ XeF32x16 logits(const char* s) const
+    // What S^T of a tile starts from: the biases
+    __device__ __forceinline__ XeF32x16 biases(const char* tile) const
     {
-        XeF32x16 acc = {};
-        if constexpr (PARTS == 2) {
-        } else if constexpr (USE == kXeWeights) {
+        XeF32x16 acc;
+        if constexpr (USE == kXeWeights) {
             float bias = start;
             asm volatile("" : "+v"(bias));  // (else sixteen copies of it are kept in registers through all tiles)
 #pragma unroll
@@ -477,58 +412,31 @@ struct XeWave {
         } else {
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                const XeF4 b = *reinterpret_cast<const XeF4*>(s + 4 * (8 * q + 4 * (lane_id() / 32)));
+                const XeF4 b = of_rows(tile, 0, q);
 #pragma unroll
                 for (int c = 0; c < 4; ++c) acc[4 * q + c] = b[c];
             }
         }
-        const auto at = [&](int k) { return s + (1 + k * PARTS) * kXeChunk; };
-        if constexpr (PARTS == 1) {
-            xe_products<kSteps, 1>(at, [&](int k, const XeOp (&a)[1]) { acc = xe_mfma<1>(a[0], kept[k][0], acc); });
-        } else {
-            xe_products<kSteps, 2>(at, [&](int k, const XeOp (&a)[2]) {
-                acc = xe_mfma<2>(a[1], kept[k][0], acc);
-                acc = xe_mfma<2>(a[0], kept[k][1], acc);
-                acc = xe_mfma<2>(a[0], kept[k][0], acc);
-            });
-        }
         return acc;
     }
+    // acc and the products of the kept rows with operands that lie one after another
+    __device__ __forceinline__ XeF32x16 logits(const char* s, XeF32x16 acc) const
+    {
+        xe_products<kKept, PARTS>([&](int k) { return s + k * PARTS * kXeChunk; }, [&](int k, const XeOp (&a)[PARTS]) { acc = xe_mfma(a, kept[k], acc); });
+        return acc;
+    }
+    // S^T of the staged tile
+    __device__ __forceinline__ XeF32x16 logits(const char* s) const { return logits(s + kXeChunk, biases(s)); }
 
     // Four values of the staged tile's rows that a lane's values 4 q .. 4 q + 3 of S^T belong to.
     static __device__ __forceinline__ XeF4 of_rows(const char* tile, int what, int q)
     {
         return *reinterpret_cast<const XeF4*>(reinterpret_cast<const float*>(tile) + what + 8 * q + 4 * (lane_id() / 32));
     }
-    static __device__ __forceinline__ int of_tile(const char* tile, int what) { return __builtin_amdgcn_readfirstlane(reinterpret_cast<const int*>(tile)[what]); }
-
-    // fp32: S^T in the tile's powers of two, and what takes it to powers of two of the shares
-    __device__ __forceinline__ float even(XeF32x16& s, const char* tile) const
-    {
-        if (of_tile(tile, kXeMixed)) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const XeF4 f = of_rows(tile, kXeRowInTile, q);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) s[4 * q + j] *= f[j];
-            }
-        }
-        return unit * (__int_as_float(of_tile(tile, kXeTile)) * kXeLog2e);
-    }
 
     // S^T -> P^T, with the running maximum, sum and the label's logit.  v0: the tile's first class.
-    __device__ __forceinline__ void shares(XeF32x16& s, const char* tile, int v0)
+    __device__ __forceinline__ void shares(XeF32x16& s, int v0)
     {
-        if constexpr (PARTS == 2) {
-            const float to2 = even(s, tile);
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const XeF4 bias = of_rows(tile, 0, q);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) s[4 * q + j] = fmaf(s[4 * q + j], to2, bias[j]);
-            }
-        }
-        constexpr float kTo2 = PARTS == 2 ? 1.0f : kXeLog2e;
         const int in_tile = label - v0;
         const bool here = label >= 0 && in_tile >= 0 && in_tile < 32;
         if (__any(here)) {
@@ -536,7 +444,7 @@ struct XeWave {
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 if (at == 8 * (i / 4) + i % 4) {
-                    own = s[i] * kTo2;
+                    own = s[i] * kXeLog2e;
                     s[i] = -INFINITY;
                 }
             }
@@ -544,7 +452,7 @@ struct XeWave {
         float most = s[0];
 #pragma unroll
         for (int i = 1; i < 16; ++i) most = fmaxf(most, s[i]);
-        most = fmaxf(most, xe_other_half(most)) * kTo2;
+        most = fmaxf(most, xe_other_half(most)) * kXeLog2e;
         if (__any(most > top + kXeStep)) {
             const float now = fmaxf(top, most);
             const float scale = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top - now);
@@ -553,23 +461,9 @@ struct XeWave {
             if constexpr (USE == kXeLossAndRows) rescale(scale);
         }
         const float shift = top == -INFINITY ? 0.0f : -top;
-        if constexpr (PARTS == 1) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], kXeLog2e, shift));
-            add_up(s, 1.0f);
-        } else {
-            // P times 2^(rise - e), at most 2^14, so that with classes times 2^e all tiles' sums are times 2^rise (the loss alone: for the same bits)
-            const int most_rise = of_tile(tile, kXeExponent) + kXeRise;
-            if (most_rise < rise) {
-                if constexpr (USE == kXeLossAndRows) rescale(most_rise - rise < -126 ? 0.0f : xe_power(most_rise - rise));
-                rise = most_rise;
-            }
-            const int below = most_rise - rise, little = below < 60 ? below : 60;  // (fp16 has nothing of 2^-60 times P; the sum has)
-            const float up = shift + (float)(kXeRise - little);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(s[i] + up);
-            add_up(s, xe_power(little - kXeRise));
-        }
+        for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], kXeLog2e, shift));
+        add_up(s);
     }
 
     __device__ __forceinline__ void rescale(float scale)
@@ -580,26 +474,24 @@ struct XeWave {
             for (int i = 0; i < 16; ++i) o[d][i] *= scale;
     }
 
-    __device__ __forceinline__ void add_up(const XeF32x16& p, float scale)
+    __device__ __forceinline__ void add_up(const XeF32x16& p)
     {
         float t[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) t[i] = p[i] + p[i + 8];
-        sum += (((t[0] + t[4]) + (t[1] + t[5])) + ((t[2] + t[6]) + (t[3] + t[7]))) * scale;
+        sum += (((t[0] + t[4]) + (t[1] + t[5])) + ((t[2] + t[6]) + (t[3] + t[7])));
     }
 
     // S^T -> the gradient of the logits, from the maxima, factors and labels of the tile's rows.  Returns whether a label is among them.
     __device__ __forceinline__ bool gradients(XeF32x16& s, const char* tile, int v0)
     {
         const int* l = reinterpret_cast<const int*>(tile);
-        float to2 = kXeLog2e;
-        if constexpr (PARTS == 2) to2 = even(s, tile);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             const XeF4 shift = of_rows(tile, kXeShift, q), factor = of_rows(tile, kXeFactor, q);
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                s[4 * q + j] = __builtin_amdgcn_exp2f(fmaf(s[4 * q + j], to2, PARTS == 2 ? shift[j] + start : shift[j])) * factor[j];
+                s[4 * q + j] = __builtin_amdgcn_exp2f(fmaf(s[4 * q + j], kXeLog2e, shift[j])) * factor[j];
         }
         const int in_tile = l[kXeLabel + lane_id() % 32] - v0;
         const bool labels_here = __any(in_tile >= 0 && in_tile < 32);
@@ -613,23 +505,7 @@ struct XeWave {
                 for (int j = 0; j < 4; ++j) s[4 * q + j] = labels[j] == label ? values[j] : s[4 * q + j];
             }
         }
-        if (bias_sum) add_up(s, 1.0f);
-        if constexpr (PARTS == 2) {
-            // Times 2^-e, for rows times 2^e, and to fp16's range: 2^14 is what a class's values are below, sixteen times the largest one when that was met
-            const float of_e = __int_as_float(of_tile(tile, kXeTile));
-            float most = fabsf(s[0]);
-#pragma unroll
-            for (int i = 1; i < 16; ++i) most = fmaxf(most, fabsf(s[i]));
-            most = fmaxf(most, xe_other_half(most)) * of_e;
-            if (__any(most > top)) {
-                const float now = most > top ? __uint_as_float((__float_as_uint(fminf(most, 0x1p122f)) & 0x7F800000u) + (4u << 23)) : top;
-                rescale(top / now);
-                top = now;
-            }
-            const float scale = fminf((float)(1 << kXeTop) / top * of_e, 0x1p120f);  // (more only where all values are zero)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] *= scale;
-        }
+        if (bias_sum) add_up(s);
         return labels_here;
     }
 
@@ -642,11 +518,10 @@ struct XeWave {
             float v[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[j] = s[8 * h + j];
-            if constexpr (PARTS == 1) w[h][0] = xe_bf16(v);
-            else xe_split(v, w[h][0], w[h][1]);
+            xe_operands<PARTS>(v, w[h]);
         }
         if constexpr (PARTS == 1) {
-            xe_products<2 * DB, 1>([&](int i) { return p + i * kXeChunk; }, [&](int i, const XeOp (&a)[1]) { o[i % DB] = xe_mfma<1>(a[0], w[i / DB][0], o[i % DB]); });
+            xe_products<2 * DB, 1>([&](int i) { return p + i * kXeChunk; }, [&](int i, const XeOp (&a)[1]) { o[i % DB] = xe_mfma(a, w[i / DB], o[i % DB]); });
             // A class's gradient is mostly its own rows' where there are many classes: those tiles take what rounding left of P too (the error
             // of dw against 64 bits, 1000 rows and 10 K classes: 2.4e-3 without, 1.7e-3 with, as its own rounding to bf16 makes).
             if (USE == kXeWeights && both) {
@@ -658,26 +533,45 @@ struct XeWave {
                     for (int j = 0; j < 8; ++j) v[j] = s[8 * h + j] - (float)high[j];
                     w[h][0] = xe_bf16(v);
                 }
-                xe_products<2 * DB, 1>([&](int i) { return p + i * kXeChunk; }, [&](int i, const XeOp (&a)[1]) { o[i % DB] = xe_mfma<1>(a[0], w[i / DB][0], o[i % DB]); });
+                xe_products<2 * DB, 1>([&](int i) { return p + i * kXeChunk; }, [&](int i, const XeOp (&a)[1]) { o[i % DB] = xe_mfma(a, w[i / DB], o[i % DB]); });
             }
         } else {
-            // O beyond eight blocks lies in the accumulator registers, and the compiler moves all of it back and forth for instructions that add to it
-            // (8192 rows, 10 K classes, forward, 300 columns 444 us so and 382 with additions of their own, 384 columns 1192 and 452; 256 columns 299
-            // and 318).
-            constexpr bool kOwn = DB > 8 || WIDE;
-            XeF32x16 sum = {};
-            xe_products<2 * DB, 2>([&](int i) { return p + (i % 2 * DB + i / 2) * 2 * kXeChunk; }, [&](int i, const XeOp (&a)[2]) {
-                XeF32x16& to = kOwn ? sum : o[i / 2];
-                to = xe_mfma<2>(a[1], w[i % 2][0], to);
-                to = xe_mfma<2>(a[0], w[i % 2][1], to);
-                to = xe_mfma<2>(a[0], w[i % 2][0], to);
-                if (kOwn && i % 2 == 1) {
+            // Where O lies in the accumulator registers, the compiler moves it back and forth for instructions that add to it: it is added to in
+            // fp32 instead, while the next block is multiplied (8192 rows, 20 K classes, forward and backward, added to so and by the matrix
+            // instructions: 256 columns 1635 us and 1797, 200 columns 1428 and 1444; 128 columns 845 and 782, 64 columns 503 and 432).
+            constexpr bool kOwn = DB > 4;
+            XeF32x16 sum[2];
+            xe_products<2 * DB, PARTS>([&](int i) { return p + (i % 2 * DB + i / 2) * PARTS * kXeChunk; }, [&](int i, const XeOp (&a)[PARTS]) {
+                if constexpr (kOwn) {
+                    XeF32x16& to = sum[i / 2 % 2];
+                    to = xe_mfma(a, w[i % 2], i % 2 == 0 ? XeF32x16{} : to);
+                    if (i >= 2 && i % 2 == 0) {
 #pragma unroll
-                    for (int c = 0; c < 16; ++c) o[i / 2][c] += sum[c];
-                    sum = XeF32x16{};
+                        for (int c = 0; c < 16; ++c) o[i / 2 - 1][c] += sum[(i / 2 - 1) % 2][c];
+                    }
+                } else {
+                    o[i / 2] = xe_mfma(a, w[i % 2], o[i / 2]);
                 }
             });
+            if constexpr (kOwn) {
+#pragma unroll
+                for (int c = 0; c < 16; ++c) o[DB - 1][c] += sum[(DB - 1) % 2][c];
+            }
         }
+    }
+
+    // The same with one half of a tile's passed rows, of a pair's wave
+    __device__ __forceinline__ void half_product(const XeOp (&w)[PARTS], const char* p)
+    {
+        XeF32x16 sum[2];
+        xe_products<DB, PARTS>([&](int i) { return p + i * PARTS * kXeChunk; }, [&](int i, const XeOp (&a)[PARTS]) {
+            sum[i % 2] = xe_mfma(a, w, XeF32x16{});
+            if (i == 0) return;
+#pragma unroll
+            for (int c = 0; c < 16; ++c) o[i - 1][c] += sum[(i - 1) % 2][c];
+        });
+#pragma unroll
+        for (int c = 0; c < 16; ++c) o[DB - 1][c] += sum[(DB - 1) % 2][c];
     }
 
     // One tile: copies what comes next to `next` while it works on `s`
@@ -691,7 +585,7 @@ struct XeWave {
         if (!active) return;
         p = logits(s);
         if constexpr (USE == kXeWeights) both = gradients(p, s, v0);
-        else shares(p, s, n0);
+        else shares(p, n0);
     }
     // The same where LDS has room for two S tiles: the next one is on its way from the start of this one
     __device__ __forceinline__ void first_half_of_two(const char* __restrict__ s, char* __restrict__ next_p, char* __restrict__ next_s, const char* src_p, const char* src_s,
@@ -702,7 +596,7 @@ struct XeWave {
         if (!active) return;
         p = logits(s);
         if constexpr (USE == kXeWeights) both = gradients(p, s, v0);
-        else shares(p, s, n0);
+        else shares(p, n0);
     }
     // The same where LDS has room for two tiles of both: the next one is on its way all the while
     __device__ __forceinline__ void tile(const char* __restrict__ s, const char* __restrict__ p_tile, char* __restrict__ next_s, char* __restrict__ next_p, const char* src_s,
@@ -716,7 +610,7 @@ struct XeWave {
         XeF32x16 p = logits(s);
         bool both = false;
         if constexpr (USE == kXeWeights) both = gradients(p, s, v0);
-        else shares(p, s, n0);
+        else shares(p, n0);
         product(p, p_tile, both);
     }
     __device__ __forceinline__ void second_half(const char* __restrict__ s, char* __restrict__ next, const char* src, const XeF32x16& p, bool both, bool active)
@@ -771,13 +665,19 @@ __global__ __launch_bounds__(kBlock, xe_waves(DB, PARTS, USE, WIDE)) void xe_ker
     // columns 345 us so and 357 with one tile, 300 columns 688 and 703, 192 columns 282 and 286; 128 columns and fp32 no difference.  The weights'
     // gradient, which has a second product for some tiles, has no registers left for the one loop body: 955 us for 353.)
     constexpr bool kAll = USE == kXeLossAndRows && PARTS == 1 && DB >= 6 && !(WIDE && DB == 8);
-    __shared__ __attribute__((aligned(16))) char s_buf[(kAll ? 2 : 1) * Wave::kSChunks * kXeChunk];
-    __shared__ __attribute__((aligned(16))) char p_buf[(kAll ? 2 : 1) * (USE == kXeLoss ? Wave::kSChunks : Wave::kPChunks) * kXeChunk];  // (the loss alone: two tiles in turn)
+    constexpr bool kPair = Wave::kPair;
+    // A pair's tile goes through LDS in four pieces, each in one of three places: the halves of S, of either wave's columns, and of P, of either half
+    // of the passed rows.
+    constexpr int kPiece = Wave::kPChunks * kXeChunk;
+    __shared__ __attribute__((aligned(16))) char s_buf[kPair ? 3 * kPiece : (kAll ? 2 : 1) * Wave::kSChunks * kXeChunk];
+    // the loss alone: two tiles in turn, or one where LDS has no room for two
+    constexpr bool kInTurn = USE == kXeLoss && 2 * Wave::kSChunks <= 156;
+    __shared__ __attribute__((aligned(16))) char p_buf[(kPair ? 1 : USE != kXeLoss ? (kAll ? 2 : 1) * Wave::kPChunks : kInTurn ? Wave::kSChunks : 1) * kXeChunk];
     // In slices S is most of the work and O too little to hide the next S tile's copy behind.  (8192 x 512, 10 K classes, backward 399 us with
     // one S tile, 348 with two; two of P as well, 1250 us for 1147 of 40 K classes, forward.  Slices of 192 columns, two waves a SIMD, have no registers left for it.)
     constexpr bool kTwo = WIDE && DB == 8 && PARTS == 1 && USE != kXeLoss;
     __shared__ __attribute__((aligned(16))) char s_other[(kTwo ? Wave::kSChunks : 1) * kXeChunk];
-    constexpr int kSlices = WIDE && USE != kXeLoss ? 2 : 1;
+    constexpr int kSlices = WIDE && USE != kXeLoss && !kPair ? 2 : 1;
     constexpr int64_t kSBytes = (int64_t)Wave::kSChunks * kXeChunk, kPBytes = (int64_t)Wave::kPChunks * (WIDE ? 2 : 1) * kXeChunk;
     const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x / kWave));
     const XePlan plan = g.plan;
@@ -812,21 +712,18 @@ __global__ __launch_bounds__(kBlock, xe_waves(DB, PARTS, USE, WIDE)) void xe_ker
     }
     const int t1 = left < plan.tiles - t0 ? t0 + left : plan.tiles;
     left -= t1 - t0;
-    const int slice = group % kSlices, tile = group / kSlices * kXeWaves + wave;
+    const int slice = kPair ? wave % 2 : group % kSlices, tile = kPair ? group * (kXeWaves / 2) + wave / 2 : group / kSlices * kXeWaves + wave;
     const bool active = tile < g.kept_tiles;
     const XeGlobal<const char>* own = xe_uniform(g.kept + (active ? tile : g.kept_tiles - 1) * kSBytes);
 
     Wave w;
 #pragma unroll
-    for (int k = 0; k < Wave::kSteps; ++k)
+    for (int k = 0; k < Wave::kKept; ++k)
 #pragma unroll
-        for (int p = 0; p < PARTS; ++p) w.kept[k][p] = xe_operand(own + kXeChunk + (k * PARTS + p) * kXeChunk);
-    w.unit = 1.0f;
-    if constexpr (PARTS == 2) w.unit = reinterpret_cast<const XeGlobal<const float>*>(own)[kXeRow + lane % 32];
-    w.rise = 1 << 20;
+        for (int p = 0; p < PARTS; ++p) w.kept[k][p] = xe_operand(own + kXeChunk + (((kPair ? slice * Wave::kKept : 0) + k) * PARTS + p) * kXeChunk);
 #pragma unroll
     for (int d = 0; d < (USE == kXeLoss ? 1 : DB); ++d) w.o[d] = XeF32x16{};
-    w.top = USE == kXeWeights ? 0x1p-100f : -INFINITY;
+    w.top = -INFINITY;
     w.sum = w.own = 0.0f;
     w.bias_sum = g.d_b != nullptr;
     if constexpr (USE == kXeWeights) {
@@ -839,10 +736,69 @@ __global__ __launch_bounds__(kBlock, xe_waves(DB, PARTS, USE, WIDE)) void xe_ker
     const int v0 = 32 * tile;
     XeF32x16 p = {};
     bool both = false;
-    xe_stage<Wave::kSChunks>(g.passed + t0 * kSBytes, s_buf);
+    if constexpr (kPair) {
+        xe_stage<1>(g.passed + t0 * kSBytes, p_buf);
+        xe_stage<2 * Wave::kPChunks>(g.passed + t0 * kSBytes + kXeChunk, s_buf);
+    } else {
+        xe_stage<Wave::kSChunks>(g.passed + t0 * kSBytes, s_buf);
+    }
     if constexpr (kAll) xe_stage<Wave::kPChunks>(g.passed_p + slice * (int64_t)Wave::kPChunks * kXeChunk + t0 * kPBytes, p_buf);
     xe_staged();
-    if constexpr (kAll) {
+    if constexpr (kPair) {
+        int s0 = 0, s1 = kPiece, p0 = 2 * kPiece;  // where the tile's S halves and its first P half lie
+        for (int t = t0; t < t1; ++t) {
+            const bool more = t + 1 < t1;
+            const char *next = g.passed + (t + 1) * kSBytes, *of_p = g.passed_p + t * kPBytes;
+            const auto stage_p = [&](int half, int to) {  // (of both slices)
+                xe_stage<Wave::kPChunks / 2>(of_p + half * (kPiece / 2), s_buf + to);
+                xe_stage<Wave::kPChunks / 2>(of_p + kPiece + half * (kPiece / 2), s_buf + to + kPiece / 2);
+            };
+            stage_p(0, p0);
+            // either wave's half of S, then the other's added (the same sum for both)
+            if (active) p = w.logits(s_buf + (slice == 0 ? s0 : s1), slice == 0 ? w.biases(p_buf) : XeF32x16{});
+            __syncthreads();
+            XeF4* mine = reinterpret_cast<XeF4*>(s_buf + s0) + wave * 4 * kWave + lane;
+            const XeF4* others = reinterpret_cast<const XeF4*>(s_buf + s0) + (wave ^ 1) * 4 * kWave + lane;
+            if (active) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) mine[q * kWave] = XeF4{p[4 * q], p[4 * q + 1], p[4 * q + 2], p[4 * q + 3]};
+            }
+            __syncthreads();
+            XeOp half[2][PARTS];
+            if (active) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const XeF4 v = others[q * kWave];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) p[4 * q + c] += v[c];
+                }
+                if constexpr (USE == kXeWeights) w.gradients(p, p_buf, v0);
+                else w.shares(p, 32 * t);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float v[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[j] = p[8 * h + j];
+                    xe_operands<PARTS>(v, half[h]);
+                }
+            }
+            xe_staged();
+            stage_p(1, s0);
+            if (more) {
+                xe_stage<1>(next, p_buf);
+                xe_stage<Wave::kPChunks>(next + kXeChunk, s_buf + s1);
+            }
+            if (active) w.half_product(half[0], s_buf + p0 + slice * (kPiece / 2));
+            xe_staged();
+            if (more) xe_stage<Wave::kPChunks>(next + kXeChunk + kPiece, s_buf + p0);
+            if (active) w.half_product(half[1], s_buf + s0 + slice * (kPiece / 2));
+            xe_staged();
+            const int second = s0;
+            s0 = s1;
+            s1 = p0;
+            p0 = second;
+        }
+    } else if constexpr (kAll) {
         const char* passed_p = g.passed_p + slice * (int64_t)Wave::kPChunks * kXeChunk;
         int at_s = 0, at_p = 0;
         for (int t = t0; t < t1; ++t) {
@@ -853,6 +809,13 @@ __global__ __launch_bounds__(kBlock, xe_waves(DB, PARTS, USE, WIDE)) void xe_ker
             xe_staged();
             at_s = to_s;
             at_p = to_p;
+        }
+    } else if constexpr (USE == kXeLoss && !kInTurn) {
+        for (int t = t0; t < t1; ++t) {
+            w.first_half(s_buf, p_buf, nullptr, p, both, 32 * t, v0, active);
+            __syncthreads();
+            if (t + 1 < t1) xe_stage<Wave::kSChunks>(g.passed + (t + 1) * kSBytes, s_buf);
+            xe_staged();
         }
     } else if constexpr (USE == kXeLoss) {
         for (int t = t0; t < t1; t += 2) {
@@ -888,8 +851,6 @@ __global__ __launch_bounds__(kBlock, xe_waves(DB, PARTS, USE, WIDE)) void xe_ker
 
     w.sum += xe_other_half(w.sum);
     w.own += xe_other_half(w.own);
-    if constexpr (PARTS == 2 && USE == kXeLossAndRows) w.rescale(xe_power(-w.rise));
-    if constexpr (PARTS == 2 && USE == kXeWeights) w.rescale(w.top / (1 << kXeTop));
     if constexpr (USE == kXeWeights) {
         if (t1 - t0 == plan.tiles) {
             xe_store_weights<typename std::conditional<PARTS == 1, __bf16, float>::type>(g, w.o, v0 + lane % 32, slice, w.sum);
@@ -978,9 +939,9 @@ __global__ __launch_bounds__(kBlock) void xe_combine_kernel(const XeCombineArgs 
     __shared__ float top_of[kEach][32], own_of[kEach][32], rest_of[kEach][32];
     __shared__ double totals[2][kXeWaves];
     __shared__ int last;
-    const int tile = (int)blockIdx.x, block = (int)blockIdx.y, group = tile / kXeWaves * g.slices + block / g.blocks;
+    const int tile = (int)blockIdx.x, block = (int)blockIdx.y, group = g.plan.group_of(tile, block / g.blocks);
     const int64_t row0 = 32LL * tile;
-    const int thread = (int)threadIdx.x, wave = tile % kXeWaves, i = thread % 32, each = thread / 32, lane = thread % kWave;
+    const int thread = (int)threadIdx.x, wave = g.plan.wave_of(tile, block / g.blocks), i = thread % 32, each = thread / 32, lane = thread % kWave;
     const int b0 = g.plan.first(group), parts = g.plan.last(group) - b0 + 1;
     const int64_t place = (int64_t)g.plan.slot(b0, group) * kXeWaves + wave, step = (int64_t)kXeWaves * g.blocks * 4 * kWave;
     const XeF4* s = reinterpret_cast<const XeF4*>(g.stats) + place * 32 + i;
@@ -1147,9 +1108,9 @@ __global__ __launch_bounds__(kBlock) void xe_finish_kernel(const XeFinishArgs g)
     const int tile = id / g.groups_per_tile, in_tile = id % g.groups_per_tile;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x / kWave)), lane = lane_id();
     const int chunk = TOGETHER ? in_tile : in_tile * kXeWaves + wave, slice = chunk / (4 * g.blocks);
-    const int group = tile / kXeWaves * g.slices + slice, b0 = g.plan.first(group), parts = g.plan.last(group) - b0 + 1;
+    const int group = g.plan.group_of(tile, slice), b0 = g.plan.first(group), parts = g.plan.last(group) - b0 + 1;
     if (parts == 1) return;  // (stored as it was formed)
-    const int64_t place = (int64_t)g.plan.slot(b0, group) * kXeWaves + tile % kXeWaves;
+    const int64_t place = (int64_t)g.plan.slot(b0, group) * kXeWaves + g.plan.wave_of(tile, slice);
     const int each = TOGETHER ? (parts + kXeWaves - 1) / kXeWaves : parts, k0 = TOGETHER ? wave * each : 0, k1 = k0 + each < parts ? k0 + each : parts;
     const int64_t step = (int64_t)kXeWaves * g.blocks * 4 * kWave;
     const XeF4* p = reinterpret_cast<const XeF4*>(g.part) + place * (g.blocks * 4 * kWave) + chunk % (4 * g.blocks) * kWave + lane;
@@ -1198,7 +1159,9 @@ __global__ __launch_bounds__(kBlock) void xe_finish_kernel(const XeFinishArgs g)
 inline XePlan xe_plan(const XeShape& s, int use, int kept_tiles, int passed_tiles)
 {
     XePlan p;
-    p.groups = (int)ceil_div(kept_tiles, kXeWaves) * (use == kXeLoss ? 1 : s.slices);
+    p.slices = use == kXeLoss ? 1 : s.slices;
+    p.pairs = xe_pair(s.parts, use, s.slices == 2);
+    p.groups = p.pairs ? (int)ceil_div(kept_tiles, kXeWaves / 2) : (int)ceil_div(kept_tiles, kXeWaves) * p.slices;
     p.tiles = passed_tiles;
     const int room = 256 * xe_waves(s.blocks, s.parts, use, s.slices == 2);
     // at least: so that a part's kept rows and results are little beside its tiles, and for a loss so many parts that the combining kernel holds their
@@ -1206,16 +1169,16 @@ inline XePlan xe_plan(const XeShape& s, int use, int kept_tiles, int passed_tile
     // parts, 53 with 128, 135 with 32, and 69 with 1024, which the kernel's first tile and last stores are much of.)
     int least = (int)ceil_div(passed_tiles, use == kXeWeights ? 512 : kXeMaxParts - 2);
     // Two tiles, unless all of them are few beside the chip.  (1000 rows x 256, 64 classes, forward and backward with one and two: bf16 31 us and 34, fp32 39 and
-    // 43; 172 classes 37 and 36, 45 and 47.  8192 rows, bf16, 64 classes 51 and 50, 172 classes 69 and 57.)
+    // 47; 172 classes 37 and 36, 47 and 51.  8192 rows, bf16, 64 classes 51 and 50, 172 classes 69 and 57.)
     const bool few = (int64_t)p.groups * passed_tiles < room / 4;
     if (least < 2 && !few) least = 2;
     if (least > passed_tiles) least = passed_tiles;
     p.shared = p.groups < room ? room / p.groups : 1;
     p.per = (int)ceil_div(passed_tiles, p.shared);
     if (p.per < least) p.per = least;
-    // The weights' gradient of a few tiles and many classes: parts would cost more to write and add up than they save.  (190 rows, 256 columns,
-    // backward, whole and in parts: bf16, 4 K classes 19 us and 20, 16 K 19 and 25, 32 K 23 and 37; fp32, 8 K classes 32 and 20, 16 K 34 and 34.)
-    if (use == kXeWeights && passed_tiles <= 6 && p.groups > 48 * s.parts) p.per = passed_tiles;
+    // The weights' gradient of a few tiles and many classes in bf16: parts would cost more to write and add up than they save.  (190 rows, 256 columns,
+    // backward, whole and in parts: bf16, 4 K classes 19 us and 20, 16 K 19 and 25, 32 K 23 and 37; fp32, 8 K classes 37 and 24, 16 K 40 and 38, 32 K 48 and 46.)
+    if (use == kXeWeights && passed_tiles <= 6 && s.parts == 1 && p.groups > 48) p.per = passed_tiles;
     p.shared = (int)ceil_div(passed_tiles, p.per);
     p.room = room;
     p.whole = 0;
@@ -1325,19 +1288,13 @@ void launch_xe_parts(const XeShape& s, const XeArgs& g, unsigned workgroups, hip
 {
     const dim3 grid(workgroups), block(kBlock);
     if (s.slices == 2) {
-        if constexpr (PARTS == 1) {
-            if (s.blocks == 6) {
-                hipLaunchKernelGGL((xe_kernel<6, PARTS, USE, true>), grid, block, 0, stream, g);
-                return;
-            }
-        }
-        hipLaunchKernelGGL((xe_kernel<8, PARTS, USE, true>), grid, block, 0, stream, g);
+        if (s.blocks == 6) hipLaunchKernelGGL((xe_kernel<6, PARTS, USE, true>), grid, block, 0, stream, g);
+        else hipLaunchKernelGGL((xe_kernel<8, PARTS, USE, true>), grid, block, 0, stream, g);
         return;
     }
-    if constexpr (PARTS == 2) {
-        if (s.blocks > 8) {
-            if (s.blocks == 10) hipLaunchKernelGGL((xe_kernel<10, PARTS, USE, false>), grid, block, 0, stream, g);
-            else hipLaunchKernelGGL((xe_kernel<12, PARTS, USE, false>), grid, block, 0, stream, g);
+    if constexpr (PARTS == 3) {
+        if (s.blocks == 10) {
+            hipLaunchKernelGGL((xe_kernel<10, PARTS, USE, false>), grid, block, 0, stream, g);
             return;
         }
     }
@@ -1357,7 +1314,7 @@ template <int USE>
 void launch_xe(const XeShape& s, XeArgs& g, int passed_tiles, hipStream_t stream)
 {
     g.plan = xe_plan(s, USE, g.kept_tiles, passed_tiles);
-    if (s.parts == 2) launch_xe_parts<2, USE>(s, g, (unsigned)g.plan.workgroups(), stream);
+    if (s.parts == 3) launch_xe_parts<3, USE>(s, g, (unsigned)g.plan.workgroups(), stream);
     else launch_xe_parts<1, USE>(s, g, (unsigned)g.plan.workgroups(), stream);
 }
 
@@ -1409,7 +1366,7 @@ FGL_EXPORT int fgl_linear_cross_entropy(const void* d_x, int64_t x_row_stride, i
     im.classes = n_classes;
     const dim3 grid((unsigned)(p.row_tiles + p.class_tiles), (unsigned)ceil_div(s.cols(), kXeCols)), block(kBlock);
     im.done = st.done;
-    if (dtype == FGL_F32) hipLaunchKernelGGL((xe_images_kernel<float, 2>), grid, block, 0, to, im);
+    if (dtype == FGL_F32) hipLaunchKernelGGL((xe_images_kernel<float, 3>), grid, block, 0, to, im);
     else hipLaunchKernelGGL((xe_images_kernel<__bf16, 1>), grid, block, 0, to, im);
     FGL_CHECK_LAUNCH("xe_images_kernel");
 

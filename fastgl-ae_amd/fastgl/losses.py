@@ -15,8 +15,9 @@ def linear_cross_entropy(x, weight, labels, bias=None, ignore_index=-100, reduct
     [d, classes] weight will do) and ``bias`` [classes]: float32 or bfloat16, all of one type, ``d`` up to 512.  The logits are formed in pieces
     and never stored; sums, maxima and losses are float32.  ``labels`` [n]: int32 or int64; rows labelled ``ignore_index`` have no loss and no
     gradient, whatever they hold; a label outside ``[0, classes)`` makes a loss that is not a number.  A bias of -1e30 or less, ``-inf`` and the type's
-    lowest value among them, leaves its class out; ``weight`` and the other rows of ``x`` are finite, logits below 1e9 in magnitude.  float32 values
-    2^39 times smaller than the largest one of their row, or in the gradients of the 32 rows or classes around it, count as zero.  Fewer than 2^29
+    lowest value among them, leaves its class out; ``weight`` and the other rows of ``x`` are finite (float32: below 3.38e38), logits below 1e9 in magnitude.
+    In float32 each term of a logit or gradient has that type's precision for itself, however far columns, rows and classes lie apart; values and
+    shares below 2^-110 have fewer bits.  Fewer than 2^29
     rows and classes together, and 2^28 pieces of 32 columns of ``x``.  ``reduction``: ``"mean"`` over the rows that have a label (not a number if
     none has), ``"sum"`` or ``"none"``.
     Under autocast, its type is taken.  No gradients of gradients."""
