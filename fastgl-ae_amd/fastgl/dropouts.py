@@ -10,6 +10,37 @@ from torch import nn
 from . import _lib as L
 from . import ops
 
+_TAG = 0x44524F50  # the counter's last word: "DROP"
+
+def _kept(x, p, seed, stream, stream_offset):
+    """Which elements of ``x`` are kept, in torch's operators: the generator's rounds on whole numbers of 64 bits."""
+    low, n = 0xFFFFFFFF, x.numel()
+    quad = torch.arange((n + 3) // 4, device=x.device)
+    c0, c1, c2, c3 = quad & low, quad >> 32, torch.full_like(quad, stream), torch.full_like(quad, _TAG)
+    if stream_offset is not None:
+        c2 = (c2 + stream_offset.long()) & low
+    k0, k1 = seed & low, seed >> 32
+    for _ in range(10):
+        a, b = c0 * 0xD2511F53, c2 * 0xCD9E8D57  # (modulo 2^64: either half is the product's)
+        c0, c1, c2, c3 = (b >> 32) & low ^ c1 ^ k0, b & low, (a >> 32) & low ^ c3 ^ k1, a & low
+        k0, k1 = (k0 + 0x9E3779B9) & low, (k1 + 0xBB67AE85) & low
+    return (torch.stack([c0, c1, c2, c3], 1).view(-1)[:n] >= round(p * 2.0 ** 32)).view(x.shape)
+
+
+def _by_operators(x, p, seed, stream, relu, stream_offset):
+    """The same values in torch's operators, for who has to see those: some hundred launches."""
+    if x.dtype not in ops._FEAT:
+        raise RuntimeError("x must have dtype in %s, got %s" % ([str(t) for t in ops._FEAT], x.dtype))
+    if not 0.0 <= p <= 1.0:
+        raise RuntimeError("p (%g) is no probability" % p)
+    if stream_offset is not None and stream_offset.numel() != 1:
+        raise RuntimeError("stream_offset must hold one int32")
+    v = torch.relu(x) if relu else x
+    if p == 0.0:
+        return v.clone() if v is x else v
+    scale = 1.0 / (1.0 - p) if p < 1.0 else 0.0
+    return torch.where(_kept(x, p, seed, stream, stream_offset), v.float() * scale, 0.0).to(x.dtype)
+
 
 def dropout(x, p=0.5, seed=0, stream=0, relu=False, training=True, stream_offset=None):
     """``x`` (``relu``: ``max(x, 0)``) with each element kept with probability ``1 - p`` and divided by it, zero otherwise, whatever it
@@ -17,7 +48,9 @@ def dropout(x, p=0.5, seed=0, stream=0, relu=False, training=True, stream_offset
     0x44524F50), key=seed)`` is at least ``round(p * 2**32)``: calls that share a ``seed`` take a ``stream`` (32 bits) of their own each.
     ``stream_offset``: a one-element int32 device tensor that is added to ``stream`` when the kernels run; a captured call draws
     another mask at every replay before which the caller changes it (after the backward pass, which reads it again).
-    ``x``: float32 or bfloat16 on the GPU, contiguous or a matrix whose rows lie apart.  ``training=False``: ``x`` itself, or its ``relu``."""
+    ``x``: float32 or bfloat16 on the GPU, contiguous or a matrix whose rows lie apart.  ``training=False``: ``x`` itself, or its ``relu``.
+    Under tracing, forward-mode differentiation, transforms of ``torch.func`` and modes that follow the operators: the same values by
+    torch's operators (``_by_operators``); a traced call keeps the seed and stream of its trace."""
     if not isinstance(x, torch.Tensor) or not x.is_cuda:
         raise RuntimeError("x must be a CUDA tensor")
     if not 0 <= seed < 1 << 64 or not 0 <= stream < 1 << 32:
@@ -28,6 +61,8 @@ def dropout(x, p=0.5, seed=0, stream=0, relu=False, training=True, stream_offset
         if not relu:
             return x
         p, stream_offset = 0.0, None
+    if ops._unseen(x, *([] if stream_offset is None else [stream_offset])):
+        return _by_operators(x, p, seed, stream, relu, stream_offset)
     return L.host().dropout(x, p, seed, stream, relu, stream_offset)
 
 

@@ -5,9 +5,40 @@ classes as a graph has nodes (which entity is it, out of all?) it saves gigabyte
 from __future__ import annotations
 
 import torch
+from torch.nn import functional as F
 
 from . import _lib as L
+from . import ops
 from .conv import _Linear
+
+
+def _by_operators(x, weight, labels, bias, ignore_index, reduction):
+    """The same in torch's operators, for who has to see those: with the logits in memory, in float32."""
+    if torch.is_autocast_enabled():
+        to = torch.get_autocast_dtype("cuda")
+        x, weight, bias = x.to(to), weight.to(to), None if bias is None else bias.to(to)
+    sized = not torch.jit.is_tracing()  # (a trace is of any sizes, and its operators have their own checks)
+    if x.dim() != 2 or weight.dim() != 2 or (sized and not (x.size(1) == weight.size(1) and weight.size(0) >= 1 and 1 <= x.size(1) <= L.XENT_MAX_DIM)):
+        raise RuntimeError("x %s and weight %s must be [n, d] and [classes, d] with 1 <= d <= %d" % (tuple(x.shape), tuple(weight.shape), L.XENT_MAX_DIM))
+    if not (x.dtype in ops._FEAT and weight.dtype == x.dtype and (bias is None or bias.dtype == x.dtype)):
+        raise RuntimeError("x, weight and bias must all be of one type in %s" % [str(t) for t in ops._FEAT])
+    if bias is not None and (bias.dim() != 1 or (sized and bias.size(0) != weight.size(0))):
+        raise RuntimeError("bias must hold a value for each class")
+    if labels.dim() != 1 or labels.dtype not in (torch.int32, torch.int64) or (sized and labels.size(0) != x.size(0)):
+        raise RuntimeError("labels must be int32 or int64, one for each row of x")
+    with torch.autocast("cuda", enabled=False):
+        valid = labels != ignore_index
+        named = (labels >= 0) & (labels < weight.size(0))
+        if bias is not None:
+            bias = bias.float()
+            bias = torch.where(bias <= -1e30, float("-inf"), bias)
+        logits = F.linear(torch.where(valid[:, None], x.float(), 0.0), weight.float(), bias)
+        losses = -torch.log_softmax(logits, 1).gather(1, torch.where(named, labels, 0).long()[:, None])[:, 0]
+        losses = torch.where(valid, losses * torch.where(valid & ~named, float("nan"), 1.0), 0.0)  # (a bad label's gradients are no numbers either)
+        if reduction == "none":
+            return losses
+        count = valid.sum()
+        return losses.sum() if reduction == "sum" else torch.where(count > 0, losses.sum() / count.clamp(min=1), float("nan"))
 
 
 def linear_cross_entropy(x, weight, labels, bias=None, ignore_index=-100, reduction="mean"):
@@ -20,11 +51,14 @@ def linear_cross_entropy(x, weight, labels, bias=None, ignore_index=-100, reduct
     shares below 2^-110 have fewer bits.  Fewer than 2^29
     rows and classes together, and 2^28 pieces of 32 columns of ``x``.  ``reduction``: ``"mean"`` over the rows that have a label (not a number if
     none has), ``"sum"`` or ``"none"``.
-    Under autocast, its type is taken.  No gradients of gradients."""
+    Under autocast, its type is taken.  No gradients of gradients.  Under tracing, forward-mode differentiation, transforms of ``torch.func`` and modes
+    that follow the operators: by torch's operators, with the logits in memory."""
     if not all(isinstance(t, torch.Tensor) and t.is_cuda for t in (x, weight, labels)) or not (bias is None or (isinstance(bias, torch.Tensor) and bias.is_cuda)):
         raise RuntimeError("x, weight, labels and bias must be CUDA tensors")
     if reduction not in L.REDUCE:
         raise RuntimeError("reduction must be one of %s" % ", ".join(L.REDUCE))
+    if ops._unseen(x, weight, labels, *([] if bias is None else [bias])):
+        return _by_operators(x, weight, labels, bias, ignore_index, reduction)
     return L.host().linear_cross_entropy(x, weight, labels, bias, ignore_index, L.REDUCE[reduction], L.XENT_MAX_DIM)
 
 

@@ -348,6 +348,15 @@ def _followed():
     return n > 0 and any(type(torch._C._get_function_stack_at(i)) is not DeviceContext for i in range(n))
 
 
+def _unseen(*tensors):
+    """Whether a kernel that is no operator of torch's would be missed by who has to see it: a tracer, forward-mode differentiation, what
+    ``_followed`` asks for, or a tensor whose class takes its operators itself.  (The compiler cannot look into these questions and breaks
+    its graph at the kernel's call, which is then made as it is.)"""
+    return not torch.compiler.is_compiling() and (
+        torch.jit.is_tracing() or torch.autograd.forward_ad._current_level >= 0 or _followed() or
+        any(type(t) is not torch.Tensor and type(t) is not torch.nn.Parameter for t in tensors))
+
+
 def _addresses(a, b):
     """Where the two tensors lie, or None if one has no memory of its own: the gradients that ``torch.autograd.grad`` hands to
     backward passes with ``is_grads_batched`` (and ``jacobian`` with ``vectorize``) look like matrices, but only torch's operators take them."""
