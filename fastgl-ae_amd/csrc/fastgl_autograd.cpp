@@ -39,6 +39,13 @@ Tensor bytes_like(const Tensor& t, size_t n)
 
 void* address(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
+// Whether t only looks like a tensor of its sizes and has no memory of its own: a gradient that torch.autograd.grad(is_grads_batched=True) and
+// jacobian(vectorize=True) hand to a backward pass, many at once
+bool is_wrapped(const Tensor& t)
+{
+    return t.key_set().has_any(c10::DispatchKeySet({c10::DispatchKey::Batched, c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper}));
+}
+
 // ---- dropout -------------------------------------------------------------------------------------------------------
 bool gaps_in_rows_only(const Tensor& x) { return x.is_contiguous() || (x.dim() == 2 && x.stride(1) == 1 && x.stride(0) >= x.size(1)); }
 
@@ -77,9 +84,11 @@ struct DropoutNode : torch::autograd::Function<DropoutNode> {
         Tensor d_x;
         if (!d_out.defined()) return {d_x, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
         const bool recorded = torch::GradMode::is_enabled();  // (a graph of the gradients is being built; they are linear in d_out)
+        const bool wrapped = is_wrapped(d_out);
+        const double scale = p < 1.0 ? 1.0 / (1.0 - p) : 0.0;
         if (ctx->saved_data["relu"].toBool()) {
-            if (recorded) {
-                d_x = torch::where(out <= 0, torch::zeros({}, d_out.options()), d_out * (p < 1.0 ? 1.0 / (1.0 - p) : 0.0));
+            if (recorded || wrapped) {
+                d_x = torch::where(out <= 0, torch::zeros({}, d_out.options()), d_out * scale);
             } else {
                 c10::hip::HIPGuard guard(out.get_device());
                 d_out = d_out.contiguous();
@@ -87,6 +96,10 @@ struct DropoutNode : torch::autograd::Function<DropoutNode> {
                 if (d_x.numel() > 0)
                     ok(fgl_dropout_relu_backward(d_out.data_ptr(), out.data_ptr(), out.numel(), type_of(out), p, d_x.data_ptr(), stream_of(out)));
             }
+        } else if (wrapped) {
+            const auto like = at::TensorOptions().dtype(d_out.scalar_type()).device(d_out.device());
+            const Tensor kept = drop(torch::ones(d_out.sizes(), like), p, seed, stream, false, offset);
+            d_x = torch::where(kept == 0, torch::zeros({}, like), d_out * scale);
         } else {
             if (!gaps_in_rows_only(d_out)) d_out = d_out.contiguous();
             if (recorded) d_x = DropoutNode::apply(d_out, p, seed, stream, false, offset.defined() ? Maybe(offset) : Maybe());
@@ -137,6 +150,46 @@ std::tuple<Tensor, Tensor> form_loss(const Tensor& x, const Tensor& w, const May
     return {loss, state};
 }
 
+// What the forward pass left in `state` -> the gradients that are asked for
+std::tuple<Tensor, Tensor, Tensor> loss_gradients(const Tensor& d_loss_of, const Tensor& state, int64_t n, int64_t classes, int64_t dim, int64_t reduction, int64_t want,
+                                                  at::ScalarType type, bool need_x, bool need_w, bool need_b)
+{
+    torch::NoGradGuard no_grad;
+    c10::hip::HIPGuard guard(state.get_device());
+    const auto of = state.options().dtype(type);
+    const int dtype = type == torch::kFloat32 ? FGL_F32 : FGL_BF16;
+    auto make = [&](at::IntArrayRef size) { return n > 0 ? torch::empty(size, of) : torch::zeros(size, of); };
+    Tensor d_x, d_w, d_b;
+    if (need_x) d_x = make({n, dim});
+    if (need_w || need_b) d_w = make({classes, dim});
+    if (need_b) d_b = make({classes});
+    if (n > 0 && (need_x || need_w || need_b)) {
+        const Tensor d_loss = d_loss_of.contiguous();
+        const size_t ws_bytes = fgl_linear_cross_entropy_workspace_bytes(n, classes, (int)dim, dtype, (int)want, 1);
+        Tensor ws;
+        if (ws_bytes > 0) ws = bytes_like(state, ws_bytes);
+        ok(fgl_linear_cross_entropy_backward(d_loss.data_ptr<float>(), n, classes, (int)dim, dtype, (int)reduction, (int)want, state.data_ptr(), (size_t)state.numel(),
+                                             address(d_x), address(d_w), address(d_b), address(ws), ws_bytes, stream_of(state)));
+    }
+    return {d_x, need_w ? d_w : Tensor(), d_b};
+}
+
+// The same as an operator of torch's, whose loop takes gradients of the loss that are many at once apart; it wants a tensor in each place.
+std::tuple<Tensor, Tensor, Tensor> loss_gradients_operator(const Tensor& d_loss, const Tensor& state, int64_t n, int64_t classes, int64_t dim, int64_t reduction, int64_t want,
+                                                           at::ScalarType type, bool need_x, bool need_w, bool need_b)
+{
+    auto made = loss_gradients(d_loss, state, n, classes, dim, reduction, want, type, need_x, need_w, need_b);
+    const auto some = [&](const Tensor& t) { return t.defined() ? t : torch::empty({0}, state.options().dtype(type)); };
+    return {some(std::get<0>(made)), some(std::get<1>(made)), some(std::get<2>(made))};
+}
+
+TORCH_LIBRARY_FRAGMENT(fastgl, m)
+{
+    m.def("linear_cross_entropy_gradients(Tensor d_loss, Tensor state, int n, int classes, int dim, int reduction, int want, ScalarType type, bool need_x, bool need_w, "
+          "bool need_b) -> (Tensor, Tensor, Tensor)",
+          torch::dispatch(c10::DispatchKey::CompositeExplicitAutograd, TORCH_FN(loss_gradients_operator)));
+}
+
 struct LossNode : torch::autograd::Function<LossNode> {
     static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Maybe& bias, const Tensor& labels, int64_t ignore, LossSizes z)
     {
@@ -159,28 +212,21 @@ struct LossNode : torch::autograd::Function<LossNode> {
         const Tensor state = ctx->get_saved_variables()[0];
         const bool with_bias = ctx->saved_data["bias"].toBool();
         const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1), need_b = with_bias && ctx->needs_input_grad(2);
-        const int64_t n = ctx->saved_data["n"].toInt(), classes = ctx->saved_data["classes"].toInt(), dim = ctx->saved_data["dim"].toInt();
-        const int reduction = (int)ctx->saved_data["reduction"].toInt(), want = (int)ctx->saved_data["want"].toInt();
-        const auto of = state.options().dtype(ctx->saved_data["type"].toScalarType());
-        const int dtype = of.dtype() == torch::kFloat32 ? FGL_F32 : FGL_BF16;
-        c10::hip::HIPGuard guard(state.get_device());
-        auto make = [&](at::IntArrayRef size) { return n > 0 ? torch::empty(size, of) : torch::zeros(size, of); };
+        const auto sizes = [&](const char* name) { return ctx->saved_data[name].toInt(); };
+        const auto form = [&](auto&& gradients) {
+            return gradients(grads[0], state, sizes("n"), sizes("classes"), sizes("dim"), sizes("reduction"), sizes("want"), ctx->saved_data["type"].toScalarType(), need_x,
+                             need_w, need_b);
+        };
         Tensor d_x, d_w, d_b;
-        {
-            torch::NoGradGuard no_grad;
-            if (need_x) d_x = make({n, dim});
-            if (need_w || need_b) d_w = make({classes, dim});
-            if (need_b) d_b = make({classes});
-            if (n > 0 && (need_x || need_w || need_b)) {
-                const Tensor d_loss = grads[0].contiguous();
-                const size_t ws_bytes = fgl_linear_cross_entropy_workspace_bytes(n, classes, (int)dim, dtype, want, 1);
-                Tensor ws;
-                if (ws_bytes > 0) ws = bytes_like(state, ws_bytes);
-                ok(fgl_linear_cross_entropy_backward(d_loss.data_ptr<float>(), n, classes, (int)dim, dtype, reduction, want, state.data_ptr(), (size_t)state.numel(),
-                                                     address(d_x), address(d_w), address(d_b), address(ws), ws_bytes, stream_of(state)));
-            }
+        if (is_wrapped(grads[0])) {
+            static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("fastgl::linear_cross_entropy_gradients", "").typed<decltype(loss_gradients)>();
+            std::tie(d_x, d_w, d_b) = form([](auto&&... a) { return op.call(a...); });
+            if (!need_x) d_x = Tensor();
+            if (!need_w) d_w = Tensor();
+            if (!need_b) d_b = Tensor();
+        } else {
+            std::tie(d_x, d_w, d_b) = form(loss_gradients);
         }
-        if (!need_w) d_w = Tensor();
         if (torch::GradMode::is_enabled()) {
             // a graph of the gradients is being built, and they have none: who asks for them is told so
             variable_list made;

@@ -172,3 +172,38 @@ def test_autocast(cuda):
         with Watch():
             got = fastgl.linear_cross_entropy(x, w, y, b)
     assert close(got, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("relu", [False, True])
+@pytest.mark.parametrize("p", [0.4, 1.0])
+def test_batched_gradients_of_dropout(cuda, dtype, relu, p):
+    """The same bits as one after another: a product in fp32, rounded once."""
+    x = make(cuda, dtype)[0].requires_grad_()
+    y = fastgl.dropout(x, p, seed=3, stream=8, relu=relu)
+    v = torch.randn(5, 60, 24, device=cuda).to(dtype)
+    got, = torch.autograd.grad(y, x, v, is_grads_batched=True, retain_graph=True)
+    assert torch.equal(got, torch.stack([torch.autograd.grad(y, x, t, retain_graph=True)[0] for t in v]))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+@pytest.mark.parametrize("needs", [(1, 1, 1), (1, 0, 0), (0, 0, 1)])
+def test_batched_gradients_of_the_loss(cuda, dtype, reduction, needs):
+    x, w, b, y = make(cuda, dtype)
+    leaves = [t.requires_grad_(bool(k)) for t, k in zip((x, w, b), needs)]
+    loss = fastgl.linear_cross_entropy(x, w, y, b, reduction=reduction)
+    v = torch.randn(4, *loss.shape, device=cuda)
+    wanted = [t for t, k in zip(leaves, needs) if k]
+    got = torch.autograd.grad(loss, wanted, v, is_grads_batched=True, retain_graph=True)
+    want = [torch.autograd.grad(loss, wanted, t, retain_graph=True) for t in v]
+    assert all(torch.equal(g, torch.stack(e)) for g, e in zip(got, zip(*want)))
+
+
+def test_vectorized_jacobian(cuda):
+    x, w, b, y = make(cuda, n=6)
+    f = lambda t: fastgl.linear_cross_entropy(t, w, y, b, reduction="none")  # noqa: E731
+    want = torch.autograd.functional.jacobian(f, x)
+    assert torch.equal(torch.autograd.functional.jacobian(f, x, vectorize=True), want)
+    g = lambda t: fastgl.dropout(t, 0.5, seed=1)  # noqa: E731
+    assert torch.equal(torch.autograd.functional.jacobian(g, x, vectorize=True), torch.autograd.functional.jacobian(g, x))
