@@ -28,7 +28,7 @@
 // two thirds of the time, 8192 x 128, 20 K classes, forward and backward 498 us for 782, but share a power of two with the values around them and
 // hold nothing below 2^-39 of the largest of those: one column of x 2^30 times the others took half of the other columns' bits.)
 // Sums, maxima and losses are fp32 in both.  x and w must be finite, and below 3.38e38 in fp32, where a part would round to infinity: others make
-// losses and gradients that are not numbers, but in rows without a label, which are taken as zeros.
+// losses and gradients that are not numbers, but in rows without a label and in classes that are left out, which are taken as zeros.
 // A bias of -1e30 or less, -infinity among them, leaves its class out: no share, no gradient.  (Shares are exp2 of one fma, whose
 // product with log2 e is not rounded where the maximum's is: logits up to some 1e9 are no matter, the difference of 2^-25 of the maximum is the
 // same for all of a row's shares and their sum.)
@@ -155,7 +155,7 @@ template <typename T, int PARTS>
 __global__ __launch_bounds__(kBlock) void xe_images_kernel(const XeImagesArgs g)
 {
     __shared__ float tile[32 * kXePitch];
-    __shared__ int live[32];  // rows that there are, and that have a label
+    __shared__ int live[32];  // rows that there are, and that have a label; classes that no bias leaves out: the others are taken as zeros
     const int64_t id = blockIdx.x;
     const bool classes = id >= g.first_tiles;
     const XeMatrix& m = g.m[classes ? 1 : 0];
@@ -176,7 +176,7 @@ __global__ __launch_bounds__(kBlock) void xe_images_kernel(const XeImagesArgs g)
                 if (y != g.ignore) label = y >= 0 && y < g.classes ? (int)y : -2;  // (-2: no such class)
             }
         }
-        live[thread] = row < m.rows && (classes || label != -1);
+        live[thread] = row < m.rows && (classes ? bias != -INFINITY : label != -1);
     }
     __syncthreads();
     if (m.col_stride == 1) {

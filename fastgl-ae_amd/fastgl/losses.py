@@ -29,10 +29,12 @@ def _by_operators(x, weight, labels, bias, ignore_index, reduction):
     with torch.autocast("cuda", enabled=False):
         valid = labels != ignore_index
         named = (labels >= 0) & (labels < weight.size(0))
+        weight = weight.float()
         if bias is not None:
             bias = bias.float()
-            bias = torch.where(bias <= -1e30, float("-inf"), bias)
-        logits = F.linear(torch.where(valid[:, None], x.float(), 0.0), weight.float(), bias)
+            left_out = bias <= -1e30
+            weight, bias = torch.where(left_out[:, None], 0.0, weight), torch.where(left_out, float("-inf"), bias)
+        logits = F.linear(torch.where(valid[:, None], x.float(), 0.0), weight, bias)
         losses = -torch.log_softmax(logits, 1).gather(1, torch.where(named, labels, 0).long()[:, None])[:, 0]
         losses = torch.where(valid, losses * torch.where(valid & ~named, float("nan"), 1.0), 0.0)  # (a bad label's gradients are no numbers either)
         if reduction == "none":
@@ -46,7 +48,8 @@ def linear_cross_entropy(x, weight, labels, bias=None, ignore_index=-100, reduct
     [d, classes] weight will do) and ``bias`` [classes]: float32 or bfloat16, all of one type, ``d`` up to 512.  The logits are formed in pieces
     and never stored; sums, maxima and losses are float32.  ``labels`` [n]: int32 or int64; rows labelled ``ignore_index`` have no loss and no
     gradient, whatever they hold; a label outside ``[0, classes)`` makes a loss that is not a number.  A bias of -1e30 or less, ``-inf`` and the type's
-    lowest value among them, leaves its class out; ``weight`` and the other rows of ``x`` are finite (float32: below 3.38e38), logits below 1e9 in magnitude.
+    lowest value among them, leaves its class out, whatever its weights hold; the others and the other rows of ``x`` are finite (float32: below 3.38e38), logits
+    below 1e9 in magnitude.
     In float32 each term of a logit or gradient has that type's precision for itself, however far columns, rows and classes lie apart; values and
     shares below 2^-110 have fewer bits.  Fewer than 2^29
     rows and classes together, and 2^28 pieces of 32 columns of ``x``.  ``reduction``: ``"mean"`` over the rows that have a label (not a number if

@@ -479,7 +479,7 @@ int fgl_dropout_relu_backward(const void* d_dout, const void* d_out, int64_t n, 
  * x [n_rows, dim] and w [n_classes, dim] of `dtype`, any strides (in elements); d_bias [n_classes] of `dtype` or NULL, where -1e30 and less, -infinity among them, leave a class out;
  * labels int32 or (label64) int64.  A row labelled ignore_index has loss 0 and no gradient; one with a label outside [0, n_classes) has a
  * loss and gradients that are not numbers.  d_loss: float, n_rows of them (FGL_REDUCE_NONE), or the sum, or the sum over the number of rows with a
- * label.  What a row without a label holds is not looked at; others and w are finite (fp32: below 3.38e38; values below 2^-110 have fewer bits
+ * label.  What a row without a label or a class that is left out holds is not looked at; others are finite (fp32: below 3.38e38; values below 2^-110 have fewer bits
  * in the products).  dim 1 .. 512, n_rows + n_classes below 2^29,
  * n_rows * ceil(dim / 32) below 2^28.
  * want: what the backward pass will be asked for, FGL_XENT_ROWS (dx; formed here up to its factor) and FGL_XENT_WEIGHTS (dw, db).  The state

@@ -80,6 +80,7 @@ def test_loss_of_labels_and_classes_that_are_not():
     for out in (float("-inf"), torch.finfo(torch.float32).min, -1e30):
         b[9] = out
         y[y == 9] = 8
+        w[9] = float("nan")
         leaves = [t.detach().requires_grad_() for t in (x, w, b)]
         loss = losses._by_operators(leaves[0], leaves[1], y, leaves[2], -100, "mean")
         got = torch.autograd.grad(loss, leaves)

@@ -119,3 +119,24 @@ def test_a_large_value_of_one_row(cuda, n, v, d, size):
 def test_gradients_of_losses_of_any_magnitude(cuda, n, v, d, power):
     x, w, b, y = problem(cuda, n, v, d)
     check(x, w, b, y, g=normal(cuda, 6, n) * 2.0 ** power)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("d", [40, 300, 500])
+@pytest.mark.parametrize("what", [float("nan"), float("inf"), 1e30])
+def test_what_classes_that_are_left_out_hold_is_nobodys_matter(cuda, dtype, d, what):
+    """A table of classes that is longer than what it holds: the same bits as with zeros there."""
+    x, w, b, y = problem(cuda, 150, 170, d)
+    out = torch.arange(170, device=cuda) % 5 == 1
+    out[128:] = True  # (a whole tile and the last ones)
+    y = torch.where(out[y], torch.full_like(y, 2), y)
+    for bias in (float("-inf"), torch.finfo(dtype).min):
+        results = []
+        for fill in (0.0, what):
+            leaves = [t.to(dtype).detach() for t in (x, torch.where(out[:, None], fill, w), torch.where(out, bias, b))]
+            for t in leaves:
+                t.requires_grad_()
+            loss = fastgl.linear_cross_entropy(leaves[0], leaves[1], y, leaves[2])
+            results.append([loss.detach(), *torch.autograd.grad(loss, leaves), fastgl.linear_cross_entropy(*(t.detach() for t in leaves[:2]), y, leaves[2].detach())])
+        assert all(torch.isfinite(t).all() and torch.equal(t, u) for t, u in zip(*results))
+        assert (results[1][2][out] == 0).all() and (results[1][3][out] == 0).all()
