@@ -6,11 +6,18 @@ from __future__ import annotations
 
 import torch
 from torch import nn
+from torch.utils._python_dispatch import _disable_current_modes
 
 from . import _lib as L
 from . import ops
 
 _TAG = 0x44524F50  # the counter's last word: "DROP"
+
+def _drawn_seed():
+    """A seed from torch's generator (of the CPU: ``torch.manual_seed`` governs it)."""
+    with _disable_current_modes():  # (a number, also where tensors hold none)
+        return int(torch.randint(0, 2 ** 63 - 1, (), device="cpu"))
+
 
 def _kept(x, p, seed, stream, stream_offset):
     """Which elements of ``x`` are kept, in torch's operators: the generator's rounds on whole numbers of 64 bits."""
@@ -42,10 +49,11 @@ def _by_operators(x, p, seed, stream, relu, stream_offset):
     return torch.where(_kept(x, p, seed, stream, stream_offset), v.float() * scale, 0.0).to(x.dtype)
 
 
-def dropout(x, p=0.5, seed=0, stream=0, relu=False, training=True, stream_offset=None):
+def dropout(x, p=0.5, seed=None, stream=0, relu=False, training=True, stream_offset=None):
     """``x`` (``relu``: ``max(x, 0)``) with each element kept with probability ``1 - p`` and divided by it, zero otherwise, whatever it
     holds.  Element ``i`` of ``x`` in row-major order is kept if word ``i % 4`` of ``philox4x32_10(counter=(i // 4 low, i // 4 high, stream,
     0x44524F50), key=seed)`` is at least ``round(p * 2**32)``: calls that share a ``seed`` take a ``stream`` (32 bits) of their own each.
+    ``seed=None``: another one for each call, from torch's generator (a captured call keeps the one of its capture).
     ``stream_offset``: a one-element int32 device tensor that is added to ``stream`` when the kernels run; a captured call draws
     another mask at every replay before which the caller changes it (after the backward pass, which reads it again).
     ``x``: float32 or bfloat16 on the GPU, contiguous or a matrix whose rows lie apart.  ``training=False``: ``x`` itself, or its ``relu``.
@@ -53,6 +61,8 @@ def dropout(x, p=0.5, seed=0, stream=0, relu=False, training=True, stream_offset
     torch's operators (``_by_operators``); a traced call keeps the seed and stream of its trace."""
     if not isinstance(x, torch.Tensor) or not x.is_cuda:
         raise RuntimeError("x must be a CUDA tensor")
+    if seed is None:
+        seed = _drawn_seed() if training and 0.0 < p < 1.0 else 0
     if not 0 <= seed < 1 << 64 or not 0 <= stream < 1 << 32:
         raise RuntimeError("seed (%d) and stream (%d) are unsigned, of 64 and 32 bits" % (seed, stream))
     if stream_offset is not None:
@@ -68,16 +78,17 @@ def dropout(x, p=0.5, seed=0, stream=0, relu=False, training=True, stream_offset
 
 class Dropout(nn.Module):
     """``dropout`` as a layer: ``seed`` makes the masks of a run, every call in training takes the next stream (``calls`` counts them;
-    set it to repeat or resume a run).  Layers of one model take a seed each, or share one instance.  ``relu=True``: the activation before it goes with it, in
+    set it to repeat or resume a run).  Layers of one model take a seed each, or share one instance; ``seed=None``: one from torch's generator
+    when the layer is made.  ``relu=True``: the activation before it goes with it, in
     evaluation too.  ``stream_offset``: as for ``dropout``, for calls that are captured in a graph (whose stream numbers are those of the
     capture: advance it by more than the calls that one replay makes).  A layer that is computed anew for its backward pass (activation
     checkpoints) would take another stream there: call ``dropout`` with a ``stream`` of its own in such a layer."""
 
-    def __init__(self, p=0.5, seed=0, relu=False):
+    def __init__(self, p=0.5, seed=None, relu=False):
         super().__init__()
         if not 0.0 <= p <= 1.0:
             raise ValueError("p (%g) is no probability" % p)
-        self.p, self.seed, self.relu = float(p), int(seed), bool(relu)
+        self.p, self.seed, self.relu = float(p), _drawn_seed() if seed is None else int(seed), bool(relu)
         self.calls = 0
         self.stream_offset = None
 

@@ -1,0 +1,48 @@
+"""fastgl.dropout without a seed, and layers without one."""
+import pytest
+import torch
+
+import fastgl
+
+pytestmark = pytest.mark.gpu
+
+
+def test_calls_without_a_seed_draw_one_each(cuda):
+    x = torch.randn(40, 30, device=cuda)
+    torch.manual_seed(3)
+    a, b = fastgl.dropout(x, 0.5), fastgl.dropout(x, 0.5)
+    torch.manual_seed(3)
+    assert torch.equal(fastgl.dropout(x, 0.5), a) and not torch.equal(a, b) and torch.equal(fastgl.dropout(x, 0.5), b)
+    # no draw where there is none to make
+    state = torch.get_rng_state()
+    assert torch.equal(fastgl.dropout(x, 0.0), x) and (fastgl.dropout(x, 1.0) == 0).all() and fastgl.dropout(x, 0.5, training=False) is x
+    fastgl.dropout(x, 0.5, seed=7)
+    assert torch.equal(torch.get_rng_state(), state)
+    # the backward pass has the forward's
+    y = x.clone().requires_grad_()
+    out = fastgl.dropout(y, 0.5)
+    g, = torch.autograd.grad(out, y, torch.ones_like(x))
+    assert torch.equal(g != 0, out != 0)
+
+
+def test_two_layers_without_a_seed_lose_different_elements(cuda):
+    x = torch.ones(1000, device=cuda)
+    first, second = fastgl.Dropout(0.5), fastgl.Dropout(0.5)
+    # (the chance that they agree in every element: 2^-1000)
+    assert not torch.equal(first(x), second(x))
+
+
+def test_recomputed_for_the_backward_pass(cuda):
+    """An activation checkpoint puts torch's generator back: a call without a seed draws the same one."""
+    from torch.utils.checkpoint import checkpoint
+    x = torch.randn(50, 20, device=cuda, requires_grad=True)
+    out = checkpoint(lambda t: fastgl.dropout(t, 0.5).sin(), x, use_reentrant=False)
+    g, = torch.autograd.grad(out, x, torch.ones_like(x))
+    assert torch.equal(g != 0, out != 0)
+
+
+def test_compiled_without_a_seed(cuda):
+    x = torch.ones(400, device=cuda)
+    compiled = torch.compile(lambda t: fastgl.dropout(t * 2.0, 0.5) + 1.0, backend="eager")
+    a, b = compiled(x), compiled(x)
+    assert not torch.equal(a, b) and set(a.tolist()) == {1.0, 5.0}
