@@ -170,9 +170,19 @@ def _stack(conv, in_feats, n_hidden, n_classes, n_layers, weight):
     return layers
 
 
+def _drop_dropout_state(module, state_dict, prefix, *rest):
+    """Before a state is loaded: torch's dropout has none."""
+    state_dict.pop(prefix + "_extra_state", None)
+
+
 def _between_layers(p, seed, relu=False):
-    """The dropout between a model's layers: torch's, or -- with a seed -- the one whose masks are a function of it (and of the call)."""
-    return nn.Dropout(p=p) if seed is None else Dropout(p, seed, relu)
+    """The dropout between a model's layers: torch's, or -- with a seed -- the one whose masks are a function of it (and of the call).  Either
+    takes the state of a model with the other."""
+    if seed is not None:
+        return Dropout(p, seed, relu)
+    plain = nn.Dropout(p=p)
+    plain.register_load_state_dict_pre_hook(_drop_dropout_state)
+    return plain
 
 
 class GCN(nn.Module):

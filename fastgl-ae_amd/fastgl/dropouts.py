@@ -78,7 +78,8 @@ def dropout(x, p=0.5, seed=None, stream=0, relu=False, training=True, stream_off
 
 class Dropout(nn.Module):
     """``dropout`` as a layer: ``seed`` makes the masks of a run, every call in training takes the next stream (``calls`` counts them;
-    set it to repeat or resume a run).  Layers of one model take a seed each, or share one instance; ``seed=None``: one from torch's generator
+    set it to repeat a run).  Both are in ``state_dict()``, so that a run that is resumed goes on with the next stream; a state without them leaves
+    them as they are.  Layers of one model take a seed each, or share one instance; ``seed=None``: one from torch's generator
     when the layer is made.  ``relu=True``: the activation before it goes with it, in
     evaluation too.  ``stream_offset``: as for ``dropout``, for calls that are captured in a graph (whose stream numbers are those of the
     capture: advance it by more than the calls that one replay makes).  A layer that is computed anew for its backward pass (activation
@@ -88,6 +89,8 @@ class Dropout(nn.Module):
         super().__init__()
         if not 0.0 <= p <= 1.0:
             raise ValueError("p (%g) is no probability" % p)
+        if seed is not None and not 0 <= int(seed) < 1 << 64:
+            raise ValueError("seed (%d) is unsigned, of 64 bits" % seed)
         self.p, self.seed, self.relu = float(p), _drawn_seed() if seed is None else int(seed), bool(relu)
         self.calls = 0
         self.stream_offset = None
@@ -98,6 +101,18 @@ class Dropout(nn.Module):
         stream = self.calls & 0xFFFFFFFF
         self.calls += 1
         return dropout(x, self.p, self.seed, stream, self.relu, True, self.stream_offset)
+
+    def get_extra_state(self):
+        return torch.tensor([self.seed - (self.seed >> 63 << 64), self.calls], dtype=torch.int64, device="cpu")
+
+    def set_extra_state(self, state):
+        seed, self.calls = state.tolist()
+        self.seed = seed % (1 << 64)
+
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs):
+        super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs)
+        if prefix + "_extra_state" in missing_keys:  # (the state of a model without a seed)
+            missing_keys.remove(prefix + "_extra_state")
 
     def extra_repr(self):
         return "p=%g, seed=%d%s" % (self.p, self.seed, ", relu=True" if self.relu else "")

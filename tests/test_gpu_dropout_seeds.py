@@ -46,3 +46,14 @@ def test_compiled_without_a_seed(cuda):
     compiled = torch.compile(lambda t: fastgl.dropout(t * 2.0, 0.5) + 1.0, backend="eager")
     a, b = compiled(x), compiled(x)
     assert not torch.equal(a, b) and set(a.tolist()) == {1.0, 5.0}
+
+
+def test_a_resumed_layer_draws_what_the_run_would_have(cuda):
+    x = torch.ones(500, device=cuda)
+    layer = fastgl.Dropout(0.5, seed=12)
+    layer(x)
+    state = layer.state_dict()
+    want = [layer(x), layer(x)]
+    resumed = fastgl.Dropout(0.5)
+    resumed.load_state_dict(state)
+    assert all(torch.equal(resumed(x), w) for w in want)
