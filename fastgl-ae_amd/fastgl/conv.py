@@ -561,13 +561,28 @@ class SAGEConv(nn.Module):
         return self.fc_self(feat_dst) + self.fc_neigh(h_neigh)
 
 
+_RELUS = (torch.relu, nn.functional.relu)  # what a seeded dropout takes along
+
+
 class SAGE(nn.Module):
     def __init__(self, in_feats, n_hidden, n_classes, n_layers, activation=torch.relu, dropout=0.0, dropout_seed=None):
         super().__init__()
         dims = [in_feats] + [n_hidden] * (n_layers - 1) + [n_classes]
         self.layers = nn.ModuleList(SAGEConv(dims[i], dims[i + 1]) for i in range(n_layers))
         self.activation = activation
-        self.dropout = _between_layers(dropout, dropout_seed, relu=activation in (torch.relu, nn.functional.relu))
+        self.dropout = _between_layers(dropout, dropout_seed, relu=activation in _RELUS)
+        self.dropout.takes_activation = dropout_seed is not None and activation in _RELUS
+
+    def _between(self, h):
+        """What is between two layers: the activation and the dropout, as one where that is what ``__init__`` made it."""
+        if getattr(self.dropout, "takes_activation", False):
+            relu = self.activation in _RELUS  # (it may be another one by now)
+            if self.activation is not None and not relu:
+                h = self.activation(h)
+            return self.dropout(h, relu)
+        if self.activation is not None and not getattr(self.dropout, "relu", False):
+            h = self.activation(h)
+        return self.dropout(h)
 
     def forward(self, blocks, features, input_nodes=None):
         """``features``: the rows of the input nodes, or -- with ``input_nodes`` given -- the
@@ -584,7 +599,5 @@ class SAGE(nn.Module):
             else:
                 h = layer(block, h)
             if i != len(self.layers) - 1:
-                if self.activation is not None and not getattr(self.dropout, "relu", False):  # (else it goes with the dropout)
-                    h = self.activation(h)
-                h = self.dropout(h)
+                h = self._between(h)
         return h

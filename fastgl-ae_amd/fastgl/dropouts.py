@@ -95,12 +95,14 @@ class Dropout(nn.Module):
         self.calls = 0
         self.stream_offset = None
 
-    def forward(self, x):
+    def forward(self, x, relu=None):
+        """``relu``: in the place of the layer's own, if given."""
+        relu = self.relu if relu is None else relu
         if not self.training:
-            return dropout(x, 0.0, relu=self.relu, training=False)
+            return dropout(x, 0.0, relu=relu, training=False)
         stream = self.calls & 0xFFFFFFFF
         self.calls += 1
-        return dropout(x, self.p, self.seed, stream, self.relu, True, self.stream_offset)
+        return dropout(x, self.p, self.seed, stream, relu, True, self.stream_offset)
 
     def get_extra_state(self):
         return torch.tensor([self.seed - (self.seed >> 63 << 64), self.calls], dtype=torch.int64, device="cpu")

@@ -57,3 +57,24 @@ def test_a_resumed_layer_draws_what_the_run_would_have(cuda):
     resumed = fastgl.Dropout(0.5)
     resumed.load_state_dict(state)
     assert all(torch.equal(resumed(x), w) for w in want)
+
+
+@pytest.mark.parametrize("activation", [None, torch.tanh, torch.nn.functional.relu])
+@pytest.mark.parametrize("training", [False, True])
+def test_an_activation_that_is_changed_is_the_one_that_is_taken(cuda, activation, training):
+    edge_ptr, edge_src = fastgl.graph.rmat_csr(2000, 20000, seed=3, device=cuda)
+    sampler = fastgl.FusedMapSampler([3, 3], rng_seed=1).set_graph(edge_ptr, edge_src)
+    inputs, _, blocks = sampler.sample_blocks(None, torch.arange(50, dtype=torch.int32, device=cuda) * 31)
+    x = torch.randn(inputs.numel(), 8, device=cuda)
+    model = fastgl.SAGE(8, 16, 5, 2, dropout=0.5, dropout_seed=4).to(cuda).train(training)
+    assert model.dropout.relu
+    model.activation = activation
+    with torch.no_grad():
+        got = model(blocks, x)
+        h = model.layers[0](blocks[0], x)
+        h = h if activation is None else activation(h)
+        h = fastgl.dropout(h, 0.5, seed=4, stream=0, training=training)
+        assert torch.equal(got, model.layers[1](blocks[1], h))
+        own = fastgl.Dropout(0.0, seed=1, relu=True)  # (a layer of the caller's is taken as it is)
+        model.dropout, model.activation = own, None
+        assert torch.equal(model(blocks, x), model.layers[1](blocks[1], model.layers[0](blocks[0], x).clamp(min=0)))
