@@ -74,8 +74,8 @@ constexpr int kXeShift = 0, kXeFactor = 32, kXeLabel = 64, kXeOwn = 96;
 
 // Sizes of a problem as the kernels see it: blocks of 32 columns, padded.  Beyond 256 columns in bf16, 320 in fp32, in two slices, each with half of O,
 // which otherwise did not fit a wave's registers.  bf16 forms S for either.  In fp32 half of the columns of the kept rows is all that fits beside half of
-// O too: two waves share them, each forms its half of S, and they add the halves up.  (8192 rows, 10 K classes, 512 columns, forward and backward: 2261
-// us, 3140 with S formed for either and the kept rows' other half read from the L2 for each tile, 2293 by the library; 384 columns 1856, 1835 with S
+// O too: two waves share them, each forms its half of S, and they add the halves up.  (8192 rows, 10 K classes, 512 columns, forward and backward: 2076
+// us, 3140 with S formed for either and the kept rows' other half read from the L2 for each tile, 2293 by the library; 384 columns 1608, 1835 with S
 // formed for either, 1800 by the library.)  (bf16 could have 384 columns whole, with one wave a SIMD instead of
 // two: 8192 rows, 20 K classes, forward, 300 columns 340 us against 352 in slices, 370 columns 556 against 352.)
 struct XeShape {
@@ -419,14 +419,16 @@ struct XeWave {
         }
         return acc;
     }
-    // acc and the products of the kept rows with operands that lie one after another
+    // acc and the products of the kept rows, from step FIRST on, with operands that lie one after another
+    template <int FIRST>
     __device__ __forceinline__ XeF32x16 logits(const char* s, XeF32x16 acc) const
     {
-        xe_products<kKept, PARTS>([&](int k) { return s + k * PARTS * kXeChunk; }, [&](int k, const XeOp (&a)[PARTS]) { acc = xe_mfma(a, kept[k], acc); });
+        constexpr int kN = kPair ? DB : kKept;
+        xe_products<kN, PARTS>([&](int k) { return s + k * PARTS * kXeChunk; }, [&](int k, const XeOp (&a)[PARTS]) { acc = xe_mfma(a, kept[FIRST + k], acc); });
         return acc;
     }
     // S^T of the staged tile
-    __device__ __forceinline__ XeF32x16 logits(const char* s) const { return logits(s + kXeChunk, biases(s)); }
+    __device__ __forceinline__ XeF32x16 logits(const char* s) const { return logits<0>(s + kXeChunk, biases(s)); }
 
     // Four values of the staged tile's rows that a lane's values 4 q .. 4 q + 3 of S^T belong to.
     static __device__ __forceinline__ XeF4 of_rows(const char* tile, int what, int q)
@@ -560,7 +562,66 @@ struct XeWave {
         }
     }
 
-    // The same with one half of a tile's passed rows, of a pair's wave
+    // Half of the steps of a pair's tile, of either slice, to one place: the first or the second half of each slice's operands of S, or of O
+    static constexpr int kPiece = 2 * DB * PARTS * kXeChunk;
+    static __device__ __forceinline__ void stage_piece(const char* tile, int half, char* to)
+    {
+        xe_stage<DB * PARTS>(tile + half * (kPiece / 2), to);
+        xe_stage<DB * PARTS>(tile + kPiece + half * (kPiece / 2), to + kPiece / 2);
+    }
+    // One tile of a pair, whose S and P go through LDS in four such pieces, each in one of three places (arrays of their own: in one array, all reads wait
+    // for the copies; 512 columns 2261 us for 2076).  At the start a and b have S, in the end b and c the next tile's; next: that, or null.
+    __device__ __forceinline__ void pair_tile(char* a, char* b, char* c, char* header, const char* of_p, const char* next, int slice, int n0, int v0, bool active)
+    {
+        const int own = slice * (kPiece / 2), wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x / kWave));
+        stage_piece(of_p, 0, c);
+        XeF32x16 p = {};
+        if (active) {
+            if (slice == 0) p = biases(header);
+            p = logits<0>(a + own, p);
+            p = logits<DB>(b + own, p);
+        }
+        __syncthreads();
+        // the other wave's half of S is added (the same sum for both)
+        XeF4* mine = reinterpret_cast<XeF4*>(a) + wave * 4 * kWave + lane_id();
+        const XeF4* others = reinterpret_cast<const XeF4*>(a) + (wave ^ 1) * 4 * kWave + lane_id();
+        if (active) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) mine[q * kWave] = XeF4{p[4 * q], p[4 * q + 1], p[4 * q + 2], p[4 * q + 3]};
+        }
+        __syncthreads();
+        XeOp w[2][PARTS];
+        if (active) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const XeF4 v = others[q * kWave];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) p[4 * q + j] += v[j];
+            }
+            if constexpr (USE == kXeWeights) gradients(p, header, v0);
+            else shares(p, n0);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float v[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = p[8 * h + j];
+                xe_operands<PARTS>(v, w[h]);
+            }
+        }
+        xe_staged();
+        stage_piece(of_p, 1, a);
+        if (next != nullptr) {
+            xe_stage<1>(next, header);
+            stage_piece(next + kXeChunk, 0, b);
+        }
+        if (active) half_product(w[0], c + own);
+        xe_staged();
+        if (next != nullptr) stage_piece(next + kXeChunk, 1, c);
+        if (active) half_product(w[1], a + own);
+        xe_staged();
+    }
+
+    // O^T += passed^T P^T of one half of a tile's passed rows
     __device__ __forceinline__ void half_product(const XeOp (&w)[PARTS], const char* p)
     {
         XeF32x16 sum[2];
@@ -666,17 +727,14 @@ __global__ __launch_bounds__(kBlock, xe_waves(DB, PARTS, USE, WIDE)) void xe_ker
     // gradient, which has a second product for some tiles, has no registers left for the one loop body: 955 us for 353.)
     constexpr bool kAll = USE == kXeLossAndRows && PARTS == 1 && DB >= 6 && !(WIDE && DB == 8);
     constexpr bool kPair = Wave::kPair;
-    // A pair's tile goes through LDS in four pieces, each in one of three places: the halves of S, of either wave's columns, and of P, of either half
-    // of the passed rows.
-    constexpr int kPiece = Wave::kPChunks * kXeChunk;
-    __shared__ __attribute__((aligned(16))) char s_buf[kPair ? 3 * kPiece : (kAll ? 2 : 1) * Wave::kSChunks * kXeChunk];
+    __shared__ __attribute__((aligned(16))) char s_buf[kPair ? Wave::kPiece : (kAll ? 2 : 1) * Wave::kSChunks * kXeChunk];
     // the loss alone: two tiles in turn, or one where LDS has no room for two
     constexpr bool kInTurn = USE == kXeLoss && 2 * Wave::kSChunks <= 156;
     __shared__ __attribute__((aligned(16))) char p_buf[(kPair ? 1 : USE != kXeLoss ? (kAll ? 2 : 1) * Wave::kPChunks : kInTurn ? Wave::kSChunks : 1) * kXeChunk];
     // In slices S is most of the work and O too little to hide the next S tile's copy behind.  (8192 x 512, 10 K classes, backward 399 us with
     // one S tile, 348 with two; two of P as well, 1250 us for 1147 of 40 K classes, forward.  Slices of 192 columns, two waves a SIMD, have no registers left for it.)
     constexpr bool kTwo = WIDE && DB == 8 && PARTS == 1 && USE != kXeLoss;
-    __shared__ __attribute__((aligned(16))) char s_other[(kTwo ? Wave::kSChunks : 1) * kXeChunk];
+    __shared__ __attribute__((aligned(16))) char s_other[kPair ? Wave::kPiece : kTwo ? Wave::kSChunks * kXeChunk : 16], third[kPair ? Wave::kPiece : 16];
     constexpr int kSlices = WIDE && USE != kXeLoss && !kPair ? 2 : 1;
     constexpr int64_t kSBytes = (int64_t)Wave::kSChunks * kXeChunk, kPBytes = (int64_t)Wave::kPChunks * (WIDE ? 2 : 1) * kXeChunk;
     const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x / kWave));
@@ -738,65 +796,23 @@ __global__ __launch_bounds__(kBlock, xe_waves(DB, PARTS, USE, WIDE)) void xe_ker
     bool both = false;
     if constexpr (kPair) {
         xe_stage<1>(g.passed + t0 * kSBytes, p_buf);
-        xe_stage<2 * Wave::kPChunks>(g.passed + t0 * kSBytes + kXeChunk, s_buf);
+        Wave::stage_piece(g.passed + t0 * kSBytes + kXeChunk, 0, s_buf);
+        Wave::stage_piece(g.passed + t0 * kSBytes + kXeChunk, 1, s_other);
     } else {
         xe_stage<Wave::kSChunks>(g.passed + t0 * kSBytes, s_buf);
     }
     if constexpr (kAll) xe_stage<Wave::kPChunks>(g.passed_p + slice * (int64_t)Wave::kPChunks * kXeChunk + t0 * kPBytes, p_buf);
     xe_staged();
     if constexpr (kPair) {
-        int s0 = 0, s1 = kPiece, p0 = 2 * kPiece;  // where the tile's S halves and its first P half lie
-        for (int t = t0; t < t1; ++t) {
-            const bool more = t + 1 < t1;
-            const char *next = g.passed + (t + 1) * kSBytes, *of_p = g.passed_p + t * kPBytes;
-            const auto stage_p = [&](int half, int to) {  // (of both slices)
-                xe_stage<Wave::kPChunks / 2>(of_p + half * (kPiece / 2), s_buf + to);
-                xe_stage<Wave::kPChunks / 2>(of_p + kPiece + half * (kPiece / 2), s_buf + to + kPiece / 2);
-            };
-            stage_p(0, p0);
-            // either wave's half of S, then the other's added (the same sum for both)
-            if (active) p = w.logits(s_buf + (slice == 0 ? s0 : s1), slice == 0 ? w.biases(p_buf) : XeF32x16{});
-            __syncthreads();
-            XeF4* mine = reinterpret_cast<XeF4*>(s_buf + s0) + wave * 4 * kWave + lane;
-            const XeF4* others = reinterpret_cast<const XeF4*>(s_buf + s0) + (wave ^ 1) * 4 * kWave + lane;
-            if (active) {
-#pragma unroll
-                for (int q = 0; q < 4; ++q) mine[q * kWave] = XeF4{p[4 * q], p[4 * q + 1], p[4 * q + 2], p[4 * q + 3]};
-            }
-            __syncthreads();
-            XeOp half[2][PARTS];
-            if (active) {
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const XeF4 v = others[q * kWave];
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) p[4 * q + c] += v[c];
-                }
-                if constexpr (USE == kXeWeights) w.gradients(p, p_buf, v0);
-                else w.shares(p, 32 * t);
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    float v[8];
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) v[j] = p[8 * h + j];
-                    xe_operands<PARTS>(v, half[h]);
-                }
-            }
-            xe_staged();
-            stage_p(1, s0);
-            if (more) {
-                xe_stage<1>(next, p_buf);
-                xe_stage<Wave::kPChunks>(next + kXeChunk, s_buf + s1);
-            }
-            if (active) w.half_product(half[0], s_buf + p0 + slice * (kPiece / 2));
-            xe_staged();
-            if (more) xe_stage<Wave::kPChunks>(next + kXeChunk + kPiece, s_buf + p0);
-            if (active) w.half_product(half[1], s_buf + s0 + slice * (kPiece / 2));
-            xe_staged();
-            const int second = s0;
-            s0 = s1;
-            s1 = p0;
-            p0 = second;
+        const auto step = [&](int t, char* a, char* b, char* c) {
+            w.pair_tile(a, b, c, p_buf, g.passed_p + t * kPBytes, t + 1 < t1 ? g.passed + (t + 1) * kSBytes : nullptr, slice, 32 * t, v0, active);
+        };
+        for (int t = t0; t < t1; t += 3) {
+            step(t, s_buf, s_other, third);
+            if (t + 1 == t1) break;
+            step(t + 1, s_other, third, s_buf);
+            if (t + 2 == t1) break;
+            step(t + 2, third, s_buf, s_other);
         }
     } else if constexpr (kAll) {
         const char* passed_p = g.passed_p + slice * (int64_t)Wave::kPChunks * kXeChunk;
