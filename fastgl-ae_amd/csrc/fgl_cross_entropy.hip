@@ -39,9 +39,9 @@
 // run).
 //
 // What bounds it: for many classes the matrix cores and, beside them, LDS, whose operands at 1 KB for an instruction of 32 cycles would take all of its
-// rate if the cores were never idle.  8192 x 256, 100 K classes, bf16: 725 .. 770 us forward, 770 .. 835 backward (the clock falls as the chip warms up),
-// 1.00 .. 1.16 PFLOP/s (a large matrix product of the library 1.24), matrix cores busy 63 and 57 % of the cycles at the 1.8 GHz that the power limit
-// leaves.  8192 x 128, 20 K classes, fp32: 242 .. 260 us and 250 .. 274, 0.92 .. 1.04 PFLOP/s of fp16, busy 54 and 50 % beside the exponentials and splits.
+// rate if the cores were never idle.  8192 x 256, 100 K classes, bf16: 690 .. 770 us forward, 735 .. 835 backward (the clock falls as the chip warms up),
+// 1.00 .. 1.22 PFLOP/s (a large matrix product of the library 1.24), matrix cores busy 63 and 57 % of the cycles at the 1.8 GHz that the power limit
+// leaves.  8192 x 128, 20 K classes, fp32: 372 .. 397 us and 386 .. 419, 1.20 .. 1.35 PFLOP/s of bf16 (six products), busy 68 and 64 % beside the exponentials and splits.
 // The loss alone, bf16, is bound by the exponentials, maxima and sums: 2000 x 100, 100 K classes 66 us, busy 34 %.  For a few classes: launches of 5 to
 // 20 us, mostly latency.
 #include "fgl_common.hpp"

@@ -71,7 +71,7 @@ def dropout(x, p=0.5, seed=None, stream=0, relu=False, training=True, stream_off
         if not relu:
             return x
         p, stream_offset = 0.0, None
-    if ops._unseen(x, *([] if stream_offset is None else [stream_offset])):
+    if ops._unseen(x, stream_offset):
         return _by_operators(x, p, seed, stream, relu, stream_offset)
     return L.host().dropout(x, p, seed, stream, relu, stream_offset)
 

@@ -352,9 +352,12 @@ def _unseen(*tensors):
     """Whether a kernel that is no operator of torch's would be missed by who has to see it: a tracer, forward-mode differentiation, what
     ``_followed`` asks for, or a tensor whose class takes its operators itself.  (The compiler cannot look into these questions and breaks
     its graph at the kernel's call, which is then made as it is.)"""
-    return not torch.compiler.is_compiling() and (
-        torch.jit.is_tracing() or torch.autograd.forward_ad._current_level >= 0 or _followed() or
-        any(type(t) is not torch.Tensor and type(t) is not torch.nn.Parameter for t in tensors))
+    if torch.compiler.is_compiling():
+        return False
+    for t in tensors:
+        if type(t) is not torch.Tensor and type(t) is not torch.nn.Parameter and t is not None:
+            return True
+    return torch.jit.is_tracing() or torch.autograd.forward_ad._current_level >= 0 or _followed()
 
 
 def _addresses(a, b):
