@@ -10,6 +10,7 @@
 #include <c10/hip/HIPGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 
 #include <string>
 #include <tuple>
@@ -228,15 +229,24 @@ struct LossNode : torch::autograd::Function<LossNode> {
             std::tie(d_x, d_w, d_b) = form(loss_gradients);
         }
         if (torch::GradMode::is_enabled()) {
-            // a graph of the gradients is being built, and they have none: who asks for them is told so
-            variable_list made;
-            for (Tensor* t : {&d_x, &d_w, &d_b})
-                if (t->defined()) made.push_back(t->detach().set_requires_grad(true));
-            auto node = std::make_shared<torch::autograd::DelayedError>("linear_cross_entropy has no gradients of its gradients", (int64_t)made.size());
-            made = (*node)(std::move(made));
-            size_t k = 0;
-            for (Tensor* t : {&d_x, &d_w, &d_b})
-                if (t->defined()) *t = made[k++];
+            // A graph of the gradients is being built, and they have none: who asks for them is told so.  By a node that leads on to what they would be of, so
+            // that it is met also where only some tensor's gradients are asked for.
+            torch::autograd::edge_list of;
+            for (const auto& edge : torch::autograd::get_current_node()->next_edges())
+                if (edge.is_valid()) of.push_back(edge);
+            const bool wrapped = is_wrapped(grads[0]);
+            if (!wrapped && grads[0].requires_grad()) of.push_back(torch::autograd::impl::gradient_edge(grads[0]));
+            const auto node = std::make_shared<torch::autograd::Error>("linear_cross_entropy has no gradients of its gradients", std::move(of));
+            Tensor zero;  // wrapped tensors get no node: one is added that has it
+            if (wrapped) {
+                zero = torch::full({}, -0.0, state.options().dtype(ctx->saved_data["type"].toScalarType()));
+                torch::autograd::set_history(zero, node);
+            }
+            for (Tensor* t : {&d_x, &d_w, &d_b}) {
+                if (!t->defined()) continue;
+                if (wrapped) *t = *t + zero;
+                else torch::autograd::set_history(*t, node);
+            }
         }
         out[0] = d_x;
         out[1] = d_w;

@@ -207,3 +207,47 @@ def test_vectorized_jacobian(cuda):
     assert torch.equal(torch.autograd.functional.jacobian(f, x, vectorize=True), want)
     g = lambda t: fastgl.dropout(t, 0.5, seed=1)  # noqa: E731
     assert torch.equal(torch.autograd.functional.jacobian(g, x, vectorize=True), torch.autograd.functional.jacobian(g, x))
+
+
+def test_vectorized_jacobian_with_a_graph(cuda):
+    x, w, b, y = make(cuda, n=6)
+    f = lambda t: fastgl.linear_cross_entropy(t, w, y, b, reduction="none")  # noqa: E731
+    x.requires_grad_()
+    made = torch.autograd.functional.jacobian(f, x, create_graph=True, vectorize=True)
+    assert torch.equal(made.detach(), torch.autograd.functional.jacobian(f, x))
+    with pytest.raises(RuntimeError, match="no gradients of its gradients"):
+        torch.autograd.grad(made.sum() + (x * x).sum(), x)
+    g = lambda t: fastgl.dropout(t, 0.5, seed=1, relu=True)  # noqa: E731
+    assert torch.equal(torch.autograd.functional.jacobian(g, x, create_graph=True, vectorize=True).detach(), torch.autograd.functional.jacobian(g, x))
+
+
+def test_a_traced_model(cuda):
+    """A whole seeded SAGE in evaluation, blocks held: another input than that of the trace."""
+    edge_ptr, edge_src = fastgl.graph.rmat_csr(2000, 20000, seed=3, device=cuda)
+    sampler = fastgl.FusedMapSampler([3, 3], rng_seed=1).set_graph(edge_ptr, edge_src)
+    inputs, _, blocks = sampler.sample_blocks(None, torch.arange(50, dtype=torch.int32, device=cuda) * 31)
+    x = torch.randn(inputs.numel(), 8, device=cuda)
+    seeded = fastgl.SAGE(8, 16, 5, 2, dropout=0.5, dropout_seed=4).to(cuda).eval()
+    with torch.no_grad(), forward_ad.dual_level():
+        y, tangent = forward_ad.unpack_dual(seeded._between(forward_ad.make_dual(x, torch.ones_like(x))))
+    assert torch.equal(y, x.clamp(min=0)) and torch.equal(tangent, (x > 0).float())
+
+
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_gradients_of_gradients_are_refused_wherever_they_are_asked_for(cuda, reduction):
+    """A penalty on a gradient beside something that has second derivatives: the sum must not come back without the penalty's part."""
+    leaves = [t.requires_grad_() for t in make(cuda)[:3]]
+    y = make(cuda)[3]
+    d = torch.ones(60 if reduction == "none" else (), device=cuda, requires_grad=True)
+    for k in range(3):
+        loss = fastgl.linear_cross_entropy(leaves[0], leaves[1], y, leaves[2], reduction=reduction)
+        grads = torch.autograd.grad(loss, leaves, d, create_graph=True)
+        assert all(torch.equal(p.detach(), q) for p, q in zip(grads, torch.autograd.grad(loss, leaves, d.detach(), retain_graph=True)))
+        total = grads[k].square().sum() + sum(t.square().sum() for t in leaves) + d.sum()
+        for of in (leaves[0], leaves[1], leaves[2], d):
+            with pytest.raises(RuntimeError, match="no gradients of its gradients"):
+                torch.autograd.grad(total, of, retain_graph=True)
+        with pytest.raises(RuntimeError, match="no gradients of its gradients"):
+            total.backward(retain_graph=True)
+    # of the losses themselves there is one
+    assert torch.isfinite(torch.autograd.grad(loss.sum() + leaves[0].square().sum(), leaves[0])[0]).all()

@@ -140,3 +140,40 @@ def test_what_classes_that_are_left_out_hold_is_nobodys_matter(cuda, dtype, d, w
             results.append([loss.detach(), *torch.autograd.grad(loss, leaves), fastgl.linear_cross_entropy(*(t.detach() for t in leaves[:2]), y, leaves[2].detach())])
         assert all(torch.isfinite(t).all() and torch.equal(t, u) for t, u in zip(*results))
         assert (results[1][2][out] == 0).all() and (results[1][3][out] == 0).all()
+
+
+@pytest.mark.parametrize("n,v,d", [(12_900, 230, 340), (230, 12_900, 500), (20_000, 3000, 400), (3000, 20_000, 330), (1, 1, 321), (65, 33, 512), (70_000, 40, 450), (33, 100_000, 350)])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_many_columns_in_whole_and_in_cut_groups(cuda, n, v, d, reduction):
+    """Two waves share their rows from 321 columns on: groups that a workgroup has alone, that several share, and that are cut anywhere."""
+    print("linear_cross_entropy %d x %d, %d classes" % (n, d, v), flush=True)
+    check(*problem(cuda, n, v, d), reduction=reduction)
+
+
+@pytest.mark.parametrize("d", [330, 500])
+def test_many_columns_captured_and_replayed(cuda, d):
+    x, w, b, y = problem(cuda, 900, 700, d)
+    y[::5] = -100
+    held, one = [x.clone(), w.clone(), b.clone()], torch.ones((), device=cuda)
+
+    def step():
+        leaves = [t.detach().requires_grad_() for t in held]
+        loss = fastgl.linear_cross_entropy(leaves[0], leaves[1], y, leaves[2])
+        return loss.detach(), *torch.autograd.grad(loss, leaves, one)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for k in range(4):
+        for t, u in zip(held, (x, w, b)):
+            t.copy_(u * (1 + k / 2))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
