@@ -13,6 +13,7 @@ from . import ops
 
 _TAG = 0x44524F50  # the counter's last word: "DROP"
 
+
 def _drawn_seed():
     """A seed from torch's generator (of the CPU: ``torch.manual_seed`` governs it)."""
     with _disable_current_modes():  # (a number, also where tensors hold none)
