@@ -4,48 +4,11 @@
 // A training step calls them once a layer, on rows that take the GPU tens of microseconds; recorded by a Python function, forward and
 // backward cost 90 us (dropout) and 130 us (the loss) of the host's time, here 46 and 73, on a host where torch's relu takes 42 (27, 45 and 24 on
 // a faster one).
-#include "fastgl_autograd.h"
-
-#include <ATen/autocast_mode.h>
-#include <c10/hip/HIPGuard.h>
-#include <c10/hip/HIPStream.h>
-#include <torch/csrc/autograd/functions/basic_ops.h>
-#include <torch/csrc/autograd/functions/utils.h>
-
-#include <string>
-#include <tuple>
-
-#include "fastgl_hip.h"
+#include "fastgl_recorded.hpp"
 
 namespace {
 
-using torch::Tensor;
-using torch::autograd::AutogradContext;
-using torch::autograd::variable_list;
-using Maybe = c10::optional<Tensor>;
-
-void ok(int rc) { TORCH_CHECK(rc == FGL_OK, "fastgl: ", fgl_last_error(), " (error ", rc, ")"); }
-
-void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
-
-int type_of(const Tensor& t) { return t.scalar_type() == torch::kFloat32 ? FGL_F32 : FGL_BF16; }
-
-bool is_feature(const Tensor& t) { return t.scalar_type() == torch::kFloat32 || t.scalar_type() == torch::kBFloat16; }
-
-// Scratch of the call's own, from torch's allocator (in stream order, also under capture)
-Tensor bytes_like(const Tensor& t, size_t n)
-{
-    return torch::empty({(int64_t)(n < 256 ? 256 : n)}, t.options().dtype(torch::kUInt8).requires_grad(false));
-}
-
-void* address(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
-
-// Whether t only looks like a tensor of its sizes and has no memory of its own: a gradient that torch.autograd.grad(is_grads_batched=True) and
-// jacobian(vectorize=True) hand to a backward pass, many at once
-bool is_wrapped(const Tensor& t)
-{
-    return t.key_set().has_any(c10::DispatchKeySet({c10::DispatchKey::Batched, c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper}));
-}
+using namespace fastgl;
 
 // ---- dropout -------------------------------------------------------------------------------------------------------
 bool gaps_in_rows_only(const Tensor& x) { return x.is_contiguous() || (x.dim() == 2 && x.stride(1) == 1 && x.stride(0) >= x.size(1)); }
@@ -228,26 +191,8 @@ struct LossNode : torch::autograd::Function<LossNode> {
         } else {
             std::tie(d_x, d_w, d_b) = form(loss_gradients);
         }
-        if (torch::GradMode::is_enabled()) {
-            // A graph of the gradients is being built, and they have none: who asks for them is told so.  By a node that leads on to what they would be of, so
-            // that it is met also where only some tensor's gradients are asked for.
-            torch::autograd::edge_list of;
-            for (const auto& edge : torch::autograd::get_current_node()->next_edges())
-                if (edge.is_valid()) of.push_back(edge);
-            const bool wrapped = is_wrapped(grads[0]);
-            if (!wrapped && grads[0].requires_grad()) of.push_back(torch::autograd::impl::gradient_edge(grads[0]));
-            const auto node = std::make_shared<torch::autograd::Error>("linear_cross_entropy has no gradients of its gradients", std::move(of));
-            Tensor zero;  // wrapped tensors get no node: one is added that has it
-            if (wrapped) {
-                zero = torch::full({}, -0.0, state.options().dtype(ctx->saved_data["type"].toScalarType()));
-                torch::autograd::set_history(zero, node);
-            }
-            for (Tensor* t : {&d_x, &d_w, &d_b}) {
-                if (!t->defined()) continue;
-                if (wrapped) *t = *t + zero;
-                else torch::autograd::set_history(*t, node);
-            }
-        }
+        refuse_gradients_of({&d_x, &d_w, &d_b}, grads[0], state.options().dtype(ctx->saved_data["type"].toScalarType()),
+                            "linear_cross_entropy has no gradients of its gradients");
         out[0] = d_x;
         out[1] = d_w;
         out[2] = d_b;

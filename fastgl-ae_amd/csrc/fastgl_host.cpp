@@ -130,4 +130,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
     m.def("sample_blocks", &sample_blocks);
     m.def("trim", &trim);
     bind_recorded_operators(m);
+    bind_layers(m);
 }

@@ -1,0 +1,66 @@
+"""What stands between the aggregations of a deep model: the norm of its rows, forward and backward in one pass over them each, with the
+activation behind it in the same pass, and with 8 bits a value kept for the backward pass where memory is what limits a batch.
+"""
+from __future__ import annotations
+
+import torch
+from torch import nn
+from torch.nn import functional as F
+
+from . import _lib as L
+from . import ops
+
+
+def _norm_by_operators(x, weight, bias, eps, relu):
+    """The same in torch's operators, for who has to see those; what the backward pass needs is kept in full."""
+    if torch.is_autocast_enabled():
+        x, weight, bias = (None if t is None else t.float() for t in (x, weight, bias))
+    if x.dtype not in ops._FEAT or x.dim() < 1 or not (torch.jit.is_tracing() or 1 <= x.size(-1) <= L.NORM_MAX_DIM):
+        raise RuntimeError("x must have dtype in %s and rows of 1 to %d columns" % ([str(t) for t in ops._FEAT], L.NORM_MAX_DIM))
+    if any(t is not None and (t.dim() != 1 or t.dtype != x.dtype or not (torch.jit.is_tracing() or t.size(0) == x.size(-1))) for t in (weight, bias)):
+        raise RuntimeError("weight and bias must hold a value of x's type for each column")
+    if not eps >= 0.0:
+        raise RuntimeError("eps (%g) must not be negative" % eps)
+    with torch.autocast("cuda", enabled=False):
+        h = x.double()
+        h = h - h.mean(-1, keepdim=True)
+        h = h * torch.rsqrt(h.square().mean(-1, keepdim=True) + eps)
+        y = h if weight is None else h * weight.double()
+        y = y if bias is None else y + bias.double()
+        return (torch.where(y <= 0, 0.0, y) if relu else y).to(x.dtype)
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5, relu=False, keep8=False):
+    """``(x - mean) / sqrt(var + eps) * weight + bias`` over the last dimension (at most 2048 columns), ``relu``: ``max(.., 0)`` of it, with gradients
+    for all three.  ``x``: float32 or bfloat16 on the GPU, any leading dimensions; rows that lie apart are taken as they are, other orders copied.
+    ``weight``, ``bias``: of x's type, or ``None`` for ones and zeros.  Mean, variance and the normed values are formed in 64 bits, so that rows far from
+    zero keep what they differ in.
+    For the backward pass ``x`` is kept with 12 bytes a row, and with ``relu`` a bit a value.  ``keep8=True``: in ``x``'s place the normed values, 8 bits each: 32
+    neighbouring columns share a step, ``2**(floor(log2(largest magnitude)) - 6)``, and the nearest of -127 .. 127 steps is held; gradients are those of
+    the values so held (32 columns with one that is not finite are held as not a number).
+    Under autocast in float32, as torch's.  No gradients of gradients.  Under tracing, forward-mode differentiation, transforms of
+    ``torch.func`` and modes that follow the operators: by torch's operators, with nothing kept in 8 bits."""
+    if not all(t is None or (isinstance(t, torch.Tensor) and t.is_cuda) for t in (weight, bias)) or not (isinstance(x, torch.Tensor) and x.is_cuda):
+        raise RuntimeError("x, weight and bias must be CUDA tensors")
+    if ops._unseen(x, weight, bias):
+        return _norm_by_operators(x, weight, bias, eps, relu)
+    return L.host().layer_norm(x, weight, bias, eps, bool(relu), bool(keep8), L.NORM_MAX_DIM)
+
+
+class LayerNorm(nn.LayerNorm):
+    """``nn.LayerNorm`` over the last dimension whose ``forward`` is ``layer_norm``; a state of either is one of the other's.  ``relu``: the activation
+    behind it goes with it (``forward(x, relu)``: in its place, if given).  ``keep8``: 8 bits a value are kept for the backward pass."""
+
+    def __init__(self, features, eps=1e-5, elementwise_affine=True, bias=True, relu=False, keep8=False):
+        super().__init__(features, eps=eps, elementwise_affine=elementwise_affine, bias=bias)
+        if len(self.normalized_shape) != 1:
+            raise ValueError("the norm is over one dimension, not %s" % (self.normalized_shape,))
+        self.relu, self.keep8 = bool(relu), bool(keep8)
+
+    def forward(self, x, relu=None):
+        if isinstance(x, torch.Tensor) and x.dim() > 0 and x.size(-1) != self.normalized_shape[0]:
+            raise RuntimeError("x has rows of %d columns, not of %d" % (x.size(-1), self.normalized_shape[0]))
+        return layer_norm(x, self.weight, self.bias, self.eps, self.relu if relu is None else relu, self.keep8)
+
+    def extra_repr(self):
+        return super().extra_repr() + (", relu=True" if self.relu else "") + (", keep8=True" if self.keep8 else "")

@@ -473,6 +473,26 @@ int fgl_dropout(const void* d_x, int64_t ldx, int64_t n_rows, int64_t n_cols, in
 int fgl_dropout_relu_backward(const void* d_dout, const void* d_out, int64_t n, int dtype, double p, void* d_dx, void* stream);
 
 /* ---------------------------------------------------------------------------------
+ * Norm of rows and its gradients (no counterpart in the reference; what nn.LayerNorm is to its nn.Dropout).  For each of n rows of
+ * d columns of x (row stride ldx), 1 <= d <= 2048:
+ *   h = (x - mean) / sqrt(var + eps) (var: of the row, divided by d),   y = h w + b,   relu not zero: y <= 0 ? 0 : y
+ * w, b: d values of `dtype`, or NULL for ones and zeros.  y: [n, d] without gaps.  Mean, variance and h are formed in 64 bits.
+ * d_state: what the backward pass needs, fgl_layer_norm_state_bytes, at a multiple of 256 bytes; NULL if there will be none.  keep8 not zero: h is
+ * kept in 8 bits a value (32 neighbouring columns share a step 2^(max(floor(log2(largest magnitude)), -120) - 6); the nearest of -127 .. 127 steps; if
+ * one is infinite or not a number, none of them is a number), and the backward pass does without x.
+ * Backward: g = dy [y > 0] w, dx = (g - mean(g) - h mean(g h)) / sqrt(var + eps), dw and db the sums over rows of dy [y > 0] h and dy [y > 0], in a
+ * fixed order; [y > 0] only with relu, h the one that is kept.  dx: [n, d] without gaps; dx, dw, db: each may be NULL.  Workspace at a multiple
+ * of 256 bytes, NULL if neither dw nor db is asked for.  The state may be read by several backward passes.
+ * ------------------------------------------------------------------------------- */
+size_t fgl_layer_norm_state_bytes(int64_t n, int d, int relu, int keep8);
+size_t fgl_layer_norm_workspace_bytes(int64_t n, int d, int dtype);
+int fgl_layer_norm(const void* d_x, int64_t ldx, const void* d_w, const void* d_b, int64_t n, int d, int dtype, double eps, int relu, int keep8,
+                   void* d_y, void* d_state, size_t state_bytes, void* stream);
+int fgl_layer_norm_backward(const void* d_dy, int64_t lddy, const void* d_x, int64_t ldx, const void* d_w, int64_t n, int d, int dtype, int relu,
+                            int keep8, const void* d_state, size_t state_bytes, void* d_dx, void* d_dw, void* d_db, void* d_ws, size_t ws_bytes,
+                            void* stream);
+
+/* ---------------------------------------------------------------------------------
  * A model's last product and its loss as one operator, without the logits ever lying in memory: softmax cross entropy of
  * x W^T + b (replaces the last layer's product followed by nn.CrossEntropyLoss, train_fastgl.py:328,383).
  *   s_iv = sum_d x[i, d] w[v, d] + b[v],   loss_i = log(sum_v exp(s_iv)) - s_i,label(i)
