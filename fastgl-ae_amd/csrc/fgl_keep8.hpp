@@ -41,6 +41,18 @@ __device__ __forceinline__ uint32_t group_max(uint32_t v)
     return v;
 }
 
+// The same lanes' bits (8 or 16 lanes), together
+template <int GROUP>
+__device__ __forceinline__ uint32_t group_or(uint32_t v)
+{
+    static_assert(GROUP == 8 || GROUP == 16, "");
+    v |= dpp_u32<kDppXor1>(v);
+    v |= dpp_u32<kDppXor2>(v);
+    v |= dpp_u32<kDppHalfMirror>(v);
+    if constexpr (GROUP == 16) v |= dpp_u32<kDppMirror>(v);
+    return v;
+}
+
 // the exponent that stands for the step, from floor(log2) of the largest magnitude
 __device__ __forceinline__ uint32_t k8_step(int log2_most) { return (uint32_t)((log2_most < -120 ? -120 : log2_most) + 121); }
 constexpr uint32_t kStepNone = 255;

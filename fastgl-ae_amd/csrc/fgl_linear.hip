@@ -1,0 +1,298 @@
+// A dense layer with what follows it, and its gradients:
+//   z = x W^T + b,   y = act(z) + residual;   dz = dy act'(z),   dx = dz W,   dW = dz^T x,   db = sum over rows of dz
+//
+// The products are fgl_row_product.hip's (fp32 on the bf16 matrix cores: fgl_split_product.hip) and fgl_wgrad.hip's; the forward one stores act(z) + residual
+// from its accumulators, and what act' will be formed from: a bit a value for relu, z itself for gelu and silu.  The backward pass forms dz in one pass over dy
+// (none where there is no activation: dz is dy).
+//
+// KEEP8: the rows of x are held in 8 bits a value (fgl_keep8.hpp) for dW, which fgl_wgrad8.hip forms from them; dx and db need no x.
+#include "fgl_activation.hpp"
+#include "fgl_common.hpp"
+#include "fgl_keep8.hpp"
+#include "fgl_kernels.hpp"
+#include "fgl_row_product.hpp"
+#include "fgl_wgrad8.hpp"
+
+namespace fgl {
+
+constexpr int kLinearMost = 4096;  // columns of x and y
+constexpr int kPackRows = 64;      // of a workgroup
+
+struct LinearState {
+    uint8_t* codes;  // KEEP8: [n][k8_columns(dim)]
+    uint8_t* steps;  // KEEP8: [k8_columns(dim) / 32][w8_step_ld(n)]
+    uint32_t* mask;  // relu: [n][mask_ld]
+    void* z;         // gelu, silu: [n][ldz] of x's type
+    int64_t mask_ld, ldz;
+    size_t bytes;
+};
+
+static LinearState linear_state(void* base, int64_t n, int dim, int out, int dtype, int act, bool keep8)
+{
+    Carver c(base);
+    LinearState s;
+    memset(&s, 0, sizeof(s));
+    s.mask_ld = (out + 31) / 32;
+    s.ldz = (out + 1) / 2 * 2;
+    if (keep8) {
+        s.codes = c.take<uint8_t>((size_t)n * (size_t)k8_columns(dim));
+        s.steps = c.take<uint8_t>((size_t)(k8_columns(dim) / 32) * (size_t)w8_step_ld(n));
+    }
+    if (act == kActRelu) s.mask = c.take<uint32_t>((size_t)n * (size_t)s.mask_ld);
+    else if (act != kActNone) s.z = c.take<uint8_t>((size_t)n * (size_t)s.ldz * (dtype == FGL_F32 ? 4 : 2));
+    s.bytes = c.used();
+    return s;
+}
+
+template <typename T>
+constexpr int kLinV = 16 / (int)sizeof(T);
+template <typename T>
+using LinVec = T __attribute__((ext_vector_type(kLinV<T>), aligned(sizeof(T))));
+
+template <typename T>
+__device__ __forceinline__ LinVec<T> lin_load(const T* p, int left)
+{
+    LinVec<T> v;
+    if (left >= kLinV<T>) {
+        v = *reinterpret_cast<const LinVec<T>*>(p);
+    } else {
+#pragma unroll
+        for (int e = 0; e < kLinV<T>; ++e) {
+            v[e] = (T)0.0f;
+            if (e < left) v[e] = p[e];
+        }
+    }
+    return v;
+}
+
+// Rows in 8 bits a value.  A workgroup takes 64 rows, a lane 16 bytes of one at a time, so that 32 columns are those of 8 lanes (bf16: 4); steps are
+// gathered in LDS, since those of a column of rows are neighbours.
+template <typename T>
+__global__ __launch_bounds__(kBlock) void pack8_kernel(const T* __restrict__ x, int64_t ldx, int64_t n, int d, int code_ld, uint8_t* __restrict__ codes,
+                                                      uint8_t* __restrict__ steps, int64_t step_ld)
+{
+    constexpr int V = kLinV<T>, kGroup = 32 / V;
+    __shared__ uint8_t s_step[kLinearMost / 32][kPackRows];
+    typedef uint32_t Codes __attribute__((ext_vector_type(V / 4)));
+    const int64_t row0 = (int64_t)blockIdx.x * kPackRows;
+    const int per_row = code_ld / V, rows = n - row0 < kPackRows ? (int)(n - row0) : kPackRows;
+    const int items = rows * per_row;
+    for (int i0 = 0; i0 < items; i0 += kBlock) {  // (the lanes of a group are all in or all out)
+        const int i = i0 + (int)threadIdx.x, r = i / per_row, c = (i - r * per_row) * V;
+        const bool in = i < items;
+        LinVec<T> v = lin_load(x + (row0 + r) * ldx + c, in ? d - c : 0);
+        uint32_t most = 0;
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const uint32_t m = __float_as_uint((float)v[e]) & 0x7FFFFFFFu;
+            most = most > m ? most : m;
+        }
+        most = group_max<kGroup>(most) >> 23;
+        const uint32_t step = most == 0xFF ? kStepNone : k8_step((int)most - 127);
+        const float inverse = step == kStepNone ? 0.0f : k8_inverse(step);
+        Codes q;
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const uint32_t code = k8_code((float)v[e] * inverse);
+            if (e % 4 == 0) q[e / 4] = code;
+            else q[e / 4] |= code << 8 * (e % 4);
+        }
+        if (in) {
+            *reinterpret_cast<Codes*>(codes + (row0 + r) * code_ld + c) = q;
+            if (c % 32 == 0) s_step[c / 32][r] = (uint8_t)step;
+        }
+    }
+    __syncthreads();
+    const int columns = code_ld / 32;
+    for (int i = (int)threadIdx.x; i < columns * kPackRows; i += kBlock) {
+        const int c = i / kPackRows, r = i % kPackRows;
+        if (r < rows) steps[c * step_ld + row0 + r] = s_step[c][r];
+    }
+}
+
+// dz = dy act'(z); rows of z and dz are ldz apart, those of dy lddy.  Lanes: 2^log_lanes neighbours take the loads of a row.
+template <typename T, bool MASK>
+__global__ __launch_bounds__(kBlock) void slope_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restrict__ z, const uint32_t* __restrict__ mask, int64_t mask_ld,
+                                                      int act, int64_t n, int d, int64_t ldz, T* __restrict__ dz, int log_lanes)
+{
+    constexpr int V = kLinV<T>;
+    const int l = (int)threadIdx.x & ((1 << log_lanes) - 1);
+    const int64_t stride = (int64_t)gridDim.x << (8 - log_lanes);
+    for (int64_t row = ((int64_t)blockIdx.x << (8 - log_lanes)) + (threadIdx.x >> log_lanes); row < n; row += stride) {
+        for (int c = l * V; c < d; c += V << log_lanes) {
+            const int left = d - c;
+            LinVec<T> g = lin_load(dy + row * lddy + c, left), q;
+            if constexpr (MASK) {
+                const uint32_t bits = mask[row * mask_ld + c / 32] >> (c % 32);
+#pragma unroll
+                for (int e = 0; e < V; ++e) q[e] = bits >> e & 1u ? g[e] : (T)0.0f;
+            } else {
+                const LinVec<T> at = lin_load(z + row * ldz + c, left);
+#pragma unroll
+                for (int e = 0; e < V; ++e) q[e] = (T)((float)g[e] * act_slope(act, (float)at[e]));
+            }
+            T* to = dz + row * ldz + c;
+            if (left >= V) {
+                *reinterpret_cast<LinVec<T>*>(to) = q;
+            } else {
+#pragma unroll
+                for (int e = 0; e < V; ++e)
+                    if (e < left) to[e] = q[e];
+            }
+        }
+    }
+}
+
+template <typename T>
+static void launch_slope(const void* dy, int64_t lddy, const LinearState& s, int act, int64_t n, int d, void* dz, hipStream_t stream)
+{
+    int log_lanes = 0;
+    while (log_lanes < 6 && (kLinV<T> << log_lanes) < d) ++log_lanes;
+    const int64_t want = ceil_div(n, 1 << (8 - log_lanes)), blocks = want < 8192 ? want : 8192;
+    if (act == kActRelu)
+        hipLaunchKernelGGL((slope_kernel<T, true>), dim3((unsigned)blocks), dim3(kBlock), 0, stream, static_cast<const T*>(dy), lddy, (const T*)nullptr, s.mask, s.mask_ld, act,
+                           n, d, s.ldz, static_cast<T*>(dz), log_lanes);
+    else
+        hipLaunchKernelGGL((slope_kernel<T, false>), dim3((unsigned)blocks), dim3(kBlock), 0, stream, static_cast<const T*>(dy), lddy, static_cast<const T*>(s.z),
+                           (const uint32_t*)nullptr, (int64_t)0, act, n, d, s.ldz, static_cast<T*>(dz), log_lanes);
+}
+
+// What the backward pass carves from its workspace: dz (where there is an activation), a weight gradient that nobody asked for, the weight gradient's sums
+struct LinearWorkspace {
+    void* dz;
+    void* dw;
+    void* sums;
+    size_t sums_bytes, bytes;
+};
+static LinearWorkspace linear_workspace(void* base, int64_t n, int dim, int out, int dtype, int act, bool keep8, bool need_w, bool need_b)
+{
+    Carver c(base);
+    LinearWorkspace w;
+    memset(&w, 0, sizeof(w));
+    const size_t size = dtype == FGL_F32 ? 4 : 2;
+    if (act != kActNone) w.dz = c.take<uint8_t>((size_t)n * (size_t)((out + 1) / 2 * 2) * size);
+    if (need_b && !need_w) w.dw = c.take<uint8_t>((size_t)dim * (size_t)out * size);
+    if (need_w || need_b) {
+        w.sums_bytes = keep8 ? wgrad8_workspace_bytes(n, out, dim, dtype) : fgl_weight_grad_workspace_bytes_for(n, out, dim, dtype);
+        w.sums = c.take<uint8_t>(w.sums_bytes);
+    }
+    w.bytes = c.used();
+    return w;
+}
+
+static bool linear_sizes(int64_t n, int dim, int out, int dtype, int act)
+{
+    return n >= 0 && n <= 0x7FFFFFFF && dim >= 1 && dim <= kLinearMost && out >= 1 && out <= kLinearMost && (dtype == FGL_F32 || dtype == FGL_BF16) && act >= kActNone &&
+           act <= kActSilu;
+}
+
+#define FGL_LINEAR_ROWS(p_, ld_, cols_)                                                                                                                  \
+    FGL_REQUIRE((ld_) >= (cols_) && (ld_) < (1 << 24), "linear: row stride %lld of %d columns", (long long)(ld_), (int)(cols_));                         \
+    FGL_REQUIRE(dtype == FGL_F32 || ((ld_) % 2 == 0 && (uintptr_t)(p_) % 4 == 0), "linear: bf16 rows must start on 4-byte boundaries")
+
+}  // namespace fgl
+
+using namespace fgl;
+
+FGL_EXPORT size_t fgl_linear_state_bytes(int64_t n, int dim, int out, int dtype, int act, int keep8)
+{
+    return linear_sizes(n, dim, out, dtype, act) ? linear_state(nullptr, n, dim, out, dtype, act, keep8 != 0).bytes : 0;
+}
+
+FGL_EXPORT size_t fgl_linear_workspace_bytes(int64_t n, int dim, int out, int dtype, int act, int keep8, int want_w, int want_b)
+{
+    return linear_sizes(n, dim, out, dtype, act) ? linear_workspace(nullptr, n, dim, out, dtype, act, keep8 != 0, want_w != 0, want_b != 0).bytes : 0;
+}
+
+FGL_EXPORT int fgl_linear(const void* d_x, int64_t ldx, const void* d_w, int64_t ldw, const void* d_bias, const void* d_residual, int64_t ldr, int64_t n, int dim, int out,
+                          int dtype, int act, int keep8, void* d_y, int64_t ldy, void* d_state, size_t state_bytes, void* stream)
+{
+    FGL_REQUIRE(linear_sizes(n, dim, out, dtype, act), "linear: %lld rows of %d by %d columns, dtype %d, activation %d", (long long)n, dim, out, dtype, act);
+    FGL_LINEAR_ROWS(d_x, ldx, dim);
+    FGL_LINEAR_ROWS(d_w, ldw, dim);
+    FGL_REQUIRE(ldy >= out && (d_residual == nullptr || ldr >= out), "linear: row stride smaller than the row length");
+    if (n == 0) return FGL_OK;
+    FGL_REQUIRE(d_x && d_w && d_y, "linear: null pointer");
+    RowProductArgs g;
+    memset(&g, 0, sizeof(g));
+    g.side[0] = RowProductSide{d_x, d_w, ldx, ldw, dim};
+    g.bias = d_bias; g.c = d_y; g.ldc = ldy; g.m = n; g.n = out;
+    g.then.act = act; g.then.residual = d_residual; g.then.ldr = d_residual != nullptr ? ldr : 0;
+    hipStream_t s = as_stream(stream);
+    if (d_state != nullptr) {
+        const LinearState kept = linear_state(d_state, n, dim, out, dtype, act, keep8 != 0);
+        if (state_bytes < kept.bytes || ((uintptr_t)d_state & 255) != 0) {
+            set_error("linear: state of %zu bytes at a multiple of 256 bytes, %zu given", kept.bytes, state_bytes);
+            return FGL_ERR_WORKSPACE;
+        }
+        if (act == kActRelu) {
+            g.then.mask = kept.mask;
+            g.then.mask_ld = kept.mask_ld;
+        } else if (act != kActNone) {
+            g.then.z = kept.z;
+            g.then.ldz = kept.ldz;
+        }
+        if (keep8) {
+            const dim3 grid((unsigned)ceil_div(n, kPackRows));
+            if (dtype == FGL_F32)
+                hipLaunchKernelGGL(pack8_kernel<float>, grid, dim3(kBlock), 0, s, static_cast<const float*>(d_x), ldx, n, dim, (int)k8_columns(dim), kept.codes, kept.steps,
+                                   w8_step_ld(n));
+            else
+                hipLaunchKernelGGL(pack8_kernel<__bf16>, grid, dim3(kBlock), 0, s, static_cast<const __bf16*>(d_x), ldx, n, dim, (int)k8_columns(dim), kept.codes, kept.steps,
+                                   w8_step_ld(n));
+            FGL_CHECK_LAUNCH("pack8_kernel");
+        }
+    }
+    return row_product_then(g, dtype, s);
+}
+
+FGL_EXPORT int fgl_linear_backward(const void* d_dy, int64_t lddy, const void* d_x, int64_t ldx, const void* d_w, int64_t ldw, int64_t n, int dim, int out, int dtype,
+                                   int act, int keep8, const void* d_state, size_t state_bytes, void* d_dx, int64_t lddx, void* d_dw, void* d_db, void* d_ws, size_t ws_bytes,
+                                   void* stream)
+{
+    FGL_REQUIRE(linear_sizes(n, dim, out, dtype, act) && n >= 1, "linear_backward: %lld rows of %d by %d columns, dtype %d, activation %d", (long long)n, dim, out, dtype, act);
+    const bool sums = d_dw != nullptr || d_db != nullptr;
+    if (d_dx == nullptr && !sums) return FGL_OK;
+    FGL_REQUIRE(d_dy != nullptr && (d_dx == nullptr || d_w != nullptr) && (!sums || keep8 || d_x != nullptr), "linear_backward: null pointer");
+    if (act == kActNone) {  // (dy is an operand itself then)
+        FGL_LINEAR_ROWS(d_dy, lddy, out);
+    } else {
+        FGL_REQUIRE(lddy >= out, "linear_backward: row stride smaller than the row length");
+    }
+    FGL_REQUIRE(d_dx == nullptr || (ldw >= dim && lddx >= dim), "linear_backward: row stride smaller than the row length");
+    if (sums && !keep8) {
+        FGL_LINEAR_ROWS(d_x, ldx, dim);
+    }
+    LinearState kept;
+    memset(&kept, 0, sizeof(kept));
+    if (keep8 || act != kActNone) {
+        kept = linear_state(const_cast<void*>(d_state), n, dim, out, dtype, act, keep8 != 0);
+        if (d_state == nullptr || state_bytes < kept.bytes || ((uintptr_t)d_state & 255) != 0) {
+            set_error("linear_backward: state of %zu bytes at a multiple of 256 bytes, %zu given", kept.bytes, state_bytes);
+            return FGL_ERR_WORKSPACE;
+        }
+    }
+    const LinearWorkspace w = linear_workspace(d_ws, n, dim, out, dtype, act, keep8 != 0, d_dw != nullptr, d_db != nullptr);
+    if (w.bytes > 0 && (d_ws == nullptr || ws_bytes < w.bytes || ((uintptr_t)d_ws & 255) != 0)) {
+        set_error("linear_backward: workspace of %zu bytes at a multiple of 256 bytes, %zu given", w.bytes, ws_bytes);
+        return FGL_ERR_WORKSPACE;
+    }
+    hipStream_t s = as_stream(stream);
+    const void* dz = d_dy;
+    int64_t lddz = lddy;
+    if (act != kActNone) {
+        if (dtype == FGL_F32) launch_slope<float>(d_dy, lddy, kept, act, n, out, w.dz, s);
+        else launch_slope<__bf16>(d_dy, lddy, kept, act, n, out, w.dz, s);
+        FGL_CHECK_LAUNCH("slope_kernel");
+        dz = w.dz;
+        lddz = kept.ldz;
+    }
+    if (d_dx != nullptr) {
+        const int rc = fgl_row_product(dz, lddz, d_w, ldw, 0, n, out, dim, dtype, nullptr, d_dx, lddx, stream);
+        if (rc != FGL_OK) return rc;
+    }
+    if (!sums) return FGL_OK;
+    void* dw = d_dw != nullptr ? d_dw : w.dw;
+    if (keep8) return launch_wgrad8(dz, lddz, kept.codes, kept.steps, w8_step_ld(n), n, out, dim, dtype, dw, dim, d_db, w.sums, w.sums_bytes, s);
+    return fgl_weight_grad(dz, lddz, d_x, ldx, n, out, dim, dtype, dw, dim, d_db, w.sums, w.sums_bytes, stream);
+}

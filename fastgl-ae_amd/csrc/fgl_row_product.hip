@@ -218,6 +218,7 @@ __global__ __launch_bounds__(kBlock, VA * VB >= 4 ? 2 : 4) void row_product_kern
 
     int col = (tn * 32 + lane % 32) * VB;
     const bool past_end = FORM == kRpAdd && col >= g.n;  // (adds nothing: the columns that it repeats are another lane's)
+    const int own_col = col;
     if (col + VB > g.n) col = g.n - VB;
     RpF32x16 acc[VA * VB];
 #pragma unroll
@@ -264,12 +265,17 @@ __global__ __launch_bounds__(kBlock, VA * VB >= 4 ? 2 : 4) void row_product_kern
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 float s = acc[i * VB + t][r] + add[t];
-                if constexpr (FORM != kRpOne && sizeof(T) == 2) s = __uint_as_float(rp_bf16_bits(s) << 16);
+                if constexpr (FORM != kRpOne && FORM != kRpThen && sizeof(T) == 2) s = __uint_as_float(rp_bf16_bits(s) << 16);
                 if constexpr (kKeep) s += __uint_as_float(r & 1 ? kept[i * VB + t][r / 2] & 0xFFFF0000u : kept[i * VB + t][r / 2] << 16);
                 asm volatile("" : "+v"(s));
                 acc[i * VB + t][r] = s;
             }
 
+    if constexpr (FORM == kRpThen) {
+#pragma unroll
+        for (int i = 0; i < VA; ++i) rp_then<T, VB>(g, row0 + 32 * i + 4 * half, own_col, [&](int t, int r) { return acc[i * VB + t][r]; });
+        return;
+    }
     // accumulator register r of lane l: row 8 (r / 4) + 4 (l / 32) + r % 4, column l % 32 of its 32x32 tile
 #pragma unroll
     for (int i = 0; i < VA; ++i)
@@ -310,7 +316,7 @@ static int launch_row_product_any(const RowProductArgs& g, bool vectors, hipStre
     for (int v = 2; v <= 4 && vectors; v *= 2) {
         const int64_t p = ceil_div(g.n, 32 * v) * 32 * v;
         const int64_t waves = ceil_div(g.m, 32) * (p / (32 * v));
-        if (g.n >= v && p * 10 <= pad1 * 12 && waves >= 1024 && (FORM != kRpAdd || g.n % v == 0)) vb = v;
+        if (g.n >= v && p * 10 <= pad1 * 12 && waves >= 1024 && ((FORM != kRpAdd && FORM != kRpThen) || g.n % v == 0)) vb = v;
     }
     // A bf16 sum keeps the first product's values besides the accumulators: no tall tiles.  An fp32 one goes on in the same accumulators; it gains by
     // tall tiles where there is enough to multiply (us, tiles of 32 / 64 rows: 87 K rows of 2 x 256 x 256 276 / 242, 2 x 100 x 256 128 / 115, 200 K of 2 x 256 x 64
@@ -364,6 +370,19 @@ static int row_product(const RowProductSide& one, const RowProductSide& two, int
     if (split) return split_product(g, b_transposed != 0, FORM, s);
     if (dtype == FGL_F32) return b_transposed ? launch_row_product_any<float, true, FORM>(g, true, s) : launch_row_product_any<float, false, FORM>(g, true, s);
     return b_transposed ? launch_row_product_any<uint16_t, true, FORM>(g, vectors, s) : launch_row_product_any<uint16_t, false, FORM>(g, vectors, s);
+}
+
+int fgl::row_product_then(const RowProductArgs& given, int dtype, hipStream_t stream)
+{
+    RowProductArgs g = given;
+    const bool split = dtype == FGL_F32 && split_product_pays(g);
+    note_product(split ? "split_product_kernel" : "row_product_kernel");
+    if (split) return split_product(g, true, kRpThen, stream);
+    if (dtype == FGL_F32) return launch_row_product_any<float, true, kRpThen>(g, true, stream);
+    // bf16 moves in words: see row_product
+    const RowProductEpilogue& e = g.then;
+    const uint64_t starts = (uintptr_t)g.c | (uintptr_t)e.residual | (uintptr_t)e.z, strides = (uint64_t)g.n | (uint64_t)g.ldc | (uint64_t)e.ldr | (uint64_t)e.ldz;
+    return launch_row_product_any<uint16_t, true, kRpThen>(g, starts % 4 == 0 && strides % 2 == 0, stream);
 }
 
 FGL_EXPORT int fgl_row_product(const void* d_a, int64_t lda, const void* d_b, int64_t ldb, int b_transposed, int64_t m, int k, int n, int dtype,

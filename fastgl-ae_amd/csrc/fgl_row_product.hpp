@@ -1,6 +1,7 @@
 // What the kernels of a dense layer's product over rows share: operands, and how a lane's columns of a row are stored.
 #pragma once
 
+#include "fgl_activation.hpp"
 #include "fgl_common.hpp"
 
 namespace fgl {
@@ -11,6 +12,16 @@ struct RowProductSide {
     int64_t lda, ldb;
     int k;  // 0: no such pair
 };
+// What follows a product: C = act(A B + bias) + residual, and what act's derivative will be formed from, the sums themselves or a bit for each
+struct RowProductEpilogue {
+    int act;               // kActNone ..
+    const void* residual;  // (may be null) of C's sizes
+    int64_t ldr;
+    void* z;               // (may be null) A B + bias in C's type
+    int64_t ldz;
+    uint32_t* mask;        // (may be null) relu: bit c % 32 of word c / 32 of a row
+    int64_t mask_ld;       // words a row
+};
 struct RowProductArgs {
     RowProductSide side[2];  // C = A0 B0 + A1 B1
     const void* bias;
@@ -20,6 +31,7 @@ struct RowProductArgs {
     int tiles_n;          // tiles of C along n
     int64_t row_blocks;   // workgroups along m
     int vec_log;          // (split products) log2 of the neighbouring columns a lane stores
+    RowProductEpilogue then;  // (kRpThen)
 };
 
 __device__ __forceinline__ uint32_t rp_bf16_bits(float v) { return (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)v); }
@@ -66,10 +78,70 @@ __device__ __forceinline__ void rp_store(T* p, const float (&v)[VB])
 // FORM: one product (kRpOne), two of them and their sum (kRpSum: a layer's own rows with one weight and its gathered rows with another, in one
 // pass over C where the products and their sum were five), or a product added to what C holds (kRpAdd).  In bf16 a product is rounded to
 // bf16 before it is added to another or to C, as it would be if it were stored in between.
-constexpr int kRpOne = 0, kRpSum = 1, kRpAdd = 2;
+// kRpThen: one product and its epilogue.
+constexpr int kRpOne = 0, kRpSum = 1, kRpAdd = 2, kRpThen = 3;
+
+// The epilogue of 16 rows of a lane, of V neighbouring columns each from `col` on; accumulator register r of tile t is value(t, r), of row row0 +
+// 8 (r / 4) + r % 4.  V > 1 only where rows are a whole number of V, so that all or none of a lane's columns exist.  Every lane of the wave has to call it.
+template <typename T, int V, typename F>
+__device__ __forceinline__ void rp_then(const RowProductArgs& g, int64_t row0, int col, F&& value)
+{
+    constexpr int kBatch = V == 4 ? 4 : 8;  // rows whose residuals are on their way together
+    constexpr int kLanes = 32 / V;          // that share a word of the mask
+    const RowProductEpilogue& e = g.then;
+    const bool there = col < g.n;
+#pragma unroll
+    for (int r0 = 0; r0 < 16; r0 += kBatch) {
+        float v[kBatch][V], add[kBatch][V];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            const int64_t row = row0 + 8 * ((r0 + i) / 4) + (r0 + i) % 4;
+#pragma unroll
+            for (int t = 0; t < V; ++t) add[i][t] = 0.0f;
+            if (e.residual != nullptr && there && row < g.m) rp_add<T, V>(static_cast<const T*>(e.residual) + row * e.ldr + col, add[i]);
+#pragma unroll
+            for (int t = 0; t < V; ++t) v[i][t] = value(t, r0 + i);
+        }
+        if (e.z != nullptr) {
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+                const int64_t row = row0 + 8 * ((r0 + i) / 4) + (r0 + i) % 4;
+                if (there && row < g.m) rp_store<T, V>(static_cast<T*>(e.z) + row * e.ldz + col, v[i]);
+            }
+        }
+        if (e.mask != nullptr) {
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+                const int64_t row = row0 + 8 * ((r0 + i) / 4) + (r0 + i) % 4;
+                uint32_t word;
+                if constexpr (V == 1) {
+                    const unsigned long long b = __ballot(there && act_passes(v[i][0]));
+                    word = lane_id() < 32 ? (uint32_t)b : (uint32_t)(b >> 32);
+                } else {
+                    uint32_t bits = 0;
+#pragma unroll
+                    for (int t = 0; t < V; ++t) bits |= there && act_passes(v[i][t]) ? 1u << t : 0u;
+                    word = group_or<kLanes>(bits << (V * (lane_id() % kLanes)));
+                }
+                if (lane_id() % kLanes == 0 && there && row < g.m) e.mask[row * e.mask_ld + col / 32] = word;
+            }
+        }
+        act_apply<kBatch, V>(e.act, v);
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            const int64_t row = row0 + 8 * ((r0 + i) / 4) + (r0 + i) % 4;
+#pragma unroll
+            for (int t = 0; t < V; ++t) v[i][t] += add[i][t];
+            if (there && row < g.m) rp_store<T, V>(static_cast<T*>(g.c) + row * g.ldc + col, v[i]);
+        }
+    }
+}
 
 // fp32 products on the bf16 matrix cores: whether they pay for these sizes, and one of them
 bool split_product_pays(const RowProductArgs& g);
 int split_product(const RowProductArgs& g, bool b_transposed, int form, hipStream_t stream);
+
+// side[0]'s product with B transposed, and its epilogue; sizes, strides and pointers have been checked (bf16: rows of A and B start on words)
+int row_product_then(const RowProductArgs& g, int dtype, hipStream_t stream);
 
 }  // namespace fgl

@@ -320,6 +320,25 @@ __device__ __forceinline__ void sp_store_tile(const RowProductArgs& g, int64_t r
     }
 }
 
+// The same with what follows the product
+template <int NT, int V>
+__device__ __forceinline__ void sp_then(const RowProductArgs& g, int64_t row0, int col0, const SpF32x16 (&acc)[NT])
+{
+    int lane = lane_id();
+    asm volatile("" : "+v"(lane));
+#pragma unroll
+    for (int q = 0; q < NT / V; ++q) {
+        const int col = col0 + 32 * V * q + lane % 32 * V;
+        float add[V];
+#pragma unroll
+        for (int t = 0; t < V; ++t) {
+            add[t] = 0.0f;
+            if (g.bias != nullptr && col + t < g.n) add[t] = static_cast<const float*>(g.bias)[col + t];
+        }
+        rp_then<float, V>(g, row0 + 4 * (lane / 32), col, [&](int t, int r) { return acc[q * V + t][r] + add[t]; });
+    }
+}
+
 template <int NT, int W, bool BT, int FORM>
 __global__ __launch_bounds__(W * kWave, 2) void split_product_kernel(const RowProductArgs g)
 {
@@ -443,7 +462,11 @@ __global__ __launch_bounds__(W * kWave, 2) void split_product_kernel(const RowPr
             }
             w.template read_b<0>(s_img + lane);  // (what was read ahead: its registers are free above)
         }
-        if (NT >= 4 && g.vec_log == 2) sp_store_tile<NT, NT < 4 ? 1 : 4, FORM>(g, row0, col0, acc);
+        if constexpr (FORM == kRpThen) {
+            if (NT >= 4 && g.vec_log == 2) sp_then<NT, NT < 4 ? 1 : 4>(g, row0, col0, acc);
+            else if (NT >= 2 && g.vec_log == 1) sp_then<NT, NT < 2 ? 1 : 2>(g, row0, col0, acc);
+            else sp_then<NT, 1>(g, row0, col0, acc);
+        } else if (NT >= 4 && g.vec_log == 2) sp_store_tile<NT, NT < 4 ? 1 : 4, FORM>(g, row0, col0, acc);
         else if (NT >= 2 && g.vec_log == 1) sp_store_tile<NT, NT < 2 ? 1 : 2, FORM>(g, row0, col0, acc);
         else sp_store_tile<NT, 1, FORM>(g, row0, col0, acc);
         tile += stride;
@@ -487,7 +510,9 @@ static int launch_split_product(RowProductArgs g, hipStream_t stream)
     int64_t per_cu = kSpLds / (int64_t)lds;
     if (per_cu > 8 / W) per_cu = 8 / W;
     // as many neighbouring columns a lane as every row's start allows
-    const uint64_t starts = (uintptr_t)g.c | (uint64_t)g.ldc * sizeof(float);
+    uint64_t starts = (uintptr_t)g.c | (uint64_t)g.ldc * sizeof(float);
+    if (FORM == kRpThen)  // (and of what goes with them; rows are a whole number of them too)
+        starts |= (uintptr_t)g.then.residual | (uintptr_t)g.then.z | (uint64_t)(g.then.ldr | g.then.ldz | g.n) * sizeof(float);
     g.vec_log = NT >= 4 && starts % 16 == 0 ? 2 : NT >= 2 && starts % 8 == 0 ? 1 : 0;
     g.row_blocks = sp_row_blocks(ceil_div(g.m, 32), W, (int)per_cu, g.tiles_n);
     const int64_t blocks = ceil_div(g.row_blocks, 8) * 8 * g.tiles_n;
@@ -556,6 +581,7 @@ static int launch_split_product_any(const RowProductArgs& g, hipStream_t stream)
 int split_product(const RowProductArgs& g, bool b_transposed, int form, hipStream_t stream)
 {
     if (form == kRpSum) return b_transposed ? launch_split_product_any<true, kRpSum>(g, stream) : launch_split_product_any<false, kRpSum>(g, stream);
+    if (form == kRpThen) return launch_split_product_any<true, kRpThen>(g, stream);
     if (form == kRpAdd) return b_transposed ? launch_split_product_any<true, kRpAdd>(g, stream) : launch_split_product_any<false, kRpAdd>(g, stream);
     return b_transposed ? launch_split_product_any<true, kRpOne>(g, stream) : launch_split_product_any<false, kRpOne>(g, stream);
 }

@@ -22,7 +22,8 @@ ZERO_COPY_SELF, ZERO_ZEROS = 0, 1
 ABI_VERSION = 11  # FGL_ABI_VERSION of include/fastgl_hip.h that the signatures below follow
 REDUCE = {"none": 0, "sum": 1, "mean": 2}
 XENT_ROWS, XENT_WEIGHTS, XENT_MAX_DIM = 1, 2, 512
-NORM_MAX_DIM = 2048
+NORM_MAX_DIM, LINEAR_MAX_DIM = 2048, 4096
+ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "silu": 3}
 STATUS_TABLE_FULL, STATUS_UNIQ_OVERFLOW, STATUS_MISSING_KEY, STATUS_BAD_SEED, STATUS_BAD_ID = 1, 2, 4, 8, 16
 IDMAP_ORDERED, IDMAP_ARRIVAL, IDMAP_FINAL, IDMAP_LEAVE_TABLE_EMPTY = 0, 1, 2, 8
 BLOCKS_TABLE_EMPTY, BLOCKS_LEAVE_TABLE_EMPTY, BLOCKS_SORT_TRANSPOSED = 4, 8, 16
@@ -89,6 +90,10 @@ SIGNATURES = {
     "fgl_layer_norm_workspace_bytes": (_sz, [_i64, _i32, _i32]),
     "fgl_layer_norm": (_i32, [_vp, _i64, _vp, _vp, _i64, _i32, _i32, C.c_double, _i32, _i32, _vp, _vp, _sz, _vp]),
     "fgl_layer_norm_backward": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _i32, _i32, _i32, _i32, _vp, _sz, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "fgl_linear_state_bytes": (_sz, [_i64, _i32, _i32, _i32, _i32, _i32]),
+    "fgl_linear_workspace_bytes": (_sz, [_i64, _i32, _i32, _i32, _i32, _i32, _i32, _i32]),
+    "fgl_linear": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i32, _i32, _i32, _i32, _i32, _vp, _i64, _vp, _sz, _vp]),
+    "fgl_linear_backward": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _i32, _i32, _i32, _i32, _i32, _vp, _sz, _vp, _i64, _vp, _vp, _vp, _sz, _vp]),
     "fgl_rmat_keys": (_i32, [_i64, _i64, _i32, _i64, _u64, _vp, _vp]),
 }
 

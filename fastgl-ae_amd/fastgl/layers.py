@@ -1,5 +1,5 @@
-"""What stands between the aggregations of a deep model: the norm of its rows, forward and backward in one pass over them each, with the
-activation behind it in the same pass, and with 8 bits a value kept for the backward pass where memory is what limits a batch.
+"""What stands between the aggregations of a deep model: the norm of its rows and dense layers, each with what follows it in the same pass, and with
+8 bits a value of their inputs kept for the backward pass where memory is what limits a batch.
 """
 from __future__ import annotations
 
@@ -64,3 +64,59 @@ class LayerNorm(nn.LayerNorm):
 
     def extra_repr(self):
         return super().extra_repr() + (", relu=True" if self.relu else "") + (", keep8=True" if self.keep8 else "")
+
+
+def _linear_by_operators(x, weight, bias, activation, residual):
+    """The same in torch's operators, for who has to see those; what the backward pass needs is kept in full."""
+    if torch.is_autocast_enabled():
+        to = torch.get_autocast_dtype("cuda")
+        x, weight, bias, residual = (None if t is None else t.to(to) for t in (x, weight, bias, residual))
+    sized = not torch.jit.is_tracing()  # (a trace is of any sizes, and its operators have their own checks)
+    if x.dim() < 1 or weight.dim() != 2 or (sized and not (x.size(-1) == weight.size(1) and all(1 <= d <= L.LINEAR_MAX_DIM for d in weight.shape))):
+        raise RuntimeError("x %s and weight %s must be [.., d] and [out, d] with 1 <= d, out <= %d" % (tuple(x.shape), tuple(weight.shape), L.LINEAR_MAX_DIM))
+    if x.dtype not in ops._FEAT or any(t is not None and t.dtype != x.dtype for t in (weight, bias, residual)):
+        raise RuntimeError("x, weight, bias and residual must all be of one type in %s" % [str(t) for t in ops._FEAT])
+    if bias is not None and (bias.dim() != 1 or (sized and bias.size(0) != weight.size(0))):
+        raise RuntimeError("bias must hold a value for each row of weight")
+    if residual is not None and sized and tuple(residual.shape) != (*x.shape[:-1], weight.size(0)):
+        raise RuntimeError("residual must be of the output's sizes")
+    with torch.autocast("cuda", enabled=False):
+        z = F.linear(x.float(), weight.float(), None if bias is None else bias.float())
+        if activation is not None:
+            z = {"relu": torch.relu, "gelu": F.gelu, "silu": F.silu}[activation](z)
+        return (z if residual is None else z + residual.float()).to(x.dtype)
+
+
+def linear(x, weight, bias=None, activation=None, residual=None, keep8=False):
+    """``activation(x weight^T + bias) + residual`` for ``x`` [.., d] and ``weight`` [out, d], with gradients for all four.  Float32 or bfloat16 on the GPU, all of one
+    type, ``d`` and ``out`` up to 4096; rows that lie apart are taken as they are (bfloat16: where they start on four bytes), other orders copied.
+    ``activation``: ``None``, ``"relu"``, ``"gelu"`` (by the normal distribution function) or ``"silu"``; ``residual``: of the output's sizes.
+    Sums are float32, and the output is rounded once; in the backward pass the gradient behind the activation is rounded to the type once more.
+    For the backward pass ``x`` and ``weight`` are kept, and for ``"relu"`` a bit a value, for ``"gelu"`` and ``"silu"`` the values that they are taken of.  ``keep8=True``: in ``x``'s place
+    8 bits a value of it, as ``layer_norm`` holds them, if ``weight`` or ``bias`` has a gradient (nothing else reads ``x``): ``weight``'s is that of the values so held,
+    all others are not touched by it.
+    Under autocast, its type is taken.  No gradients of gradients.  Under tracing, forward-mode differentiation, transforms of ``torch.func`` and modes
+    that follow the operators: by torch's operators, with nothing kept in 8 bits."""
+    if not all(isinstance(t, torch.Tensor) and t.is_cuda for t in (x, weight)) or not all(t is None or (isinstance(t, torch.Tensor) and t.is_cuda) for t in (bias, residual)):
+        raise RuntimeError("x, weight, bias and residual must be CUDA tensors")
+    if activation not in L.ACTIVATIONS:
+        raise RuntimeError("activation must be one of %s" % ", ".join(map(repr, L.ACTIVATIONS)))
+    if ops._unseen(x, weight, bias, residual):
+        return _linear_by_operators(x, weight, bias, activation, residual)
+    return L.host().linear(x, weight, bias, L.ACTIVATIONS[activation], residual, bool(keep8), L.LINEAR_MAX_DIM)
+
+
+class Linear(nn.Linear):
+    """``nn.Linear`` whose ``forward(x, residual=None)`` is ``linear``, with its ``activation`` and ``keep8``; a state of either is one of the other's."""
+
+    def __init__(self, in_features, out_features, bias=True, activation=None, keep8=False):
+        super().__init__(in_features, out_features, bias=bias)
+        if activation not in L.ACTIVATIONS:
+            raise ValueError("activation must be one of %s" % ", ".join(map(repr, L.ACTIVATIONS)))
+        self.activation, self.keep8 = activation, bool(keep8)
+
+    def forward(self, x, residual=None):
+        return linear(x, self.weight, self.bias, self.activation, residual, self.keep8)
+
+    def extra_repr(self):
+        return super().extra_repr() + (", activation=%s" % self.activation if self.activation else "") + (", keep8=True" if self.keep8 else "")

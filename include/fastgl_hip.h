@@ -493,6 +493,25 @@ int fgl_layer_norm_backward(const void* d_dy, int64_t lddy, const void* d_x, int
                             void* stream);
 
 /* ---------------------------------------------------------------------------------
+ * A dense layer with what follows it, and its gradients (the reference's torch::mm, aggregate_acc.cpp:144, with what its models do
+ * to the result): z = x W^T + bias, y = act(z) + residual, for n rows x [n, dim] and W [out, dim] of `dtype`, 1 <= dim, out <= 4096, n < 2^31.
+ * act: 0 none, 1 relu (z <= 0 ? 0 : z), 2 gelu (z times the normal distribution function of z), 3 silu (z / (1 + exp(-z))).  bias [out], residual [n, out]: may be
+ * NULL.  bf16: rows of x and W (and, without an activation, of dy) start on 4-byte boundaries; strides below 2^24.
+ * d_state: what the backward pass needs, fgl_linear_state_bytes, at a multiple of 256 bytes (a bit a value for relu, z for gelu and silu; keep8
+ * not zero: the rows of x in 8 bits a value, as fgl_layer_norm keeps its own); NULL if there will be none.
+ * Backward: dz = dy act'(z), rounded to `dtype`; dx = dz W, dw = dz^T x (of the values that are held, with keep8: x may be NULL then), db = sums of dz over
+ * rows.  dx (row stride lddx), dw [out, dim] and db [out] may each be NULL; the residual's gradient is dy.  The state may be read by several backward passes.
+ * The same bits on every run.
+ * ------------------------------------------------------------------------------- */
+size_t fgl_linear_state_bytes(int64_t n, int dim, int out, int dtype, int act, int keep8);
+size_t fgl_linear_workspace_bytes(int64_t n, int dim, int out, int dtype, int act, int keep8, int want_dw, int want_db);
+int fgl_linear(const void* d_x, int64_t ldx, const void* d_w, int64_t ldw, const void* d_bias, const void* d_residual, int64_t ldr, int64_t n, int dim, int out,
+               int dtype, int act, int keep8, void* d_y, int64_t ldy, void* d_state, size_t state_bytes, void* stream);
+int fgl_linear_backward(const void* d_dy, int64_t lddy, const void* d_x, int64_t ldx, const void* d_w, int64_t ldw, int64_t n, int dim, int out, int dtype,
+                        int act, int keep8, const void* d_state, size_t state_bytes, void* d_dx, int64_t lddx, void* d_dw, void* d_db, void* d_ws, size_t ws_bytes,
+                        void* stream);
+
+/* ---------------------------------------------------------------------------------
  * A model's last product and its loss as one operator, without the logits ever lying in memory: softmax cross entropy of
  * x W^T + b (replaces the last layer's product followed by nn.CrossEntropyLoss, train_fastgl.py:328,383).
  *   s_iv = sum_d x[i, d] w[v, d] + b[v],   loss_i = log(sum_v exp(s_iv)) - s_i,label(i)
