@@ -12,7 +12,7 @@ Tensor as_rows(const Tensor& x, bool even)
     const int64_t d = x.size(-1);
     Tensor m = x.dim() == 2 ? x : x.reshape({-1, d});
     if (m.size(0) == 0 || d == 0) return m;
-    if ((d > 1 && m.stride(1) != 1) || (m.size(0) > 1 && m.stride(0) < d)) m = m.contiguous();
+    if ((d > 1 && m.stride(1) != 1) || (m.size(0) > 1 && (m.stride(0) < d || m.stride(0) >= 1 << 24))) m = m.contiguous();
     if (even && ((m.size(0) > 1 && m.stride(0) % 2 != 0) || (reinterpret_cast<uintptr_t>(m.data_ptr()) & 3) != 0)) {
         Tensor wider = torch::empty({m.size(0), (d + 1) / 2 * 2}, m.options().requires_grad(false));
         Tensor copy = wider.narrow(1, 0, d);

@@ -33,20 +33,27 @@ __device__ __forceinline__ float act_normal(float z, float& e)
 
 __device__ __forceinline__ bool act_passes(float z) { return !(z <= 0.0f); }  // (what is not a number stays it)
 
-template <int N, int V>
-__device__ __forceinline__ void act_apply(int act, float (&v)[N][V])
+template <int N, int V, typename F>
+__device__ __forceinline__ void act_each(float (&v)[N][V], F&& f)
 {
-    if (act == kActNone) return;
 #pragma unroll
     for (int i = 0; i < N; ++i)
 #pragma unroll
-        for (int t = 0; t < V; ++t) {
-            const float z = v[i][t];
+        for (int t = 0; t < V; ++t) v[i][t] = f(v[i][t]);
+}
+template <int N, int V>
+__device__ __forceinline__ void act_apply(int act, float (&v)[N][V])
+{
+    if (act == kActRelu) {
+        act_each(v, [](float z) { return act_passes(z) ? z : 0.0f; });
+    } else if (act == kActGelu) {
+        act_each(v, [](float z) {
             float unused;
-            if (act == kActRelu) v[i][t] = act_passes(z) ? z : 0.0f;
-            else if (act == kActGelu) v[i][t] = z * act_normal(z, unused);
-            else v[i][t] = z * __builtin_amdgcn_rcpf(1.0f + act_exp(-z));
-        }
+            return z * act_normal(z, unused);
+        });
+    } else if (act == kActSilu) {
+        act_each(v, [](float z) { return z * __builtin_amdgcn_rcpf(1.0f + act_exp(-z)); });
+    }
 }
 
 // the derivative (not relu's, which is a bit)

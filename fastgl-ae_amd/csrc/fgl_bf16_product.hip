@@ -1,0 +1,237 @@
+// Products over the rows of a block in bf16 (what fgl_row_product.hip forms, which see) where there are enough rows to keep the weights on the CUs:
+// C[m, n] = A[m, k] B[k, n], or act(A B + bias) + residual.
+//
+// Split: as in fgl_split_product.hip a workgroup keeps its 32 NT columns of B in LDS, in the order in which the lanes take them, and its waves go over the rows
+// of A, here in tiles of 64, each by itself: no barrier after the first.  A lane reads its two rows of A straight to registers, 64 k (a line of 128 bytes a row) ahead;
+// an operand of B from LDS serves two matrix instructions, which is what LDS delivers at the matrix cores' rate with room to spare.
+//
+// What bounds it: for short k and few columns the pass over A and C, beyond that the matrix cores.
+//
+// k past the end: a lane's eight k begin where they would or eight before the end of the row, and B's image is zero for those that an eight before has.
+// Rows past the end repeat the last one and are not stored, nor are columns past the end, which repeat the last one too.  No access leaves the operands.
+#include "fgl_common.hpp"
+#include "fgl_kernels.hpp"
+#include "fgl_row_product.hpp"
+#include "fgl_split.hpp"
+
+namespace fgl {
+
+constexpr int kBpLds = 158 * 1024;
+typedef uint32_t BpU4 __attribute__((ext_vector_type(4), aligned(2)));
+
+__device__ __host__ __forceinline__ int bp_chunks(int k) { return (k + 63) / 64; }
+// Where the eight k of number `oct` are read
+__device__ __forceinline__ int bp_first(int oct, int k) { return 8 * oct + 8 <= k ? 8 * oct : k - 8; }
+
+// (the lanes' columns: fgl_split_product.hip)
+__device__ __forceinline__ int bp_column(int vl, int t, int i) { return ((t >> vl) << (5 + vl)) + (i << vl) + (t & ((1 << vl) - 1)); }
+
+// B's columns from col0 on -> img[step * NT + tile][lane], a step being 16 k
+template <int NT, bool BT, int THREADS>
+__device__ __forceinline__ void bp_stage(const RowProductSide& x, int col0, int n, int vl, SpU4* img)
+{
+    constexpr int kCols = 32 * NT, kBatch = 8;  // (so many loads a thread on their way; the accumulators' registers are free yet)
+    const uint16_t* b = static_cast<const uint16_t*>(x.b);
+    const int items = bp_chunks(x.k) * 8 * kCols;
+    // A transposed B is read along its rows, a line of 128 bytes by eight lanes, another one along its columns.
+    auto place = [&](int at, int& oct, int& c) {
+        if constexpr (BT) {
+            oct = at / (8 * kCols) * 8 + at % 8;
+            c = at / 8 % kCols;
+        } else {
+            oct = at / kCols;
+            c = at % kCols;
+        }
+    };
+    for (int first = (int)threadIdx.x; first < items; first += THREADS * kBatch) {
+        SpU4 v[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            int oct, c;
+            place(first + i * THREADS < items ? first + i * THREADS : items - 1, oct, c);
+            const int col = col0 + c < n ? col0 + c : n - 1, k0 = bp_first(oct, x.k);
+            if constexpr (BT) {
+                const BpU4 w = *reinterpret_cast<const BpU4*>(b + (int64_t)col * x.ldb + k0);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[i][j] = w[j];
+            } else {
+                const uint16_t* p = b + (int64_t)k0 * x.ldb + col;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[i][j] = (uint32_t)p[2 * j * x.ldb] | (uint32_t)p[(2 * j + 1) * x.ldb] << 16;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            const int at = first + i * THREADS;
+            if (at >= items) break;
+            int oct, c;
+            place(at, oct, c);
+            const int k0 = bp_first(oct, x.k), own = 8 * oct;
+            if (k0 != own) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (k0 + 2 * j < own) v[i][j] &= 0xFFFF0000u;
+                    if (k0 + 2 * j + 1 < own) v[i][j] &= 0x0000FFFFu;
+                }
+            }
+            const int t = (c >> (5 + vl) << vl) + (c & ((1 << vl) - 1)), lane = (c >> vl) & 31;
+            img[((oct / 2) * NT + t) * kWave + oct % 2 * 32 + lane] = v[i];
+        }
+    }
+}
+
+template <int NT, int V>
+__device__ __forceinline__ void bp_then(const RowProductArgs& g, int64_t row0, int col0, const SpF32x16 (&acc)[2][NT])
+{
+    int lane = lane_id();
+    asm volatile("" : "+v"(lane));
+#pragma unroll
+    for (int q = 0; q < NT / V; ++q) {
+        const int col = col0 + 32 * V * q + lane % 32 * V;
+        float add[V];
+#pragma unroll
+        for (int t = 0; t < V; ++t) {
+            add[t] = 0.0f;
+            if (g.bias != nullptr && col + t < g.n) add[t] = __uint_as_float((uint32_t)static_cast<const uint16_t*>(g.bias)[col + t] << 16);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) rp_then<uint16_t, V>(g, row0 + 32 * i, lane / 32, col, [&](int t, int r) { return acc[i][q * V + t][r] + add[t]; });
+    }
+}
+
+// V: neighbouring columns a lane stores
+template <int NT, int W, bool BT, int V>
+__global__ __launch_bounds__(W * kWave, 2) void bf16_product_kernel(const RowProductArgs g)
+{
+    extern __shared__ SpU4 s_img[];
+    const int lane = lane_id(), half = lane / 32;
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x / kWave));
+    const unsigned per_group = 8u * (unsigned)g.tiles_n;
+    const int64_t rb = (int64_t)(blockIdx.x / per_group) * 8 + blockIdx.x % per_group % 8;
+    const int col0 = (int)(blockIdx.x % per_group / 8) * 32 * NT;
+    const int64_t row_tiles = (g.m + 63) / 64, stride = g.row_blocks * W;
+    if (rb * W >= row_tiles) return;  // (uniform over the workgroup: no row tile for it)
+    const int k = g.side[0].k, chunks = bp_chunks(k);
+    const int64_t lda = g.side[0].lda;
+    int64_t tile = rb * W + wave, ahead = tile;
+    int at = 0;
+    const uint16_t *p0, *p1;
+    auto rows_of = [&](int64_t t) {
+        int64_t row = t * 64 + lane % 32;
+        const int64_t last = g.m - 1;
+        p0 = static_cast<const uint16_t*>(g.side[0].a) + (row < last ? row : last) * lda;
+        row += 32;
+        p1 = static_cast<const uint16_t*>(g.side[0].a) + (row < last ? row : last) * lda;
+    };
+    rows_of(ahead);
+    auto load = [&](SpU4 (&a)[2][4]) {
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            const int k0 = bp_first(8 * at + 2 * s + half, k);
+            const BpU4 u = *reinterpret_cast<const BpU4*>(p0 + k0), v = *reinterpret_cast<const BpU4*>(p1 + k0);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                a[0][s][j] = u[j];
+                a[1][s][j] = v[j];
+            }
+        }
+        if (++at == chunks) {
+            at = 0;
+            if (ahead + stride < row_tiles) ahead += stride;
+            rows_of(ahead);
+        }
+    };
+    SpU4 cur[2][4], next[2][4];
+    load(cur);
+    bp_stage<NT, BT, W * kWave>(g.side[0], col0, g.n, V == 4 ? 2 : V == 2 ? 1 : 0, s_img);
+    __syncthreads();
+    if (tile >= row_tiles) return;  // (uniform over the wave; no barrier follows)
+    for (;;) {
+        SpF32x16 acc[2][NT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) acc[0][t] = acc[1][t] = SpF32x16{};
+        const SpU4* img = s_img + lane;
+        for (int c = 0; c < chunks; ++c) {
+            load(next);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                SpU4 b[NT];
+#pragma unroll
+                for (int t = 0; t < NT; ++t) b[t] = img[(s * NT + t) * kWave];
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+                        acc[i][t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(Bf16x8, cur[i][s]), __builtin_bit_cast(Bf16x8, b[t]), acc[i][t], 0, 0, 0);
+            }
+            img += 4 * NT * kWave;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int s = 0; s < 4; ++s) cur[i][s] = next[i][s];
+        }
+        // The sums may be read so many cycles after the last product; a branch lies between the two, across which the compiler was seen not to keep them.
+        if constexpr (NT == 4)
+            asm volatile("s_nop 15\n\ts_nop 15" : "+v"(acc[0][0]), "+v"(acc[0][1]), "+v"(acc[0][2]), "+v"(acc[0][3]), "+v"(acc[1][0]), "+v"(acc[1][1]), "+v"(acc[1][2]), "+v"(acc[1][3]));
+        else if constexpr (NT == 2)
+            asm volatile("s_nop 15\n\ts_nop 15" : "+v"(acc[0][0]), "+v"(acc[0][1]), "+v"(acc[1][0]), "+v"(acc[1][1]));
+        else
+            asm volatile("s_nop 15\n\ts_nop 15" : "+v"(acc[0][0]), "+v"(acc[1][0]));
+        const int64_t row0 = tile * 64;
+        bp_then<NT, V>(g, row0, col0, acc);
+        tile += stride;
+        if (tile >= row_tiles) return;
+    }
+}
+
+static size_t bp_lds(int k, int nt) { return (size_t)bp_chunks(k) * 4 * nt * kWave * sizeof(SpU4); }
+
+static int bp_tiles(int k, int n)
+{
+    if (n > 64 && bp_lds(k, 4) <= (size_t)kBpLds) return 4;
+    return n > 32 && bp_lds(k, 2) <= (size_t)kBpLds ? 2 : 1;
+}
+
+bool bf16_product_pays(const RowProductArgs& g)
+{
+    const int k = g.side[0].k;
+    return k >= 16 && bp_lds(k, 1) <= (size_t)kBpLds && g.m >= 8192;
+}
+
+template <int NT, int W, bool BT>
+static int launch_bf16_product(RowProductArgs g, hipStream_t stream)
+{
+    const size_t lds = bp_lds(g.side[0].k, NT);
+    g.tiles_n = (int)ceil_div(g.n, 32 * NT);
+    int64_t per_cu = kBpLds / (int64_t)lds;
+    if (per_cu > 8 / W) per_cu = 8 / W;
+    const uint64_t starts = (uintptr_t)g.c | (uintptr_t)g.then.residual | (uintptr_t)g.then.z | (uint64_t)(g.ldc | g.then.ldr | g.then.ldz | g.n) * 2;
+    const int v = NT >= 4 && starts % 8 == 0 ? 4 : NT >= 2 && starts % 4 == 0 ? 2 : 1;
+    g.row_blocks = sp_row_blocks(ceil_div(g.m, 64), W, (int)per_cu, g.tiles_n);
+    const int64_t blocks = ceil_div(g.row_blocks, 8) * 8 * g.tiles_n;
+    FGL_REQUIRE(blocks <= 0x7FFFFFFF, "row_product: grid too large");
+    const dim3 grid((unsigned)blocks), block(W * kWave);
+    if (v == 4) hipLaunchKernelGGL((bf16_product_kernel<NT, W, BT, NT >= 4 ? 4 : 1>), grid, block, lds, stream, g);
+    else if (v == 2) hipLaunchKernelGGL((bf16_product_kernel<NT, W, BT, NT >= 2 ? 2 : 1>), grid, block, lds, stream, g);
+    else hipLaunchKernelGGL((bf16_product_kernel<NT, W, BT, 1>), grid, block, lds, stream, g);
+    FGL_CHECK_LAUNCH("bf16_product_kernel");
+    return FGL_OK;
+}
+
+template <bool BT>
+static int launch_bf16_product_any(const RowProductArgs& g, hipStream_t stream)
+{
+    const int nt = bp_tiles(g.side[0].k, g.n);
+    const bool one_a_cu = bp_lds(g.side[0].k, nt) * 2 > (size_t)kBpLds;  // then of eight waves, otherwise two of four
+    if (nt == 4) return one_a_cu ? launch_bf16_product<4, 8, BT>(g, stream) : launch_bf16_product<4, 4, BT>(g, stream);
+    if (nt == 2) return one_a_cu ? launch_bf16_product<2, 8, BT>(g, stream) : launch_bf16_product<2, 4, BT>(g, stream);
+    return one_a_cu ? launch_bf16_product<1, 8, BT>(g, stream) : launch_bf16_product<1, 4, BT>(g, stream);
+}
+
+int bf16_product(const RowProductArgs& g, bool b_transposed, hipStream_t stream)
+{
+    return b_transposed ? launch_bf16_product_any<true>(g, stream) : launch_bf16_product_any<false>(g, stream);
+}
+
+}  // namespace fgl

@@ -210,7 +210,8 @@ FGL_EXPORT int fgl_linear(const void* d_x, int64_t ldx, const void* d_w, int64_t
     FGL_REQUIRE(linear_sizes(n, dim, out, dtype, act), "linear: %lld rows of %d by %d columns, dtype %d, activation %d", (long long)n, dim, out, dtype, act);
     FGL_LINEAR_ROWS(d_x, ldx, dim);
     FGL_LINEAR_ROWS(d_w, ldw, dim);
-    FGL_REQUIRE(ldy >= out && (d_residual == nullptr || ldr >= out), "linear: row stride smaller than the row length");
+    FGL_REQUIRE(ldy >= out && ldy < (1 << 24) && (d_residual == nullptr || (ldr >= out && ldr < (1 << 24))), "linear: row strides %lld and %lld of %d columns", (long long)ldy,
+                (long long)ldr, out);
     if (n == 0) return FGL_OK;
     FGL_REQUIRE(d_x && d_w && d_y, "linear: null pointer");
     RowProductArgs g;
@@ -243,7 +244,7 @@ FGL_EXPORT int fgl_linear(const void* d_x, int64_t ldx, const void* d_w, int64_t
             FGL_CHECK_LAUNCH("pack8_kernel");
         }
     }
-    return row_product_then(g, dtype, s);
+    return row_product_then(g, true, dtype, s);
 }
 
 FGL_EXPORT int fgl_linear_backward(const void* d_dy, int64_t lddy, const void* d_x, int64_t ldx, const void* d_w, int64_t ldw, int64_t n, int dim, int out, int dtype,
@@ -259,7 +260,8 @@ FGL_EXPORT int fgl_linear_backward(const void* d_dy, int64_t lddy, const void* d
     } else {
         FGL_REQUIRE(lddy >= out, "linear_backward: row stride smaller than the row length");
     }
-    FGL_REQUIRE(d_dx == nullptr || (ldw >= dim && lddx >= dim), "linear_backward: row stride smaller than the row length");
+    FGL_REQUIRE(d_dx == nullptr || (ldw >= dim && lddx >= dim && ldw < (1 << 24) && lddx < (1 << 24)), "linear_backward: row strides %lld and %lld of %d columns", (long long)ldw,
+                (long long)lddx, dim);
     if (sums && !keep8) {
         FGL_LINEAR_ROWS(d_x, ldx, dim);
     }
@@ -288,7 +290,11 @@ FGL_EXPORT int fgl_linear_backward(const void* d_dy, int64_t lddy, const void* d
         lddz = kept.ldz;
     }
     if (d_dx != nullptr) {
-        const int rc = fgl_row_product(dz, lddz, d_w, ldw, 0, n, out, dim, dtype, nullptr, d_dx, lddx, stream);
+        RowProductArgs g;
+        memset(&g, 0, sizeof(g));
+        g.side[0] = RowProductSide{dz, d_w, lddz, ldw, out};
+        g.c = d_dx; g.ldc = lddx; g.m = n; g.n = dim;
+        const int rc = row_product_then(g, false, dtype, s);
         if (rc != FGL_OK) return rc;
     }
     if (!sums) return FGL_OK;

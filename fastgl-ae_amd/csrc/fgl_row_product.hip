@@ -273,7 +273,7 @@ __global__ __launch_bounds__(kBlock, VA * VB >= 4 ? 2 : 4) void row_product_kern
 
     if constexpr (FORM == kRpThen) {
 #pragma unroll
-        for (int i = 0; i < VA; ++i) rp_then<T, VB>(g, row0 + 32 * i + 4 * half, own_col, [&](int t, int r) { return acc[i * VB + t][r]; });
+        for (int i = 0; i < VA; ++i) rp_then<T, VB>(g, row0 + 32 * i, half, own_col, [&](int t, int r) { return acc[i * VB + t][r]; });
         return;
     }
     // accumulator register r of lane l: row 8 (r / 4) + 4 (l / 32) + r % 4, column l % 32 of its 32x32 tile
@@ -372,9 +372,14 @@ static int row_product(const RowProductSide& one, const RowProductSide& two, int
     return b_transposed ? launch_row_product_any<uint16_t, true, FORM>(g, vectors, s) : launch_row_product_any<uint16_t, false, FORM>(g, vectors, s);
 }
 
-int fgl::row_product_then(const RowProductArgs& given, int dtype, hipStream_t stream)
+int fgl::row_product_then(const RowProductArgs& g, bool b_transposed, int dtype, hipStream_t stream)
 {
-    RowProductArgs g = given;
+    if (dtype == FGL_BF16 && bf16_product_pays(g)) {
+        note_product("bf16_product_kernel");
+        return bf16_product(g, b_transposed, stream);
+    }
+    const RowProductSide& x = g.side[0];
+    if (!b_transposed) return fgl_row_product(x.a, x.lda, x.b, x.ldb, 0, g.m, x.k, g.n, dtype, g.bias, g.c, g.ldc, stream);
     const bool split = dtype == FGL_F32 && split_product_pays(g);
     note_product(split ? "split_product_kernel" : "row_product_kernel");
     if (split) return split_product(g, true, kRpThen, stream);

@@ -82,57 +82,75 @@ __device__ __forceinline__ void rp_store(T* p, const float (&v)[VB])
 constexpr int kRpOne = 0, kRpSum = 1, kRpAdd = 2, kRpThen = 3;
 
 // The epilogue of 16 rows of a lane, of V neighbouring columns each from `col` on; accumulator register r of tile t is value(t, r), of row row0 +
-// 8 (r / 4) + r % 4.  V > 1 only where rows are a whole number of V, so that all or none of a lane's columns exist.  Every lane of the wave has to call it.
+// 4 half + 8 (r / 4) + r % 4, half being the lane's half of the wave and row0 the wave's.  V > 1 only where rows are a whole number of V, so that all or none of a lane's
+// columns exist.  Every lane of the wave has to call it.
+// A lane's place within a group of rows is 32 bits for each array, and the rest of an address the wave's (scalar): addresses of 64 bits a lane and row take what
+// registers the accumulators leave.
 template <typename T, int V, typename F>
-__device__ __forceinline__ void rp_then(const RowProductArgs& g, int64_t row0, int col, F&& value)
+__device__ __forceinline__ void rp_then(const RowProductArgs& g, int64_t row0, int half, int col, F&& value)
 {
     constexpr int kBatch = V == 4 ? 4 : 8;  // rows whose residuals are on their way together
     constexpr int kLanes = 32 / V;          // that share a word of the mask
     const RowProductEpilogue& e = g.then;
-    const bool there = col < g.n;
+    const int64_t rows = g.m - row0 - 4 * half;
+    const int left = col < g.n ? (rows < 64 ? (int)rows : 64) : 0;  // rows of the lane, from its first
+    auto place = [&](int64_t ld) { return (uint32_t)(4 * half * (int)ld + col) * (uint32_t)sizeof(T); };
+    const uint32_t at_c = place(g.ldc), at_r = place(e.ldr), at_z = place(e.ldz);
+    uint32_t words[V == 4 ? 2 : 1];  // of the mask, of row number lane % kLanes (and that plus kLanes): all lanes store at once what one of each kLanes would row by row
+    auto row_of = [&](const void* base, int64_t ld, int r) { return static_cast<const char*>(base) + (row0 + 8 * (r / 4) + r % 4) * ld * (int64_t)sizeof(T); };
 #pragma unroll
     for (int r0 = 0; r0 < 16; r0 += kBatch) {
         float v[kBatch][V], add[kBatch][V];
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
-            const int64_t row = row0 + 8 * ((r0 + i) / 4) + (r0 + i) % 4;
+            const int r = r0 + i;
 #pragma unroll
             for (int t = 0; t < V; ++t) add[i][t] = 0.0f;
-            if (e.residual != nullptr && there && row < g.m) rp_add<T, V>(static_cast<const T*>(e.residual) + row * e.ldr + col, add[i]);
+            if (e.residual != nullptr && 8 * (r / 4) + r % 4 < left) rp_add<T, V>(reinterpret_cast<const T*>(row_of(e.residual, e.ldr, r) + at_r), add[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i)
 #pragma unroll
             for (int t = 0; t < V; ++t) v[i][t] = value(t, r0 + i);
-        }
         if (e.z != nullptr) {
 #pragma unroll
             for (int i = 0; i < kBatch; ++i) {
-                const int64_t row = row0 + 8 * ((r0 + i) / 4) + (r0 + i) % 4;
-                if (there && row < g.m) rp_store<T, V>(static_cast<T*>(e.z) + row * e.ldz + col, v[i]);
+                const int r = r0 + i;
+                if (8 * (r / 4) + r % 4 < left) rp_store<T, V>(reinterpret_cast<T*>(const_cast<char*>(row_of(e.z, e.ldz, r)) + at_z), v[i]);
             }
         }
         if (e.mask != nullptr) {
 #pragma unroll
             for (int i = 0; i < kBatch; ++i) {
-                const int64_t row = row0 + 8 * ((r0 + i) / 4) + (r0 + i) % 4;
+                const int r = r0 + i;
                 uint32_t word;
                 if constexpr (V == 1) {
-                    const unsigned long long b = __ballot(there && act_passes(v[i][0]));
-                    word = lane_id() < 32 ? (uint32_t)b : (uint32_t)(b >> 32);
+                    const unsigned long long b = __ballot(left > 0 && act_passes(v[i][0]));
+                    word = half == 0 ? (uint32_t)b : (uint32_t)(b >> 32);
                 } else {
                     uint32_t bits = 0;
 #pragma unroll
-                    for (int t = 0; t < V; ++t) bits |= there && act_passes(v[i][t]) ? 1u << t : 0u;
+                    for (int t = 0; t < V; ++t) bits |= left > 0 && act_passes(v[i][t]) ? 1u << t : 0u;
                     word = group_or<kLanes>(bits << (V * (lane_id() % kLanes)));
                 }
-                if (lane_id() % kLanes == 0 && there && row < g.m) e.mask[row * e.mask_ld + col / 32] = word;
+                if (lane_id() % kLanes == r % kLanes) words[r / kLanes] = word;
             }
         }
         act_apply<kBatch, V>(e.act, v);
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
-            const int64_t row = row0 + 8 * ((r0 + i) / 4) + (r0 + i) % 4;
+            const int r = r0 + i;
 #pragma unroll
             for (int t = 0; t < V; ++t) v[i][t] += add[i][t];
-            if (there && row < g.m) rp_store<T, V>(static_cast<T*>(g.c) + row * g.ldc + col, v[i]);
+            if (8 * (r / 4) + r % 4 < left) rp_store<T, V>(reinterpret_cast<T*>(const_cast<char*>(row_of(g.c, g.ldc, r)) + at_c), v[i]);
+        }
+    }
+    if (e.mask != nullptr && (V != 1 || lane_id() % kLanes < 16)) {
+#pragma unroll
+        for (int q = 0; q < (V == 4 ? 2 : 1); ++q) {
+            const int r = q * kLanes + lane_id() % kLanes, row = 8 * (r / 4) + r % 4;
+            // (a lane whose columns do not exist stores a row's word all the same, if the word does)
+            if (row < rows && col - V * (lane_id() % kLanes) < g.n) (e.mask + row0 * e.mask_ld)[(4 * half + row) * (int)e.mask_ld + col / 32] = words[q];
         }
     }
 }
@@ -141,7 +159,14 @@ __device__ __forceinline__ void rp_then(const RowProductArgs& g, int64_t row0, i
 bool split_product_pays(const RowProductArgs& g);
 int split_product(const RowProductArgs& g, bool b_transposed, int form, hipStream_t stream);
 
-// side[0]'s product with B transposed, and its epilogue; sizes, strides and pointers have been checked (bf16: rows of A and B start on words)
-int row_product_then(const RowProductArgs& g, int dtype, hipStream_t stream);
+// Row blocks, eight at a time, of a kernel that keeps B's columns on the CUs (fgl_split_product.hip)
+int64_t sp_row_blocks(int64_t row_tiles, int waves, int per_cu, int64_t tiles_n);
+
+// bf16 products with B kept on the CUs, side[0]'s with bias and epilogue: whether they pay for these sizes, and one of them
+bool bf16_product_pays(const RowProductArgs& g);
+int bf16_product(const RowProductArgs& g, bool b_transposed, hipStream_t stream);
+
+// side[0]'s product, B transposed or (without an epilogue) not, and its epilogue; sizes, strides and pointers have been checked (bf16: rows of A and B start on words)
+int row_product_then(const RowProductArgs& g, bool b_transposed, int dtype, hipStream_t stream);
 
 }  // namespace fgl

@@ -335,7 +335,7 @@ __device__ __forceinline__ void sp_then(const RowProductArgs& g, int64_t row0, i
             add[t] = 0.0f;
             if (g.bias != nullptr && col + t < g.n) add[t] = static_cast<const float*>(g.bias)[col + t];
         }
-        rp_then<float, V>(g, row0 + 4 * (lane / 32), col, [&](int t, int r) { return acc[q * V + t][r] + add[t]; });
+        rp_then<float, V>(g, row0, lane / 32, col, [&](int t, int r) { return acc[q * V + t][r] + add[t]; });
     }
 }
 
@@ -483,7 +483,7 @@ static size_t sp_lds(const RowProductArgs& g, int nt) { return (size_t)(sp_chunk
 // row tiles, and two tiles' time to stage B; six tenths of that in a last round that has the CUs to itself, so that half rounds count too.
 // (us, with one block more than fits / with this: 209 K x 64 x 896 248 / 209, 100 K x 128 x 376 95 / 77, added to C 168 / 112, 119 K x (256 +
 // 256) x 165 302 / 210, 80 K x 256 x 1064 424 / 302; whole rounds only / with this: 19 K x 128 x 2970 126 / 113.)
-static int64_t sp_row_blocks(int64_t row_tiles, int waves, int per_cu, int64_t tiles_n)
+int64_t sp_row_blocks(int64_t row_tiles, int waves, int per_cu, int64_t tiles_n)
 {
     const int64_t places = 32 * per_cu, want = ceil_div(ceil_div(row_tiles, waves), 8);  // (of an XCD: a tile a wave)
     int64_t best = 1, least = INT64_MAX;
