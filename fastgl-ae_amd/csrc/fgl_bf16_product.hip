@@ -99,9 +99,12 @@ __device__ __forceinline__ void bp_then(const RowProductArgs& g, int64_t row0, i
     }
 }
 
+// Waves a SIMD: as the accumulators' registers allow
+constexpr int bp_waves(int nt) { return nt >= 4 ? 2 : nt == 2 ? 3 : 4; }
+
 // V: neighbouring columns a lane stores
 template <int NT, int W, bool BT, int V>
-__global__ __launch_bounds__(W * kWave, 2) void bf16_product_kernel(const RowProductArgs g)
+__global__ __launch_bounds__(W * kWave, bp_waves(NT)) void bf16_product_kernel(const RowProductArgs g)
 {
     extern __shared__ SpU4 s_img[];
     const int lane = lane_id(), half = lane / 32;
@@ -205,7 +208,7 @@ static int launch_bf16_product(RowProductArgs g, hipStream_t stream)
     const size_t lds = bp_lds(g.side[0].k, NT);
     g.tiles_n = (int)ceil_div(g.n, 32 * NT);
     int64_t per_cu = kBpLds / (int64_t)lds;
-    if (per_cu > 8 / W) per_cu = 8 / W;
+    if (per_cu > bp_waves(NT) * 4 / W) per_cu = bp_waves(NT) * 4 / W;
     const uint64_t starts = (uintptr_t)g.c | (uintptr_t)g.then.residual | (uintptr_t)g.then.z | (uint64_t)(g.ldc | g.then.ldr | g.then.ldz | g.n) * 2;
     const int v = NT >= 4 && starts % 8 == 0 ? 4 : NT >= 2 && starts % 4 == 0 ? 2 : 1;
     g.row_blocks = sp_row_blocks(ceil_div(g.m, 64), W, (int)per_cu, g.tiles_n);

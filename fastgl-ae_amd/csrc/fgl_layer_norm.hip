@@ -113,10 +113,10 @@ __device__ __forceinline__ double ln_rsqrt(double v)
 
 // The lane's values of a chunk, of which the first `left` exist (others: `fill`).  WHOLE: rows are a whole number of chunks, all or none exist.
 template <bool WHOLE, typename T>
-__device__ __forceinline__ LnVec<T> ln_load(const T* p, int left, float fill = 0.0f)
+__device__ __forceinline__ LnVec<T> ln_load(const T* p, bool inside, int left, float fill = 0.0f)
 {
     LnVec<T> v;
-    if (left >= kLnV<T>) {
+    if (inside || left >= kLnV<T>) {
         v = *reinterpret_cast<const LnVec<T>*>(p);
     } else {
 #pragma unroll
@@ -129,8 +129,10 @@ __device__ __forceinline__ LnVec<T> ln_load(const T* p, int left, float fill = 0
     }
     return v;
 }
+// Of a lane's loads, how many lie within the row whatever the row (ln_shape): those that a shape with fewer would have
+constexpr int ln_inside(int lanes, int loads) { return lanes < 16 ? 0 : loads == 8 ? 6 : lanes == 64 && loads == 6 ? 4 : loads - 1; }
 template <bool WHOLE>
-__device__ __forceinline__ bool ln_there(int e, int left) { return WHOLE ? left > 0 : e < left; }
+__device__ __forceinline__ bool ln_there(bool inside, int e, int left) { return inside || (WHOLE ? left > 0 : e < left); }
 // Keeps what is made of a parameter (its 32 or 64-bit value) from being formed before the loop over rows and held in twice or four times the registers
 template <typename T>
 __device__ __forceinline__ void ln_as_held(LnVec<T>& v)
@@ -141,9 +143,9 @@ __device__ __forceinline__ void ln_as_held(LnVec<T>& v)
     v = __builtin_bit_cast(LnVec<T>, u);
 }
 template <bool WHOLE, typename T>
-__device__ __forceinline__ void ln_store(T* p, int left, const LnVec<T>& v)
+__device__ __forceinline__ void ln_store(T* p, bool inside, int left, const LnVec<T>& v)
 {
-    if (left >= kLnV<T>) {
+    if (inside || left >= kLnV<T>) {
         *reinterpret_cast<LnVec<T>*>(p) = v;
     } else if constexpr (!WHOLE) {
 #pragma unroll
@@ -169,8 +171,8 @@ __global__ __launch_bounds__(kLnThreads, C * kLnV<T> <= 16 ? 4 : 2) void layer_n
 #pragma unroll
     for (int j = 0; j < C; ++j) {
         const int c = (j * G + l) * V, left = g.d - c;
-        w[j] = ln_load<WHOLE>(static_cast<const T*>(g.w) + c, g.w != nullptr ? left : 0, 1.0f);
-        b[j] = ln_load<WHOLE>(static_cast<const T*>(g.b) + c, g.b != nullptr ? left : 0, 0.0f);
+        w[j] = ln_load<WHOLE>(static_cast<const T*>(g.w) + c, false, g.w != nullptr ? left : 0, 1.0f);
+        b[j] = ln_load<WHOLE>(static_cast<const T*>(g.b) + c, false, g.b != nullptr ? left : 0, 0.0f);
     }
     const int64_t stride = (int64_t)gridDim.x * kLnWaves * kRows;
     for (int64_t row0 = ((int64_t)blockIdx.x * kLnWaves + wave) * kRows; row0 < g.n; row0 += stride) {
@@ -182,7 +184,7 @@ __global__ __launch_bounds__(kLnThreads, C * kLnV<T> <= 16 ? 4 : 2) void layer_n
             ln_as_held<T>(w[j]);
             ln_as_held<T>(b[j]);
             const int c = (j * G + l) * V;
-            v[j] = ln_load<WHOLE>(x + row * g.ldx + c, g.d - c);
+            v[j] = ln_load<WHOLE>(x + row * g.ldx + c, j < ln_inside(G, C), g.d - c);
         }
         double sum = 0.0;
 #pragma unroll
@@ -198,7 +200,7 @@ __global__ __launch_bounds__(kLnThreads, C * kLnV<T> <= 16 ? 4 : 2) void layer_n
 #pragma unroll
             for (int e = 0; e < V; ++e) {
                 const double t = (double)(float)v[j][e] - mean;
-                if (ln_there<WHOLE>(e, g.d - (j * G + l) * V)) square = fma(t, t, square);
+                if (ln_there<WHOLE>(j < ln_inside(G, C), e, g.d - (j * G + l) * V)) square = fma(t, t, square);
             }
         const double rstd = ln_rsqrt(fma(ln_sum<G>(square), g.inv_d64, g.eps));
         if (g.state.rstd != nullptr && l == 0 && mine) {
@@ -211,7 +213,7 @@ __global__ __launch_bounds__(kLnThreads, C * kLnV<T> <= 16 ? 4 : 2) void layer_n
             double h[V];
             float out[V];
 #pragma unroll
-            for (int e = 0; e < V; ++e) h[e] = ln_there<WHOLE>(e, left) ? ((double)(float)v[j][e] - mean) * rstd : 0.0;
+            for (int e = 0; e < V; ++e) h[e] = ln_there<WHOLE>(j < ln_inside(G, C), e, left) ? ((double)(float)v[j][e] - mean) * rstd : 0.0;
             if (g.relu) {
                 uint32_t bits = 0;
 #pragma unroll
@@ -229,7 +231,7 @@ __global__ __launch_bounds__(kLnThreads, C * kLnV<T> <= 16 ? 4 : 2) void layer_n
             LnVec<T> q;
 #pragma unroll
             for (int e = 0; e < V; ++e) q[e] = (T)out[e];
-            if (mine) ln_store<WHOLE>(y + row * g.d + c, left, q);
+            if (mine) ln_store<WHOLE>(y + row * g.d + c, j < ln_inside(G, C), left, q);
             if constexpr (KEEP8) {
                 uint32_t most = 0;  // the largest magnitude's upper word: exponent and first bits
 #pragma unroll
@@ -243,8 +245,9 @@ __global__ __launch_bounds__(kLnThreads, C * kLnV<T> <= 16 ? 4 : 2) void layer_n
                 LnCodes<V> codes;
 #pragma unroll
                 for (int e = 0; e < V; ++e) {
-                    const double r = rint(h[e] * inverse);
-                    const uint32_t code = (uint32_t)((int)(r > 127.0 ? 127.0 : r < -127.0 ? -127.0 : r) + 128);
+                    // the nearest whole number, 128 more, in the lower word (what the sum with 1.5 2^52 rounds to)
+                    const int r = __double2loint(fma(h[e], inverse, 0x1.8p52 + 128.0));
+                    const uint32_t code = (uint32_t)(r < 1 ? 1 : r > 255 ? 255 : r);
                     if (e % 4 == 0) codes[e / 4] = code;
                     else codes[e / 4] |= code << 8 * (e % 4);
                 }
@@ -272,7 +275,7 @@ __global__ __launch_bounds__(kLnThreads, C * kLnV<T> <= 16 ? 4 : 2) void layer_n
 #pragma unroll
     for (int j = 0; j < C; ++j) {
         const int c = (j * G + l) * V;
-        w[j] = ln_load<WHOLE>(static_cast<const T*>(g.w) + c, g.w != nullptr ? g.d - c : 0, 1.0f);
+        w[j] = ln_load<WHOLE>(static_cast<const T*>(g.w) + c, false, g.w != nullptr ? g.d - c : 0, 1.0f);
 #pragma unroll
         for (int e = 0; e < V; ++e) dw[j][e] = db[j][e] = 0.0f;
     }
@@ -288,13 +291,13 @@ __global__ __launch_bounds__(kLnThreads, C * kLnV<T> <= 16 ? 4 : 2) void layer_n
         for (int j = 0; j < C; ++j) {
             ln_as_held<T>(w[j]);
             const int c = (j * G + l) * V, left = g.d - c;
-            vd[j] = ln_load<WHOLE>(dy + row * g.lddy + c, mine ? left : 0);  // (past the end: zeros, which add nothing)
+            vd[j] = ln_load<WHOLE>(dy + row * g.lddy + c, false, mine ? left : 0);  // (past the end: zeros, which add nothing)
             if constexpr (KEEP8) {
                 const int at = c < g.code_ld ? c : 0;
                 codes[j] = *reinterpret_cast<const LnCodes<V>*>(g.state.codes + row * g.code_ld + at);
                 step[j] = g.state.steps[row * (g.code_ld / 32) + at / 32];
             } else {
-                vx[j] = ln_load<WHOLE>(x + row * g.ldx + c, left);
+                vx[j] = ln_load<WHOLE>(x + row * g.ldx + c, j < ln_inside(G, C), left);
             }
             bits[j] = 0xFFu;
             if (g.relu && left > 0) bits[j] = (uint32_t)g.state.mask[row * g.mask_ld + c / 8] >> (c % 8);
@@ -306,7 +309,7 @@ __global__ __launch_bounds__(kLnThreads, C * kLnV<T> <= 16 ? 4 : 2) void layer_n
         for (int j = 0; j < C; ++j)
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                const bool there = ln_there<WHOLE>(e, g.d - (j * G + l) * V);
+                const bool there = ln_there<WHOLE>(j < ln_inside(G, C), e, g.d - (j * G + l) * V);
                 if constexpr (KEEP8) h[j][e] = there ? k8_value(codes[j][e / 4] >> 8 * (e % 4) & 0xFFu, step[j]) : 0.0f;
                 else h[j][e] = there ? (float)((double)(float)vx[j][e] - mean) * rstd : 0.0f;
                 const float d = bits[j] >> e & 1u ? (float)vd[j][e] : 0.0f;
@@ -326,7 +329,7 @@ __global__ __launch_bounds__(kLnThreads, C * kLnV<T> <= 16 ? 4 : 2) void layer_n
             LnVec<T> q;
 #pragma unroll
             for (int e = 0; e < V; ++e) q[e] = (T)(rstd * (t[j][e] - sum - h[j][e] * with_h));
-            if (mine) ln_store<WHOLE>(dx + row * g.d + c, g.d - c, q);
+            if (mine) ln_store<WHOLE>(dx + row * g.d + c, j < ln_inside(G, C), g.d - c, q);
         }
     }
     if (g.partial == nullptr) return;
@@ -358,26 +361,30 @@ __global__ __launch_bounds__(kLnThreads, C * kLnV<T> <= 16 ? 4 : 2) void layer_n
     }
 }
 
-// dw and db from the workgroups' sums: 32 columns a workgroup, eight lanes of rows
+// dw and db from the workgroups' sums: 32 columns a workgroup, 32 lanes of rows, eight loads of each on their way (of 1024 rows of 2 x 256 columns: 12 us with
+// a quarter of the lanes and half of the loads, XXX so)
+constexpr int kLnReduce = 1024;
 template <typename T>
-__global__ __launch_bounds__(kBlock) void layer_norm_reduce_kernel(const float* __restrict__ partial, int rows, int d, T* __restrict__ dw, T* __restrict__ db)
+__global__ __launch_bounds__(kLnReduce) void layer_norm_reduce_kernel(const float* __restrict__ partial, int rows, int d, T* __restrict__ dw, T* __restrict__ db)
 {
-    __shared__ float s_sum[8][33];
+    constexpr int kLanes = kLnReduce / 32, kBatch = 8;
+    __shared__ float s_sum[kLanes][33];
     const int i = (int)(threadIdx.x % 32), r = (int)(threadIdx.x / 32), c = (int)blockIdx.x * 32 + i;
     float s = 0.0f;
     if (c < 2 * d) {
-        const float* p = partial + c;
-        int q = r;
-        for (; q + 24 < rows; q += 32) {
-            const float v0 = p[(int64_t)q * 2 * d], v1 = p[(int64_t)(q + 8) * 2 * d], v2 = p[(int64_t)(q + 16) * 2 * d], v3 = p[(int64_t)(q + 24) * 2 * d];
-            s += (v0 + v1) + (v2 + v3);
+        for (int q = r; q < rows; q += kLanes * kBatch) {
+            float v[kBatch];
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) v[k] = q + k * kLanes < rows ? partial[(int64_t)(q + k * kLanes) * 2 * d + c] : 0.0f;
+            s += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
         }
-        for (; q < rows; q += 8) s += p[(int64_t)q * 2 * d];
     }
     s_sum[r][i] = s;
     __syncthreads();
     if (r != 0 || c >= 2 * d) return;
-    s = ((s_sum[0][i] + s_sum[1][i]) + (s_sum[2][i] + s_sum[3][i])) + ((s_sum[4][i] + s_sum[5][i]) + (s_sum[6][i] + s_sum[7][i]));
+    s = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kLanes; k += 4) s += (s_sum[k][i] + s_sum[k + 1][i]) + (s_sum[k + 2][i] + s_sum[k + 3][i]);
     if (c < d) {
         if (dw != nullptr) dw[c] = (T)s;
     } else if (db != nullptr) {
@@ -385,49 +392,55 @@ __global__ __launch_bounds__(kBlock) void layer_norm_reduce_kernel(const float* 
     }
 }
 
-// Lanes of a row and loads of a lane.  16 lanes as long as four loads are enough for them (sums over 16 lanes need no LDS exchange); fewer where a row
-// has no more.
+// Lanes of a row and loads of a lane.  16 lanes as long as their registers hold a row: four rows a wave share what is done once a row, sums over 16 lanes need no
+// exchange through LDS, and a lane has many loads on their way (200 K x 602 in bf16, of which 64 lanes take two loads each and leave two fifths of them empty: XXX).
+// In the backward pass a lane holds four values for each element of its loads, two of them sums, and a row of more than 40 takes 64 lanes.
 struct LnShape {
     int lanes, loads;
 };
-static LnShape ln_shape(int d, int v)
+static LnShape ln_shape(int d, int v, bool backward)
 {
     const int chunks = (d + v - 1) / v;
     if (chunks <= 32 / v) return {32 / v, 1};
-    if (chunks <= 16) return {16, 1};
-    if (chunks <= 32) return {16, 2};
-    if (chunks <= 64) return {16, 4};
-    if (chunks <= 128) return {64, 2};
-    return chunks <= 256 ? LnShape{64, 4} : LnShape{64, 8};
+    const int most = backward && v == 8 ? 80 : 128;
+    if (chunks <= most) return {16, chunks > 96 ? 8 : (chunks + 15) / 16};
+    const int loads = (chunks + 63) / 64;
+    return {64, loads > 6 ? 8 : loads > 4 ? 6 : loads};
 }
 
 // Calls f with integral constants: ln_shape's lanes and loads, whether rows are whole numbers of loads.
-template <typename T, typename F>
+template <typename T, bool BACKWARD, typename F>
 static void ln_dispatch(int d, F&& f)
 {
     constexpr int V = kLnV<T>;
-    const LnShape s = ln_shape(d, V);
-    const int key = s.lanes * 100 + s.loads;
+    const LnShape s = ln_shape(d, V, BACKWARD);
     auto call = [&](auto lanes, auto loads) {
+        if (s.lanes != decltype(lanes)::value || s.loads != decltype(loads)::value) return;
         if (d % V == 0) f(lanes, loads, std::true_type{});
         else f(lanes, loads, std::false_type{});
     };
+    auto each = [&](auto lanes, auto... loads) { (call(lanes, loads), ...); };
     using std::integral_constant;
-    switch (key) {
-        case 32 / V * 100 + 1: return call(integral_constant<int, 32 / V>{}, integral_constant<int, 1>{});
-        case 1601: return call(integral_constant<int, 16>{}, integral_constant<int, 1>{});
-        case 1602: return call(integral_constant<int, 16>{}, integral_constant<int, 2>{});
-        case 1604: return call(integral_constant<int, 16>{}, integral_constant<int, 4>{});
-        case 6402: return call(integral_constant<int, 64>{}, integral_constant<int, 2>{});
-        case 6404: return call(integral_constant<int, 64>{}, integral_constant<int, 4>{});
-        default:
-            if constexpr (V == 4) return call(integral_constant<int, 64>{}, integral_constant<int, 8>{});
-    }
+    constexpr integral_constant<int, 1> k1{};
+    constexpr integral_constant<int, 2> k2{};
+    constexpr integral_constant<int, 3> k3{};
+    constexpr integral_constant<int, 4> k4{};
+    constexpr integral_constant<int, 5> k5{};
+    constexpr integral_constant<int, 6> k6{};
+    constexpr integral_constant<int, 8> k8{};
+    constexpr integral_constant<int, 16> k16{};
+    constexpr integral_constant<int, 64> k64{};
+    call(integral_constant<int, 32 / V>{}, k1);
+    each(k16, k1, k2, k3, k4, k5);
+    if constexpr (!(BACKWARD && V == 8)) each(k16, k6, k8);
+    else call(k64, k2);
+    each(k64, k3, k4);
+    if constexpr (V == 4) each(k64, k6, k8);
 }
 
-static int64_t ln_blocks(int64_t n, int d, int dtype, int64_t most)
+static int64_t ln_blocks(int64_t n, int d, int dtype, bool backward, int64_t most)
 {
-    const int rows = kWave / ln_shape(d, dtype == FGL_F32 ? 4 : 8).lanes * kLnWaves;
+    const int rows = kWave / ln_shape(d, dtype == FGL_F32 ? 4 : 8, backward).lanes * kLnWaves;
     const int64_t want = ceil_div(n, rows);
     return want < most ? want : most;
 }
@@ -460,7 +473,7 @@ FGL_EXPORT size_t fgl_layer_norm_state_bytes(int64_t n, int d, int relu, int kee
 
 FGL_EXPORT size_t fgl_layer_norm_workspace_bytes(int64_t n, int d, int dtype)
 {
-    return ln_sizes(n, d, dtype) ? (size_t)ln_blocks(n, d, dtype, kLnMostBlocks) * 2 * (size_t)d * sizeof(float) : 0;
+    return ln_sizes(n, d, dtype) ? (size_t)ln_blocks(n, d, dtype, true, kLnMostBlocks) * 2 * (size_t)d * sizeof(float) : 0;
 }
 
 FGL_EXPORT int fgl_layer_norm(const void* d_x, int64_t ldx, const void* d_w, const void* d_b, int64_t n, int d, int dtype, double eps, int relu, int keep8,
@@ -481,10 +494,10 @@ FGL_EXPORT int fgl_layer_norm(const void* d_x, int64_t ldx, const void* d_w, con
         }
     }
     const bool codes = keep8 != 0 && d_state != nullptr;
-    const dim3 grid((unsigned)ln_blocks(n, d, dtype, 4096));
+    const dim3 grid((unsigned)ln_blocks(n, d, dtype, false, 4096));
     auto launch = [&](auto type) {
         using T = decltype(type);
-        ln_dispatch<T>(d, [&](auto lanes, auto loads, auto whole) {
+        ln_dispatch<T, false>(d, [&](auto lanes, auto loads, auto whole) {
             constexpr int G = decltype(lanes)::value, C = decltype(loads)::value;
             constexpr bool W = decltype(whole)::value;
             if (codes) hipLaunchKernelGGL((layer_norm_kernel<T, G, C, true, W>), grid, dim3(kLnThreads), 0, as_stream(stream), g);
@@ -512,7 +525,7 @@ FGL_EXPORT int fgl_layer_norm_backward(const void* d_dy, int64_t lddy, const voi
     }
     const bool sums = d_dw != nullptr || d_db != nullptr;
     if (d_dx == nullptr && !sums) return FGL_OK;
-    const int64_t blocks = ln_blocks(n, d, dtype, kLnMostBlocks);
+    const int64_t blocks = ln_blocks(n, d, dtype, true, kLnMostBlocks);
     if (sums && (d_ws == nullptr || ws_bytes < (size_t)blocks * 2 * d * sizeof(float) || ((uintptr_t)d_ws & 255) != 0)) {
         set_error("layer_norm_backward: workspace too small (%zu < %zu) or not at a multiple of 256 bytes", ws_bytes, (size_t)blocks * 2 * d * sizeof(float));
         return FGL_ERR_WORKSPACE;
@@ -521,14 +534,14 @@ FGL_EXPORT int fgl_layer_norm_backward(const void* d_dy, int64_t lddy, const voi
     g.partial = sums ? static_cast<float*>(d_ws) : nullptr;
     auto launch = [&](auto type) {
         using T = decltype(type);
-        ln_dispatch<T>(d, [&](auto lanes, auto loads, auto whole) {
+        ln_dispatch<T, true>(d, [&](auto lanes, auto loads, auto whole) {
             constexpr int G = decltype(lanes)::value, C = decltype(loads)::value;
             constexpr bool W = decltype(whole)::value;
             if (keep8) hipLaunchKernelGGL((layer_norm_backward_kernel<T, G, C, true, W>), dim3((unsigned)blocks), dim3(kLnThreads), 0, as_stream(stream), g);
             else hipLaunchKernelGGL((layer_norm_backward_kernel<T, G, C, false, W>), dim3((unsigned)blocks), dim3(kLnThreads), 0, as_stream(stream), g);
         });
         if (sums)
-            hipLaunchKernelGGL((layer_norm_reduce_kernel<T>), dim3((unsigned)ceil_div(2 * d, 32)), dim3(kBlock), 0, as_stream(stream), g.partial, (int)blocks, d,
+            hipLaunchKernelGGL((layer_norm_reduce_kernel<T>), dim3((unsigned)ceil_div(2 * d, 32)), dim3(kLnReduce), 0, as_stream(stream), g.partial, (int)blocks, d,
                                static_cast<T*>(d_dw), static_cast<T*>(d_db));
     };
     if (dtype == FGL_F32) launch(float{});
