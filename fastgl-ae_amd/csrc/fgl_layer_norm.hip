@@ -362,7 +362,7 @@ __global__ __launch_bounds__(kLnThreads, C * kLnV<T> <= 16 ? 4 : 2) void layer_n
 }
 
 // dw and db from the workgroups' sums: 32 columns a workgroup, 32 lanes of rows, eight loads of each on their way (of 1024 rows of 2 x 256 columns: 12 us with
-// a quarter of the lanes and half of the loads, XXX so)
+// a quarter of the lanes and half of the loads, 4 so)
 constexpr int kLnReduce = 1024;
 template <typename T>
 __global__ __launch_bounds__(kLnReduce) void layer_norm_reduce_kernel(const float* __restrict__ partial, int rows, int d, T* __restrict__ dw, T* __restrict__ db)
@@ -393,8 +393,10 @@ __global__ __launch_bounds__(kLnReduce) void layer_norm_reduce_kernel(const floa
 }
 
 // Lanes of a row and loads of a lane.  16 lanes as long as their registers hold a row: four rows a wave share what is done once a row, sums over 16 lanes need no
-// exchange through LDS, and a lane has many loads on their way (200 K x 602 in bf16, of which 64 lanes take two loads each and leave two fifths of them empty: XXX).
-// In the backward pass a lane holds four values for each element of its loads, two of them sums, and a row of more than 40 takes 64 lanes.
+// exchange through LDS, and a lane has many loads on their way (200 K x 602 in bf16, of
+// which 64 lanes would take two loads each and leave two fifths of them empty: 235 us forward and 265 back, 137 and 191 so).
+// In bf16 a row of more than 48 elements a lane takes 64 lanes,
+// in the backward pass, where a lane holds four values for each, two of them sums, one of more than 40.
 struct LnShape {
     int lanes, loads;
 };
@@ -402,7 +404,7 @@ static LnShape ln_shape(int d, int v, bool backward)
 {
     const int chunks = (d + v - 1) / v;
     if (chunks <= 32 / v) return {32 / v, 1};
-    const int most = backward && v == 8 ? 80 : 128;
+    const int most = v == 4 ? 128 : backward ? 80 : 96;
     if (chunks <= most) return {16, chunks > 96 ? 8 : (chunks + 15) / 16};
     const int loads = (chunks + 63) / 64;
     return {64, loads > 6 ? 8 : loads > 4 ? 6 : loads};
@@ -432,7 +434,8 @@ static void ln_dispatch(int d, F&& f)
     constexpr integral_constant<int, 64> k64{};
     call(integral_constant<int, 32 / V>{}, k1);
     each(k16, k1, k2, k3, k4, k5);
-    if constexpr (!(BACKWARD && V == 8)) each(k16, k6, k8);
+    if constexpr (V == 4 || !BACKWARD) call(k16, k6);
+    if constexpr (V == 4) call(k16, k8);
     else call(k64, k2);
     each(k64, k3, k4);
     if constexpr (V == 4) each(k64, k6, k8);

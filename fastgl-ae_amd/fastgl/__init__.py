@@ -30,7 +30,7 @@ from .ops import (  # noqa: F401
     transfer_edge_id,
 )
 from .dropouts import Dropout, dropout  # noqa: F401
-from .layers import LayerNorm, Linear, layer_norm, linear  # noqa: F401
+from .layers import FeedForward, LayerNorm, Linear, layer_norm, linear  # noqa: F401
 from .sampler import Block, DataLoader, FusedMapSampler, PendingBatch, transpose_blocks  # noqa: F401
 from .conv import (  # noqa: F401
     GAT,

@@ -20,6 +20,7 @@ from torch import nn
 
 from . import ops
 from .dropouts import Dropout
+from .layers import FeedForward, LayerNorm
 from .sampler import Block
 
 
@@ -185,17 +186,44 @@ def _between_layers(p, seed, relu=False):
     return plain
 
 
+def _add_depth(model, n_hidden, n_between, norm, feed_forward, keep8):
+    """What a model may have between its layers besides dropout (none of it: no modules, and a state without them): a ``FeedForward`` block with ``feed_forward`` hidden
+    columns, and behind it a norm of the rows (``norm="layer"``)."""
+    if norm not in (None, "layer"):
+        raise ValueError("norm must be None or 'layer', not %r" % (norm,))
+    if feed_forward < 0:
+        raise ValueError("feed_forward (%d) is a number of columns" % feed_forward)
+    if norm is None and not feed_forward:
+        if keep8:
+            raise ValueError("keep8 is of the norms and feed-forward blocks between the layers: there are none")
+        return
+    if feed_forward:
+        model.blocks_between = nn.ModuleList(FeedForward(n_hidden, feed_forward, keep8=keep8) for _ in range(n_between))
+    if norm is not None:
+        model.norms = nn.ModuleList(LayerNorm(n_hidden, keep8=keep8) for _ in range(n_between))
+
+
+def _deepened(model, i, h, relu=False):
+    """``h`` behind layer ``i``, through what ``_add_depth`` put there; ``relu`` goes with the norm."""
+    between = getattr(model, "blocks_between", None)
+    if between is not None:
+        h = between[i](h)
+    norms = getattr(model, "norms", None)
+    return h if norms is None else norms[i](h, relu)
+
+
 class GCN(nn.Module):
-    def __init__(self, in_feats, n_hidden, n_classes, n_layers, activation, weight, dropout, dropout_seed=None):
+    def __init__(self, in_feats, n_hidden, n_classes, n_layers, activation, weight, dropout, dropout_seed=None, norm=None, feed_forward=0, keep8=False):
         super().__init__()
         self.layers = _stack(GCNConv, in_feats, n_hidden, n_classes, n_layers, weight)
         self.dropout = _between_layers(dropout, dropout_seed)
+        _add_depth(self, n_hidden, len(self.layers) - 1, norm, feed_forward, keep8)
 
     def forward(self, blocks, features, neighbor_list=[5, 10, 15]):
         h = features
         for i, layer in enumerate(self.layers):
             if i != 0:
-                h = self.dropout(h)
+                h = self.dropout(_deepened(self, i - 1, h))
             graph = blocks[i]
             dst_nodes = graph.num_dst_nodes()
             if isinstance(graph, Block):
@@ -242,16 +270,17 @@ class GINConv(_Conv):
 
 
 class GIN(nn.Module):
-    def __init__(self, in_feats, n_hidden, n_classes, n_layers, activation, weight, dropout, dropout_seed=None):
+    def __init__(self, in_feats, n_hidden, n_classes, n_layers, activation, weight, dropout, dropout_seed=None, norm=None, feed_forward=0, keep8=False):
         super().__init__()
         self.layers = _stack(GINConv, in_feats, n_hidden, n_classes, n_layers, weight)
         self.dropout = _between_layers(dropout, dropout_seed)
+        _add_depth(self, n_hidden, len(self.layers) - 1, norm, feed_forward, keep8)
 
     def forward(self, blocks, features, neighbor_list=[5, 10, 15]):
         h = features
         for i, layer in enumerate(self.layers):
             if i != 0:
-                h = self.dropout(h)
+                h = self.dropout(_deepened(self, i - 1, h))
             graph = blocks[i]
             dst_nodes = graph.num_dst_nodes()
             edge_ptr, src_edges = (graph.edge_ptr, graph.src_local) if isinstance(graph, Block) else _block_csr(graph)[:2]
@@ -565,16 +594,25 @@ _RELUS = (torch.relu, nn.functional.relu)  # what a seeded dropout takes along
 
 
 class SAGE(nn.Module):
-    def __init__(self, in_feats, n_hidden, n_classes, n_layers, activation=torch.relu, dropout=0.0, dropout_seed=None):
+    def __init__(self, in_feats, n_hidden, n_classes, n_layers, activation=torch.relu, dropout=0.0, dropout_seed=None, norm=None, feed_forward=0, keep8=False):
         super().__init__()
         dims = [in_feats] + [n_hidden] * (n_layers - 1) + [n_classes]
         self.layers = nn.ModuleList(SAGEConv(dims[i], dims[i + 1]) for i in range(n_layers))
         self.activation = activation
         self.dropout = _between_layers(dropout, dropout_seed, relu=activation in _RELUS)
         self.dropout.takes_activation = dropout_seed is not None and activation in _RELUS
+        _add_depth(self, n_hidden, len(self.layers) - 1, norm, feed_forward, keep8)
 
-    def _between(self, h):
-        """What is between two layers: the activation and the dropout, as one where that is what ``__init__`` made it."""
+    def _between(self, h, i=0):
+        """What is between layer ``i`` and the next: the activation and the dropout, as one where that is what ``__init__`` made it; before them what
+        ``_add_depth`` put there, and with a norm the activation as one with that where it can be."""
+        if getattr(self, "norms", None) is not None:
+            relu = self.activation in _RELUS
+            h = _deepened(self, i, h, relu)
+            if self.activation is not None and not relu:
+                h = self.activation(h)
+            return self.dropout(h, False) if isinstance(self.dropout, Dropout) else self.dropout(h)
+        h = _deepened(self, i, h)
         if getattr(self.dropout, "takes_activation", False):
             relu = self.activation in _RELUS  # (it may be another one by now)
             if self.activation is not None and not relu:
@@ -599,5 +637,5 @@ class SAGE(nn.Module):
             else:
                 h = layer(block, h)
             if i != len(self.layers) - 1:
-                h = self._between(h)
+                h = self._between(h, i)
         return h

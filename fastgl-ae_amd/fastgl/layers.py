@@ -120,3 +120,18 @@ class Linear(nn.Linear):
 
     def extra_repr(self):
         return super().extra_repr() + (", activation=%s" % self.activation if self.activation else "") + (", keep8=True" if self.keep8 else "")
+
+
+class FeedForward(nn.Module):
+    """``x + down(activation(up(norm(x))))``, the block that a deep model has between its aggregations: a norm and two dense layers, ``features`` to ``hidden`` and
+    back, with the activation behind the first and the residual behind the second.  ``keep8``: all three keep 8 bits a value of what their backward passes need of
+    their inputs (``x`` itself is kept by nobody: the residual's gradient is the output's)."""
+
+    def __init__(self, features, hidden, activation="gelu", eps=1e-5, keep8=False):
+        super().__init__()
+        self.norm = LayerNorm(features, eps=eps, keep8=keep8)
+        self.up = Linear(features, hidden, activation=activation, keep8=keep8)
+        self.down = Linear(hidden, features, keep8=keep8)
+
+    def forward(self, x):
+        return self.down(self.up(self.norm(x)), residual=x)

@@ -38,17 +38,20 @@ def make_dataset(n_nodes, n_draws, feat_dim, n_classes, train_frac, seed, device
     return edge_ptr, edge_src, feat, label, train_nids
 
 
-def build_model(name, in_feats, n_hidden, n_classes, n_layers, dropout, dropout_seed=None):
+def build_model(name, in_feats, n_hidden, n_classes, n_layers, dropout, dropout_seed=None, norm=None, feed_forward=0, keep8=False):
+    depth = dict(norm=norm, feed_forward=feed_forward, keep8=keep8)
     if name == "gcn":
-        return fastgl.GCN(in_feats, n_hidden, n_classes, n_layers, None, True, dropout, dropout_seed)
+        return fastgl.GCN(in_feats, n_hidden, n_classes, n_layers, None, True, dropout, dropout_seed, **depth)
     if name == "gin":
-        return fastgl.GIN(in_feats, n_hidden, n_classes, n_layers, None, True, dropout, dropout_seed)
+        return fastgl.GIN(in_feats, n_hidden, n_classes, n_layers, None, True, dropout, dropout_seed, **depth)
     if name == "gat":
+        if norm is not None or feed_forward or keep8:
+            raise ValueError("GAT has no norms or feed-forward blocks between its layers")
         if dropout_seed is not None:
             raise ValueError("GAT has no dropout between its layers")
         return fastgl.GAT(in_feats, n_hidden, n_classes, n_layers, None, dropout, heads=4)
     if name == "sage":
-        return fastgl.SAGE(in_feats, n_hidden, n_classes, n_layers, dropout=dropout, dropout_seed=dropout_seed)
+        return fastgl.SAGE(in_feats, n_hidden, n_classes, n_layers, dropout=dropout, dropout_seed=dropout_seed, **depth)
     raise ValueError("unknown model %r" % name)
 
 
@@ -65,7 +68,8 @@ def run(args):
                                      deterministic=bool(args.deterministic)).set_graph(edge_ptr, edge_src)
     # the last layer gives the classes' logits, or hidden rows that a layer of its own turns into the loss at once
     outputs = args.classes if args.head == "layer" else args.num_hidden
-    model = build_model(args.model, args.feat_dim, args.num_hidden, outputs, len(args.fanout), args.dropout, args.dropout_seed).to(device)
+    model = build_model(args.model, args.feat_dim, args.num_hidden, outputs, len(args.fanout), args.dropout, args.dropout_seed,
+                        None if args.norm == "none" else args.norm, args.feed_forward, bool(args.keep8)).to(device)
     loss_fcn = torch.nn.CrossEntropyLoss() if args.head == "layer" else fastgl.LinearCrossEntropy(args.num_hidden, args.classes).to(device)
     optimizer = torch.optim.Adam([*model.parameters(), *loss_fcn.parameters()], lr=args.lr, weight_decay=args.weight_decay)
     sync = torch.cuda.synchronize
@@ -168,6 +172,10 @@ def parse_args(argv=None):
     ap.add_argument("--head", default="layer", choices=["layer", "linear"],
                     help="linear: the model gives num_hidden columns, and fastgl.LinearCrossEntropy the loss over the classes, without the "
                          "logits in memory (for very many classes)")
+    ap.add_argument("--norm", default="none", choices=["none", "layer"], help="gcn, gin, sage: layer: a norm of the rows between the layers")
+    ap.add_argument("--feed_forward", type=int, default=0,
+                    help="gcn, gin, sage: a feed-forward block (norm, two dense layers, residual) with so many hidden columns behind every layer but the last")
+    ap.add_argument("--keep8", type=int, default=0, help="1: those norms and blocks keep 8 bits a value of their inputs for the backward pass")
     ap.add_argument("--weight_decay", type=float, default=0.0005)
     ap.add_argument("--seed", type=int, default=0)
     ap.add_argument("--id_order", default="first", choices=["first", "arrival"])
