@@ -56,16 +56,30 @@ __device__ __forceinline__ void act_apply(int act, float (&v)[N][V])
     }
 }
 
-// the derivative (not relu's, which is a bit)
-__device__ __forceinline__ float act_slope(int act, float z)
+// gelu or silu of v, and their derivatives
+template <int N, int V>
+__device__ __forceinline__ void act_with_slope(int act, float (&v)[N][V], float (&slope)[N][V])
 {
     if (act == kActGelu) {
-        float e;
-        const float p = act_normal(z, e);
-        return fmaf(z * 0.39894228040f, e, p);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int t = 0; t < V; ++t) {
+                float e;
+                const float z = v[i][t], p = act_normal(z, e);
+                slope[i][t] = fmaf(z * 0.39894228040f, e, p);
+                v[i][t] = z * p;
+            }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int t = 0; t < V; ++t) {
+                const float z = v[i][t], p = __builtin_amdgcn_rcpf(1.0f + act_exp(-z));
+                slope[i][t] = p * fmaf(z, 1.0f - p, 1.0f);
+                v[i][t] = z * p;
+            }
     }
-    const float p = __builtin_amdgcn_rcpf(1.0f + act_exp(-z));
-    return p * fmaf(z, 1.0f - p, 1.0f);
 }
 
 #endif  // __HIPCC__

@@ -209,7 +209,7 @@ static int launch_bf16_product(RowProductArgs g, hipStream_t stream)
     g.tiles_n = (int)ceil_div(g.n, 32 * NT);
     int64_t per_cu = kBpLds / (int64_t)lds;
     if (per_cu > bp_waves(NT) * 4 / W) per_cu = bp_waves(NT) * 4 / W;
-    const uint64_t starts = (uintptr_t)g.c | (uintptr_t)g.then.residual | (uintptr_t)g.then.z | (uint64_t)(g.ldc | g.then.ldr | g.then.ldz | g.n) * 2;
+    const uint64_t starts = (uintptr_t)g.c | (uintptr_t)g.then.residual | (uintptr_t)g.then.slope | (uint64_t)(g.ldc | g.then.ldr | g.then.lds | g.n) * 2;
     const int v = NT >= 4 && starts % 8 == 0 ? 4 : NT >= 2 && starts % 4 == 0 ? 2 : 1;
     g.row_blocks = sp_row_blocks(ceil_div(g.m, 64), W, (int)per_cu, g.tiles_n);
     const int64_t blocks = ceil_div(g.row_blocks, 8) * 8 * g.tiles_n;

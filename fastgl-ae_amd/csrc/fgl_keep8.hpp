@@ -61,11 +61,10 @@ constexpr uint32_t kStepNone = 255;
 __device__ __forceinline__ float k8_inverse(uint32_t step) { return __uint_as_float((254u - step) << 23); }
 __device__ __forceinline__ double k8_inverse64(uint32_t step) { return __hiloint2double((int)((1023u + 127u - step) << 20), 0); }
 
-__device__ __forceinline__ uint32_t k8_code(float steps)
-{
-    const float r = rintf(steps);
-    return (uint32_t)((int)(r > 127.0f ? 127.0f : r < -127.0f ? -127.0f : r) + 128);
-}
+// the code of v: its sum with 1.5 2^23 + 128 is rounded to a whole number, the nearest, in its lower bits (64 bits: 1.5 2^52)
+__device__ __forceinline__ uint32_t k8_clamp(int r) { return (uint32_t)(r < 1 ? 1 : r > 255 ? 255 : r); }
+__device__ __forceinline__ uint32_t k8_code(float v, float inverse) { return k8_clamp((int)__float_as_uint(fmaf(v, inverse, 0x1.8p23f + 128.0f)) - 0x4B400000); }
+__device__ __forceinline__ uint32_t k8_code(double v, double inverse) { return k8_clamp(__double2loint(fma(v, inverse, 0x1.8p52 + 128.0))); }
 
 // value of a code: two instructions (255: infinity times something minus infinity, which is no number)
 __device__ __forceinline__ float k8_value(uint32_t code, uint32_t step)

@@ -245,9 +245,7 @@ __global__ __launch_bounds__(kLnThreads, C * kLnV<T> <= 16 ? 4 : 2) void layer_n
                 LnCodes<V> codes;
 #pragma unroll
                 for (int e = 0; e < V; ++e) {
-                    // the nearest whole number, 128 more, in the lower word (what the sum with 1.5 2^52 rounds to)
-                    const int r = __double2loint(fma(h[e], inverse, 0x1.8p52 + 128.0));
-                    const uint32_t code = (uint32_t)(r < 1 ? 1 : r > 255 ? 255 : r);
+                    const uint32_t code = k8_code(h[e], inverse);
                     if (e % 4 == 0) codes[e / 4] = code;
                     else codes[e / 4] |= code << 8 * (e % 4);
                 }

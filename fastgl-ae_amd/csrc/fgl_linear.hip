@@ -2,8 +2,9 @@
 //   z = x W^T + b,   y = act(z) + residual;   dz = dy act'(z),   dx = dz W,   dW = dz^T x,   db = sum over rows of dz
 //
 // The products are fgl_row_product.hip's (fp32 on the bf16 matrix cores: fgl_split_product.hip) and fgl_wgrad.hip's; the forward one stores act(z) + residual
-// from its accumulators, and what act' will be formed from: a bit a value for relu, z itself for gelu and silu.  The backward pass forms dz in one pass over dy
-// (none where there is no activation: dz is dy).
+// from its accumulators, and act': a bit a value for relu, the slope itself for gelu and silu (in bf16 as fp16, whose eleven bits leave dz the one rounding that the
+// matrix cores ask for; z in bf16 in its place added as much again: 2-norm 2.5e-3 instead of 2.4e-3).  The backward pass forms dz in one pass over dy (none where there is no
+// activation: dz is dy).
 //
 // KEEP8: the rows of x are held in 8 bits a value (fgl_keep8.hpp) for dW, which fgl_wgrad8.hip forms from them; dx and db need no x.
 #include "fgl_activation.hpp"
@@ -13,16 +14,19 @@
 #include "fgl_row_product.hpp"
 #include "fgl_wgrad8.hpp"
 
+#include <type_traits>
+
 namespace fgl {
 
 constexpr int kLinearMost = 4096;  // columns of x and y
-constexpr int kPackRows = 64;      // of a workgroup
+constexpr int kPackRows = 16;      // of a workgroup
+constexpr int kPackLoads = 4;      // of a lane, on their way together
 
 struct LinearState {
     uint8_t* codes;  // KEEP8: [n][k8_columns(dim)]
     uint8_t* steps;  // KEEP8: [k8_columns(dim) / 32][w8_step_ld(n)]
     uint32_t* mask;  // relu: [n][mask_ld]
-    void* z;         // gelu, silu: [n][ldz] of x's type
+    void* slope;     // gelu, silu: [n][ldz] fp32, or fp16 for bf16
     int64_t mask_ld, ldz;
     size_t bytes;
 };
@@ -39,7 +43,7 @@ static LinearState linear_state(void* base, int64_t n, int dim, int out, int dty
         s.steps = c.take<uint8_t>((size_t)(k8_columns(dim) / 32) * (size_t)w8_step_ld(n));
     }
     if (act == kActRelu) s.mask = c.take<uint32_t>((size_t)n * (size_t)s.mask_ld);
-    else if (act != kActNone) s.z = c.take<uint8_t>((size_t)n * (size_t)s.ldz * (dtype == FGL_F32 ? 4 : 2));
+    else if (act != kActNone) s.slope = c.take<uint8_t>((size_t)n * (size_t)s.ldz * (dtype == FGL_F32 ? 4 : 2));
     s.bytes = c.used();
     return s;
 }
@@ -65,8 +69,8 @@ __device__ __forceinline__ LinVec<T> lin_load(const T* p, int left)
     return v;
 }
 
-// Rows in 8 bits a value.  A workgroup takes 64 rows, a lane 16 bytes of one at a time, so that 32 columns are those of 8 lanes (bf16: 4); steps are
-// gathered in LDS, since those of a column of rows are neighbours.
+// Rows in 8 bits a value.  A workgroup takes 16 rows, a lane 16 bytes of one at a time, so that 32 columns are those of 8 lanes (bf16: 4); steps are
+// gathered in LDS, since those of a column of rows are neighbours.  (64 rows a workgroup and a load at a time: 8192 x 602 fp32 25 us, XXX so, 87 K x 512 bf16 34, YYY.)
 template <typename T>
 __global__ __launch_bounds__(kBlock) void pack8_kernel(const T* __restrict__ x, int64_t ldx, int64_t n, int d, int code_ld, uint8_t* __restrict__ codes,
                                                       uint8_t* __restrict__ steps, int64_t step_ld)
@@ -77,29 +81,38 @@ __global__ __launch_bounds__(kBlock) void pack8_kernel(const T* __restrict__ x, 
     const int64_t row0 = (int64_t)blockIdx.x * kPackRows;
     const int per_row = code_ld / V, rows = n - row0 < kPackRows ? (int)(n - row0) : kPackRows;
     const int items = rows * per_row;
-    for (int i0 = 0; i0 < items; i0 += kBlock) {  // (the lanes of a group are all in or all out)
-        const int i = i0 + (int)threadIdx.x, r = i / per_row, c = (i - r * per_row) * V;
-        const bool in = i < items;
-        LinVec<T> v = lin_load(x + (row0 + r) * ldx + c, in ? d - c : 0);
-        uint32_t most = 0;
+    for (int i0 = (int)threadIdx.x; i0 - (int)threadIdx.x < items; i0 += kBlock * kPackLoads) {  // (the lanes of a group are all in or all out)
+        LinVec<T> v[kPackLoads];
+        int r[kPackLoads], c[kPackLoads];
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-            const uint32_t m = __float_as_uint((float)v[e]) & 0x7FFFFFFFu;
-            most = most > m ? most : m;
+        for (int k = 0; k < kPackLoads; ++k) {
+            const int i = i0 + k * kBlock;
+            r[k] = i / per_row;
+            c[k] = (i - r[k] * per_row) * V;
+            v[k] = lin_load(x + (row0 + r[k]) * ldx + c[k], i < items ? d - c[k] : 0);
         }
-        most = group_max<kGroup>(most) >> 23;
-        const uint32_t step = most == 0xFF ? kStepNone : k8_step((int)most - 127);
-        const float inverse = step == kStepNone ? 0.0f : k8_inverse(step);
-        Codes q;
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-            const uint32_t code = k8_code((float)v[e] * inverse);
-            if (e % 4 == 0) q[e / 4] = code;
-            else q[e / 4] |= code << 8 * (e % 4);
-        }
-        if (in) {
-            *reinterpret_cast<Codes*>(codes + (row0 + r) * code_ld + c) = q;
-            if (c % 32 == 0) s_step[c / 32][r] = (uint8_t)step;
+        for (int k = 0; k < kPackLoads; ++k) {
+            uint32_t most = 0;
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const uint32_t m = __float_as_uint((float)v[k][e]) & 0x7FFFFFFFu;
+                most = most > m ? most : m;
+            }
+            most = group_max<kGroup>(most) >> 23;
+            const uint32_t step = most == 0xFF ? kStepNone : k8_step((int)most - 127);
+            const float inverse = step == kStepNone ? 0.0f : k8_inverse(step);
+            Codes q;
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const uint32_t code = k8_code((float)v[k][e], inverse);
+                if (e % 4 == 0) q[e / 4] = code;
+                else q[e / 4] |= code << 8 * (e % 4);
+            }
+            if (i0 + k * kBlock < items) {
+                *reinterpret_cast<Codes*>(codes + (row0 + r[k]) * code_ld + c[k]) = q;
+                if (c[k] % 32 == 0) s_step[c[k] / 32][r[k]] = (uint8_t)step;
+            }
         }
     }
     __syncthreads();
@@ -110,28 +123,41 @@ __global__ __launch_bounds__(kBlock) void pack8_kernel(const T* __restrict__ x, 
     }
 }
 
-// dz = dy act'(z); rows of z and dz are ldz apart, those of dy lddy.  Lanes: 2^log_lanes neighbours take the loads of a row.
+// dz = dy act'(z); rows of the slopes and of dz are ldz apart, those of dy lddy.  2^log_lanes neighbouring lanes take the loads of a row, and a lane those of
+// kSlopeRows rows at a time.
+constexpr int kSlopeRows = 4;
+template <typename T>
+using SlopeOf = std::conditional_t<sizeof(T) == 4, float, _Float16>;
+
 template <typename T, bool MASK>
-__global__ __launch_bounds__(kBlock) void slope_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restrict__ z, const uint32_t* __restrict__ mask, int64_t mask_ld,
-                                                      int act, int64_t n, int d, int64_t ldz, T* __restrict__ dz, int log_lanes)
+__global__ __launch_bounds__(kBlock) void slope_kernel(const T* __restrict__ dy, int64_t lddy, const SlopeOf<T>* __restrict__ slope, const uint32_t* __restrict__ mask,
+                                                      int64_t mask_ld, int64_t n, int d, int64_t ldz, T* __restrict__ dz, int log_lanes)
 {
     constexpr int V = kLinV<T>;
-    const int l = (int)threadIdx.x & ((1 << log_lanes) - 1);
-    const int64_t stride = (int64_t)gridDim.x << (8 - log_lanes);
-    for (int64_t row = ((int64_t)blockIdx.x << (8 - log_lanes)) + (threadIdx.x >> log_lanes); row < n; row += stride) {
-        for (int c = l * V; c < d; c += V << log_lanes) {
-            const int left = d - c;
-            LinVec<T> g = lin_load(dy + row * lddy + c, left), q;
-            if constexpr (MASK) {
-                const uint32_t bits = mask[row * mask_ld + c / 32] >> (c % 32);
+    const int l = (int)threadIdx.x & ((1 << log_lanes) - 1), rows = kBlock >> log_lanes;
+    const int64_t first = (int64_t)blockIdx.x * rows * kSlopeRows + (threadIdx.x >> log_lanes);
+    for (int c = l * V; c < d; c += V << log_lanes) {
+        const int left = d - c;
+        LinVec<T> g[kSlopeRows];
+        LinVec<SlopeOf<T>> s[kSlopeRows];
+        uint32_t bits[kSlopeRows];
 #pragma unroll
-                for (int e = 0; e < V; ++e) q[e] = bits >> e & 1u ? g[e] : (T)0.0f;
-            } else {
-                const LinVec<T> at = lin_load(z + row * ldz + c, left);
+        for (int i = 0; i < kSlopeRows; ++i) {
+            const int64_t row = first + i * rows < n ? first + i * rows : n - 1;
+            g[i] = lin_load(dy + row * lddy + c, left);
+            if constexpr (MASK) bits[i] = mask[row * mask_ld + c / 32] >> (c % 32);
+            else s[i] = lin_load(slope + row * ldz + c, left);
+        }
 #pragma unroll
-                for (int e = 0; e < V; ++e) q[e] = (T)((float)g[e] * act_slope(act, (float)at[e]));
+        for (int i = 0; i < kSlopeRows; ++i) {
+            LinVec<T> q;
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                if constexpr (MASK) q[e] = bits[i] >> e & 1u ? g[i][e] : (T)0.0f;
+                else q[e] = (T)((float)g[i][e] * (float)s[i][e]);
             }
-            T* to = dz + row * ldz + c;
+            if (first + i * rows >= n) break;
+            T* to = dz + (first + i * rows) * ldz + c;
             if (left >= V) {
                 *reinterpret_cast<LinVec<T>*>(to) = q;
             } else {
@@ -144,17 +170,20 @@ __global__ __launch_bounds__(kBlock) void slope_kernel(const T* __restrict__ dy,
 }
 
 template <typename T>
-static void launch_slope(const void* dy, int64_t lddy, const LinearState& s, int act, int64_t n, int d, void* dz, hipStream_t stream)
+static int launch_slope(const void* dy, int64_t lddy, const LinearState& s, int act, int64_t n, int d, void* dz, hipStream_t stream)
 {
     int log_lanes = 0;
     while (log_lanes < 6 && (kLinV<T> << log_lanes) < d) ++log_lanes;
-    const int64_t want = ceil_div(n, 1 << (8 - log_lanes)), blocks = want < 8192 ? want : 8192;
+    const int64_t blocks = ceil_div(n, (int64_t)(kBlock >> log_lanes) * kSlopeRows);
+    const dim3 grid((unsigned)blocks);  // (n below 2^31, 16 rows and more a workgroup)
     if (act == kActRelu)
-        hipLaunchKernelGGL((slope_kernel<T, true>), dim3((unsigned)blocks), dim3(kBlock), 0, stream, static_cast<const T*>(dy), lddy, (const T*)nullptr, s.mask, s.mask_ld, act,
-                           n, d, s.ldz, static_cast<T*>(dz), log_lanes);
+        hipLaunchKernelGGL((slope_kernel<T, true>), grid, dim3(kBlock), 0, stream, static_cast<const T*>(dy), lddy, (const SlopeOf<T>*)nullptr, s.mask, s.mask_ld, n, d, s.ldz,
+                           static_cast<T*>(dz), log_lanes);
     else
-        hipLaunchKernelGGL((slope_kernel<T, false>), dim3((unsigned)blocks), dim3(kBlock), 0, stream, static_cast<const T*>(dy), lddy, static_cast<const T*>(s.z),
-                           (const uint32_t*)nullptr, (int64_t)0, act, n, d, s.ldz, static_cast<T*>(dz), log_lanes);
+        hipLaunchKernelGGL((slope_kernel<T, false>), grid, dim3(kBlock), 0, stream, static_cast<const T*>(dy), lddy, static_cast<const SlopeOf<T>*>(s.slope),
+                           (const uint32_t*)nullptr, (int64_t)0, n, d, s.ldz, static_cast<T*>(dz), log_lanes);
+    FGL_CHECK_LAUNCH("slope_kernel");
+    return FGL_OK;
 }
 
 // What the backward pass carves from its workspace: dz (where there is an activation), a weight gradient that nobody asked for, the weight gradient's sums
@@ -230,8 +259,8 @@ FGL_EXPORT int fgl_linear(const void* d_x, int64_t ldx, const void* d_w, int64_t
             g.then.mask = kept.mask;
             g.then.mask_ld = kept.mask_ld;
         } else if (act != kActNone) {
-            g.then.z = kept.z;
-            g.then.ldz = kept.ldz;
+            g.then.slope = kept.slope;
+            g.then.lds = kept.ldz;
         }
         if (keep8) {
             const dim3 grid((unsigned)ceil_div(n, kPackRows));
@@ -283,9 +312,8 @@ FGL_EXPORT int fgl_linear_backward(const void* d_dy, int64_t lddy, const void* d
     const void* dz = d_dy;
     int64_t lddz = lddy;
     if (act != kActNone) {
-        if (dtype == FGL_F32) launch_slope<float>(d_dy, lddy, kept, act, n, out, w.dz, s);
-        else launch_slope<__bf16>(d_dy, lddy, kept, act, n, out, w.dz, s);
-        FGL_CHECK_LAUNCH("slope_kernel");
+        const int rc = dtype == FGL_F32 ? launch_slope<float>(d_dy, lddy, kept, act, n, out, w.dz, s) : launch_slope<__bf16>(d_dy, lddy, kept, act, n, out, w.dz, s);
+        if (rc != FGL_OK) return rc;
         dz = w.dz;
         lddz = kept.ldz;
     }
@@ -299,6 +327,6 @@ FGL_EXPORT int fgl_linear_backward(const void* d_dy, int64_t lddy, const void* d
     }
     if (!sums) return FGL_OK;
     void* dw = d_dw != nullptr ? d_dw : w.dw;
-    if (keep8) return launch_wgrad8(dz, lddz, kept.codes, kept.steps, w8_step_ld(n), n, out, dim, dtype, dw, dim, d_db, w.sums, w.sums_bytes, s);
+    if (keep8) return launch_wgrad8(dz, lddz, kept.codes, kept.steps, n, out, dim, dtype, dw, dim, d_db, w.sums, w.sums_bytes, s);
     return fgl_weight_grad(dz, lddz, d_x, ldx, n, out, dim, dtype, dw, dim, d_db, w.sums, w.sums_bytes, stream);
 }

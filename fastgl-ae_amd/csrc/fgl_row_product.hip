@@ -386,7 +386,7 @@ int fgl::row_product_then(const RowProductArgs& g, bool b_transposed, int dtype,
     if (dtype == FGL_F32) return launch_row_product_any<float, true, kRpThen>(g, true, stream);
     // bf16 moves in words: see row_product
     const RowProductEpilogue& e = g.then;
-    const uint64_t starts = (uintptr_t)g.c | (uintptr_t)e.residual | (uintptr_t)e.z, strides = (uint64_t)g.n | (uint64_t)g.ldc | (uint64_t)e.ldr | (uint64_t)e.ldz;
+    const uint64_t starts = (uintptr_t)g.c | (uintptr_t)e.residual | (uintptr_t)e.slope, strides = (uint64_t)g.n | (uint64_t)g.ldc | (uint64_t)e.ldr | (uint64_t)e.lds;
     return launch_row_product_any<uint16_t, true, kRpThen>(g, starts % 4 == 0 && strides % 2 == 0, stream);
 }
 

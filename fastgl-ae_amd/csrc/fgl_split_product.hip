@@ -512,7 +512,7 @@ static int launch_split_product(RowProductArgs g, hipStream_t stream)
     // as many neighbouring columns a lane as every row's start allows
     uint64_t starts = (uintptr_t)g.c | (uint64_t)g.ldc * sizeof(float);
     if (FORM == kRpThen)  // (and of what goes with them; rows are a whole number of them too)
-        starts |= (uintptr_t)g.then.residual | (uintptr_t)g.then.z | (uint64_t)(g.then.ldr | g.then.ldz | g.n) * sizeof(float);
+        starts |= (uintptr_t)g.then.residual | (uintptr_t)g.then.slope | (uint64_t)(g.then.ldr | g.then.lds | g.n) * sizeof(float);
     g.vec_log = NT >= 4 && starts % 16 == 0 ? 2 : NT >= 2 && starts % 8 == 0 ? 1 : 0;
     g.row_blocks = sp_row_blocks(ceil_div(g.m, 32), W, (int)per_cu, g.tiles_n);
     const int64_t blocks = ceil_div(g.row_blocks, 8) * 8 * g.tiles_n;

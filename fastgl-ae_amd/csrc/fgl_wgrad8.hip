@@ -182,12 +182,13 @@ __device__ __forceinline__ int w8_column(int tile, int i, int m)
 }
 
 // Where a wave's lanes read: rows first, first + kStep, ..; col_a, col_b: the lane's first columns
-template <typename T>
+template <typename T, int VB>
 struct W8Walk {
     static constexpr int64_t kStep = 16 * (kBlock / kWave);
     const T* a;
     const uint8_t* codes;
     const uint8_t* steps;
+    int at = 0;
     int whole, last_rows;  // steps before the last one, which has so many rows of the lane's eight (none or fewer than none, it may be)
     __device__ __forceinline__ W8Walk(const Wgrad8Args& g, int64_t k0, int64_t k1, int wave, int col_a, int col_b)
     {
@@ -201,26 +202,31 @@ struct W8Walk {
         codes = g.codes + row * g.code_ld + col_b;
         steps = g.steps + (int64_t)(col_b / 32) * g.step_ld + row;
     }
-    template <int VA, int VB>
-    __device__ __forceinline__ void load(const Wgrad8Args& g, int i, W8Rows<T, VA>& ra, W8Codes<VB>& rb)
+    // the steps in order: the whole ones (at least one; after the last, that one again), the last one
+    template <int VA>
+    __device__ __forceinline__ void load(const Wgrad8Args& g, W8Rows<T, VA>& ra, W8Codes<VB>& rb)
     {
-        if (i < whole) {
-            ra.load(a, g.lda);
-            rb.load(codes, g.code_ld, steps);
-        } else {
-            const int n = i > whole ? 0 : last_rows;
-            ra.load_tail(a, g.lda, n);
-            rb.load_tail(codes, g.code_ld, steps, n);
-        }
-        a += kStep * g.lda;
-        codes += kStep * g.code_ld;
-        steps += kStep;
+        ra.load(a, g.lda);
+        rb.load(codes, g.code_ld, steps);
+        advance(g, ++at < whole ? kStep : 0);
     }
-    template <int VB>
+    template <int VA>
+    __device__ __forceinline__ void load_tail(const Wgrad8Args& g, W8Rows<T, VA>& ra, W8Codes<VB>& rb)
+    {
+        if (whole > 0) advance(g, kStep);
+        ra.load_tail(a, g.lda, last_rows);
+        rb.load_tail(codes, g.code_ld, steps, last_rows);
+    }
     __device__ __forceinline__ void load_steps(int i, W8Codes<VB>& rb)
     {
         rb.load_steps_tail(steps, i < whole ? 8 : last_rows);
         steps += kStep;
+    }
+    __device__ __forceinline__ void advance(const Wgrad8Args& g, int64_t rows)
+    {
+        a += rows * g.lda;
+        codes += rows * g.code_ld;
+        steps += rows;
     }
 };
 
@@ -228,11 +234,12 @@ struct W8Walk {
 template <int VA, int VB>
 __device__ __forceinline__ void w8_plain(const Wgrad8Args& g, int64_t k0, int64_t k1, int wave, int col_a, int col_b, W8F32x16 (&acc)[VA * VB])
 {
-    W8Walk<float> walk(g, k0, k1, wave, col_a, col_b);
+    W8Walk<float, VB> walk(g, k0, k1, wave, col_a, col_b);
     W8Rows<float, VA> a;
     W8Codes<VB> b;
     for (int i = 0; i <= walk.whole; ++i) {
-        walk.load(g, i, a, b);
+        if (i < walk.whole) walk.load(g, a, b);
+        else walk.load_tail(g, a, b);
 #pragma unroll
         for (int r = 0; r < 8; ++r)
 #pragma unroll
@@ -258,14 +265,18 @@ template <int VA, int VB>
 __device__ __forceinline__ bool w8_rows(const Wgrad8Args& g, int64_t k0, int64_t k1, int wave, int col_a, int col_b, bool sums, W8F32x16 (&acc)[VA * VB], float (&sum)[VA])
 {
     const int half = lane_id() / 32;
-    W8Walk<float> walk(g, k0, k1, wave, col_a, col_b);
+    W8Walk<float, VB> walk(g, k0, k1, wave, col_a, col_b);
     W8Rows<float, VA> a;
     W8Codes<VB> b;
     uint32_t rest[VA];
 #pragma unroll
     for (int i = 0; i < VA; ++i) rest[i] = 0;
     float sign = 1.0f;
-    walk.load(g, 0, a, b);
+    auto load = [&](int i) {
+        if (i < walk.whole) walk.load(g, a, b);
+        else walk.load_tail(g, a, b);
+    };
+    load(0);
     for (int s = 0; s <= walk.whole; ++s) {
         if (sums) a.add_columns(sum);
         SpU4 pa[VA][3], pb[VB];
@@ -277,7 +288,7 @@ __device__ __forceinline__ bool w8_rows(const Wgrad8Args& g, int64_t k0, int64_t
             for (int r = 0; r < 8; ++r) v[r] = a.r[r][i] * sign;
             sp_split<true>(v, pa[i], rest[i]);
         }
-        if (s < walk.whole) walk.load(g, s + 1, a, b);  // (on the way while these are multiplied)
+        if (s < walk.whole) load(s + 1);  // (on the way while these are multiplied)
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < VA; ++i) {
@@ -307,7 +318,7 @@ __device__ __forceinline__ bool w8_rows(const Wgrad8Args& g, int64_t k0, int64_t
     }
     if (__any(loses)) {
         // the largest value that the lane's codes may stand for, from their steps
-        W8Walk<float> again(g, k0, k1, wave, col_a, col_b);
+        W8Walk<float, VB> again(g, k0, k1, wave, col_a, col_b);
         uint32_t most = 0;
         for (int s = 0; s <= again.whole; ++s) {
             W8Codes<VB> t;
@@ -332,31 +343,43 @@ __device__ __forceinline__ bool w8_rows(const Wgrad8Args& g, int64_t k0, int64_t
     return odd;
 }
 
-// The wave's rows in bf16
-template <int VA, int VB>
-__device__ __forceinline__ void w8_rows(const Wgrad8Args& g, int64_t k0, int64_t k1, int wave, int col_a, int col_b, bool sums, W8F32x16 (&acc)[VA * VB], float (&sum)[VA],
-                                        uint16_t)
+// The wave's rows in bf16.  Steps are on their way three ahead of the one that is multiplied.  (87 K x 256 x 512: in tiles of 128 x 128, one wave a SIMD and one step ahead 65 us,
+// 128 x 64 so 53, at 10 TB/s of the L2s.)
+template <int VA, int VB, bool SUMS>
+__device__ __forceinline__ void w8_rows(const Wgrad8Args& g, int64_t k0, int64_t k1, int wave, int col_a, int col_b, W8F32x16 (&acc)[VA * VB], float (&sum)[VA])
 {
-    W8Walk<uint16_t> walk(g, k0, k1, wave, col_a, col_b);
-    W8Rows<uint16_t, VA> a, next_a;
-    W8Codes<VB> b, next_b;
-    walk.load(g, 0, a, b);
-    for (int s = 0; s <= walk.whole; ++s) {
-        if (s < walk.whole) walk.load(g, s + 1, next_a, next_b);
-        if (sums) a.add_columns(sum);
-        __builtin_amdgcn_sched_barrier(0);
-        SpU4 pb[VB];
-        b.columns(pb);
+    constexpr int kAhead = 3;
+    W8Walk<uint16_t, VB> walk(g, k0, k1, wave, col_a, col_b);
+    W8Rows<uint16_t, VA> a[kAhead];
+    W8Codes<VB> b[kAhead];
+    auto multiply = [&](const W8Rows<uint16_t, VA>& ra, const W8Codes<VB>& rb, auto&& then) {
+        if constexpr (SUMS) ra.add_columns(sum);
+        SpU4 pa[VA], pb[VB];
+        rb.columns(pb);
 #pragma unroll
-        for (int i = 0; i < VA; ++i) {
-            const Bf16x8 fa = bf16_column(a.r, i);
+        for (int i = 0; i < VA; ++i) pa[i] = __builtin_bit_cast(SpU4, bf16_column(ra.r, i));
+        then();
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < VA; ++i)
 #pragma unroll
             for (int j = 0; j < VB; ++j)
-                acc[i * VB + j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa, __builtin_bit_cast(Bf16x8, pb[j]), acc[i * VB + j], 0, 0, 0);
-        }
-        a = next_a;
-        b = next_b;
+                acc[i * VB + j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(Bf16x8, pa[i]), __builtin_bit_cast(Bf16x8, pb[j]), acc[i * VB + j], 0, 0, 0);
+    };
+    // (nothing branches around the loads: past the last whole step that one is read again, and not used)
+    if (walk.whole > 0) {
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) walk.load(g, a[u], b[u]);
+        int s = 0;
+        for (; s + kAhead <= walk.whole; s += kAhead)
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) multiply(a[u], b[u], [&] { walk.load(g, a[u], b[u]); });
+#pragma unroll
+        for (int u = 0; u + 1 < kAhead; ++u)
+            if (s + u < walk.whole) multiply(a[u], b[u], [] {});
     }
+    walk.load_tail(g, a[0], b[0]);
+    multiply(a[0], b[0], [] {});
 #pragma unroll
     for (int t = 0; t < VA * VB; ++t)  // (no branch between the last products and the first reads)
         acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(Bf16x8{}, Bf16x8{}, acc[t], 0, 0, 0);
@@ -371,7 +394,7 @@ __device__ __forceinline__ void w8_rows(const Wgrad8Args& g, int64_t k0, int64_t
 }
 
 template <typename T, int VA, int VB>
-__global__ __launch_bounds__(kBlock, VA * VB >= 16 ? 1 : 2) void wgrad8_kernel(const Wgrad8Args g)
+__global__ __launch_bounds__(kBlock, 2) void wgrad8_kernel(const Wgrad8Args g)
 {
     constexpr int kTiles = VA * VB, kChunk = kTiles < 4 ? kTiles : 4, kWaves = kBlock / kWave;
     __shared__ float s_acc[kWaves][kChunk * 16][kWave];
@@ -400,7 +423,8 @@ __global__ __launch_bounds__(kBlock, VA * VB >= 16 ? 1 : 2) void wgrad8_kernel(c
             w8_plain<VA, VB>(g, k0, k1, wave, col_a, col_b, acc);
         }
     } else {
-        w8_rows<VA, VB>(g, k0, k1, wave, col_a, col_b, sums, acc, sum, T{});
+        if (sums) w8_rows<VA, VB, true>(g, k0, k1, wave, col_a, col_b, acc, sum);
+        else w8_rows<VA, VB, false>(g, k0, k1, wave, col_a, col_b, acc, sum);
     }
     float* out = g.partial + ((int64_t)split * g.tiles + tile) * (kTiles * 16) * kWave;
 #pragma unroll
@@ -503,10 +527,10 @@ static Wgrad8Plan w8_plan(int64_t k, int m, int n, int dtype, bool vectors)
 {
     Wgrad8Plan p;
     p.va = w8_vec(m, vectors, dtype == FGL_F32 ? 2 : 4);
-    p.vb = w8_vec((int)k8_columns(n), true, dtype == FGL_F32 ? 2 : 4);
+    p.vb = w8_vec((int)k8_columns(n), true, dtype == FGL_F32 || p.va == 4 ? 2 : 4);
     p.tiles_n = (int)ceil_div(n, 32 * p.vb);
     p.tiles = p.tiles_n * (int)ceil_div(m, 32 * p.va);
-    const int per_cu = p.va * p.vb >= 16 ? 1 : dtype == FGL_F32 || p.va * p.vb >= 8 ? 2 : 4;
+    const int per_cu = dtype == FGL_F32 || p.va * p.vb >= 8 ? 2 : 4;
     int64_t splits = 256 * per_cu / p.tiles;
     const int64_t most = ceil_div(k, 256);  // 256 rows and more a split: the sum over the splits costs as much as they do otherwise
     if (splits > most) splits = most;
@@ -536,23 +560,22 @@ static void launch_wgrad8(const Wgrad8Args& g, hipStream_t stream)
     hipLaunchKernelGGL((wgrad8_reduce_kernel<T, VA, VB>), dim3((unsigned)(g.tiles * VA * VB * 16 + sum_blocks)), dim3(kBlock), 0, stream, g);
 }
 
-int launch_wgrad8(const void* a, int64_t lda, const uint8_t* codes, const uint8_t* steps, int64_t step_ld, int64_t k, int m, int n, int dtype, void* c, int64_t ldc,
-                  void* sum_a, void* ws, size_t ws_bytes, hipStream_t stream)
+int launch_wgrad8(const void* a, int64_t lda, const uint8_t* codes, const uint8_t* steps, int64_t k, int m, int n, int dtype, void* c, int64_t ldc, void* sum_a, void* ws,
+                  size_t ws_bytes, hipStream_t stream)
 {
     const Wgrad8Plan p = w8_plan(k, m, n, dtype, dtype == FGL_F32 || (m % 2 == 0 && lda % 2 == 0 && ((uintptr_t)a & 3) == 0));
     if (ws == nullptr || ws_bytes < p.ws_bytes) {
-        set_error("weight gradient of 8-bit rows: workspace too small (%zu < %zu)", ws_bytes, p.ws_bytes);
+        set_error("weight gradient: workspace too small (%zu < %zu)", ws_bytes, p.ws_bytes);
         return FGL_ERR_WORKSPACE;
     }
     Wgrad8Args g;
     memset(&g, 0, sizeof(g));
-    g.a = a; g.lda = lda; g.codes = codes; g.steps = steps; g.step_ld = step_ld; g.code_ld = (int)k8_columns(n); g.k = k; g.m = m; g.n = n;
+    g.a = a; g.lda = lda; g.codes = codes; g.steps = steps; g.step_ld = w8_step_ld(k); g.code_ld = (int)k8_columns(n); g.k = k; g.m = m; g.n = n;
     g.tiles_n = p.tiles_n; g.tiles = p.tiles; g.splits = p.splits; g.k_per_split = p.k_per_split; g.partial = static_cast<float*>(ws); g.c = c; g.ldc = ldc;
     g.sum_a = sum_a; g.partial_sum = reinterpret_cast<float*>(static_cast<char*>(ws) + p.sum_offset);
     auto wide = [&](auto type) {
         using T = decltype(type);
         if constexpr (sizeof(T) == 2) {
-            if (p.va == 4 && p.vb == 4) return launch_wgrad8<T, 4, 4>(g, stream);
             if (p.va == 4 && p.vb == 2) return launch_wgrad8<T, 4, 2>(g, stream);
             if (p.va == 4) return launch_wgrad8<T, 4, 1>(g, stream);
             if (p.va == 2 && p.vb == 4) return launch_wgrad8<T, 2, 4>(g, stream);
