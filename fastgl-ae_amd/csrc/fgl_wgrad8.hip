@@ -264,31 +264,27 @@ __device__ __forceinline__ void w8_plain(const Wgrad8Args& g, int64_t k0, int64_
 template <int VA, int VB>
 __device__ __forceinline__ bool w8_rows(const Wgrad8Args& g, int64_t k0, int64_t k1, int wave, int col_a, int col_b, bool sums, W8F32x16 (&acc)[VA * VB], float (&sum)[VA])
 {
+    constexpr int kAhead = 2;
     const int half = lane_id() / 32;
     W8Walk<float, VB> walk(g, k0, k1, wave, col_a, col_b);
-    W8Rows<float, VA> a;
-    W8Codes<VB> b;
+    W8Rows<float, VA> a[kAhead];
+    W8Codes<VB> b[kAhead];
     uint32_t rest[VA];
 #pragma unroll
     for (int i = 0; i < VA; ++i) rest[i] = 0;
     float sign = 1.0f;
-    auto load = [&](int i) {
-        if (i < walk.whole) walk.load(g, a, b);
-        else walk.load_tail(g, a, b);
-    };
-    load(0);
-    for (int s = 0; s <= walk.whole; ++s) {
-        if (sums) a.add_columns(sum);
+    auto multiply = [&](const W8Rows<float, VA>& ra, const W8Codes<VB>& rb, auto&& then) {
+        if (sums) ra.add_columns(sum);
         SpU4 pa[VA][3], pb[VB];
-        b.columns(pb);
+        rb.columns(pb);
 #pragma unroll
         for (int i = 0; i < VA; ++i) {
             float v[8];
 #pragma unroll
-            for (int r = 0; r < 8; ++r) v[r] = a.r[r][i] * sign;
+            for (int r = 0; r < 8; ++r) v[r] = ra.r[r][i] * sign;
             sp_split<true>(v, pa[i], rest[i]);
         }
-        if (s < walk.whole) load(s + 1);  // (on the way while these are multiplied)
+        then();
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < VA; ++i) {
@@ -304,7 +300,21 @@ __device__ __forceinline__ bool w8_rows(const Wgrad8Args& g, int64_t k0, int64_t
                 for (int r = 0; r < 16; ++r) acc[i * VB + j][r] = fmaf(part[j][r], sign, acc[i * VB + j][r]);
         }
         sign = -sign;
+    };
+    // (nothing branches around the loads: past the last whole step that one is read again, and not used)
+    if (walk.whole > 0) {
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) walk.load(g, a[u], b[u]);
+        int s = 0;
+        for (; s + kAhead <= walk.whole; s += kAhead)
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) multiply(a[u], b[u], [&] { walk.load(g, a[u], b[u]); });
+#pragma unroll
+        for (int u = 0; u + 1 < kAhead; ++u)
+            if (s + u < walk.whole) multiply(a[u], b[u], [] {});
     }
+    walk.load_tail(g, a[0], b[0]);
+    multiply(a[0], b[0], [] {});
     bool odd = false;
 #pragma unroll
     for (int t = 0; t < VA * VB; ++t)
