@@ -93,6 +93,24 @@ def test_rows_far_from_zero(cuda):
     check(x, w, b, dy, 1e-5, False, False, y, torch.autograd.grad(y, (x, w, b), dy))
 
 
+def test_offsets_beyond_32_bits(cuda):
+    n, d = (1 << 32) // 512 + 37, 512
+    x = torch.empty((n, d), device=cuda, dtype=torch.bfloat16).normal_().requires_grad_()
+    w, b = torch.randn(d, device=cuda).bfloat16().requires_grad_(), torch.randn(d, device=cuda).bfloat16().requires_grad_()
+    y = fastgl.layer_norm(x, w, b, relu=True, keep8=True)
+    dy = torch.zeros((n, d), device=cuda, dtype=torch.bfloat16)
+    some = torch.cat([torch.arange(40), torch.arange(n - 90, n)]).to(cuda)
+    dy[some] = torch.randn((130, d), device=cuda).bfloat16()
+    g = torch.autograd.grad(y, (x, w, b), dy)
+    xs = x.detach()[some].clone().requires_grad_()
+    ys = fastgl.layer_norm(xs, w, b, relu=True, keep8=True)
+    assert torch.equal(ys, y[some])
+    s = torch.autograd.grad(ys, (xs, w, b), dy[some])
+    assert torch.equal(s[0], g[0][some]) and not g[0][100:1000].any()
+    for p, q in zip(g[1:], s[1:]):  # (sums in another order, each rounded)
+        assert torch.allclose(p.float(), q.float(), rtol=2.0 ** -7, atol=2.0 ** -7)
+
+
 def test_constant_rows_and_no_eps(cuda):
     x = torch.full((6, 40), 3.5, device=cuda, requires_grad=True)
     w, b = torch.randn(40, device=cuda), torch.randn(40, device=cuda)
@@ -136,7 +154,7 @@ def test_any_shape_order_and_gradients_from_views(cuda):
     x, w, b, dy = problem(cuda, 24, 36, torch.float32)
     y = fastgl.layer_norm(x, w, b, relu=True)
     g = torch.autograd.grad(y, (x, w, b), dy)
-    for view in (x.detach().view(2, 3, 4, 36), x.detach().t().contiguous().t()):
+    for view in (x.detach().view(2, 3, 4, 36), x.detach().t().contiguous().t()):  # (another order is copied)
         v = view.requires_grad_()
         z = fastgl.layer_norm(v, w, b, relu=True)
         assert z.shape == v.shape and torch.equal(z.reshape(24, 36), y)

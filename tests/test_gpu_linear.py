@@ -104,6 +104,58 @@ def test_values_and_gradients(cuda, dtype, act, keep8, n, d, out):
         assert torch.equal(fastgl.linear(x, w, b, activation=act, residual=r), y)
 
 
+# bf16 with the weights kept on the CUs, from 8192 rows on: columns and lanes at the ends of tiles, vectors and pairs, k at the ends of a piece of 8 and a chunk of 64, and as
+# long as 128, 64 and 32 columns of weights have room
+@pytest.mark.parametrize("act", [None, "relu", "gelu"])
+@pytest.mark.parametrize("n,d,out", [(8192, 16, 64), (8193, 17, 129), (10_000, 47, 33), (8255, 64, 30), (8999, 640, 128), (8200, 641, 132), (9000, 1216, 62), (8192, 1217, 60), (8300, 2400, 24),
+                                     (8321, 72, 260), (9999, 128, 127), (70_001, 24, 68), (8192, 4096, 8), (8193, 15, 40)])
+def test_many_rows_in_bf16(cuda, act, n, d, out):
+    x, w, b, r, dy = problem(cuda, n, d, out, torch.bfloat16, True, out % 4 != 1, stride=d + d % 2 + 2 * (n % 2))
+    y = fastgl.linear(x, w, b, activation=act, residual=r)
+    check(x, w, b, r, dy, act, False, y, torch.autograd.grad(y, [t for t in (x, w, b, r) if t is not None], dy))
+
+
+def test_offsets_beyond_32_bits(cuda):
+    n = (1 << 32) // 256 + 70
+    w, b = torch.randn((256, 16), device=cuda).bfloat16().requires_grad_(), torch.randn(256, device=cuda).bfloat16().requires_grad_()
+    x = torch.randn((n, 16), device=cuda).bfloat16().requires_grad_()
+    y = fastgl.linear(x, w, b, "relu", keep8=True)
+    d = torch.zeros((n, 256), device=cuda, dtype=torch.bfloat16)
+    some = torch.cat([torch.arange(40), torch.arange(n - 90, n)]).to(cuda)
+    d[some] = torch.randn((130, 256), device=cuda).bfloat16()
+    gx, gw, gb = torch.autograd.grad(y, (x, w, b), d)
+    xs = x.detach()[some].clone().requires_grad_()
+    ys = fastgl.linear(xs, w, b, "relu", keep8=True)
+    assert torch.equal(ys, y[some])
+    sx, sw, sb = torch.autograd.grad(ys, (xs, w, b), d[some])
+    assert torch.equal(sx, gx[some]) and not gx[100:1000].any()
+    for p, q in ((gw, sw), (gb, sb)):  # (sums in another order, each rounded)
+        assert torch.allclose(p.float(), q.float(), rtol=2.0 ** -7, atol=2.0 ** -7)
+
+
+def test_from_several_threads_on_streams_of_their_own(cuda):
+    import threading
+
+    x, w, b, r, dy = problem(cuda, 9000, 100, 130, torch.float32, True, True)
+    step = lambda: (lambda y: (y.detach(), *torch.autograd.grad(y, (x, w, b, r), dy)))(fastgl.linear(x, w, b, "gelu", r, keep8=True))  # noqa: E731
+    want = step()
+    torch.cuda.synchronize()
+    results = [None] * 4
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            out = [step() for _ in range(5)]
+            torch.cuda.current_stream().synchronize()
+        results[i] = out
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert all(torch.equal(p, q) for out in results for one in out for p, q in zip(one, want))
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("act", [None, "relu", "silu"])
 @pytest.mark.parametrize("keep8", [False, True])
@@ -142,6 +194,24 @@ def test_any_shape_order_and_gradients_from_views(cuda):
             z = fastgl.linear(e, w, b, "gelu", keep8=keep8)
             ge = torch.autograd.grad(z, (e, w, b), torch.zeros((0, 33), device=cuda, dtype=dtype))
             assert z.shape == (0, 33) and ge[0].shape == (0, 35) and not ge[1].any() and not ge[2].any()
+
+
+def test_gradients_are_those_of_differences(cuda):
+    """y along a direction, forward by two steps in 64 bits of the formula's arguments, against the gradient's product with it."""
+    for act in ("gelu", "silu"):
+        x, w, b, r, dy = problem(cuda, 40, 30, 20, torch.float32, True, True)
+        y = fastgl.linear(x, w, b, act, r)
+        grads = torch.autograd.grad(y, (x, w, b, r), dy)
+        for i, t in enumerate((x, w, b, r)):
+            v = torch.randn_like(t)
+            h = 2.0 ** -8
+            moved = [[u.detach() + (s * h * v if j == i else 0) for j, u in enumerate((x, w, b, r))] for s in (1, -1)]
+            up, down = (fastgl.linear(m[0], m[1], m[2], act, m[3]).double() for m in moved)
+            slope, want = float(((up - down) / (2 * h) * dy).sum()), float((grads[i].double() * v).sum())
+            # rounding: 2^-24 of values below 8 over 2 h, 800 of them times dy; the third derivative (below 2) times h^2 / 6
+            size = float(dy.abs().sum())
+            third = 2 * h * h / 6 * size * float((v.abs().max() * (1 + w.abs().sum(1).max())) ** 3)
+            assert abs(slope - want) < 8 * 2.0 ** -24 / h * size + third
 
 
 @pytest.mark.parametrize("keep8", [False, True])
