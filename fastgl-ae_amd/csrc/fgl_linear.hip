@@ -70,7 +70,7 @@ __device__ __forceinline__ LinVec<T> lin_load(const T* p, int left)
 }
 
 // Rows in 8 bits a value.  A workgroup takes 16 rows, a lane 16 bytes of one at a time, so that 32 columns are those of 8 lanes (bf16: 4); steps are
-// gathered in LDS, since those of a column of rows are neighbours.  (64 rows a workgroup and a load at a time: 8192 x 602 fp32 25 us, XXX so, 87 K x 512 bf16 34, YYY.)
+// gathered in LDS, since those of a column of rows are neighbours.  (64 rows a workgroup and a load at a time: 8192 x 602 fp32 25 us, 8 so, 87 K x 512 bf16 34, 28.)
 template <typename T>
 __global__ __launch_bounds__(kBlock) void pack8_kernel(const T* __restrict__ x, int64_t ldx, int64_t n, int d, int code_ld, uint8_t* __restrict__ codes,
                                                       uint8_t* __restrict__ steps, int64_t step_ld)

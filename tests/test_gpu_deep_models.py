@@ -105,7 +105,8 @@ def test_what_is_kept(cuda):
         y.sum().backward()
         del y, block
     # the norm's output and the activation's in full, or 33 / 32 bytes a value of them and of the normed rows; a bit a value of the hidden ones for relu, 12 or 4 bytes a row
-    assert kept[0] < n * (4 * d + 4 * hidden + hidden // 8 + 12) * 1.02 and kept[1] < n * ((2 * d + hidden) * 33 // 32 + hidden // 8 + 4) * 1.02
+    # (torch's allocator hands out cached blocks up to 1 MiB larger than what is asked for as they are; five of them are kept at most)
+    assert kept[0] < n * (4 * d + 4 * hidden + hidden // 8 + 12) + 5 * 2 ** 20 and kept[1] < n * ((2 * d + hidden) * 33 // 32 + hidden // 8 + 4) + 5 * 2 ** 20
     assert kept[1] < 0.4 * kept[0]
 
 

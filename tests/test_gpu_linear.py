@@ -104,11 +104,11 @@ def test_values_and_gradients(cuda, dtype, act, keep8, n, d, out):
         assert torch.equal(fastgl.linear(x, w, b, activation=act, residual=r), y)
 
 
-# bf16 with the weights kept on the CUs, from 8192 rows on: columns and lanes at the ends of tiles, vectors and pairs, k at the ends of a piece of 8 and a chunk of 64, and as
+# bf16 with the weights kept on the CUs, from 3.3 M outputs on (and 100 K rows where k is short): columns and lanes at the ends of tiles, vectors and pairs, k at the ends of a piece of 8 and a chunk of 64, and as
 # long as 128, 64 and 32 columns of weights have room
 @pytest.mark.parametrize("act", [None, "relu", "gelu"])
-@pytest.mark.parametrize("n,d,out", [(8192, 16, 64), (8193, 17, 129), (10_000, 47, 33), (8255, 64, 30), (8999, 640, 128), (8200, 641, 132), (9000, 1216, 62), (8192, 1217, 60), (8300, 2400, 24),
-                                     (8321, 72, 260), (9999, 128, 127), (70_001, 24, 68), (8192, 4096, 8), (8193, 15, 40)])
+@pytest.mark.parametrize("n,d,out", [(100_000, 16, 64), (100_193, 17, 129), (120_000, 47, 33), (110_255, 64, 30), (26_999, 640, 128), (20_200, 641, 132), (26_000, 1216, 62), (26_192, 1217, 60),
+                                     (26_300, 2400, 24), (12_321, 96, 260), (26_999, 128, 127), (50_001, 104, 68), (60_000, 512, 256), (30_000, 4096, 8), (26_193, 15, 40), (140_001, 100, 40)])
 def test_many_rows_in_bf16(cuda, act, n, d, out):
     x, w, b, r, dy = problem(cuda, n, d, out, torch.bfloat16, True, out % 4 != 1, stride=d + d % 2 + 2 * (n % 2))
     y = fastgl.linear(x, w, b, activation=act, residual=r)
