@@ -2,7 +2,7 @@
 //   h = (x - mean) / sqrt(var + eps),   y = h w + b,   relu: y = max(y, 0)
 //   g = dy [y > 0] w,   dx = (g - mean(g) - h mean(g h)) / sqrt(var + eps),   dw = sum over rows of dy [y > 0] h,   db = sum of dy [y > 0]
 //
-// One pass over the rows each way: 4, 16 or 64 lanes hold a row in registers, 16 bytes a lane and load, so a wave has 16, 4 or one of them; sums
+// One pass over the rows each way: 4 (fp32: 8), 16 or 64 lanes hold a row in registers, 16 bytes a lane and load, so a wave has 16 (8), 4 or one of them; sums
 // over a row are exchanges between its lanes.  In the backward pass a lane adds up dw and db of its columns over all rows that its wave takes, a
 // workgroup those of its waves through LDS, and a second launch those of the workgroups, in a fixed order.
 //
@@ -12,7 +12,9 @@
 //
 // For the backward pass a row leaves its mean (64 bits) and 1 / sqrt (32), with relu a bit a value, and with KEEP8 h in 8 bits a value in x's place.
 //
-// What bounds it: the pass over memory.
+// What bounds it: the pass over memory.  us forward / back (and 4 .. 7 for the second launch): 60 K x 256 fp32 22 / 37 (5.6 and 4.9 TB/s; relu in it), 87 K x 256 bf16 with relu and KEEP8
+// 27 / 26, where codes and relu's decision take as long as the memory forward, 2.4 M x 64 fp32 of rows of 100 columns with KEEP8 325 / 262.  Rows that do not begin on 16 bytes cost
+// loads and stores across lines: 200 K x 602 bf16 137 / 191, 600 columns 107 / 161.
 #include "fgl_common.hpp"
 #include "fgl_keep8.hpp"
 #include "fgl_kernels.hpp"
