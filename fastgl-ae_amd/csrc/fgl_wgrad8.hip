@@ -14,9 +14,9 @@
 // step those of A's negative, since it is cut downwards.  Rows past the end are zeros on both sides.  Where a value of A has bits below 2^-133, bf16's last, that a sum is not
 // large beside, or a sum is no number, a workgroup forms its rows again in fp32 instructions.
 //
-// What bounds it: in fp32 the vector unit (per step of 64 x 64: 88 instructions split A, 64 make the codes' operands, 64 add the products to the accumulators, beside 12 matrix
-// instructions of 32 cycles), in bf16 the L2s, from which every tile takes its rows.  us with the second launch: 107 K x 100 x 256 fp32 51 (from rows in full, fgl_wgrad.hip, 70), one step
-// ahead instead of two 59; 8192 x 602 x 256 fp32 33; 87 K x 512 x 256 bf16 58.
+// What bounds it: in fp32 the vector unit (a step of 32 x 128: 44 instructions split A, 104 make the codes' operands, 64 add the products to the accumulators, beside 12 matrix
+// instructions of 32 cycles) and the L2s, from which every tile takes its rows, in bf16 those.  us with the second launch: 107 K x 100 x 256 fp32 47 (from rows in full, fgl_wgrad.hip,
+// 65; one step ahead instead of two 59, tiles of 64 x 64 52), 8192 x 602 x 256 fp32 30; 87 K x 512 x 256 bf16 52 (tiles of 128 x 64 58).
 #include "fgl_common.hpp"
 #include "fgl_keep8.hpp"
 #include "fgl_kernels.hpp"
@@ -357,8 +357,8 @@ __device__ __forceinline__ bool w8_rows(const Wgrad8Args& g, int64_t k0, int64_t
     return odd;
 }
 
-// The wave's rows in bf16.  Steps are on their way three ahead of the one that is multiplied.  (87 K x 256 x 512: in tiles of 128 x 128, one wave a SIMD and one step ahead 65 us,
-// 128 x 64 so 53, at 10 TB/s of the L2s.)
+// The wave's rows in bf16.  Steps are on their way three ahead of the one that is multiplied.  (87 K x 512 x 256: in tiles of 128 x 128, one wave a SIMD and one step ahead, 65 us,
+// 128 x 64 so 53, 64 x 128 47.)
 template <int VA, int VB, bool SUMS>
 __device__ __forceinline__ void w8_rows(const Wgrad8Args& g, int64_t k0, int64_t k1, int wave, int col_a, int col_b, W8F32x16 (&acc)[VA * VB], float (&sum)[VA])
 {
@@ -540,8 +540,9 @@ struct Wgrad8Plan {
 static Wgrad8Plan w8_plan(int64_t k, int m, int n, int dtype, bool vectors)
 {
     Wgrad8Plan p;
-    p.va = w8_vec(m, vectors, dtype == FGL_F32 ? 2 : 4);
-    p.vb = w8_vec((int)k8_columns(n), true, dtype == FGL_F32 || p.va == 4 ? 2 : 4);
+    // codes are the fewer bytes: a tile is wide in them, and narrow in A where both could be
+    p.vb = w8_vec((int)k8_columns(n), true, 4);
+    p.va = w8_vec(m, vectors, dtype == FGL_F32 ? (p.vb == 4 ? 1 : 2) : (p.vb == 4 ? 2 : 4));
     p.tiles_n = (int)ceil_div(n, 32 * p.vb);
     p.tiles = p.tiles_n * (int)ceil_div(m, 32 * p.va);
     const int per_cu = dtype == FGL_F32 || p.va * p.vb >= 8 ? 2 : 4;
@@ -593,8 +594,8 @@ int launch_wgrad8(const void* a, int64_t lda, const uint8_t* codes, const uint8_
             if (p.va == 4 && p.vb == 2) return launch_wgrad8<T, 4, 2>(g, stream);
             if (p.va == 4) return launch_wgrad8<T, 4, 1>(g, stream);
             if (p.va == 2 && p.vb == 4) return launch_wgrad8<T, 2, 4>(g, stream);
-            if (p.vb == 4) return launch_wgrad8<T, 1, 4>(g, stream);
         }
+        if (p.vb == 4) return launch_wgrad8<T, 1, 4>(g, stream);
         if (p.va == 2 && p.vb == 2) return launch_wgrad8<T, 2, 2>(g, stream);
         if (p.va == 2) return launch_wgrad8<T, 2, 1>(g, stream);
         if (p.vb == 2) return launch_wgrad8<T, 1, 2>(g, stream);
