@@ -193,3 +193,121 @@ def test_training_by_the_command(cuda, model, tmp_path):
     assert all(x == x and x < 1e3 for x in losses)
     with pytest.raises(ValueError):
         train.build_model("gat", 8, 8, 4, 2, 0.0, None, "layer")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n", [1, 15, 17, 700, 13_001])
+def test_memory_that_held_something_else(cuda, dtype, n):
+    """States, workspaces and outputs come from torch's cache with whatever was there: not a number in all of it changes nothing."""
+    torch.manual_seed(n)
+    block = fastgl.FeedForward(100, 260, keep8=True).to(cuda).to(dtype)
+    x = torch.randn((n, 100), device=cuda).to(dtype).requires_grad_()
+    d = torch.randn((n, 100), device=cuda).to(dtype)
+    step = lambda: (lambda y: [y.detach(), *torch.autograd.grad(y, [x, *block.parameters()], d)])(block(x))  # noqa: E731
+    runs = []
+    for fill in (0.0, float("nan"), 3e38):
+        torch.cuda.synchronize()
+        torch.cuda.empty_cache()
+        held = [torch.full((size,), fill, device=cuda) for size in (1 << 26, 1 << 17, 1 << 17, 1 << 17, 100, 100, 100, 100)]
+        del held
+        runs.append(step())
+    assert all(torch.equal(p, q) for r in runs[1:] for p, q in zip(runs[0], r)) and all(t.isfinite().all() for t in runs[0])
+
+
+def test_nothing_is_written_past_the_outputs(cuda):
+    from fastgl import _lib as L
+
+    lib = L.lib()
+    for dtype, code in ((torch.float32, 0), (torch.bfloat16, 1)):
+        for n, d, out in ((1, 1, 1), (37, 47, 33), (130, 64, 96), (2500, 100, 130), (26_000, 130, 128)):
+            size = torch.finfo(dtype).bits // 8
+            even = d + d % 2
+            x = torch.zeros((n, even), device=cuda, dtype=dtype)
+            w = torch.randn((out, even), device=cuda).to(dtype)
+            x[:, :d] = torch.randn((n, d), device=cuda).to(dtype)
+            dy = torch.randn((n, out + out % 2), device=cuda).to(dtype)
+
+            def guarded(count, of=dtype):
+                t = torch.full((count + 256,), 7.0, device=cuda, dtype=of) if of != torch.uint8 else torch.full((count + 4096,), 77, device=cuda, dtype=of)
+                return t
+
+            for act in (0, 1, 2):
+                for keep8 in (0, 1):
+                    state_bytes = lib.fgl_linear_state_bytes(n, d, out, code, act, keep8)
+                    ws_bytes = lib.fgl_linear_workspace_bytes(n, d, out, code, act, keep8, 1, 1)
+                    y, dx, dw, db = guarded(n * out), guarded(n * d), guarded(out * d), guarded(out)
+                    state, ws = guarded(state_bytes, torch.uint8), guarded(ws_bytes, torch.uint8)
+                    L.check(lib.fgl_linear(x.data_ptr(), even, w.data_ptr(), even, None, None, 0, n, d, out, code, act, keep8, y.data_ptr(), out, state.data_ptr(), state_bytes,
+                                           L.stream_handle()))
+                    L.check(lib.fgl_linear_backward(dy.data_ptr(), out + out % 2, x.data_ptr(), even, w.data_ptr(), even, n, d, out, code, act, keep8, state.data_ptr(), state_bytes,
+                                                    dx.data_ptr(), d, dw.data_ptr(), db.data_ptr(), ws.data_ptr(), ws_bytes, L.stream_handle()))
+                    for t, used in ((y, n * out), (dx, n * d), (dw, out * d), (db, out)):
+                        assert (t[used:] == 7.0).all() and t[:used].isfinite().all()
+                    assert (state[state_bytes:] == 77).all() and (ws[ws_bytes:] == 77).all()
+            for relu in (0, 1):
+                for keep8 in (0, 1):
+                    state_bytes, ws_bytes = lib.fgl_layer_norm_state_bytes(n, d, relu, keep8), lib.fgl_layer_norm_workspace_bytes(n, d, code)
+                    y, dx, dw, db = guarded(n * d), guarded(n * d), guarded(d), guarded(d)
+                    state, ws = guarded(state_bytes, torch.uint8), guarded(ws_bytes, torch.uint8)
+                    L.check(lib.fgl_layer_norm(x.data_ptr(), even, None, None, n, d, code, 1e-5, relu, keep8, y.data_ptr(), state.data_ptr(), state_bytes, L.stream_handle()))
+                    L.check(lib.fgl_layer_norm_backward(x.data_ptr(), even, x.data_ptr(), even, None, n, d, code, relu, keep8, state.data_ptr(), state_bytes, dx.data_ptr(),
+                                                        dw.data_ptr(), db.data_ptr(), ws.data_ptr(), ws_bytes, L.stream_handle()))
+                    for t, used in ((y, n * d), (dx, n * d), (dw, d), (db, d)):
+                        assert (t[used:] == 7.0).all() and t[:used].isfinite().all()
+                    assert (state[state_bytes:] == 77).all() and (ws[ws_bytes:] == 77).all()
+
+
+def test_compiled_modules(cuda):
+    """The compiler breaks its graph at the kernels' calls and makes them as they are."""
+    torch.manual_seed(4)
+    block = fastgl.FeedForward(48, 96).to(cuda)
+    x = torch.randn((300, 48), device=cuda, requires_grad=True)
+    d = torch.randn_like(x)
+    y = block(x)
+    want = torch.autograd.grad(y, [x, *block.parameters()], d)
+    z = torch.compile(block, backend="eager")(x)
+    got = torch.autograd.grad(z, [x, *block.parameters()], d)
+    assert torch.equal(y, z) and all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+def test_computed_anew_for_the_backward_pass(cuda):
+    from torch.utils.checkpoint import checkpoint
+
+    torch.manual_seed(5)
+    block = fastgl.FeedForward(48, 96, keep8=True).to(cuda)
+    x = torch.randn((300, 48), device=cuda, requires_grad=True)
+    d = torch.randn_like(x)
+    want = torch.autograd.grad(block(x), [x, *block.parameters()], d)
+    y = checkpoint(block, x, use_reentrant=False)
+    got = torch.autograd.grad(y, [x, *block.parameters()], d)
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+def test_two_captured_steps(cuda):
+    """Two graphs of steps over the same parameters, replayed in turn with eager steps in between."""
+    torch.manual_seed(6)
+    block = fastgl.FeedForward(64, 128, keep8=True).to(cuda)
+    inputs = [torch.randn((n, 64), device=cuda, requires_grad=True) for n in (300, 5000)]
+    grads = [torch.randn_like(t) for t in inputs]
+    step = lambda i: (lambda y: [y.detach(), *torch.autograd.grad(y, [inputs[i], *block.parameters()], grads[i])])(block(inputs[i]))  # noqa: E731
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for i in range(2):
+            step(i)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, outs = [], []
+    for i in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(step(i))
+        graphs.append(g)
+    for turn in range(3):
+        with torch.no_grad():
+            for t in inputs:
+                t.copy_(torch.randn(t.shape, generator=torch.Generator(device=cuda).manual_seed(turn), device=cuda))
+        for i in (turn % 2, 1 - turn % 2):
+            graphs[i].replay()
+        torch.cuda.synchronize()
+        for i in range(2):
+            assert all(torch.equal(p, q) for p, q in zip(outs[i], step(i)))
