@@ -8,7 +8,7 @@
 // What bounds it: for short k and few columns the pass over A and C (2.4 M x 64 x 100 164 us, 4.8 TB/s), beyond that the loads' latency, with as many rows on their way as the
 // registers hold: the matrix cores are busy for a fifth to a quarter of the time (87 K x 512 x 256 45 us, 0.51 PFLOP/s; the old kernel of fgl_row_product.hip 67).
 //
-// k past the end: a lane's eight k begin where they would or eight before the end of the row, and B's image is zero for those that an eight before has.
+// k past the end: a lane's eight k begin where they would or eight before the end of the row, and those that an eight before has are zero on both sides.
 // Rows past the end repeat the last one and are not stored, nor are columns past the end, which repeat the last one too.  No access leaves the operands.
 #include "fgl_common.hpp"
 #include "fgl_kernels.hpp"
@@ -26,6 +26,35 @@ constexpr int bp_steps(int k, int nt) { return nt <= 2 && k > 64 && k <= 128 ? 8
 __device__ __host__ __forceinline__ int bp_chunks(int k, int steps) { return (k + 16 * steps - 1) / (16 * steps); }
 // Where the eight k of number `oct` are read
 __device__ __forceinline__ int bp_first(int oct, int k) { return 8 * oct + 8 <= k ? 8 * oct : k - 8; }
+
+// Of a row's last S steps, how many are whole whatever the row
+constexpr int bp_whole(int steps) { return steps == 8 ? 4 : 0; }
+
+// Clears what of a row's last S steps, from number `step` on, an eight before has: infinite, it would make a zero of B's image no number.  One step at most has
+// both, of which a lane's eight are those from `again` on.
+template <int VA, int S>
+__device__ __forceinline__ void bp_own(SpU4 (&a)[VA][S], int step, int half, int k)
+{
+    const int mixed = k / 16 - step;
+#pragma unroll
+    for (int s = bp_whole(S); s < S; ++s) {
+        if (s < mixed) continue;
+        if (s > mixed) {
+#pragma unroll
+            for (int i = 0; i < VA; ++i) a[i][s] = SpU4{};
+            continue;
+        }
+        int oct = 2 * (step + s) + half;
+        asm volatile("" : "+v"(oct));  // (what is made of it is not kept over the rows)
+        const int again = 8 * oct - bp_first(oct, k);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t own = again <= 2 * j ? 0xFFFFFFFFu : again == 2 * j + 1 ? 0xFFFF0000u : 0u;
+#pragma unroll
+            for (int i = 0; i < VA; ++i) a[i][s][j] &= own;
+        }
+    }
+}
 
 // (the lanes' columns: fgl_split_product.hip)
 __device__ __forceinline__ int bp_column(int vl, int t, int i) { return ((t >> vl) << (5 + vl)) + (i << vl) + (t & ((1 << vl) - 1)); }
@@ -132,6 +161,7 @@ __global__ __launch_bounds__(W * kWave, bp_waves(VA, NT, S)) void bf16_product_k
     const int64_t row_tiles = (g.m + 32 * VA - 1) / (32 * VA), stride = g.row_blocks * W;
     if (rb * W >= row_tiles) return;  // (uniform over the workgroup: no row tile for it)
     const int k = g.side[0].k, chunks = bp_chunks(k, S);
+    const bool ragged = k % (16 * S) != 0;
     const int64_t lda = g.side[0].lda;
     int64_t tile = rb * W + wave, ahead = tile;
     int at = 0;
@@ -178,6 +208,7 @@ __global__ __launch_bounds__(W * kWave, bp_waves(VA, NT, S)) void bf16_product_k
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int s = 0; s < S; ++s) {
+                if (s == bp_whole(S) && ragged && c == chunks - 1) bp_own<VA, S>(cur, S * c, half, k);
                 SpU4 b[NT];
 #pragma unroll
                 for (int t = 0; t < NT; ++t) b[t] = img[(s * NT + t) * kWave];

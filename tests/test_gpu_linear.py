@@ -237,6 +237,30 @@ def test_values_that_are_no_numbers(cuda, keep8):
         assert not gw[:, ~columns].isfinite().any()
 
 
+@pytest.mark.parametrize("n", [300, 27_000])
+@pytest.mark.parametrize("d", [96, 100, 129, 250])
+def test_infinite_values_in_bf16(cuda, n, d):
+    """A row with one infinite value is infinite by its weights' signs, wherever in the row that is, and its gradient's by theirs."""
+    x, w, b, r, dy = problem(cuda, n, d, 130, torch.bfloat16, True, False)
+    x, dy, w = x.detach().clone(), dy.clone(), w.detach().clone()
+    w[w.abs() < 2.0 ** -10] = 0.5
+    places = [(0, d - 1), (1, d - 2), (70, d - 8), (133, 0), (n - 1, d - 5)]
+    for row, c in places:
+        x[row, c] = float("inf")
+        dy[row, 130 - d + c if c > d - 10 else 0] = float("-inf")
+    x.requires_grad_()
+    y = fastgl.linear(x, w, b)
+    z = fastgl.linear(x, w, b, "relu")
+    gx, = torch.autograd.grad(y, x, dy)
+    bad = torch.zeros(n, dtype=torch.bool, device=cuda)
+    for row, c in places:
+        assert torch.equal(y[row].float(), float("inf") * w[:, c].sign().float())
+        assert torch.equal(z[row].float(), torch.where(w[:, c] > 0, float("inf"), 0.0))
+        assert torch.equal(gx[row].float(), float("-inf") * w[130 - d + c if c > d - 10 else 0].sign().float())
+        bad[row] = True
+    assert y[~bad].isfinite().all() and gx[~bad].isfinite().all()
+
+
 @pytest.mark.parametrize("act", [None, "silu"])
 def test_magnitudes_that_have_no_three_parts(cuda, act):
     """Gradients below 2^-110 and rows of zeros beside large ones, kept in 8 bits: each sum to its own terms' precision."""
