@@ -1,5 +1,5 @@
 // Rows held in 8 bits a value for a backward pass.  32 neighbouring columns of a row share a step, a power of two:
-//   step = 2^(max(floor(log2(largest magnitude)), -120) - 6),   code = clamp(nearest whole number to v / step, -127, 127) + 128
+//   step = 2^(max(floor(log2(largest magnitude)), -120) - 6),   code = clamp(nearest whole number to v / step, -127, 127), a signed byte
 // so a value is off by half a step, 2^-7 of its neighbours' largest at most (by a whole one where that lies in the last half step below a power of
 // two).  A step is held as the exponent of an fp32 value, 255 where one of the 32 is infinite or not a number; all of them are not a number then.
 //
@@ -61,17 +61,21 @@ constexpr uint32_t kStepNone = 255;
 __device__ __forceinline__ float k8_inverse(uint32_t step) { return __uint_as_float((254u - step) << 23); }
 __device__ __forceinline__ double k8_inverse64(uint32_t step) { return __hiloint2double((int)((1023u + 127u - step) << 20), 0); }
 
-// the code of v: its sum with 1.5 2^23 + 128 is rounded to a whole number, the nearest, in its lower bits (64 bits: 1.5 2^52)
+// the code of v plus 128: its sum with 1.5 2^23 + 128 is rounded to a whole number, the nearest, in its lower bits (64 bits: 1.5 2^52).  Four of them at a time become signed
+// bytes by their upper bits.
+constexpr uint32_t kSigned = 0x80808080u;
 __device__ __forceinline__ uint32_t k8_clamp(int r) { return (uint32_t)(r < 1 ? 1 : r > 255 ? 255 : r); }
 __device__ __forceinline__ uint32_t k8_code(float v, float inverse) { return k8_clamp((int)__float_as_uint(fmaf(v, inverse, 0x1.8p23f + 128.0f)) - 0x4B400000); }
 __device__ __forceinline__ uint32_t k8_code(double v, double inverse) { return k8_clamp(__double2loint(fma(v, inverse, 0x1.8p52 + 128.0))); }
 
-// value of a code: two instructions (255: infinity times something minus infinity, which is no number)
-__device__ __forceinline__ float k8_value(uint32_t code, uint32_t step)
+// the step that an exponent stands for, exactly (255: no number, which infinity times zero is)
+__device__ __forceinline__ float k8_step_value(uint32_t step)
 {
     const float s = __uint_as_float(step << 23);
-    return fmaf((float)code, s, s * -128.0f);
+    return fmaf(s, 0.0f, s);
 }
+// code number c of a word, exactly.  Signed bytes, so that a value is one product: next to the largest finite values 128 steps, which an offset would take off, are infinite.
+__device__ __forceinline__ float k8_code_value(uint32_t word, int c) { return (float)(int)__builtin_amdgcn_sbfe((int)word, 8 * c, 8); }
 
 #endif  // __HIPCC__
 

@@ -251,6 +251,7 @@ __global__ __launch_bounds__(kLnThreads, C * kLnV<T> <= 16 ? 4 : 2) void layer_n
                     if (e % 4 == 0) codes[e / 4] = code;
                     else codes[e / 4] |= code << 8 * (e % 4);
                 }
+                codes ^= kSigned;
                 if (mine && c < g.code_ld) {
                     *reinterpret_cast<LnCodes<V>*>(g.state.codes + row * g.code_ld + c) = codes;
                     if (l % kGroup == 0) g.state.steps[row * (g.code_ld / 32) + c / 32] = (uint8_t)step;
@@ -310,7 +311,7 @@ __global__ __launch_bounds__(kLnThreads, C * kLnV<T> <= 16 ? 4 : 2) void layer_n
 #pragma unroll
             for (int e = 0; e < V; ++e) {
                 const bool there = ln_there<WHOLE>(j < ln_inside(G, C), e, g.d - (j * G + l) * V);
-                if constexpr (KEEP8) h[j][e] = there ? k8_value(codes[j][e / 4] >> 8 * (e % 4) & 0xFFu, step[j]) : 0.0f;
+                if constexpr (KEEP8) h[j][e] = there ? k8_code_value(codes[j][e / 4], e % 4) * k8_step_value(step[j]) : 0.0f;
                 else h[j][e] = there ? (float)((double)(float)vx[j][e] - mean) * rstd : 0.0f;
                 const float d = bits[j] >> e & 1u ? (float)vd[j][e] : 0.0f;
                 // (rows past the end leave dw as it is, also where the last one's h is no number)

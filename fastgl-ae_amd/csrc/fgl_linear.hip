@@ -111,6 +111,7 @@ __global__ __launch_bounds__(kBlock) void pack8_kernel(const T* __restrict__ x, 
                 if (e % 4 == 0) q[e / 4] = code;
                 else q[e / 4] |= code << 8 * (e % 4);
             }
+            q ^= kSigned;
             if (i0 + k * kBlock < items) {
                 *reinterpret_cast<Codes*>(codes + (row0 + r[k]) * code_ld + c[k]) = q;
                 if (c[k] % 32 == 0) s_step[c[k] / 32][r[k]] = (uint8_t)step;

@@ -7,7 +7,7 @@
 // workgroups by a second launch in a fixed order.
 //
 // A code times its step is a bf16 value, so there is nothing to split on that side: fp32 takes three products, of A's three bf16 parts (fgl_split.hpp), instead of six.
-// A code becomes one in two and a half instructions: byte to float, one multiply-add, two of them rounded to bf16 (exactly) at a time.
+// A code becomes one in two and a half instructions: byte to float, one product, two of them rounded to bf16 (exactly) at a time.
 // Steps lie by columns, so that a lane has those of its eight rows with one load.
 //
 // fp32: a step's products are added up from zero before they go to the accumulators, as what a matrix instruction adds is cut to 26 bits of its largest term; every other
@@ -154,24 +154,21 @@ struct W8Codes {
         if (n < 4) steps[0] &= n <= 0 ? 0u : (1u << 8 * n) - 1u;
         if (n < 8) steps[1] &= n <= 4 ? 0u : (1u << 8 * (n - 4)) - 1u;
     }
-    __device__ __forceinline__ float value(int i, int c) const { return k8_value(r[i] >> 8 * c & 0xFFu, steps[i / 4] >> 8 * (i % 4) & 0xFFu); }
+    __device__ __forceinline__ float value(int i, int c) const { return k8_code_value(r[i], c) * k8_step_value(steps[i / 4] >> 8 * (i % 4) & 0xFFu); }
     // column c of the eight rows, as the matrix instruction's operand
     __device__ __forceinline__ void columns(SpU4 (&to)[V]) const
     {
-        float s[8], least[8];
+        float s[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            s[i] = __uint_as_float((steps[i / 4] >> 8 * (i % 4) & 0xFFu) << 23);
-            least[i] = s[i] * -128.0f;
-        }
+        for (int i = 0; i < 8; ++i) s[i] = k8_step_value(steps[i / 4] >> 8 * (i % 4) & 0xFFu);
 #pragma unroll
         for (int c = 0; c < V; ++c)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 typedef __bf16 B2 __attribute__((ext_vector_type(2)));
                 B2 h;
-                h[0] = (__bf16)fmaf((float)(r[2 * j] >> 8 * c & 0xFFu), s[2 * j], least[2 * j]);
-                h[1] = (__bf16)fmaf((float)(r[2 * j + 1] >> 8 * c & 0xFFu), s[2 * j + 1], least[2 * j + 1]);
+                h[0] = (__bf16)(k8_code_value(r[2 * j], c) * s[2 * j]);
+                h[1] = (__bf16)(k8_code_value(r[2 * j + 1], c) * s[2 * j + 1]);
                 to[c][j] = __builtin_bit_cast(uint32_t, h);
             }
     }
