@@ -505,9 +505,10 @@ __global__ __launch_bounds__(kBlock) void wgrad8_reduce_kernel(const Wgrad8Args 
     // accumulator register r of lane l: row 8 (r / 4) + 4 (l / 32) + r % 4, column l % 32 of its 32x32 tile
     const int r = reg % 16, t = reg / 16;
     const int row = 8 * (r / 4) + 4 * (lane / 32) + r % 4;
-    const int mm = w8_column<VA>(tile / g.tiles_n, row, g.m) + t / VB;
+    const int own_m = (tile / g.tiles_n * 32 + row) * VA, mm = w8_column<VA>(tile / g.tiles_n, row, g.m) + t / VB;
     const int nn = (tile % g.tiles_n * 32 + lane % 32) * VB + t % VB;
     if (nn >= g.n) return;  // (columns of the codes that fill up a step's 32, and repeated ones)
+    if (mm < own_m) return;  // (repeated columns of A: one may be another tile's, whose sum has other bits where only one of the two formed its rows again)
     if constexpr (sizeof(T) == 4) static_cast<float*>(g.c)[(int64_t)mm * g.ldc + nn] = s;
     else static_cast<__bf16*>(g.c)[(int64_t)mm * g.ldc + nn] = (__bf16)s;
 }
