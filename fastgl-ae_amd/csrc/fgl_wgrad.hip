@@ -38,8 +38,9 @@
 // 128 x 128 through LDS, in which every value is split once (65 us for the first of these, but 34 and 41 for 256 x 256 and 602 x
 // 256), and two steps ahead, for which the registers do not suffice (89).
 //
-// A lane whose columns would leave the row takes the row's last VA columns instead (its sums are then bit-equal copies of
-// its neighbour's); rows past the end are replaced by zeros.  No access leaves the operands.
+// A lane whose columns would leave the row takes the row's last VA columns instead, of which those that are its neighbour's are not
+// stored (the neighbour may be another tile's, and of two tiles one alone may form its rows again); rows past the end are replaced by
+// zeros.  No access leaves the operands.
 #include "fgl_common.hpp"
 #include "fgl_kernels.hpp"
 #include "fgl_split.hpp"
@@ -493,8 +494,9 @@ __global__ __launch_bounds__(kBlock) void wgrad_reduce_kernel(const WgradArgs g)
     // accumulator register r of lane l: row 8 (r / 4) + 4 (l / 32) + r % 4, column l % 32 of its 32x32 tile
     const int r = reg % 16, t = reg / 16;
     const int row = 8 * (r / 4) + 4 * (lane / 32) + r % 4;
-    const int mm = wgrad_column<VA>(tile / g.tiles_n, row, g.m) + t / VB;
-    const int nn = wgrad_column<VB>(tile % g.tiles_n, lane % 32, g.n) + t % VB;
+    const int own_m = (tile / g.tiles_n * 32 + row) * VA, mm = wgrad_column<VA>(tile / g.tiles_n, row, g.m) + t / VB;
+    const int own_n = (tile % g.tiles_n * 32 + lane % 32) * VB, nn = wgrad_column<VB>(tile % g.tiles_n, lane % 32, g.n) + t % VB;
+    if (mm < own_m || nn < own_n) return;
     if constexpr (sizeof(T) == 4) static_cast<float*>(g.c)[(int64_t)mm * g.ldc + nn] = s;
     else static_cast<__bf16*>(g.c)[(int64_t)mm * g.ldc + nn] = (__bf16)s;
 }

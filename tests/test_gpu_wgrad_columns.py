@@ -10,7 +10,7 @@ pytestmark = pytest.mark.gpu
 
 
 @pytest.mark.parametrize("odd", [float("inf"), 2.0 ** -130])
-@pytest.mark.parametrize("keep8,n,d,out,side", [(True, 4000, 64, 193, "out"), (True, 9001, 96, 129, "out")])
+@pytest.mark.parametrize("keep8,n,d,out,side", [(True, 4000, 64, 193, "out"), (True, 9001, 96, 129, "out"), (False, 4000, 64, 193, "out"), (False, 4000, 193, 64, "in")])
 def test_a_column_is_its_own_tiles(cuda, keep8, n, d, out, side, odd):
     """Columns before the last one, beside a last one that is formed again, have the bits that they have beside one that is not."""
     gen = torch.Generator(device=cuda).manual_seed(n + d + out)
