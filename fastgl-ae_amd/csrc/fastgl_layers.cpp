@@ -203,7 +203,7 @@ std::tuple<Tensor, Tensor, Tensor> linear_gradients(const Tensor& d_y, const Ten
         const int dtype = type_of(w);
         const Tensor weights = as_rows(w, false);
         Tensor rows, ws;
-        if (x.defined() && (need_w || need_b)) rows = as_rows(x, even);
+        if (x.defined() && need_w) rows = as_rows(x, even);
         const size_t ws_bytes = fgl_linear_workspace_bytes(n, (int)dim, (int)out, dtype, (int)act, keep8, need_w, need_b);
         if (ws_bytes > 0) ws = bytes_like(w, ws_bytes);
         ok(fgl_linear_backward(g.data_ptr(), row_stride(g, out), address(rows), rows.defined() ? row_stride(rows, dim) : 0, weights.data_ptr(), row_stride(weights, dim), n,
@@ -231,16 +231,16 @@ TORCH_LIBRARY_FRAGMENT(fastgl, m)
 struct LinearNode : torch::autograd::Function<LinearNode> {
     static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Maybe& bias, const Maybe& residual, LinearSizes z)
     {
-        const bool sums = w.requires_grad() || (bias.has_value() && bias->requires_grad());
-        z.keep8 = z.keep8 && sums;  // (nothing else reads x)
+        const bool keep8 = z.keep8, sums = w.requires_grad();  // (nothing but the weight's gradient reads x)
+        z.keep8 = keep8 && sums;
         const bool kept = z.keep8 || z.act != 0;
         auto [y, state] = form_linear(x, w, bias.value_or(Tensor()), residual.value_or(Tensor()), z, kept);
         ctx->saved_data["dim"] = (int64_t)z.dim;
         ctx->saved_data["act"] = (int64_t)z.act;
-        ctx->saved_data["keep8"] = z.keep8;
+        ctx->saved_data["keep8"] = keep8;
         ctx->saved_data["bias"] = bias.has_value();
         ctx->saved_data["residual"] = residual.has_value();
-        ctx->save_for_backward({sums && !z.keep8 ? x : Tensor(), w, state});
+        ctx->save_for_backward({sums && !keep8 ? x : Tensor(), w, state});
         return y;
     }
 

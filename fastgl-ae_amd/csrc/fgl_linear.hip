@@ -6,10 +6,12 @@
 // matrix cores ask for: gradients off by 2.4e-3 in the 2-norm, results rounded once alone by 1.7e-3; with z kept in bf16 2.5e-3).  The backward pass forms dz in one pass over dy
 // (none where there is no activation: dz is dy).
 //
-// KEEP8: the rows of x are held in 8 bits a value (fgl_keep8.hpp) for dW, which fgl_wgrad8.hip forms from them; dx and db need no x.
+// KEEP8: the rows of x are held in 8 bits a value (fgl_keep8.hpp) for dW, which fgl_wgrad8.hip forms from them; dx and db need no x.  db comes with dW, or alone from
+// fgl_column_sums.hip (60 K x 256 fp32 17 us, where dW with it takes 82).
 //
 // What bounds it: the products (their files say); dz the pass over memory (2.4 M x 64 bf16 173 us, 5.3 TB/s; 107 K x 256 fp32 60 us, 5.5 TB/s), and so the rows in 8 bits.
 #include "fgl_activation.hpp"
+#include "fgl_column_sums.hpp"
 #include "fgl_common.hpp"
 #include "fgl_keep8.hpp"
 #include "fgl_kernels.hpp"
@@ -25,10 +27,10 @@ constexpr int kPackRows = 16;      // of a workgroup
 constexpr int kPackLoads = 4;      // of a lane, on their way together
 
 struct LinearState {
-    uint8_t* codes;  // KEEP8: [n][k8_columns(dim)]
-    uint8_t* steps;  // KEEP8: [k8_columns(dim) / 32][w8_step_ld(n)]
     uint32_t* mask;  // relu: [n][mask_ld]
     void* slope;     // gelu, silu: [n][ldz] fp32, or fp16 for bf16
+    uint8_t* codes;  // KEEP8, behind those, which are all that there is without it: [n][k8_columns(dim)]
+    uint8_t* steps;  // KEEP8: [k8_columns(dim) / 32][w8_step_ld(n)]
     int64_t mask_ld, ldz;
     size_t bytes;
 };
@@ -40,12 +42,12 @@ static LinearState linear_state(void* base, int64_t n, int dim, int out, int dty
     memset(&s, 0, sizeof(s));
     s.mask_ld = (out + 31) / 32;
     s.ldz = (out + 1) / 2 * 2;
+    if (act == kActRelu) s.mask = c.take<uint32_t>((size_t)n * (size_t)s.mask_ld);
+    else if (act != kActNone) s.slope = c.take<uint8_t>((size_t)n * (size_t)s.ldz * (dtype == FGL_F32 ? 4 : 2));
     if (keep8) {
         s.codes = c.take<uint8_t>((size_t)n * (size_t)k8_columns(dim));
         s.steps = c.take<uint8_t>((size_t)(k8_columns(dim) / 32) * (size_t)w8_step_ld(n));
     }
-    if (act == kActRelu) s.mask = c.take<uint32_t>((size_t)n * (size_t)s.mask_ld);
-    else if (act != kActNone) s.slope = c.take<uint8_t>((size_t)n * (size_t)s.ldz * (dtype == FGL_F32 ? 4 : 2));
     s.bytes = c.used();
     return s;
 }
@@ -189,13 +191,17 @@ static int launch_slope(const void* dy, int64_t lddy, const LinearState& s, int 
     return FGL_OK;
 }
 
-// What the backward pass carves from its workspace: dz (where there is an activation), a weight gradient that nobody asked for, the weight gradient's sums
+// What the backward pass carves from its workspace: dz (where there is an activation), the sums of the weight's gradient, or of the bias's alone
 struct LinearWorkspace {
     void* dz;
-    void* dw;
     void* sums;
     size_t sums_bytes, bytes;
 };
+// The bias's gradient is the one that it has beside the weight's
+static ColumnSplit linear_column_split(int64_t n, int dim, int out, int dtype, bool keep8)
+{
+    return keep8 ? wgrad8_column_split(n, out, dim, dtype) : wgrad_column_split(n, out, dim, dtype);
+}
 static LinearWorkspace linear_workspace(void* base, int64_t n, int dim, int out, int dtype, int act, bool keep8, bool need_w, bool need_b)
 {
     Carver c(base);
@@ -203,9 +209,9 @@ static LinearWorkspace linear_workspace(void* base, int64_t n, int dim, int out,
     memset(&w, 0, sizeof(w));
     const size_t size = dtype == FGL_F32 ? 4 : 2;
     if (act != kActNone) w.dz = c.take<uint8_t>((size_t)n * (size_t)((out + 1) / 2 * 2) * size);
-    if (need_b && !need_w) w.dw = c.take<uint8_t>((size_t)dim * (size_t)out * size);
     if (need_w || need_b) {
-        w.sums_bytes = keep8 ? wgrad8_workspace_bytes(n, out, dim, dtype) : fgl_weight_grad_workspace_bytes_for(n, out, dim, dtype);
+        if (!need_w) w.sums_bytes = column_sums_workspace_bytes(linear_column_split(n, dim, out, dtype, keep8), out);
+        else w.sums_bytes = keep8 ? wgrad8_workspace_bytes(n, out, dim, dtype) : fgl_weight_grad_workspace_bytes_for(n, out, dim, dtype);
         w.sums = c.take<uint8_t>(w.sums_bytes);
     }
     w.bytes = c.used();
@@ -286,7 +292,7 @@ FGL_EXPORT int fgl_linear_backward(const void* d_dy, int64_t lddy, const void* d
     FGL_REQUIRE(linear_sizes(n, dim, out, dtype, act) && n >= 1, "linear_backward: %lld rows of %d by %d columns, dtype %d, activation %d", (long long)n, dim, out, dtype, act);
     const bool sums = d_dw != nullptr || d_db != nullptr;
     if (d_dx == nullptr && !sums) return FGL_OK;
-    FGL_REQUIRE(d_dy != nullptr && (d_dx == nullptr || d_w != nullptr) && (!sums || keep8 || d_x != nullptr), "linear_backward: null pointer");
+    FGL_REQUIRE(d_dy != nullptr && (d_dx == nullptr || d_w != nullptr) && (d_dw == nullptr || keep8 || d_x != nullptr), "linear_backward: null pointer");
     if (act == kActNone) {  // (dy is an operand itself then)
         FGL_LINEAR_ROWS(d_dy, lddy, out);
     } else {
@@ -294,13 +300,14 @@ FGL_EXPORT int fgl_linear_backward(const void* d_dy, int64_t lddy, const void* d
     }
     FGL_REQUIRE(d_dx == nullptr || (ldw >= dim && lddx >= dim && ldw < (1 << 24) && lddx < (1 << 24)), "linear_backward: row strides %lld and %lld of %d columns", (long long)ldw,
                 (long long)lddx, dim);
-    if (sums && !keep8) {
+    if (d_dw != nullptr && !keep8) {
         FGL_LINEAR_ROWS(d_x, ldx, dim);
     }
     LinearState kept;
     memset(&kept, 0, sizeof(kept));
-    if (keep8 || act != kActNone) {
-        kept = linear_state(const_cast<void*>(d_state), n, dim, out, dtype, act, keep8 != 0);
+    const bool codes = keep8 && d_dw != nullptr;  // (nothing else reads them)
+    if (codes || act != kActNone) {
+        kept = linear_state(const_cast<void*>(d_state), n, dim, out, dtype, act, codes);
         if (d_state == nullptr || state_bytes < kept.bytes || ((uintptr_t)d_state & 255) != 0) {
             set_error("linear_backward: state of %zu bytes at a multiple of 256 bytes, %zu given", kept.bytes, state_bytes);
             return FGL_ERR_WORKSPACE;
@@ -329,7 +336,7 @@ FGL_EXPORT int fgl_linear_backward(const void* d_dy, int64_t lddy, const void* d
         if (rc != FGL_OK) return rc;
     }
     if (!sums) return FGL_OK;
-    void* dw = d_dw != nullptr ? d_dw : w.dw;
-    if (keep8) return launch_wgrad8(dz, lddz, kept.codes, kept.steps, n, out, dim, dtype, dw, dim, d_db, w.sums, w.sums_bytes, s);
-    return fgl_weight_grad(dz, lddz, d_x, ldx, n, out, dim, dtype, dw, dim, d_db, w.sums, w.sums_bytes, stream);
+    if (d_dw == nullptr) return launch_column_sums(dz, lddz, n, out, dtype, linear_column_split(n, dim, out, dtype, keep8 != 0), d_db, w.sums, w.sums_bytes, s);
+    if (keep8) return launch_wgrad8(dz, lddz, kept.codes, kept.steps, n, out, dim, dtype, d_dw, dim, d_db, w.sums, w.sums_bytes, s);
+    return fgl_weight_grad(dz, lddz, d_x, ldx, n, out, dim, dtype, d_dw, dim, d_db, w.sums, w.sums_bytes, stream);
 }

@@ -41,6 +41,7 @@
 // A lane whose columns would leave the row takes the row's last VA columns instead, of which those that are its neighbour's are not
 // stored (the neighbour may be another tile's, and of two tiles one alone may form its rows again); rows past the end are replaced by
 // zeros.  No access leaves the operands.
+#include "fgl_column_sums.hpp"
 #include "fgl_common.hpp"
 #include "fgl_kernels.hpp"
 #include "fgl_split.hpp"
@@ -576,6 +577,13 @@ static bool wgrad_split_pays(int64_t k, int m, int n)
 static bool wgrad_vectors(int dtype, int cols, int64_t ld, const void* ptr)
 {
     return dtype == FGL_F32 || (cols % 2 == 0 && ld % 2 == 0 && ((uintptr_t)ptr & 3) == 0);
+}
+
+ColumnSplit wgrad_column_split(int64_t k, int m, int n, int dtype)
+{
+    const bool f32 = dtype == FGL_F32, split = f32 && wgrad_split_pays(k, m, n);
+    const WgradPlan p = wgrad_plan(k, m, n, f32 || m % 2 == 0, f32 || n % 2 == 0, split);
+    return {p.splits, p.k_per_split, f32 && !split};
 }
 
 template <typename T, int VA, int VB, bool SPLIT>

@@ -17,6 +17,7 @@
 // What bounds it: in fp32 the vector unit (a step of 32 x 128: 44 instructions split A, 104 make the codes' operands, 64 add the products to the accumulators, beside 12 matrix
 // instructions of 32 cycles) and the L2s, from which every tile takes its rows, in bf16 those.  us with the second launch: 107 K x 100 x 256 fp32 47 (from rows in full, fgl_wgrad.hip,
 // 65; one step ahead instead of two 59, tiles of 64 x 64 52), 8192 x 602 x 256 fp32 30; 87 K x 512 x 256 bf16 52 (tiles of 128 x 64 58).
+#include "fgl_column_sums.hpp"
 #include "fgl_common.hpp"
 #include "fgl_keep8.hpp"
 #include "fgl_kernels.hpp"
@@ -562,6 +563,12 @@ size_t wgrad8_workspace_bytes(int64_t k, int m, int n, int dtype)
 {
     const size_t a = w8_plan(k, m, n, dtype, true).ws_bytes, b = w8_plan(k, m, n, dtype, false).ws_bytes;
     return a > b ? a : b;
+}
+
+ColumnSplit wgrad8_column_split(int64_t k, int m, int n, int dtype)
+{
+    const Wgrad8Plan p = w8_plan(k, m, n, dtype, dtype == FGL_F32 || m % 2 == 0);
+    return {p.splits, p.k_per_split, false};
 }
 
 template <typename T, int VA, int VB>

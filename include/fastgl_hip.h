@@ -500,7 +500,8 @@ int fgl_layer_norm_backward(const void* d_dy, int64_t lddy, const void* d_x, int
  * d_state: what the backward pass needs, fgl_linear_state_bytes, at a multiple of 256 bytes (for relu a bit a value, for gelu and silu the derivative, fp32 or beside bf16 fp16; keep8
  * not zero: the rows of x in 8 bits a value, as fgl_layer_norm keeps its own); NULL if there will be none.
  * Backward: dz = dy act'(z), rounded to `dtype`; dx = dz W, dw = dz^T x (of the values that are held, with keep8: x may be NULL then), db = sums of dz over
- * rows.  dx (row stride lddx), dw [out, dim] and db [out] may each be NULL; the residual's gradient is dy.  The state may be read by several backward passes.
+ * rows, the same bits with dw and without.  dx (row stride lddx), dw [out, dim] and db [out] may each be NULL; the residual's gradient is dy.  Without dw neither x nor what keep8
+ * holds of it is read: x may be NULL, and the state one of a forward pass without keep8.  The state may be read by several backward passes.
  * The same bits on every run.
  * ------------------------------------------------------------------------------- */
 size_t fgl_linear_state_bytes(int64_t n, int dim, int out, int dtype, int act, int keep8);
