@@ -94,7 +94,7 @@ def linear(x, weight, bias=None, activation=None, residual=None, keep8=False):
     Sums are float32, and the output is rounded once (a float32 sum that an infinite value takes part in may be no number: values are multiplied in parts); in the backward pass the gradient behind the activation is rounded to the type once more.
     For the backward pass ``weight`` is kept, ``x`` if ``weight`` has a gradient (no other reads it), and for ``"relu"`` a bit a value, for ``"gelu"`` and ``"silu"`` their derivatives (float32, or float16 beside bfloat16).  ``keep8=True``: in ``x``'s place
     8 bits a value of it, as ``layer_norm`` holds them: ``weight``'s gradient is that of the values so held, all others are not touched by it.
-    Under autocast, its type is taken, which must be one of the two.  No gradients of gradients.  Under tracing, forward-mode differentiation, transforms of ``torch.func`` and modes
+    Under autocast, its type is taken, which must be one of the two, for the residual and the output too.  No gradients of gradients.  Under tracing, forward-mode differentiation, transforms of ``torch.func`` and modes
     that follow the operators: by torch's operators, with nothing kept in 8 bits."""
     if not all(isinstance(t, torch.Tensor) and t.is_cuda for t in (x, weight)) or not all(t is None or (isinstance(t, torch.Tensor) and t.is_cuda) for t in (bias, residual)):
         raise RuntimeError("x, weight, bias and residual must be CUDA tensors")
@@ -124,7 +124,8 @@ class Linear(nn.Linear):
 class FeedForward(nn.Module):
     """``x + down(activation(up(norm(x))))``, the block that a deep model has between its aggregations: a norm and two dense layers, ``features`` to ``hidden`` and
     back, with the activation behind the first and the residual behind the second.  ``keep8``: all three keep 8 bits a value of what their backward passes need of
-    their inputs (``x`` itself is kept by nobody: the residual's gradient is the output's)."""
+    their inputs (``x`` itself is kept by nobody: the residual's gradient is the output's).
+    Under autocast ``x`` keeps its type, as beside torch's modules: what is added to rows of another type than autocast's is added by an operator of its own."""
 
     def __init__(self, features, hidden, activation="gelu", eps=1e-5, keep8=False):
         super().__init__()
@@ -133,4 +134,7 @@ class FeedForward(nn.Module):
         self.down = Linear(hidden, features, keep8=keep8)
 
     def forward(self, x):
-        return self.down(self.up(self.norm(x)), residual=x)
+        h = self.up(self.norm(x))
+        if torch.is_autocast_enabled() and x.dtype != torch.get_autocast_dtype("cuda"):
+            return x + self.down(h)
+        return self.down(h, residual=x)
