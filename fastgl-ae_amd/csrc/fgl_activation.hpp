@@ -11,6 +11,10 @@
 
 namespace fgl {
 
+// Derivatives are kept in fp16 beside bf16 values, times 2^15: they are at most 1.13, and so have eleven bits down to 2^-29 (silu's at -23) and are off by 2^-40 at
+// most below that.
+constexpr float kSlopeScale = 0x1p15f;
+
 constexpr int kActNone = 0, kActRelu = 1, kActGelu = 2, kActSilu = 3;
 
 #if defined(__HIPCC__)

@@ -2,7 +2,7 @@
 //   z = x W^T + b,   y = act(z) + residual;   dz = dy act'(z),   dx = dz W,   dW = dz^T x,   db = sum over rows of dz
 //
 // The products are fgl_row_product.hip's (fp32 on the bf16 matrix cores: fgl_split_product.hip) and fgl_wgrad.hip's; the forward one stores act(z) + residual
-// from its accumulators, and act': a bit a value for relu, the slope itself for gelu and silu (in bf16 as fp16, whose eleven bits leave dz with the one rounding that the
+// from its accumulators, and act': a bit a value for relu, the slope itself for gelu and silu (in bf16 as fp16, whose eleven bits, down to 2^-29, leave dz with the one rounding that the
 // matrix cores ask for: gradients off by 2.4e-3 in the 2-norm, results rounded once alone by 1.7e-3; with z kept in bf16 2.5e-3).  The backward pass forms dz in one pass over dy
 // (none where there is no activation: dz is dy).
 //
@@ -28,7 +28,7 @@ constexpr int kPackLoads = 4;      // of a lane, on their way together
 
 struct LinearState {
     uint32_t* mask;  // relu: [n][mask_ld]
-    void* slope;     // gelu, silu: [n][ldz] fp32, or fp16 for bf16
+    void* slope;     // gelu, silu: [n][ldz] fp32, or fp16 times kSlopeScale for bf16
     uint8_t* codes;  // KEEP8, behind those, which are all that there is without it: [n][k8_columns(dim)]
     uint8_t* steps;  // KEEP8: [k8_columns(dim) / 32][w8_step_ld(n)]
     int64_t mask_ld, ldz;
@@ -159,7 +159,7 @@ __global__ __launch_bounds__(kBlock) void slope_kernel(const T* __restrict__ dy,
 #pragma unroll
             for (int e = 0; e < V; ++e) {
                 if constexpr (MASK) q[e] = bits[i] >> e & 1u ? g[i][e] : (T)0.0f;
-                else q[e] = (T)((float)g[i][e] * (float)s[i][e]);
+                else q[e] = (T)((float)g[i][e] * ((float)s[i][e] * (sizeof(T) == 4 ? 1.0f : 1.0f / kSlopeScale)));
             }
             if (first + i * rows >= n) break;
             T* to = dz + (first + i * rows) * ldz + c;

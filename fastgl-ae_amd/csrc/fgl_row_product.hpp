@@ -19,7 +19,7 @@ struct RowProductEpilogue {
     int act;               // kActNone ..
     const void* residual;  // (may be null) of C's sizes
     int64_t ldr;
-    void* slope;           // (may be null) gelu, silu: the derivative, fp32 or, where C is bf16, fp16
+    void* slope;           // (may be null) gelu, silu: the derivative, fp32 or, where C is bf16, fp16 times kSlopeScale
     int64_t lds;
     uint32_t* mask;        // (may be null) relu: bit c % 32 of word c / 32 of a row
     int64_t mask_ld;       // words a row
@@ -100,7 +100,7 @@ __device__ __forceinline__ void rp_store(T* p, const float (&v)[VB])
     }
 }
 
-// V values as words of memory: fp32, bf16, or (KIND 1) derivatives beside bf16, fp16
+// V values as words of memory: fp32, bf16, or (KIND 1) derivatives beside bf16, fp16 times kSlopeScale
 template <typename T, int V, int KIND>
 struct RpWords {
     static constexpr int kWords = sizeof(T) == 4 ? V : (V + 1) / 2;
@@ -115,8 +115,9 @@ struct RpWords {
 #pragma unroll
             for (int t = 0; t < V; t += 2) {
                 E2 h;
-                h[0] = (E)v[t];
-                h[1] = (E)v[t + 1 < V ? t + 1 : t];
+                const float scale = KIND == 1 ? kSlopeScale : 1.0f;
+                h[0] = (E)(v[t] * scale);
+                h[1] = (E)(v[t + 1 < V ? t + 1 : t] * scale);
                 w[t / 2] = __builtin_bit_cast(uint32_t, h);
             }
         }

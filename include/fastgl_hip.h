@@ -497,7 +497,7 @@ int fgl_layer_norm_backward(const void* d_dy, int64_t lddy, const void* d_x, int
  * to the result): z = x W^T + bias, y = act(z) + residual, for n rows x [n, dim] and W [out, dim] of `dtype`, 1 <= dim, out <= 4096, n < 2^31.
  * act: 0 none, 1 relu (z <= 0 ? 0 : z), 2 gelu (z times the normal distribution function of z), 3 silu (z / (1 + exp(-z))).  bias [out], residual [n, out]: may be
  * NULL.  bf16: rows of x and W (and, without an activation, of dy) start on 4-byte boundaries; strides below 2^24.
- * d_state: what the backward pass needs, fgl_linear_state_bytes, at a multiple of 256 bytes (for relu a bit a value, for gelu and silu the derivative, fp32 or beside bf16 fp16; keep8
+ * d_state: what the backward pass needs, fgl_linear_state_bytes, at a multiple of 256 bytes (for relu a bit a value, for gelu and silu the derivative, fp32 or beside bf16 fp16 times 2^15; keep8
  * not zero: the rows of x in 8 bits a value, as fgl_layer_norm keeps its own); NULL if there will be none.
  * Backward: dz = dy act'(z), rounded to `dtype`; dx = dz W, dw = dz^T x (of the values that are held, with keep8: x may be NULL then), db = sums of dz over
  * rows, the same bits with dw and without.  dx (row stride lddx), dw [out, dim] and db [out] may each be NULL; the residual's gradient is dy.  Without dw neither x nor what keep8
