@@ -91,7 +91,7 @@ def linear(x, weight, bias=None, activation=None, residual=None, keep8=False):
     """``activation(x weight^T + bias) + residual`` for ``x`` [.., d] and ``weight`` [out, d], with gradients for all four.  Float32 or bfloat16 on the GPU, all of one
     type, ``d`` and ``out`` up to 4096; rows that lie apart are taken as they are (bfloat16: where they start on four bytes), other orders copied.
     ``activation``: ``None``, ``"relu"``, ``"gelu"`` (by the normal distribution function) or ``"silu"``; ``residual``: of the output's sizes.
-    Sums are float32, and the output is rounded once (a float32 sum that an infinite value takes part in may be no number: values are multiplied in parts); in the backward pass the gradient behind the activation is rounded to the type once more.
+    Sums are float32, and the output is rounded once; a row with an infinite value is infinite by its weights' signs.  In the backward pass the gradient behind the activation is rounded to the type once more.
     For the backward pass ``weight`` is kept, ``x`` if ``weight`` has a gradient (no other reads it), and for ``"relu"`` a bit a value, for ``"gelu"`` and ``"silu"`` their derivatives (float32, or beside bfloat16 2**15 times it in float16: eleven bits down to 2**-29).  ``keep8=True``: in ``x``'s place
     8 bits a value of it, as ``layer_norm`` holds them: ``weight``'s gradient is that of the values so held, all others are not touched by it.
     Under autocast, its type is taken, which must be one of the two, for the residual and the output too.  No gradients of gradients.  Under tracing, forward-mode differentiation, transforms of ``torch.func`` and modes
