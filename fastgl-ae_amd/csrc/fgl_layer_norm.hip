@@ -10,7 +10,7 @@
 // than the row's spread), relu's decision and the code of a value in 8 bits (fgl_keep8.hpp) are those of the formula, not of an order of summation.
 // The 64-bit instructions issue like the 32-bit ones here, and there is room for them beside the pass over memory.
 //
-// For the backward pass a row leaves its mean (64 bits) and 1 / sqrt (32), with relu a bit a value, and with KEEP8 h in 8 bits a value in x's place.
+// For the backward pass a row leaves its mean and 1 / sqrt (64 bits each: 1 / sqrt, and differences from the mean, may be past fp32's range where h is not), with relu a bit a value, and with KEEP8 h in 8 bits a value in x's place.
 //
 // What bounds it: the pass over memory.  us forward / back (and 4 .. 7 for the second launch): 60 K x 256 fp32 22 / 37 (5.6 and 4.9 TB/s; relu in it), 87 K x 256 bf16 with relu and KEEP8
 // 27 / 26, where codes and relu's decision take as long as the memory forward, 2.4 M x 64 fp32 of rows of 100 columns with KEEP8 325 / 262.  Rows that do not begin on 16 bytes cost
@@ -29,7 +29,7 @@ constexpr int kLnMostBlocks = 1024;  // of the backward pass: rows of partial su
 
 struct LnState {
     double* mean;    // without KEEP8
-    float* rstd;
+    double* rstd;
     uint8_t* mask;   // relu: [n][mask_ld], bit c % 8 of byte c / 8
     uint8_t* codes;  // KEEP8: [n][k8_columns(d)]
     uint8_t* steps;  // KEEP8: [n][k8_columns(d) / 32]
@@ -42,7 +42,7 @@ static LnState ln_state(void* base, int64_t n, int d, bool relu, bool keep8)
     LnState s;
     memset(&s, 0, sizeof(s));
     if (!keep8) s.mean = c.take<double>((size_t)n);
-    s.rstd = c.take<float>((size_t)n);
+    s.rstd = c.take<double>((size_t)n);
     if (relu) s.mask = c.take<uint8_t>((size_t)n * (size_t)((d + 7) / 8));
     if (keep8) {
         s.codes = c.take<uint8_t>((size_t)n * (size_t)k8_columns(d));
@@ -206,7 +206,7 @@ __global__ __launch_bounds__(kLnThreads, C * kLnV<T> <= 16 ? 4 : 2) void layer_n
             }
         const double rstd = ln_rsqrt(fma(ln_sum<G>(square), g.inv_d64, g.eps));
         if (g.state.rstd != nullptr && l == 0 && mine) {
-            g.state.rstd[row] = (float)rstd;
+            g.state.rstd[row] = rstd;
             if constexpr (!KEEP8) g.state.mean[row] = mean;
         }
 #pragma unroll
@@ -303,7 +303,7 @@ __global__ __launch_bounds__(kLnThreads, C * kLnV<T> <= 16 ? 4 : 2) void layer_n
             bits[j] = 0xFFu;
             if (g.relu && left > 0) bits[j] = (uint32_t)g.state.mask[row * g.mask_ld + c / 8] >> (c % 8);
         }
-        const float rstd = g.state.rstd[row];
+        const double rstd = g.state.rstd[row];
         const double mean = KEEP8 ? 0.0 : g.state.mean[row];
         float sum = 0.0f, with_h = 0.0f;
 #pragma unroll
@@ -312,7 +312,7 @@ __global__ __launch_bounds__(kLnThreads, C * kLnV<T> <= 16 ? 4 : 2) void layer_n
             for (int e = 0; e < V; ++e) {
                 const bool there = ln_there<WHOLE>(j < ln_inside(G, C), e, g.d - (j * G + l) * V);
                 if constexpr (KEEP8) h[j][e] = there ? k8_code_value(codes[j][e / 4], e % 4) * k8_step_value(step[j]) : 0.0f;
-                else h[j][e] = there ? (float)((double)(float)vx[j][e] - mean) * rstd : 0.0f;
+                else h[j][e] = there ? (float)(((double)(float)vx[j][e] - mean) * rstd) : 0.0f;
                 const float d = bits[j] >> e & 1u ? (float)vd[j][e] : 0.0f;
                 // (rows past the end leave dw as it is, also where the last one's h is no number)
                 dw[j][e] = fmaf(d, mine ? h[j][e] : 0.0f, dw[j][e]);
@@ -324,12 +324,21 @@ __global__ __launch_bounds__(kLnThreads, C * kLnV<T> <= 16 ? 4 : 2) void layer_n
         if (dx == nullptr) continue;
         sum = ln_sum<G>(sum) * g.inv_d;
         with_h = ln_sum<G>(with_h) * g.inv_d;
+        // bf16: 1 / sqrt in two factors, the second a power of two, one unless the whole is next to fp32's ends or past them (rows of tiny values without eps, rows next to the
+        // largest).  fp32: in 64 bits, which cost less there than the registers of the factors, and more than they in bf16 (us forward and back: 60 K x 256 fp32 64.3 / 66.4 in factors,
+        // 200 K x 602 bf16 335 / 330).
+        const float more = rstd > 0x1p100 ? 0x1p100f : rstd < 0x1p-100 ? 0x1p-100f : 1.0f;
+        const float scale = (float)(rstd * (rstd > 0x1p100 ? 0x1p-100 : rstd < 0x1p-100 ? 0x1p100 : 1.0));
 #pragma unroll
         for (int j = 0; j < C; ++j) {
             const int c = (j * G + l) * V;
             LnVec<T> q;
 #pragma unroll
-            for (int e = 0; e < V; ++e) q[e] = (T)(rstd * (t[j][e] - sum - h[j][e] * with_h));
+            for (int e = 0; e < V; ++e) {
+                const float v = t[j][e] - sum - h[j][e] * with_h;
+                if constexpr (sizeof(T) == 4) q[e] = (float)(rstd * (double)v);
+                else q[e] = (T)(scale * v * more);
+            }
             if (mine) ln_store<WHOLE>(dx + row * g.d + c, j < ln_inside(G, C), g.d - c, q);
         }
     }
