@@ -3,7 +3,8 @@
 //
 // P by the error function's rational approximation 7.1.26 of Abramowitz and Stegun's Handbook (absolute error 1.5e-7, so that P is off by 0.75e-7): the
 // exponential in it is the derivative's too, and one reciprocal and five products go with it, where a library's erf branches.  Below zero P is the
-// small term itself, with no difference taken.  Exponentials and reciprocals are the instructions', 2^-22 and better.
+// small term itself, with no difference taken.  Exponentials and reciprocals are the instructions', 2^-23 or so, and an
+// exponential's argument v is rounded before: |v| 2^-23 of the result at most (2^-17 at the ends of the range, where the result is next to nothing).
 #pragma once
 
 #include "fgl_common.hpp"

@@ -8,12 +8,13 @@
 //
 // Mean, variance and h are formed in 64 bits: rows far from zero keep what they differ in (a mean in 32 bits is off by 2^-24 of itself, which may be more
 // than the row's spread), relu's decision and the code of a value in 8 bits (fgl_keep8.hpp) are those of the formula, not of an order of summation.
-// The 64-bit instructions issue like the 32-bit ones here, and there is room for them beside the pass over memory.
+// The 64-bit instructions issue like the 32-bit ones here, and there is room for them beside the pass over memory; but where a bf16 row's codes and relu's decision are formed too, they
+// are what the forward pass takes.
 //
 // For the backward pass a row leaves its mean and 1 / sqrt (64 bits each: 1 / sqrt, and differences from the mean, may be past fp32's range where h is not), with relu a bit a value, and with KEEP8 h in 8 bits a value in x's place.
 //
 // What bounds it: the pass over memory.  us forward / back (and 4 .. 7 for the second launch): 60 K x 256 fp32 22 / 37 (5.6 and 4.9 TB/s; relu in it), 87 K x 256 bf16 with relu and KEEP8
-// 27 / 26, where codes and relu's decision take as long as the memory forward, 2.4 M x 64 fp32 of rows of 100 columns with KEEP8 325 / 262.  Rows that do not begin on 16 bytes cost
+// 27 / 28, where the 64-bit instructions of codes and relu's decision take longer than the memory forward, 2.4 M x 64 fp32 of rows of 100 columns with KEEP8 325 / 266.  Rows that do not begin on 16 bytes cost
 // loads and stores across lines: 200 K x 602 bf16 137 / 191, 600 columns 107 / 161.
 #include "fgl_common.hpp"
 #include "fgl_keep8.hpp"

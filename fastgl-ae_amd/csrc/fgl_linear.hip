@@ -3,7 +3,8 @@
 //
 // The products are fgl_row_product.hip's (fp32 on the bf16 matrix cores: fgl_split_product.hip) and fgl_wgrad.hip's; the forward one stores act(z) + residual
 // from its accumulators, and act': a bit a value for relu, the slope itself for gelu and silu (in bf16 as fp16, whose eleven bits, down to 2^-29, leave dz with the one rounding that the
-// matrix cores ask for: gradients off by 2.4e-3 in the 2-norm, results rounded once alone by 1.7e-3; with z kept in bf16 2.5e-3).  The backward pass forms dz in one pass over dy
+// matrix cores ask for: gradients off by 2.36e-3 in the 2-norm, results rounded once alone by 1.66e-3, torch's layer in bf16 2.43e-3; with z kept in bf16 2.5e-3.  dz in two bf16 parts would
+// leave the results' rounding alone, for twice the products and a pass over n x out values more in each of three kernels).  The backward pass forms dz in one pass over dy
 // (none where there is no activation: dz is dy).
 //
 // KEEP8: the rows of x are held in 8 bits a value (fgl_keep8.hpp) for dW, which fgl_wgrad8.hip forms from them; dx and db need no x.  db comes with dW, or alone from

@@ -15,7 +15,8 @@
 // large beside, or a sum is no number, a workgroup forms its rows again in fp32 instructions.
 //
 // What bounds it: in fp32 the vector unit (a step of 32 x 128: 44 instructions split A, 104 make the codes' operands, 64 add the products to the accumulators, beside 12 matrix
-// instructions of 32 cycles) and the L2s, from which every tile takes its rows, in bf16 those.  us with the second launch: 107 K x 100 x 256 fp32 47 (from rows in full, fgl_wgrad.hip,
+// instructions of 32 cycles; busy for 55 % and 19 % of the time) and the L2s, from which every tile takes its rows, in bf16 those.  With more than 64 tiles there are
+// fewer than eight splits, each of one XCD, and the others have no work: 602 x 512 fp32 runs on six, 1024 x 1024 on two.  us with the second launch: 107 K x 100 x 256 fp32 47 (from rows in full, fgl_wgrad.hip,
 // 65; one step ahead instead of two 59, tiles of 64 x 64 52), 8192 x 602 x 256 fp32 30; 87 K x 512 x 256 bf16 52 (tiles of 128 x 64 58).
 #include "fgl_column_sums.hpp"
 #include "fgl_common.hpp"
