@@ -11,7 +11,7 @@
 // The 64-bit instructions issue like the 32-bit ones here, and there is room for them beside the pass over memory; but where a bf16 row's codes and relu's decision are formed too, they
 // are what the forward pass takes.
 //
-// For the backward pass a row leaves its mean and 1 / sqrt (64 bits each: 1 / sqrt, and differences from the mean, may be past fp32's range where h is not), with relu a bit a value, and with KEEP8 h in 8 bits a value in x's place.
+// For the backward pass a row leaves its mean (64 bits) and 1 / sqrt (32, of a wider range: it, and differences from the mean, may be past fp32's where h is not), with relu a bit a value, and with KEEP8 h in 8 bits a value in x's place.
 //
 // What bounds it: the pass over memory.  us forward / back (and 4 .. 7 for the second launch): 60 K x 256 fp32 22 / 37 (5.6 and 4.9 TB/s; relu in it), 87 K x 256 bf16 with relu and KEEP8
 // 27 / 28, where the 64-bit instructions of codes and relu's decision take longer than the memory forward, 2.4 M x 64 fp32 of rows of 100 columns with KEEP8 325 / 266.  Rows that do not begin on 16 bytes cost
@@ -30,7 +30,7 @@ constexpr int kLnMostBlocks = 1024;  // of the backward pass: rows of partial su
 
 struct LnState {
     double* mean;    // without KEEP8
-    double* rstd;
+    float* rstd;     // ln_held
     uint8_t* mask;   // relu: [n][mask_ld], bit c % 8 of byte c / 8
     uint8_t* codes;  // KEEP8: [n][k8_columns(d)]
     uint8_t* steps;  // KEEP8: [n][k8_columns(d) / 32]
@@ -43,7 +43,7 @@ static LnState ln_state(void* base, int64_t n, int d, bool relu, bool keep8)
     LnState s;
     memset(&s, 0, sizeof(s));
     if (!keep8) s.mean = c.take<double>((size_t)n);
-    s.rstd = c.take<double>((size_t)n);
+    s.rstd = c.take<float>((size_t)n);
     if (relu) s.mask = c.take<uint8_t>((size_t)n * (size_t)((d + 7) / 8));
     if (keep8) {
         s.codes = c.take<uint8_t>((size_t)n * (size_t)k8_columns(d));
@@ -112,6 +112,19 @@ __device__ __forceinline__ double ln_rsqrt(double v)
 {
     const double r = __builtin_amdgcn_rsq(v), e = fma(-v * r, r, 1.0);
     return fma(r * e, fma(0.375, e, 0.5), r);
+}
+
+// 1 / sqrt in 32 bits: as it is from 2^-100 to 2^100; negative, times 2^-36 above (up to 2^162: rows of one value and an eps below 2^-324 alone have more) and times 2^150 below
+__device__ __forceinline__ float ln_held(double r)
+{
+    if (r > 0x1p100) return -(float)(fmin(r, 0x1p162) * 0x1p-36);
+    if (r < 0x1p-100) return -(float)(r * 0x1p150);
+    return (float)r;
+}
+__device__ __forceinline__ double ln_of_held(float v)
+{
+    const double r = v;
+    return v < 0.0f ? r * (v < -0x1p57f ? -0x1p36 : -0x1p-150) : r;
 }
 
 // The lane's values of a chunk, of which the first `left` exist (others: `fill`).  WHOLE: rows are a whole number of chunks, all or none exist.
@@ -207,7 +220,7 @@ __global__ __launch_bounds__(kLnThreads, C * kLnV<T> <= 16 ? 4 : 2) void layer_n
             }
         const double rstd = ln_rsqrt(fma(ln_sum<G>(square), g.inv_d64, g.eps));
         if (g.state.rstd != nullptr && l == 0 && mine) {
-            g.state.rstd[row] = rstd;
+            g.state.rstd[row] = ln_held(rstd);
             if constexpr (!KEEP8) g.state.mean[row] = mean;
         }
 #pragma unroll
@@ -304,7 +317,7 @@ __global__ __launch_bounds__(kLnThreads, C * kLnV<T> <= 16 ? 4 : 2) void layer_n
             bits[j] = 0xFFu;
             if (g.relu && left > 0) bits[j] = (uint32_t)g.state.mask[row * g.mask_ld + c / 8] >> (c % 8);
         }
-        const double rstd = g.state.rstd[row];
+        const double rstd = ln_of_held(g.state.rstd[row]);
         const double mean = KEEP8 ? 0.0 : g.state.mean[row];
         float sum = 0.0f, with_h = 0.0f;
 #pragma unroll

@@ -35,7 +35,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, relu=False, keep8=False):
     for all three.  ``x``: float32 or bfloat16 on the GPU, any leading dimensions; rows that lie apart are taken as they are, other orders copied.
     ``weight``, ``bias``: of x's type, or ``None`` for ones and zeros.  Mean, variance and the normed values are formed in 64 bits, so that rows far from
     zero keep what they differ in.
-    For the backward pass ``x`` is kept with 16 bytes a row, and with ``relu`` a bit a value.  ``keep8=True``: in ``x``'s place the normed values, 8 bits each: 32
+    For the backward pass ``x`` is kept with 12 bytes a row, and with ``relu`` a bit a value.  ``keep8=True``: in ``x``'s place the normed values, 8 bits each: 32
     neighbouring columns share a step, ``2**(floor(log2(largest magnitude)) - 6)``, and the nearest of -127 .. 127 steps is held; gradients are those of
     the values so held (32 columns with one that is not finite are held as not a number).
     Under autocast in float32, as torch's.  No gradients of gradients.  Under tracing, forward-mode differentiation, transforms of
