@@ -85,3 +85,30 @@ def test_many_gradients_at_once(cuda):
     got, = torch.autograd.grad(y, b, many, is_grads_batched=True, retain_graph=True)
     for i in range(5):
         assert torch.equal(got[i], torch.autograd.grad(y, b, many[i], retain_graph=True)[0])
+
+
+@pytest.mark.parametrize("act", [0, 1, 3])
+@pytest.mark.parametrize("code,dtype", [(0, torch.float32), (1, torch.bfloat16)])
+@pytest.mark.parametrize("n,d,out", [(1, 1, 1), (37, 47, 33), (2500, 100, 130), (9001, 600, 257)])
+def test_entry_point_without_the_input(cuda, act, code, dtype, n, d, out):
+    """Neither x nor 8 bits of it: the state of a forward pass without keep8, workspaces to the byte and full of no numbers, nothing written past the outputs."""
+    from fastgl import _lib as L
+
+    lib = L.lib()
+    gen = torch.Generator(device=cuda).manual_seed(n)
+    even, wide = d + d % 2, out + out % 2
+    x, w, dy = (torch.randn(s, generator=gen, device=cuda).to(dtype) for s in ((n, even), (out, even), (n, wide)))
+    y = torch.empty((n, out), device=cuda, dtype=dtype)
+    for keep8 in (0, 1):
+        held = []
+        for kept, need_w in ((keep8, 1), (keep8, 0), (0, 0)):
+            size = lib.fgl_linear_state_bytes(n, d, out, code, act, kept)
+            room = lib.fgl_linear_workspace_bytes(n, d, out, code, act, keep8, need_w, 1)
+            state, ws = (torch.full((b + 256,), 255, device=cuda, dtype=torch.uint8) for b in (size, room))
+            db, dw, dx = (torch.full((c + 64,), 7.0, device=cuda, dtype=dtype) for c in (out, out * d, n * d))
+            L.check(lib.fgl_linear(x.data_ptr(), even, w.data_ptr(), even, None, None, 0, n, d, out, code, act, kept, y.data_ptr(), out, state.data_ptr(), size, L.stream_handle()))
+            L.check(lib.fgl_linear_backward(dy.data_ptr(), wide, x.data_ptr() if need_w else None, even if need_w else 0, w.data_ptr(), even, n, d, out, code, act, keep8,
+                                            state.data_ptr(), size, dx.data_ptr(), d, dw.data_ptr() if need_w else None, db.data_ptr(), ws.data_ptr(), room, L.stream_handle()))
+            assert (state[size:] == 255).all() and (ws[room:] == 255).all() and (db[out:] == 7).all() and (dx[n * d:] == 7).all()
+            held.append((db[:out].clone(), dx[:n * d].clone()))
+        assert all(torch.equal(p, q) for one in held[1:] for p, q in zip(one, held[0])) and held[0][0].isfinite().all()
