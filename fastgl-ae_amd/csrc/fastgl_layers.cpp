@@ -233,7 +233,7 @@ struct LinearNode : torch::autograd::Function<LinearNode> {
     {
         const bool keep8 = z.keep8, sums = w.requires_grad();  // (nothing but the weight's gradient reads x)
         z.keep8 = keep8 && sums;
-        const bool kept = z.keep8 || z.act != 0;
+        const bool kept = z.keep8 || (z.act != 0 && (x.requires_grad() || sums || (bias.has_value() && bias->requires_grad())));  // (the residual's gradient is the output's)
         auto [y, state] = form_linear(x, w, bias.value_or(Tensor()), residual.value_or(Tensor()), z, kept);
         ctx->saved_data["dim"] = (int64_t)z.dim;
         ctx->saved_data["act"] = (int64_t)z.act;

@@ -1,4 +1,4 @@
-"""A dense layer whose bias has a gradient and whose weight has none: the bias's needs nothing of the input."""
+"""A dense layer whose bias, or residual, has a gradient and whose weight has none: neither needs anything of the input, and the residual's nothing at all."""
 import pytest
 import torch
 
@@ -55,6 +55,18 @@ def test_keeps_nothing_of_the_input(cuda, act, keep8):
     got, = torch.autograd.grad(y, b, dy)
     assert torch.equal(got, want)
     assert torch.cuda.max_memory_allocated() - held < (2.5 if act else 1) * room + (1 << 20)  # (no gradient of the weight)
+
+
+def test_residual_alone_keeps_nothing(cuda):
+    x, w, b, dy = problem(cuda, 20_000, 64, 64, torch.float32)
+    b, r = b.detach(), torch.randn((20_000, 64), device=cuda, requires_grad=True)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    y = fastgl.linear(x, w, b, "gelu", r, keep8=True)
+    assert torch.cuda.memory_allocated() - before < 1.5 * 20_000 * 64 * 4  # (the output)
+    assert torch.equal(torch.autograd.grad(y, r, dy)[0], dy)
+    with torch.no_grad():
+        assert torch.equal(fastgl.linear(x, w, b, "gelu", r), y)
 
 
 def test_captured(cuda):
